@@ -206,7 +206,9 @@ int kda_b200_device_error(int reset);
  *   8     the forward chunk kernel's wait for its prefetched inputs ran out;
  *   9     a chunk kernel's dynamic shared memory was not 1 KB aligned (its
  *         swizzled tensor-core tiles need it): the kernel did nothing;
- *   10    a tensor-core completion wait of the forward chunk kernel ran out.
+ *   10    a tensor-core completion wait of the forward chunk kernel ran out;
+ *   11    a single-token call named a state slot past its pool (that row was
+ *         treated as padding).
  * A kernel that records a timeout lets its copies in flight land (a second
  * bounded wait), frees what it holds and returns; later calls are unaffected.
  */
@@ -293,6 +295,120 @@ int kda_b200_gated_norm_fwd(const void* o, const void* g, const float* weight, l
 int kda_b200_gated_norm_bwd(const void* dy, const void* o, const void* g, const float* weight, long long rows,
                             int D, float eps, int fp32_io, void* d_o, void* d_g, float* d_weight, void* workspace,
                             size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * State-space operators: the short causal convolution and the selective scan,
+ * for prompts (forward and backward) and for single tokens, and the global
+ * gradient norm with clipping.  The reference has no counterpart (its mixers are
+ * KDA and attention); they share this ABI's conventions.
+ *
+ * Activations are KDA_IO_F32, KDA_IO_BF16 or KDA_IO_F16, all of one type per call,
+ * rows [B, T, width] whose last dimension is contiguous; *_sb and *_st are
+ * their batch and token strides in elements, so slices of a wider projection
+ * are read in place.  Outputs are contiguous.  Parameters, states and their
+ * gradients are fp32.  cu_seqlens (int32 [N+1], device; then B == 1) packs N
+ * sequences along T; every sequence starts from its own initial state.  An
+ * empty sequence's final state is its initial state.  A malformed table sets
+ * kda_b200_device_error() to 3.  Every element of every output is written.
+ */
+#define KDA_IO_F32 0
+#define KDA_IO_BF16 1
+#define KDA_IO_F16 2
+
+/*
+ * Causal depthwise convolution over tokens, 1 <= W <= 4 taps:
+ *     c[t] = bias + sum_k w[k] x[t - (W-1) + k],   y = silu(c) or c (silu = 0)
+ * x: [B, T, C]; w: [C][W], bias: [C] or NULL; h0 / ht: [N][C][W-1] (the last W-1
+ * inputs, oldest first) or NULL; y: [B, T, C].  The backward takes the output
+ * gradient dy (strides of its own) and the final state's dht (NULL = zero) and writes
+ * dx [B, T, C], dw [C][W], dbias [C] (may be NULL) and dh0 (may be NULL).  The sums over
+ * tokens have a fixed order.
+ */
+size_t kda_b200_short_conv_workspace_bytes(int64_t B, int64_t T, int C, int W, int packed, int backward);
+int kda_b200_short_conv_fwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias,
+                            const float* h0, const int32_t* cu_seqlens, int64_t B, int64_t T, int C, int W, int N,
+                            int dtype, int silu, void* y, float* ht, void* workspace, size_t workspace_bytes,
+                            void* stream);
+int kda_b200_short_conv_bwd(const void* x, int64_t x_sb, int64_t x_st, const float* w, const float* bias,
+                            const float* h0, const int32_t* cu_seqlens, int64_t B, int64_t T, int C, int W, int N,
+                            int dtype, int silu, const void* dy, int64_t dy_sb, int64_t dy_st, const float* dht,
+                            void* dx, float* dw, float* dbias, float* dh0, void* workspace, size_t workspace_bytes,
+                            void* stream);
+/*
+ * One token for each of `rows` requests.  x: [rows, C], row stride x_sr; state: a pool
+ * [pool][C][W-1], rewritten in place; slots: int32 [rows], the pool entry of each
+ * row, or NULL (row r uses entry r).  A negative slot marks a padding row: y = 0, no
+ * state is touched; a slot >= pool does the same and sets
+ * kda_b200_device_error() to 11.  Two rows must not name one slot.
+ */
+int kda_b200_short_conv_step(const void* x, int64_t x_sr, const float* w, const float* bias, float* state,
+                             const int32_t* slots, int rows, int C, int W, int pool, int dtype, int silu, void* y,
+                             void* stream);
+
+/*
+ * Selective state space scan.  Per sequence, channel e and state n, with
+ * d = softplus(dt + dt_bias) (or dt + dt_bias, softplus = 0):
+ *     h[t] = exp(d A[e][n]) h[t-1] + d x[t] B[t][n]
+ *     s[t] = sum_n C[t][n] h[t][n] + D[e] x[t],   y[t] = s[t] silu(z[t])  (or s[t])
+ * Channels are split evenly over G groups; a group shares its rows of B and C.
+ * 1 <= N <= 64.  Unused pointers are NULL: z, D, dt_bias, h0, ht, dht, dh0, cu_seqlens;
+ * saved (kda_b200_scan_saved_bytes() bytes) is NULL for inference.
+ * kda_b200_selective_scan_bwd takes the same inputs, the saved buffer of the
+ * forward, dy and dht, and writes dx, ddt, dz, dB, dC ([B, T, G, N]) in the activations' type
+ * and dA [E][N], dD, ddt_bias [E] (either may be NULL) and dh0 in fp32; all sums have a
+ * fixed order.
+ * kda_b200_selective_scan_step takes `rows` single tokens: x, dt, z [rows, E], B and C
+ * [rows, G, N] (*_sb: row strides), a pool of states [pool][E][N] rewritten in place, and slots as
+ * kda_b200_short_conv_step; y [rows, E].
+ */
+typedef struct kda_b200_scan_args {
+  int64_t B, T;
+  int32_t E, N, G, nseq, dtype, softplus;
+  const void *x, *dt, *z, *B_, *C_;
+  int64_t x_sb, x_st, dt_sb, dt_st, z_sb, z_st, B_sb, B_st, B_sg, C_sb, C_st, C_sg;
+  const float *A, *D, *dt_bias, *h0;
+  const int32_t* cu_seqlens;
+  void* y;
+  float* ht;
+  void* saved;
+  size_t saved_bytes;
+  /* backward */
+  const void* dy;
+  int64_t dy_sb, dy_st;
+  const float* dht;
+  void *dx, *ddt, *dz, *dB, *dC;
+  float *dA, *dD, *ddt_bias, *dh0;
+  /* single tokens */
+  float* state;
+  const int32_t* slots;
+  int32_t rows, pool;
+} kda_b200_scan_args;
+size_t kda_b200_scan_saved_bytes(int64_t B, int64_t T, int E, int N, int G);
+size_t kda_b200_scan_workspace_bytes(int64_t B, int64_t T, int E, int N, int G, int packed, int backward);
+int kda_b200_selective_scan_fwd(const kda_b200_scan_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int kda_b200_selective_scan_bwd(const kda_b200_scan_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int kda_b200_selective_scan_step(const kda_b200_scan_args* args, void* stream);
+
+/*
+ * Global gradient norm over `count` tensors, and clipping:
+ *     norm = sqrt(sum g^2);   out = g * min(1, max_norm / (norm + eps))
+ * in, numel, in_type (and out, out_type): HOST arrays of device addresses, element
+ * counts and KDA_IO_* types, read during the call; out NULL computes the norm
+ * alone.  out[i] == in[i] clips in place (nothing is written when the factor is 1); a
+ * tensor and an output must not overlap otherwise.  norm: device fp32 [1].  Squares are summed
+ * in an order that the sizes alone decide.  A non-finite norm leaves as it is: with it
+ * the outputs are NaN (norm NaN) or 0 and NaN (norm infinite).
+ */
+typedef struct kda_b200_grad_args {
+  int64_t count;
+  const uint64_t *in, *out;
+  const int64_t* numel;
+  const uint8_t *in_type, *out_type;
+  float max_norm, eps;
+  float* norm;
+} kda_b200_grad_args;
+size_t kda_b200_grad_workspace_bytes(int64_t count);
+int kda_b200_grad_clip(const kda_b200_grad_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

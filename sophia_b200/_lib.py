@@ -17,6 +17,30 @@ KDA_ERR_INVALID = 1
 KDA_ERR_UNSUPPORTED = 2
 KDA_ERR_CUDA = 3
 
+
+
+class ScanArgs(ctypes.Structure):
+    """``kda_b200_scan_args``."""
+
+    _fields_ = ([(n, c_int64) for n in ("B", "T")]
+                + [(n, ctypes.c_int32) for n in ("E", "N", "G", "nseq", "dtype", "softplus")]
+                + [(n, c_void_p) for n in ("x", "dt", "z", "B_", "C_")]
+                + [(n, c_int64) for n in ("x_sb", "x_st", "dt_sb", "dt_st", "z_sb", "z_st", "B_sb", "B_st", "B_sg",
+                                          "C_sb", "C_st", "C_sg")]
+                + [(n, c_void_p) for n in ("A", "D", "dt_bias", "h0", "cu_seqlens", "y", "ht", "saved")]
+                + [("saved_bytes", c_size_t), ("dy", c_void_p), ("dy_sb", c_int64), ("dy_st", c_int64)]
+                + [(n, c_void_p) for n in ("dht", "dx", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias", "dh0", "state",
+                                           "slots")]
+                + [("rows", ctypes.c_int32), ("pool", ctypes.c_int32)])
+
+
+class GradArgs(ctypes.Structure):
+    """``kda_b200_grad_args`` (host arrays; the types as bytes objects)."""
+
+    _fields_ = [("count", c_int64), ("in_", c_void_p), ("out", c_void_p), ("numel", c_void_p), ("in_type", c_char_p),
+                ("out_type", c_char_p), ("max_norm", c_float), ("eps", c_float), ("norm", c_void_p)]
+
+
 # every symbol the header declares, with its ctypes signature
 SIGNATURES = {
     "kda_b200_version": ([], c_char_p),
@@ -52,6 +76,19 @@ SIGNATURES = {
                                 c_int),
     "kda_b200_gated_norm_bwd": ([c_void_p] * 4 + [c_int64, c_int, c_float, c_int] + [c_void_p] * 4
                                 + [c_size_t, c_void_p], c_int),
+    "kda_b200_short_conv_workspace_bytes": ([c_int64, c_int64] + [c_int] * 4, c_size_t),
+    "kda_b200_short_conv_fwd": ([c_void_p, c_int64, c_int64] + [c_void_p] * 4 + [c_int64, c_int64] + [c_int] * 5
+                                + [c_void_p, c_void_p, c_void_p, c_size_t, c_void_p], c_int),
+    "kda_b200_short_conv_bwd": ([c_void_p, c_int64, c_int64] + [c_void_p] * 4 + [c_int64, c_int64] + [c_int] * 5
+                                + [c_void_p, c_int64, c_int64] + [c_void_p] * 5 + [c_void_p, c_size_t, c_void_p], c_int),
+    "kda_b200_short_conv_step": ([c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 6 + [c_void_p, c_void_p], c_int),
+    "kda_b200_scan_saved_bytes": ([c_int64, c_int64] + [c_int] * 3, c_size_t),
+    "kda_b200_scan_workspace_bytes": ([c_int64, c_int64] + [c_int] * 5, c_size_t),
+    "kda_b200_selective_scan_fwd": ([ctypes.POINTER(ScanArgs), c_void_p, c_size_t, c_void_p], c_int),
+    "kda_b200_selective_scan_bwd": ([ctypes.POINTER(ScanArgs), c_void_p, c_size_t, c_void_p], c_int),
+    "kda_b200_selective_scan_step": ([ctypes.POINTER(ScanArgs), c_void_p], c_int),
+    "kda_b200_grad_workspace_bytes": ([c_int64], c_size_t),
+    "kda_b200_grad_clip": ([ctypes.POINTER(GradArgs), c_void_p, c_size_t, c_void_p], c_int),
 }
 
 _lib = None

@@ -33,12 +33,12 @@ def sources() -> list[Path]:
 
 def build(verbose: bool = False, force: bool = False) -> Path:
     srcs = sources()
-    deps = srcs + sorted(CSRC.glob("*.cuh")) + [PKG.parent / "include" / "kda_b200.h"]
+    deps = srcs + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + [PKG.parent / "include" / "kda_b200.h"]
     if LIB.exists() and not force:
         newest = max(p.stat().st_mtime for p in deps)
         if LIB.stat().st_mtime >= newest:
             return LIB
-    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17",
+    cmd = [nvcc(), *ARCH, "-O3", "-lineinfo", "-std=c++17", "--threads", "0",
            "-Xcompiler", "-fPIC", "-shared", "-o", str(LIB) + ".tmp",
            *[str(s) for s in srcs]]
     if verbose:

@@ -1,0 +1,125 @@
+"""Global gradient norm and clipping, between the gradient all-reduce and the
+optimizer: ``grad_norm`` and ``clip_grad_norm_`` take any number of gradient
+tensors of any supported types in two kernel launches, without a host wait (a
+training step stays capturable).  The reference clips in its trainer with torch's
+own utility.
+"""
+
+from __future__ import annotations
+
+import math
+from array import array
+from typing import Iterable, Sequence
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from ._lib import GradArgs
+from .ssm import _IO, _on, _stream
+
+__all__ = ["grad_norm", "clip_grad_norm_"]
+
+
+def _list(what: str, grads) -> list[Tensor]:
+    ts = [grads] if isinstance(grads, Tensor) else list(grads)
+    for t in ts:
+        if not isinstance(t, Tensor):
+            raise ValueError(f"{what} takes gradient tensors, got {type(t).__name__}")
+        if t.dtype not in _IO:
+            raise NotImplementedError(f"{what}: gradients must be float32, bfloat16 or float16, got {t.dtype}")
+        if not t.is_cuda:
+            raise RuntimeError(f"{what} runs on the CUDA kernels only: gradients must be CUDA tensors")
+    if len({t.device for t in ts}) > 1:
+        raise RuntimeError(f"{what}: gradients are on several devices")
+    return ts
+
+
+def _dense(t: Tensor) -> bool:
+    """Whether the tensor's elements fill one run of memory, in whatever order."""
+    if t.is_contiguous():
+        return True
+    at = 1
+    for stride, size in sorted((st, s) for st, s in zip(t.stride(), t.shape) if s != 1):
+        if stride != at:
+            return False
+        at *= size
+    return True
+
+
+def _addresses(ts: Sequence[Tensor]) -> array:
+    return array("Q", [t.data_ptr() for t in ts])
+
+
+def _types(ts: Sequence[Tensor]) -> bytes:
+    return bytes([_IO[t.dtype] for t in ts])
+
+
+def _call(ts: list[Tensor], out: list[Tensor] | None, max_norm: float, eps: float) -> Tensor:
+    norm = torch.empty((), device=ts[0].device, dtype=torch.float32)
+    lib = _lib.load()
+    ws = torch.empty(lib.kda_b200_grad_workspace_bytes(len(ts)), device=ts[0].device, dtype=torch.uint8)
+    src, numel, tin = _addresses(ts), array("q", [t.numel() for t in ts]), _types(ts)
+    dst, tout = (None, None) if out is None else (_addresses(out), _types(out))
+    addr = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
+    args = GradArgs(len(ts), addr(src), addr(dst), addr(numel), tin, tout, max_norm, eps, norm.data_ptr())
+    _lib.check(lib.kda_b200_grad_clip(args, ws.data_ptr(), ws.numel(), _stream()))
+    return norm
+
+
+def grad_norm(grads: Tensor | Iterable[Tensor]) -> Tensor:
+    """``sqrt(sum g^2)`` over all elements of all tensors (float32, bfloat16 or
+    float16, any mix), as a 0-d float32 CUDA tensor; 0 on an empty list is on the
+    current device.  No host wait.  The result does not depend on timing: sums have a
+    fixed order."""
+    with torch.no_grad():
+        ts = _list("grad_norm", grads)
+        if not ts:
+            return torch.zeros((), device="cuda", dtype=torch.float32)
+        with _on(ts[0]):
+            return _call([t if _dense(t) else t.contiguous() for t in ts], None, 0.0, 0.0)
+
+
+def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: float = 1e-6,
+                    out: Sequence[Tensor] | Tensor | None = None) -> Tensor:
+    """Scales the gradients by ``min(1, max_norm / (norm + eps))``, ``norm``
+    their global 2-norm, and returns the norm (0-d float32 CUDA tensor, before
+    clipping).  In place by default; with ``out``, tensors of the gradients' shapes and of any
+    supported type (an optimizer's float32 gradients), every element of which is
+    written, the gradients stay as they are.  ``out[i] is grads[i]`` is allowed; otherwise no two
+    tensors may overlap.  A NaN norm makes the scaled gradients NaN, an infinite one 0 (and
+    NaN where a gradient is infinite), as the formula says; there is no host wait to look."""
+    what = "clip_grad_norm_"
+    max_norm, eps = float(max_norm), float(eps)
+    if math.isnan(max_norm) or max_norm < 0 or not eps >= 0:
+        raise ValueError(f"{what}: max_norm and eps must be >= 0, got {max_norm} and {eps}")
+    with torch.no_grad():
+        ts = _list(what, grads)
+        outs = ts if out is None else _list(what, out)
+        if len(outs) != len(ts):
+            raise ValueError(f"{what}: {len(ts)} gradients but {len(outs)} outputs")
+        if not ts:
+            return torch.zeros((), device="cuda", dtype=torch.float32)
+        for g, o in zip(ts, outs):
+            if g.shape != o.shape:
+                raise ValueError(f"{what}: an output of shape {list(o.shape)} for a gradient of {list(g.shape)}")
+        if outs[0].device != ts[0].device:
+            raise RuntimeError(f"{what}: gradients and outputs are on different devices")
+        where = [o.data_ptr() for o in outs if o.numel()]
+        if len(set(where)) != len(where):
+            raise ValueError(f"{what}: one tensor is named twice")
+        src, dst, back = list(ts), list(outs), []
+        for i, (g, o) in enumerate(zip(ts, outs)):
+            if g.is_contiguous() and o.is_contiguous():
+                continue
+            if g.stride() == o.stride() and _dense(g):  # the same order of elements in both
+                continue
+            src[i] = g.contiguous()
+            if not o.is_contiguous():
+                dst[i] = torch.empty(o.shape, device=o.device, dtype=o.dtype)
+                back.append(i)
+        with _on(ts[0]):
+            norm = _call(src, dst, max_norm, eps)
+        for i in back:
+            outs[i].copy_(dst[i])
+        return norm

@@ -1,0 +1,179 @@
+// Global gradient norm over many tensors, and clipping:
+//   norm = sqrt(sum over all elements of g^2),
+//   out  = g * min(1, max_norm / (norm + eps)).
+//
+// Memory bound: the gradients are read once for the norm and once more for the
+// scaling, which writes the output; a sum below the L2's size finds its second
+// read there, so the scaling walks the chunks backwards.  The tensors' addresses travel
+// as a kernel parameter (no copy, no host wait); each launch takes up to
+// GRAD_MAX_TENSORS of them.  A CTA strides over chunks of GRAD_CHUNK elements,
+// finding a chunk's tensor by a binary search of the chunk prefix.  Squares
+// are summed in fp32 over at most GRAD_CHUNK / GRAD_THREADS elements of a thread
+// and in fp64 from there on, in an order that depends on the sizes alone.
+#pragma once
+
+#include "ssm_common.cuh"
+
+namespace kda {
+
+constexpr int GRAD_THREADS = 256;
+constexpr int GRAD_CHUNK = 8192;
+constexpr int GRAD_MAX_TENSORS = 1024;  // 30 KB of kernel parameters
+constexpr int GRAD_FEW_TENSORS = 64;    // the smaller table: 2 KB
+
+template <int M>
+struct GradTable {
+  const void* in[M];
+  void* out[M];
+  long long numel[M];
+  int chunk0[M + 1];  // chunks before tensor i
+  unsigned char tin[M], tout[M];  // 0 fp32, 1 bf16, 2 fp16
+  int n;
+};
+
+template <int M>
+__device__ __forceinline__ int grad_find(const GradTable<M>& tab, int chunk) {
+  int lo = 0, hi = tab.n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (tab.chunk0[mid] <= chunk) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+// 16-byte vectors of T per thread and step when the address allows, else elements.
+template <typename T>
+__device__ __forceinline__ float grad_sumsq(const T* p, int n) {
+  constexpr int V = 16 / sizeof(T);
+  float acc = 0.f;
+  if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const int nv = n / V;
+    int i = threadIdx.x;
+    for (; i + 3 * GRAD_THREADS < nv; i += 4 * GRAD_THREADS) {
+      float f[4][V];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) io_load<T, V>(p + (long long)(i + u * GRAD_THREADS) * V, f[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc = fmaf(f[u][k], f[u][k], acc);
+    }
+    for (; i < nv; i += GRAD_THREADS) {
+      float f[V];
+      io_load<T, V>(p + (long long)i * V, f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc = fmaf(f[k], f[k], acc);
+    }
+    for (int k = nv * V + threadIdx.x; k < n; k += GRAD_THREADS) {
+      const float v = io_to_f(p[k]);
+      acc = fmaf(v, v, acc);
+    }
+  } else {
+    for (int k = threadIdx.x; k < n; k += GRAD_THREADS) {
+      const float v = io_to_f(p[k]);
+      acc = fmaf(v, v, acc);
+    }
+  }
+  return acc;
+}
+
+// Sum over the CTA in a fixed order; valid in thread 0.
+__device__ __forceinline__ double grad_block_sum(double v) {
+  __shared__ double red[GRAD_THREADS / 32];
+#pragma unroll
+  for (int m = 16; m >= 1; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  double t = 0;
+  if (threadIdx.x == 0)
+    for (int i = 0; i < GRAD_THREADS / 32; ++i) t += red[i];
+  __syncthreads();
+  return t;
+}
+
+template <int M>
+__global__ void __launch_bounds__(GRAD_THREADS) grad_norm_kernel(const __grid_constant__ GradTable<M> tab,
+                                                                 double* partial) {
+  const int chunks = tab.chunk0[tab.n];
+  double acc = 0;
+  for (int ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
+    const int i = grad_find(tab, ch);
+    const long long at = (long long)(ch - tab.chunk0[i]) * GRAD_CHUNK;
+    const int n = (int)min((long long)GRAD_CHUNK, tab.numel[i] - at);
+    float s;
+    if (tab.tin[i] == 0) s = grad_sumsq(static_cast<const float*>(tab.in[i]) + at, n);
+    else if (tab.tin[i] == 1) s = grad_sumsq(static_cast<const bf16*>(tab.in[i]) + at, n);
+    else s = grad_sumsq(static_cast<const f16*>(tab.in[i]) + at, n);
+    acc += s;
+  }
+  acc = grad_block_sum(acc);
+  if (threadIdx.x == 0) partial[blockIdx.x] = acc;
+}
+
+template <typename TI, typename TO>
+__device__ __forceinline__ void grad_scale(const TI* p, TO* q, int n, float coef) {
+  constexpr int V = 16 / sizeof(TI);
+  if (((reinterpret_cast<uintptr_t>(p) & 15) | (reinterpret_cast<uintptr_t>(q) & (V * sizeof(TO) - 1))) == 0) {
+    const int nv = n / V;
+    for (int i = threadIdx.x; i < nv; i += GRAD_THREADS) {
+      float f[V];
+      io_load<TI, V>(p + (long long)i * V, f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) f[k] *= coef;
+      io_store<TO, V>(q + (long long)i * V, f);
+    }
+    for (int k = nv * V + threadIdx.x; k < n; k += GRAD_THREADS) q[k] = io_from_f<TO>(io_to_f(p[k]) * coef);
+  } else {
+    for (int k = threadIdx.x; k < n; k += GRAD_THREADS) q[k] = io_from_f<TO>(io_to_f(p[k]) * coef);
+  }
+}
+
+template <typename TI>
+__device__ __forceinline__ void grad_scale_to(const TI* p, void* q, long long at, int n, float coef, int tout) {
+  if (tout == 0) grad_scale(p, static_cast<float*>(q) + at, n, coef);
+  else if (tout == 1) grad_scale(p, static_cast<bf16*>(q) + at, n, coef);
+  else grad_scale(p, static_cast<f16*>(q) + at, n, coef);
+}
+
+// Every CTA sums the same `parts` partials in the same order.
+__device__ __forceinline__ double grad_total(const double* partial, int parts) {
+  double v = 0;
+  for (int i = threadIdx.x; i < parts; i += GRAD_THREADS) v += partial[i];
+  return grad_block_sum(v);
+}
+
+// norm = sqrt(sum of partials), alone.
+__global__ void __launch_bounds__(GRAD_THREADS) grad_norm_finish_kernel(const double* partial, int parts, float* norm) {
+  const double t = grad_total(partial, parts);
+  if (threadIdx.x == 0) *norm = (float)sqrt(t);
+}
+
+template <int M>
+__global__ void __launch_bounds__(GRAD_THREADS) grad_scale_kernel(const __grid_constant__ GradTable<M> tab,
+                                                                  const double* partial, int parts, float max_norm,
+                                                                  float eps, float* norm) {
+  __shared__ float s_coef;
+  const double t = grad_total(partial, parts);
+  if (threadIdx.x == 0) {
+    const float nrm = (float)sqrt(t);
+    const float c = max_norm / (nrm + eps);
+    s_coef = c > 1.f ? 1.f : c;  // a NaN norm stays NaN
+    if (blockIdx.x == 0 && norm) *norm = nrm;
+  }
+  __syncthreads();
+  const float coef = s_coef;
+  const int chunks = tab.chunk0[tab.n];
+  for (int ch = chunks - 1 - (int)blockIdx.x; ch >= 0; ch -= gridDim.x) {
+    const int i = grad_find(tab, ch);
+    if (coef == 1.f && tab.in[i] == tab.out[i]) continue;  // a product by one, in place
+    const long long at = (long long)(ch - tab.chunk0[i]) * GRAD_CHUNK;
+    const int n = (int)min((long long)GRAD_CHUNK, tab.numel[i] - at);
+    if (tab.tin[i] == 0) grad_scale_to(static_cast<const float*>(tab.in[i]) + at, tab.out[i], at, n, coef, tab.tout[i]);
+    else if (tab.tin[i] == 1)
+      grad_scale_to(static_cast<const bf16*>(tab.in[i]) + at, tab.out[i], at, n, coef, tab.tout[i]);
+    else
+      grad_scale_to(static_cast<const f16*>(tab.in[i]) + at, tab.out[i], at, n, coef, tab.tout[i]);
+  }
+}
+
+}  // namespace kda

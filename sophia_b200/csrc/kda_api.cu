@@ -20,34 +20,13 @@
 #include "kda_gated_norm.cuh"
 #include "kda_f32.cuh"
 #include "kda_pack.cuh"
+#include "kda_host.h"
 
 using namespace kda;
 
 namespace {
 
-thread_local std::string g_last_error;
-
-int fail(int code, const std::string& msg) {
-  g_last_error = msg;
-  return code;
-}
-
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-
 int64_t max_chunks(int64_t tokens, int N) { return tokens / C + N; }
-
-// Sub-buffer carving of a caller buffer.
-struct Carver {
-  char* base;
-  size_t off = 0;
-  explicit Carver(void* p) : base(static_cast<char*>(p)) {}
-  template <typename T>
-  T* take(size_t bytes) {
-    T* p = base ? reinterpret_cast<T*>(base + off) : nullptr;
-    off += align256(bytes);
-    return p;
-  }
-};
 
 struct SavedView {
   bf16 *W, *U, *Qt, *Kb, *E, *M, *hs;
@@ -129,8 +108,6 @@ BwdView carve_bwd(Carver& cv, int64_t TT, int H, int64_t mc) {
   return b;
 }
 
-bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
-
 struct Problem {
   int B, T, H, N;
   bool packed, conv;
@@ -180,55 +157,6 @@ int check_common(const void* q, const void* k, const void* v, const void* g, con
   return KDA_OK;
 }
 
-// ---- optional per-launch device timing (CUDA events on the launch stream)
-enum KernelId {
-  K_TABLE = 0, K_FWD_INTRA, K_FWD_STATE, K_BWD_STATE, K_BWD_INTRA, K_BWD_POST, K_REDUCE, K_RECURRENT,
-  K_GNORM_FWD, K_GNORM_BWD, K_F32_PREP, K_F32_FWD, K_F32_BWD, K_F32_DC, K_F32_CONV, K_DOC_BOUNDS, K_COUNT
-};
-const char* const kKernelNames[K_COUNT] = {"chunk_table", "fwd_intra", "fwd_state",       "bwd_state",
-                                           "bwd_intra",   "bwd_post",  "reduce",          "recurrent",
-                                           "gated_norm_fwd", "gated_norm_bwd", "f32_prep", "f32_fwd",
-                                           "f32_bwd",     "f32_dc",    "f32_conv_bwd",    "doc_bounds"};
-
-struct Timing {
-  std::mutex mu;
-  bool on = false;
-  std::vector<cudaEvent_t> pool;  // pairs (start, stop)
-  std::vector<int> ids;           // kernel id of each recorded pair
-  size_t used = 0;
-};
-Timing g_timing;
-
-struct TimedLaunch {
-  cudaEvent_t stop = nullptr;
-  cudaStream_t st;
-  TimedLaunch(int id, cudaStream_t s) : st(s) {
-    if (!g_timing.on) return;
-    std::lock_guard<std::mutex> lk(g_timing.mu);
-    if (g_timing.used + 2 > g_timing.pool.size()) {
-      for (int i = 0; i < 64; ++i) {
-        cudaEvent_t e;
-        if (cudaEventCreate(&e) != cudaSuccess) return;
-        g_timing.pool.push_back(e);
-      }
-    }
-    cudaEvent_t start = g_timing.pool[g_timing.used];
-    stop = g_timing.pool[g_timing.used + 1];
-    g_timing.used += 2;
-    g_timing.ids.push_back(id);
-    cudaEventRecord(start, st);
-  }
-  ~TimedLaunch() {
-    if (stop) cudaEventRecord(stop, st);
-  }
-};
-
-int launch_check(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
-  return KDA_OK;
-}
-
 // Poll limit of the forward chunk kernel's wait for its prefetched inputs
 // (kda_b200_debug_set_input_wait_polls lowers it in tests).
 constexpr uint32_t kDefaultWaitPolls = 1u << 26;
@@ -236,18 +164,6 @@ std::atomic<uint32_t> g_input_wait_polls{kDefaultWaitPolls};
 // The forward state pass's test hook (kda_b200_debug_set_state_wait).
 std::atomic<uint32_t> g_state_wait_polls{kDefaultWaitPolls};
 std::atomic<int> g_state_withhold_loads{0};
-
-// SMs of the current device (queried once per device).
-int sm_count() {
-  static std::atomic<int> counts[64];  // zero-initialised (static storage); concurrent first calls store the same value
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  int n = counts[dev].load(std::memory_order_relaxed);
-  if (n > 0) return n;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) n = 148;
-  counts[dev].store(n, std::memory_order_relaxed);
-  return n;
-}
 
 // cuTensorMapEncodeTiled from the driver, looked up once through the runtime
 // (no link-time dependency on libcuda).
@@ -429,6 +345,12 @@ int gn_check(long long rows, int D_, const void* a, const void* b, const float* 
   return KDA_OK;
 }
 }  // namespace
+
+int* kda::device_error_flag() {
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_kda_device_error) != cudaSuccess) return nullptr;
+  return static_cast<int*>(p);
+}
 
 extern "C" {
 

@@ -1,0 +1,154 @@
+// Shared device helpers of the state-space operators (short_conv,
+// selective_scan and their single-token steps).
+//
+// Activations are fp32, bf16 or fp16 rows [B, T, width] whose last dimension is
+// contiguous; batch and token strides are free (a slice of a wider projection
+// is read in place).  Arithmetic, states and sums are fp32; a value is rounded
+// to the activations' type once, when it is stored.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "kda_common.cuh"
+
+namespace kda {
+
+typedef __half f16;
+
+__device__ __forceinline__ float io_to_f(float v) { return v; }
+__device__ __forceinline__ float io_to_f(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float io_to_f(f16 v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T io_from_f(float v);
+template <> __device__ __forceinline__ float io_from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 io_from_f<bf16>(float v) { return __float2bfloat16(v); }
+template <> __device__ __forceinline__ f16 io_from_f<f16>(float v) { return __float2half(v); }
+
+// V consecutive elements as one load or store of V * sizeof(T) bytes (the
+// address is a multiple of that).
+template <typename T, int V> struct alignas(sizeof(T) * V) IoVec { T v[V]; };
+template <typename T, int V>
+__device__ __forceinline__ void io_load(const T* p, float (&f)[V]) {
+  const IoVec<T, V> r = *reinterpret_cast<const IoVec<T, V>*>(p);
+#pragma unroll
+  for (int i = 0; i < V; ++i) f[i] = io_to_f(r.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ void io_store(T* p, const float (&f)[V]) {
+  IoVec<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.v[i] = io_from_f<T>(f[i]);
+  *reinterpret_cast<IoVec<T, V>*>(p) = r;
+}
+
+// A strided activation: element (b, t, c) at p + b*sb + t*st + c.
+struct RowView {
+  const void* p;
+  long long sb, st;
+};
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const RowView& r, long long b, long long t) {
+  return static_cast<const T*>(r.p) + b * r.sb + t * r.st;
+}
+
+// Where sequences start and end.  Without the maps row b is one sequence of T
+// tokens; with them (packed, one row) start[t] / end[t] is the sequence whose
+// first / last token is t, or -1.
+struct SeqMap {
+  const int *start, *end;
+  int T;
+};
+__device__ __forceinline__ int seq_start_at(const SeqMap& m, int b, int t) {
+  return m.start ? __ldg(m.start + t) : (t == 0 ? b : -1);
+}
+__device__ __forceinline__ int seq_end_at(const SeqMap& m, int b, int t) {
+  return m.end ? __ldg(m.end + t) : (t == m.T - 1 ? b : -1);
+}
+
+// softplus(x) = max(x, 0) + log(1 + e), e = e^-|x|, with log(1 + e) = 2 atanh(s),
+// s = e / (2 + e) in [0, 1/3]: atanh(s) / s is a polynomial in s^2 (a Chebyshev
+// fit, relative error 8e-9), so the result keeps fp32 relative accuracy where e
+// is tiny and 1 + e would lose it.
+__device__ __forceinline__ float softplusf_(float x) {
+  const float e = ex2(-fabsf(x) * LOG2E), s = e * rcp(2.f + e), v = s * s;
+  float q = fmaf(0.140807271f, v, 0.139821723f);
+  q = fmaf(q, v, 0.20012325f);
+  q = fmaf(q, v, 0.333331615f);
+  q = fmaf(q, v, 1.f);
+  return fmaf(2.f * s, q, fmaxf(x, 0.f));
+}
+// silu(v) and its derivative p (1 + v (1 - p)), p = logistic(v)
+__device__ __forceinline__ float siluf_(float v) { return v * sigmoidf_(v); }
+__device__ __forceinline__ float silu_slopef_(float v) {
+  const float p = sigmoidf_(v);
+  return p * fmaf(v, 1.f - p, 1.f);
+}
+
+constexpr int SEQ_MAP_THREADS = 256;
+
+struct SeqMapParams {
+  const int* cu;  // [nseq + 1]
+  int nseq, T;
+  int *start, *end;
+  const float* src;  // per-sequence rows that an empty sequence hands through (null = zeros)
+  float* dst;        // null = nothing to hand through
+  long long per;     // elements of a row
+  int* err;
+};
+
+// Packed sequences: the maps of first and last tokens, by a binary search of
+// every token in cu_seqlens (the last sequence that starts at or before it; an
+// empty sequence holds no token), and the states of empty sequences.  A table
+// that does not start at 0, decreases or does not end at T sets the device
+// error 3; the maps still hold only valid sequence numbers.
+__global__ void __launch_bounds__(SEQ_MAP_THREADS) ssm_seq_map_kernel(SeqMapParams P) {
+  const int tok_blocks = (P.T + SEQ_MAP_THREADS - 1) / SEQ_MAP_THREADS;
+  if ((int)blockIdx.x < tok_blocks) {
+    const int t = blockIdx.x * SEQ_MAP_THREADS + threadIdx.x;
+    if (t >= P.T) return;
+    int lo = 0, hi = P.nseq;  // the answer is in [lo, hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(P.cu + mid) <= t) lo = mid; else hi = mid;
+    }
+    P.start[t] = __ldg(P.cu + lo) == t ? lo : -1;
+    P.end[t] = __ldg(P.cu + lo + 1) == t + 1 ? lo : -1;
+    return;
+  }
+  const int first = (int)blockIdx.x - tok_blocks, step = (int)gridDim.x - tok_blocks;
+  for (int i = first; i < P.nseq; i += step) {
+    const int a = __ldg(P.cu + i), b = __ldg(P.cu + i + 1);
+    if (threadIdx.x == 0 && (a > b || (i == 0 && a != 0) || (i == P.nseq - 1 && b != P.T))) atomicExch(P.err, 3);
+    if (P.dst && a >= b)
+      for (long long k = threadIdx.x; k < P.per; k += SEQ_MAP_THREADS)
+        P.dst[i * P.per + k] = P.src ? P.src[i * P.per + k] : 0.f;
+  }
+}
+
+// Sums `parts` rows of `cols` = q * w1 columns, w1 = w0 + 1 or w0 + 2: 8 strided slices
+// of the rows in order, then the slices in order -- a fixed order for a given
+// number of rows.  Columns r < w0 of item q go to out0[q * w0 + r], the next to
+// out1[q], the one after it to out2[q] (null: dropped).
+constexpr int SSM_REDUCE_COLS = 32, SSM_REDUCE_SLICES = 8;
+__global__ void __launch_bounds__(SSM_REDUCE_COLS * SSM_REDUCE_SLICES)
+    ssm_reduce_kernel(const float* partial, long long parts, long long cols, int w0, int w1, float* out0, float* out1,
+                      float* out2) {
+  __shared__ float part[SSM_REDUCE_SLICES][SSM_REDUCE_COLS];
+  const int c = threadIdx.x % SSM_REDUCE_COLS, sl = threadIdx.x / SSM_REDUCE_COLS;
+  const long long k = (long long)blockIdx.x * SSM_REDUCE_COLS + c;
+  float acc = 0.f;
+  if (k < cols)
+    for (long long b = sl; b < parts; b += SSM_REDUCE_SLICES) acc += partial[b * cols + k];
+  part[sl][c] = acc;
+  __syncthreads();
+  if (sl != 0 || k >= cols) return;
+  float t = 0.f;
+#pragma unroll
+  for (int i = 0; i < SSM_REDUCE_SLICES; ++i) t += part[i][c];
+  const long long q = k / w1;
+  const int r = (int)(k - q * w1);
+  if (r < w0) out0[q * w0 + r] = t;
+  else if (r == w0 && out1) out1[q] = t;
+  else if (r > w0 && out2) out2[q] = t;
+}
+
+}  // namespace kda
