@@ -11,7 +11,7 @@
 #include "grad_clip.cuh"
 #include "kda_host.h"
 #include "ssm_conv.cuh"
-#include "ssm_scan.cuh"
+#include "ssm_scan_launch.cuh"
 
 using namespace kda;
 
@@ -159,28 +159,6 @@ int conv_step(const ConvStepParams& p, cudaStream_t st) {
 
 constexpr int SCAN_MAX_N = 64;
 
-// Lanes along time.  8 lanes (64-token tiles, 64 channels per CTA) scan in three
-// shuffle steps and write a quarter of the dB / dC partial sums; 32 lanes
-// (256-token tiles, 16 channels) make four times the CTAs where rows are few.
-int scan_lt(long long B, int E, int N, int G) {
-  if (N > 16) return 8;
-  const long long ctas = B * G * ((E / G + 63) / 64);
-  return ctas >= sm_count() ? 8 : 32;
-}
-
-struct ScanShape {
-  int lt, tl, cpb, tiles, blocks;
-};
-ScanShape scan_shape(long long B, long long T, int E, int N, int G) {
-  ScanShape s;
-  s.lt = scan_lt(B, E, N, G);
-  s.tl = s.lt * SCAN_K;
-  s.cpb = SCAN_WARPS * (32 / s.lt) * 2;
-  s.tiles = (int)((T + s.tl - 1) / s.tl);
-  s.blocks = (E / G + s.cpb - 1) / s.cpb;
-  return s;
-}
-
 int check_scan(const kda_b200_scan_args* a, bool step) {
   int rc;
   if (!a) return fail(KDA_ERR_INVALID, "null arguments");
@@ -202,7 +180,7 @@ int check_scan(const kda_b200_scan_args* a, bool step) {
   return KDA_OK;
 }
 
-ScanParams scan_params(const kda_b200_scan_args* a, const ScanShape& sh) {
+ScanParams scan_params(const kda_b200_scan_args* a) {
   ScanParams p{};
   p.x = {a->x, a->x_sb, a->x_st};
   p.dt = {a->dt, a->dt_sb, a->dt_st};
@@ -211,71 +189,15 @@ ScanParams scan_params(const kda_b200_scan_args* a, const ScanShape& sh) {
   p.Cm = a->C_; p.c_sb = a->C_sb; p.c_st = a->C_st; p.c_sg = a->C_sg;
   p.A = a->A; p.D = a->D; p.dt_bias = a->dt_bias; p.h0 = a->h0;
   p.B = (int)a->B; p.T = (int)a->T; p.E = a->E; p.N = a->N; p.G = a->G;
-  p.tiles = sh.tiles; p.blocks = sh.blocks;
   p.softplus = a->softplus != 0;
   const size_t esz = io_size(a->dtype);
   const int V = (int)(16 / esz);
   p.vec = a->E % V == 0 && (a->G == 1 || (a->E / a->G) % V == 0) &&
           vec_rows(a->x, a->x_sb, a->x_st, a->B, a->T, V, esz) && vec_rows(a->dt, a->dt_sb, a->dt_st, a->B, a->T, V, esz) &&
           (!a->z || vec_rows(a->z, a->z_sb, a->z_st, a->B, a->T, V, esz));
+  p.vec_bc = a->N % V == 0 && vec_rows(a->B_, a->B_sb, a->B_st, a->B, a->T, V, esz) &&
+             vec_rows(a->C_, a->C_sb, a->C_st, a->B, a->T, V, esz) && (a->G == 1 || (a->B_sg % V == 0 && a->C_sg % V == 0));
   return p;
-}
-
-int pow2_at_least(int n) {
-  int p = 1;
-  while (p < n) p <<= 1;
-  return p;
-}
-
-template <typename T, int LT, bool PACKED>
-int launch_scan_fwd(const ScanParams& p, cudaStream_t st) {
-  const int smem = scan_smem_bytes<T, LT>(p.N, p.z.p ? 3 : 2, false);
-  auto kernel = ssm_scan_fwd_kernel<T, LT, PACKED>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan forward smem: ") + cudaGetErrorString(e));
-  {
-    TimedLaunch tl(K_SCAN_FWD, st);
-    kernel<<<dim3(p.G * p.blocks, p.B), SCAN_THREADS, smem, st>>>(p, pow2_at_least(p.N));
-  }
-  return launch_check("scan forward");
-}
-
-template <typename T>
-int scan_fwd(const ScanParams& p, const ScanShape& sh, cudaStream_t st) {
-  const bool packed = p.seq.start != nullptr;
-  if (sh.lt == 8) return packed ? launch_scan_fwd<T, 8, true>(p, st) : launch_scan_fwd<T, 8, false>(p, st);
-  return packed ? launch_scan_fwd<T, 32, true>(p, st) : launch_scan_fwd<T, 32, false>(p, st);
-}
-
-template <typename T, int LT, bool PACKED>
-int launch_scan_bwd(const ScanParams& p, const ScanShape& sh, float* dA, float* dD, float* ddt_bias, void* dB, void* dC,
-                    cudaStream_t st) {
-  const int smem = scan_smem_bytes<T, LT>(p.N, p.z.p ? 4 : 3, true);
-  auto kernel = ssm_scan_bwd_kernel<T, LT, PACKED>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan backward smem: ") + cudaGetErrorString(e));
-  const long long cols = (long long)p.E * (p.N + 2);
-  const int per = 2 * p.N * sh.tl;
-  {
-    TimedLaunch tl(K_SCAN_BWD, st);
-    kernel<<<dim3(p.G * p.blocks, p.B), SCAN_THREADS, smem, st>>>(p, pow2_at_least(p.N));
-    ssm_scan_bc_kernel<T, LT><<<dim3((unsigned)((long long)p.B * p.tiles * p.G), (per + SCAN_BC_THREADS - 1) / SCAN_BC_THREADS),
-                                SCAN_BC_THREADS, 0, st>>>(p.bc_part, p.T, p.tiles, p.G, p.blocks, p.N,
-                                                          static_cast<T*>(dB), static_cast<T*>(dC));
-    ssm_reduce_kernel<<<(unsigned)((cols + SSM_REDUCE_COLS - 1) / SSM_REDUCE_COLS), SSM_REDUCE_COLS * SSM_REDUCE_SLICES,
-                        0, st>>>(p.e_part, p.B, cols, p.N, p.N + 2, dA, dD, ddt_bias);
-  }
-  return launch_check("scan backward");
-}
-
-template <typename T>
-int scan_bwd(const ScanParams& p, const ScanShape& sh, const kda_b200_scan_args* a, cudaStream_t st) {
-  const bool packed = p.seq.start != nullptr;
-  if (sh.lt == 8)
-    return packed ? launch_scan_bwd<T, 8, true>(p, sh, a->dA, a->dD, a->ddt_bias, a->dB, a->dC, st)
-                  : launch_scan_bwd<T, 8, false>(p, sh, a->dA, a->dD, a->ddt_bias, a->dB, a->dC, st);
-  return packed ? launch_scan_bwd<T, 32, true>(p, sh, a->dA, a->dD, a->ddt_bias, a->dB, a->dC, st)
-                : launch_scan_bwd<T, 32, false>(p, sh, a->dA, a->dD, a->ddt_bias, a->dB, a->dC, st);
 }
 
 template <typename T, int LP>
@@ -442,16 +364,14 @@ int kda_b200_short_conv_step(const void* x, int64_t x_sr, const float* w, const 
 
 size_t kda_b200_scan_saved_bytes(int64_t B, int64_t T, int E, int N, int G) {
   if (B < 1 || T < 0 || E < 1 || N < 1 || N > SCAN_MAX_N || G < 1 || E % G) return 0;
-  const ScanShape s = scan_shape(B, T, E, N, G);
-  return std::max<size_t>(16, (size_t)B * s.tiles * G * s.blocks * N * s.cpb * 4);
+  return std::max<size_t>(16, (size_t)B * ((T + SCAN_SEG - 1) / SCAN_SEG) * E * N * 4);
 }
 
 size_t kda_b200_scan_workspace_bytes(int64_t B, int64_t T, int E, int N, int G, int packed, int backward) {
   if (B < 1 || T < 0 || E < 1 || N < 1 || N > SCAN_MAX_N || G < 1 || E % G) return 0;
   size_t b = map_bytes(T, packed != 0);
   if (backward) {
-    const ScanShape s = scan_shape(B, T, E, N, G);
-    b += align256((size_t)B * s.tiles * G * s.blocks * 2 * N * s.tl * 4) + align256((size_t)B * E * (N + 2) * 4);
+    b += align256((size_t)scan_part_floats(B, T, E, N, G) * 4) + align256((size_t)B * E * (N + 2) * 4);
   }
   return std::max<size_t>(b, 16);
 }
@@ -467,15 +387,14 @@ int kda_b200_selective_scan_fwd(const kda_b200_scan_args* a, void* workspace, si
     return fail(KDA_ERR_INVALID, "workspace too small: kda_b200_scan_workspace_bytes() bytes are needed");
   if (a->saved && (!aligned(a->saved, 16) || a->saved_bytes < kda_b200_scan_saved_bytes(a->B, a->T, a->E, a->N, a->G)))
     return fail(KDA_ERR_INVALID, "saved buffer too small: kda_b200_scan_saved_bytes() bytes are needed");
-  const ScanShape sh = scan_shape(a->B, a->T, a->E, a->N, a->G);
-  ScanParams p = scan_params(a, sh);
+  ScanParams p = scan_params(a);
   p.y = a->y;
   p.ht = a->ht;
   p.ckpt = static_cast<float*>(a->saved);
   p.vec = p.vec && aligned(a->y, 16);
   Carver cv(workspace);
   if ((rc = build_map(p.seq, cv, a->cu_seqlens, p.T, a->nseq, a->h0, a->ht, (long long)a->E * a->N, st))) return rc;
-  return SSM_DISPATCH(a->dtype, scan_fwd, p, sh, st);
+  return SSM_DISPATCH(a->dtype, scan_fwd, p, st);
 }
 
 int kda_b200_selective_scan_bwd(const kda_b200_scan_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -496,8 +415,7 @@ int kda_b200_selective_scan_bwd(const kda_b200_scan_args* a, void* workspace, si
   if (!workspace || !aligned(workspace, 16) ||
       workspace_bytes < kda_b200_scan_workspace_bytes(a->B, a->T, a->E, a->N, a->G, a->cu_seqlens != nullptr, 1))
     return fail(KDA_ERR_INVALID, "workspace too small: kda_b200_scan_workspace_bytes() bytes are needed");
-  const ScanShape sh = scan_shape(a->B, a->T, a->E, a->N, a->G);
-  ScanParams p = scan_params(a, sh);
+  ScanParams p = scan_params(a);
   p.dy = {a->dy, a->dy_sb, a->dy_st};
   p.ckpt = static_cast<float*>(a->saved);
   p.dht = a->dht; p.dh0 = a->dh0;
@@ -507,9 +425,10 @@ int kda_b200_selective_scan_bwd(const kda_b200_scan_args* a, void* workspace, si
           aligned(a->ddt, 16) && (!a->z || aligned(a->dz, 16));
   Carver cv(workspace);
   if ((rc = build_map(p.seq, cv, a->cu_seqlens, p.T, a->nseq, a->dht, a->dh0, (long long)a->E * a->N, st))) return rc;
-  p.bc_part = cv.take<float>((size_t)p.B * sh.tiles * p.G * sh.blocks * 2 * p.N * sh.tl * 4);
+  p.bc_part = cv.take<float>((size_t)scan_part_floats(p.B, p.T, p.E, p.N, p.G) * 4);
   p.e_part = cv.take<float>((size_t)p.B * p.E * (p.N + 2) * 4);
-  return SSM_DISPATCH(a->dtype, scan_bwd, p, sh, a, st);
+  const ScanGrads g{a->dA, a->dD, a->ddt_bias, a->dB, a->dC};
+  return SSM_DISPATCH(a->dtype, scan_bwd, p, g, st);
 }
 
 int kda_b200_selective_scan_step(const kda_b200_scan_args* a, void* stream) {

@@ -83,6 +83,17 @@ __device__ __forceinline__ float silu_slopef_(float v) {
   return p * fmaf(v, 1.f - p, 1.f);
 }
 
+// The pool entry of a single-token call's row: negative for a padding row; an entry past the pool is
+// reported (device error 11) and treated as one.
+__device__ __forceinline__ int step_slot(const int* slots, int r, int pool, int* err) {
+  const int s = slots ? __ldg(slots + r) : r;
+  if (s >= pool) {
+    atomicExch(err, 11);
+    return -1;
+  }
+  return s;
+}
+
 constexpr int SEQ_MAP_THREADS = 256;
 
 struct SeqMapParams {
@@ -100,7 +111,7 @@ struct SeqMapParams {
 // empty sequence holds no token), and the states of empty sequences.  A table
 // that does not start at 0, decreases or does not end at T sets the device
 // error 3; the maps still hold only valid sequence numbers.
-__global__ void __launch_bounds__(SEQ_MAP_THREADS) ssm_seq_map_kernel(SeqMapParams P) {
+static __global__ void __launch_bounds__(SEQ_MAP_THREADS) ssm_seq_map_kernel(SeqMapParams P) {
   const int tok_blocks = (P.T + SEQ_MAP_THREADS - 1) / SEQ_MAP_THREADS;
   if ((int)blockIdx.x < tok_blocks) {
     const int t = blockIdx.x * SEQ_MAP_THREADS + threadIdx.x;
@@ -129,7 +140,7 @@ __global__ void __launch_bounds__(SEQ_MAP_THREADS) ssm_seq_map_kernel(SeqMapPara
 // number of rows.  Columns r < w0 of item q go to out0[q * w0 + r], the next to
 // out1[q], the one after it to out2[q] (null: dropped).
 constexpr int SSM_REDUCE_COLS = 32, SSM_REDUCE_SLICES = 8;
-__global__ void __launch_bounds__(SSM_REDUCE_COLS * SSM_REDUCE_SLICES)
+static __global__ void __launch_bounds__(SSM_REDUCE_COLS * SSM_REDUCE_SLICES)
     ssm_reduce_kernel(const float* partial, long long parts, long long cols, int w0, int w1, float* out0, float* out1,
                       float* out2) {
   __shared__ float part[SSM_REDUCE_SLICES][SSM_REDUCE_COLS];

@@ -283,15 +283,6 @@ struct ConvStepParams {
   int* err;
 };
 
-__device__ __forceinline__ int step_slot(const int* slots, int r, int pool, int* err) {
-  const int s = slots ? __ldg(slots + r) : r;
-  if (s >= pool) {
-    atomicExch(err, 11);
-    return -1;
-  }
-  return s;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(CONV_THREADS) ssm_conv_step_kernel(ConvStepParams P) {
   const int c = blockIdx.x * CONV_THREADS + threadIdx.x;

@@ -9,17 +9,23 @@
 //   dd = sum_n q A + x sum_n g B,   dx = d sum_n g B + D ds,   dA = sum_t q d,
 //   dz = dy s silu'(z),   d dt = dd softplus',   dD = sum_t ds x.
 //
-// Layout.  Time runs over lanes: a lane owns K = 8 consecutive tokens of two
-// neighbouring channels (one fp32 pair in packed arithmetic), LT lanes make
-// a tile of 8 LT tokens, 32 / LT channel pairs share a warp.  Per state, a lane
-// composes its tokens' steps to (decay, value), the LT lanes combine theirs by a
-// shuffle scan that starts from the state carried over the tiles, and a second
-// pass over the tokens gives h.  So each decay's exponential is evaluated once and
-// a tile needs no step-by-step pass; B and C rows are shared by all lanes of a
-// token; and in the backward the sums over channels in dB and dC are, in each
-// lane, sums over the channels that its warp takes, for fixed tokens.
-// Tiles of x, dt, z (and dy) are staged in shared memory, rows of one token
-// skewed by 16 bytes per 8 tokens so that lanes 8 tokens apart use other banks.
+// Layout.  Time runs in order: a channel's N states are spread over L lanes with S
+// states each (L S >= N), its recurrence stays in registers, and 32 / L channels
+// share a warp.  The decay's exponential (16 a clock and SM) is evaluated once per
+// token, channel and state.  Four warps run the recurrences of a tile of tokens while
+// four others do what depends on the token and channel alone: they fetch the tile
+// after the next (cp.async), turn the next one into d, d x and fp32 rows of B and C
+// (softplus, gates), and finish the one before (sum of the lanes' parts, skip, gate,
+// store).  The two sides exchange double buffers in shared memory, one barrier per tile.
+//
+// Backward.  Tiles from last to first, in segments of SCAN_SEG tokens: a segment's
+// states are rebuilt from the checkpoint that the forward saved at its start and kept in
+// registers with their decays, then its tokens run backwards.  dB and dC are sums
+// over channels: the lanes of one warp that hold the same states of different channels
+// exchange halves of their values (each lane orders its states by its channel, n = n0 +
+// (i xor m), so that what a lane keeps sits in the same registers everywhere), the
+// warps' sums meet in shared memory and the CTAs' in a buffer that a last kernel sums in
+// block order.  No atomics: every sum has a fixed order.
 #pragma once
 
 #include <type_traits>
@@ -28,6 +34,71 @@
 
 namespace kda {
 
+constexpr int SCAN_MAIN = 128;                // threads with recurrences
+constexpr int SCAN_WARPS = SCAN_MAIN / 32;
+constexpr int SCAN_TOKENS = 128;              // threads of the token side
+constexpr int SCAN_THREADS = SCAN_MAIN + SCAN_TOKENS;
+constexpr int SCAN_SEG = 8;      // tokens between checkpoints
+constexpr int SCAN_TT_BWD = 8;   // tokens per tile of the backward
+constexpr int SCAN_STAGES = 4;   // raw tiles in shared memory
+
+__host__ __device__ constexpr int ilog2(int v) { return v <= 1 ? 0 : 1 + ilog2(v / 2); }
+
+// Geometry of a variant: L lanes per channel, S states per lane, tiles of TT tokens.
+template <typename T, int L_, int S_, int TT_>
+struct ScanGeo {
+  static constexpr int L = L_, S = S_, TT = TT_, TOKENS = SCAN_TOKENS;
+  static constexpr int NP = L * S;               // states with padding
+  static constexpr int CH = 32 / L;              // channels per warp
+  static constexpr int CPB = SCAN_WARPS * CH;    // channels per CTA
+  static constexpr int RAW = TT * CPB;           // elements of a staged tensor
+  static constexpr int PAIRS = CPB / 2;          // channel pairs: a thread's share of a token pass
+  static constexpr int TSTEP = TOKENS / PAIRS < TT ? TOKENS / PAIRS : TT;  // tokens per pass of the side
+  static constexpr bool SPARE = TOKENS / PAIRS > TT;  // threads without a token
+  static constexpr int V = 16 / (int)sizeof(T), NV = CPB / V;  // 16-byte pieces of a row
+};
+template <typename T, int L, int S>
+using ScanFwdGeo = ScanGeo<T, L, S, sizeof(T) == 2 ? 32 : 16>;
+template <typename T, int L, int S>
+using ScanBwdGeo = ScanGeo<T, L, S, SCAN_TT_BWD>;
+
+struct ScanParams {
+  RowView x, dt, z, dy;            // [B, T, E]; z.p null = no gate
+  const void *Bm, *Cm;             // [B, T, G, N], rows of N contiguous
+  long long b_sb, b_st, b_sg, c_sb, c_st, c_sg;
+  const float *A, *D, *dt_bias;    // [E][N], [E] or null, [E] or null
+  const float* h0;                 // [nseq][E][N] or null
+  SeqMap seq;
+  int B, T, E, N, G;
+  int blocks;                      // channel blocks per group
+  bool softplus, vec, vec_bc;      // vec: x, dt, z, dy and the outputs allow 16-byte pieces; vec_bc: B and C
+  void* y;                         // [B, T, E] contiguous
+  float* ht;                       // [nseq][E][N] or null
+  float* ckpt;                     // [B][segments][E][N]: states in front of each segment; null = not kept
+  // backward
+  const float* dht;
+  void *dx, *ddt, *dz;
+  float* dh0;
+  float* bc_part;                  // [B][tiles][G][blocks][TT][2][N]
+  float* e_part;                   // [B][E][N + 2]: dA, dD, d dt_bias
+};
+
+struct ScanBlock {
+  int g, blk, c0, nc, b;  // group, block in it, first channel, channels, row
+};
+template <int CPB>
+__device__ __forceinline__ ScanBlock scan_block(const ScanParams& P) {
+  ScanBlock s;
+  const int eg = P.E / P.G;
+  s.g = blockIdx.x / P.blocks;
+  s.blk = blockIdx.x - s.g * P.blocks;
+  s.c0 = s.g * eg + s.blk * CPB;
+  s.nc = min(CPB, eg - s.blk * CPB);
+  s.b = blockIdx.y;
+  return s;
+}
+
+// A lane's S values of one kind, pairs in packed fp32 arithmetic.
 typedef unsigned long long u64;
 __device__ __forceinline__ u64 pk2(float lo, float hi) {
   u64 r;
@@ -54,690 +125,824 @@ __device__ __forceinline__ u64 add2(u64 a, u64 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ u64 ex2_2(u64 a) {
-  const float2 v = upk2(a);
-  return pk2(ex2(v.x), ex2(v.y));
+template <int S>
+struct Lane {
+  static_assert(S % 2 == 0, "pairs");
+  u64 p[S / 2];
+  __device__ __forceinline__ float get(int i) const { return i & 1 ? upk2(p[i / 2]).y : upk2(p[i / 2]).x; }
+  __device__ __forceinline__ void set(int i, float v) {
+    const float2 o = upk2(p[i / 2]);
+    p[i / 2] = i & 1 ? pk2(o.x, v) : pk2(v, o.y);
+  }
+  __device__ __forceinline__ static Lane load(const float* q) {  // S * 4 bytes, aligned
+    Lane r;
+    if (S % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < S / 4; ++k) {
+        const ulonglong2 v = reinterpret_cast<const ulonglong2*>(q)[k];
+        r.p[2 * k] = v.x;
+        r.p[2 * k + 1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < S / 2; ++k) r.p[k] = reinterpret_cast<const u64*>(q)[k];
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(float* q) const {
+    if (S % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < S / 4; ++k) reinterpret_cast<ulonglong2*>(q)[k] = make_ulonglong2(p[2 * k], p[2 * k + 1]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < S / 2; ++k) reinterpret_cast<u64*>(q)[k] = p[k];
+    }
+  }
+  __device__ __forceinline__ static Lane all(float v) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = pk2(v, v);
+    return r;
+  }
+  __device__ __forceinline__ float sum() const {
+    u64 t = p[0];
+#pragma unroll
+    for (int k = 1; k < S / 2; ++k) t = add2(t, p[k]);
+    const float2 f = upk2(t);
+    return f.x + f.y;
+  }
+  __device__ __forceinline__ Lane exp2() const {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) {
+      const float2 f = upk2(p[k]);
+      r.p[k] = pk2(ex2(f.x), ex2(f.y));
+    }
+    return r;
+  }
+  friend __device__ __forceinline__ Lane operator*(const Lane& a, const Lane& b) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = mul2(a.p[k], b.p[k]);
+    return r;
+  }
+  friend __device__ __forceinline__ Lane fma(const Lane& a, const Lane& b, const Lane& c) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = fma2(a.p[k], b.p[k], c.p[k]);
+    return r;
+  }
+};
+// The decays 2^(d a2).  ex2.approx is low by 0.5e-8 to 2.9e-8 on average where decays are close
+// to 1 (measured: 0.5e-8 for exponents of -3e-4 to -3e-3, 2.4e-8 for -0.005 to -0.08, 1.8e-8 for
+// -0.08 to -0.3), which adds up over the tokens that a state remembers.  An exponent
+// raised by 1e-8 / ln 2 takes the middle of that off, at no cost (an fma for a product); 2^0
+// stays 1.
+constexpr float SCAN_EXP_SHIFT = 1.44e-8f;
+template <int S>
+__device__ __forceinline__ Lane<S> lane_decay(const Lane<S>& a2, float d) {
+  return fma(a2, Lane<S>::all(d), Lane<S>::all(SCAN_EXP_SHIFT)).exp2();
+}
+// sum += v with the rounding errors carried along (a compensated sum: its error does not
+// grow with the number of tokens).
+__device__ __forceinline__ void sum_add(float& sum, float& err, float v) {
+  const float y = __fadd_rn(v, -err), t = __fadd_rn(sum, y);
+  err = __fadd_rn(__fadd_rn(t, -sum), -y);
+  sum = t;
 }
 
-constexpr int SCAN_K = 8;          // tokens per lane
-constexpr int SCAN_THREADS = 256;  // 8 warps
-constexpr int SCAN_WARPS = SCAN_THREADS / 32;
-
-// Geometry of a variant with LT lanes along time and elements of T.
-template <typename T, int LT>
-struct ScanGeo {
-  static constexpr int TL = LT * SCAN_K;                   // tokens per tile
-  static constexpr int CL = 32 / LT;                       // channel pairs per warp
-  static constexpr int CPB = SCAN_WARPS * CL * 2;          // channels per CTA
-  static constexpr int ROWB = CPB * (int)sizeof(T);        // bytes of a staged row
-  static constexpr int RAW = TL * ROWB + (TL / 8) * 16;    // bytes of a staged tensor
-  static constexpr int BCP = TL + 4;                       // floats per state of staged B or C
-  static __host__ __device__ int raw_off(int t, int c) { return t * ROWB + (t >> 3) * 16 + c * (int)sizeof(T); }
-  // B and C: tokens 8l .. 8l+3 of every lane l first, then 8l+4 .. 8l+7, so that a
-  // lane's two 16-byte reads are conflict-free
-  static __host__ __device__ int bc_off(int t) { return ((t >> 2) & 1) * (TL / 2) + (t >> 3) * 4 + (t & 3); }
-};
-
-struct ScanParams {
-  RowView x, dt, z, dy;            // [B, T, E]; z.p null = no gate
-  const void *Bm, *Cm;             // [B, T, G, N], rows of N contiguous
-  long long b_sb, b_st, b_sg, c_sb, c_st, c_sg;
-  const float *A, *D, *dt_bias;    // [E][N], [E] or null, [E] or null
-  const float* h0;                 // [nseq][E][N] or null
-  SeqMap seq;
-  int B, T, E, N, G;
-  int tiles, blocks;               // tiles per row, channel blocks per group
-  bool softplus, vec;              // vec: 16-byte staging is aligned for x, dt, z, dy and the outputs
-  void* y;                         // [B, T, E] contiguous
-  float* ht;                       // [nseq][E][N] or null
-  float* ckpt;                     // [B][tiles][G * blocks][N][CPB] states at the tiles' starts, or null
-  // backward
-  const float* dht;
-  void *dx, *ddt, *dz;
-  float* dh0;
-  float* bc_part;                  // [B][tiles][G][blocks][2][N][TL]
-  float* e_part;                   // [B][E][N + 2]: dA, dD, d dt_bias
-};
-
-struct ScanBlock {
-  int g, blk, c0, nc, b;  // group, block in it, first channel, channels, row
-};
-template <int CPB>
-__device__ __forceinline__ ScanBlock scan_block(const ScanParams& P) {
-  ScanBlock s;
-  const int eg = P.E / P.G;
-  s.g = blockIdx.x / P.blocks;
-  s.blk = blockIdx.x - s.g * P.blocks;
-  s.c0 = s.g * eg + s.blk * CPB;
-  s.nc = min(CPB, eg - s.blk * CPB);
-  s.b = blockIdx.y;
-  return s;
+// Zero in the states that do not exist (PAD: N < L S), whatever arithmetic made of them.
+template <bool PAD, int S>
+__device__ __forceinline__ Lane<S> lane_keep(Lane<S> v, unsigned ok) {
+  if (PAD) {
+#pragma unroll
+    for (int i = 0; i < S; ++i) v.set(i, ok >> i & 1 ? v.get(i) : 0.f);
+  }
+  return v;
 }
 
-// Stages rows t0 .. t0+TL-1 (zeros past T and past the block's channels).
-template <typename T, int LT>
-__device__ __forceinline__ void scan_stage(char* dst, const RowView& r, const ScanParams& P, const ScanBlock& s, int t0) {
-  using G = ScanGeo<T, LT>;
-  constexpr int V = 16 / (int)sizeof(T), NV = G::CPB / V;
-  if (P.vec) {
-#pragma unroll 4
-    for (int i = threadIdx.x; i < G::TL * NV; i += SCAN_THREADS) {
-      const int t = i / NV, c = (i - t * NV) * V;
-      IoVec<T, V> v;
+// The token side's fetches.  Every thread keeps where its pieces of a tile come from
+// (the aligned case: 16-byte pieces by cp.async, zeros past T and, whole pieces, past the
+// block's channels); else elements are copied one by one.  Rows of B and C likewise.
+template <typename T, typename G, int TENSORS>
+struct ScanFetch {
+  static constexpr int PIECES = G::TT * G::NV, SLOTS = (TENSORS * PIECES + G::TOKENS - 1) / G::TOKENS;
+  static constexpr int BC_SLOTS = (2 * G::TT * (G::NP < G::V ? 1 : G::NP / G::V) + G::TOKENS - 1) / G::TOKENS;
+  static constexpr int SL = SLOTS > 0 ? SLOTS : 1;
+  const T* src[SL];      // the piece in the tile to come
+  const T* safe[SL];     // an address to name where nothing is read
+  long long step[SL];    // elements to the next tile
+  int dst[SL], row[SL];  // token in the tile; far past it: zeros
+  const T* bc_src[BC_SLOTS];
+  int bc_dst[BC_SLOTS], bc_row[BC_SLOTS];
+  long long bc_step[BC_SLOTS];
+
+  // `tile` is fetched first, then its neighbour in direction `dir`, and so on.
+  __device__ __forceinline__ void init(const ScanParams& P, const ScanBlock& s, const RowView (&r)[TENSORS], int tid,
+                                       int bc_at, int npad, int tile, int dir) {
+    const long long t0 = (long long)tile * G::TT;
+    if (P.vec) {
 #pragma unroll
-      for (int k = 0; k < V; ++k) v.v[k] = io_from_f<T>(0.f);
-      if (t0 + t < P.T) {
-        const T* p = row_ptr<T>(r, s.b, t0 + t) + s.c0 + c;
-        if (c + V <= s.nc) {
-          v = *reinterpret_cast<const IoVec<T, V>*>(p);
-        } else {
+      for (int k = 0; k < SLOTS; ++k) {
+        const int i = k * G::TOKENS + tid, w = i / PIECES, j = i - w * PIECES;
+        row[k] = j / (G::NV > 0 ? G::NV : 1);
+        const int c = (j - row[k] * G::NV) * G::V;
+        src[k] = safe[k] = nullptr;
+        step[k] = 0;
+        dst[k] = w * G::RAW + row[k] * G::CPB + c;
 #pragma unroll
-          for (int k = 0; k < V; ++k)
-            if (c + k < s.nc) v.v[k] = p[k];
+        for (int q = 0; q < TENSORS; ++q)
+          if (w == q && r[q].p) {
+            safe[k] = static_cast<const T*>(r[q].p);
+            src[k] = safe[k] + s.b * r[q].sb + (t0 + row[k]) * r[q].st + s.c0 + c;
+            step[k] = dir * G::TT * r[q].st;
+          }
+        if (c >= s.nc) row[k] = 1 << 30;  // past the channels: zeros
+      }
+    }
+    if (P.vec_bc) {
+      const int nv = P.N / G::V, per = G::TT * nv;
+#pragma unroll
+      for (int k = 0; k < BC_SLOTS; ++k) {
+        const int i = k * G::TOKENS + tid, w = i / per, j = i - w * per;
+        bc_row[k] = j / nv;
+        const int n = (j - bc_row[k] * nv) * G::V;
+        bc_src[k] = nullptr;
+        if (w == 0) bc_src[k] = static_cast<const T*>(P.Bm) + s.b * P.b_sb + s.g * P.b_sg + (t0 + bc_row[k]) * P.b_st + n;
+        if (w == 1) bc_src[k] = static_cast<const T*>(P.Cm) + s.b * P.c_sb + s.g * P.c_sg + (t0 + bc_row[k]) * P.c_st + n;
+        bc_step[k] = dir * G::TT * (w ? P.c_st : P.b_st);
+        bc_dst[k] = bc_at + w * G::TT * npad + bc_row[k] * P.N + n;
+      }
+    }
+  }
+  __device__ __forceinline__ void fetch(const ScanParams& P, const ScanBlock& s, const RowView (&r)[TENSORS], T* stage, int t0,
+                                        int tid) {
+    if (P.vec) {
+#pragma unroll
+      for (int k = 0; k < SLOTS; ++k)
+        if (safe[k]) {
+          const bool in = row[k] < P.T - t0;
+          cp_async16(stage + dst[k], in ? src[k] : safe[k], in);
+          src[k] += step[k];
+        }
+    } else {
+#pragma unroll
+      for (int q = 0; q < TENSORS; ++q)
+        if (r[q].p)
+          for (int i = tid; i < G::TT * G::CPB; i += G::TOKENS) {
+            const int t = i / G::CPB, c = i - t * G::CPB;
+            stage[q * G::RAW + i] =
+                t0 + t < P.T && c < s.nc ? row_ptr<T>(r[q], s.b, t0 + t)[s.c0 + c] : io_from_f<T>(0.f);
+          }
+    }
+    if (P.vec_bc) {
+#pragma unroll
+      for (int k = 0; k < BC_SLOTS; ++k)
+        if (bc_src[k]) {
+          const bool in = bc_row[k] < P.T - t0;
+          cp_async16(stage + bc_dst[k], in ? bc_src[k] : static_cast<const T*>(P.Bm), in);
+          bc_src[k] += bc_step[k];
+        }
+    }
+    cp_async_commit();
+  }
+};
+// vec: a block's channels are whole 16-byte pieces, or end with the tensor's row
+// (E a multiple of the piece), so a piece never mixes two blocks' channels.
+
+// B and C of a tile as fp32 [TT][VERS][NP], version v holding state n0 + (i ^ v) at n0 + i of a
+// lane's S states (zeros past T and past N); from the staged rows or from global memory.
+// Reads (load) and writes (store) apart, as the compiler must assume that they alias.
+template <typename T, typename G, int VERS, bool PAD>
+struct ScanBC {
+  static constexpr int ITEMS = 2 * G::TT * G::L, SLOTS = (ITEMS + G::TOKENS - 1) / G::TOKENS;
+  float v[SLOTS][G::S];
+  __device__ __forceinline__ void load(const T* raw, int npad, const ScanParams& P, const ScanBlock& s, int t0, int tid) {
+#pragma unroll
+    for (int k = 0; k < SLOTS; ++k) {
+      const int i = k * G::TOKENS + tid;
+      if (ITEMS % G::TOKENS != 0 && i >= ITEMS) break;
+      const bool is_c = i >= G::TT * G::L;
+      const int j = is_c ? i - G::TT * G::L : i, t = j / G::L, n0 = (j - t * G::L) * G::S;
+      if (P.vec_bc && !PAD) {
+        io_load<T, G::S>(raw + (is_c ? G::TT * npad : 0) + t * P.N + n0, v[k]);
+        continue;
+      }
+#pragma unroll
+      for (int q = 0; q < G::S; ++q) {
+        v[k][q] = 0.f;
+        if (n0 + q < P.N) {
+          if (P.vec_bc) {
+            v[k][q] = io_to_f(raw[(is_c ? G::TT * npad : 0) + t * P.N + n0 + q]);
+          } else if (t0 + t < P.T) {
+            const T* p = is_c ? static_cast<const T*>(P.Cm) + s.b * P.c_sb + s.g * P.c_sg + (t0 + t) * P.c_st
+                              : static_cast<const T*>(P.Bm) + s.b * P.b_sb + s.g * P.b_sg + (t0 + t) * P.b_st;
+            v[k][q] = io_to_f(p[n0 + q]);
+          }
         }
       }
-      *reinterpret_cast<IoVec<T, V>*>(dst + G::raw_off(t, c)) = v;
-    }
-  } else {
-    for (int i = threadIdx.x; i < G::TL * G::CPB; i += SCAN_THREADS) {
-      const int t = i / G::CPB, c = i - t * G::CPB;
-      T v = io_from_f<T>(0.f);
-      if (t0 + t < P.T && c < s.nc) v = row_ptr<T>(r, s.b, t0 + t)[s.c0 + c];
-      *reinterpret_cast<T*>(dst + G::raw_off(t, c)) = v;
     }
   }
-}
-
-// Writes a staged tile to a contiguous [B, T, E] output.
-template <typename T, int LT>
-__device__ __forceinline__ void scan_unstage(const char* src, void* out, const ScanParams& P, const ScanBlock& s, int t0) {
-  using G = ScanGeo<T, LT>;
-  constexpr int V = 16 / (int)sizeof(T), NV = G::CPB / V;
-  T* base = static_cast<T*>(out) + ((long long)s.b * P.T + t0) * P.E + s.c0;
-  if (P.vec) {
-    for (int i = threadIdx.x; i < G::TL * NV; i += SCAN_THREADS) {
-      const int t = i / NV, c = (i - t * NV) * V;
-      if (t0 + t >= P.T || c >= s.nc) continue;
-      const IoVec<T, V> v = *reinterpret_cast<const IoVec<T, V>*>(src + G::raw_off(t, c));
-      T* p = base + (long long)t * P.E + c;
-      if (c + V <= s.nc) {
-        *reinterpret_cast<IoVec<T, V>*>(p) = v;
-      } else {
+  __device__ __forceinline__ void store(float* Bs, float* Cs, int tid) const {
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (c + k < s.nc) p[k] = v.v[k];
+    for (int k = 0; k < SLOTS; ++k) {
+      const int i = k * G::TOKENS + tid;
+      if (ITEMS % G::TOKENS != 0 && i >= ITEMS) break;
+      const bool is_c = i >= G::TT * G::L;
+      const int j = is_c ? i - G::TT * G::L : i, t = j / G::L, n0 = (j - t * G::L) * G::S;
+      float* dst = is_c ? Cs : Bs;
+#pragma unroll
+      for (int w = 0; w < VERS; ++w) {
+        IoVec<float, G::S> o;
+#pragma unroll
+        for (int q = 0; q < G::S; ++q) o.v[q] = v[k][q ^ w];
+        *reinterpret_cast<IoVec<float, G::S>*>(dst + (t * VERS + w) * G::NP + n0) = o;
       }
     }
-  } else {
-    for (int i = threadIdx.x; i < G::TL * G::CPB; i += SCAN_THREADS) {
-      const int t = i / G::CPB, c = i - t * G::CPB;
-      if (t0 + t < P.T && c < s.nc) base[(long long)t * P.E + c] = *reinterpret_cast<const T*>(src + G::raw_off(t, c));
-    }
   }
-}
+};
 
-// Stages B or C of a tile as fp32 [N][BCP] (zeros past T).
-template <typename T, int LT>
-__device__ __forceinline__ void scan_stage_bc(float* dst, const void* src, long long sb, long long st, long long sg,
-                                              const ScanParams& P, const ScanBlock& s, int t0, int np2) {
-  using G = ScanGeo<T, LT>;
-  const T* p = static_cast<const T*>(src) + s.b * sb + s.g * sg;
-  const int n = threadIdx.x & (np2 - 1);  // np2: the power of two at or above N
-  if (n >= P.N) return;
-  const int step = SCAN_THREADS / np2;
-#pragma unroll 4
-  for (int t = threadIdx.x / np2; t < G::TL; t += step)
-    dst[n * G::BCP + G::bc_off(t)] = t0 + t < P.T ? io_to_f(p[(long long)(t0 + t) * st + n]) : 0.f;
-}
-
+// Pair of neighbouring channels of a staged row.
 template <typename T>
-__device__ __forceinline__ u64 scan_pair(const char* p) {
-  const IoVec<T, 2> v = *reinterpret_cast<const IoVec<T, 2>*>(p);
-  return pk2(io_to_f(v.v[0]), io_to_f(v.v[1]));
+__device__ __forceinline__ float2 scan_pair(const T* p) {
+  float f[2];
+  io_load<T, 2>(p, f);
+  return make_float2(f[0], f[1]);
 }
+// Stores a pair of a row's channels c, c+1 (of nc).
 template <typename T>
-__device__ __forceinline__ void scan_put(char* p, float2 v) {
-  IoVec<T, 2> r;
-  r.v[0] = io_from_f<T>(v.x);
-  r.v[1] = io_from_f<T>(v.y);
-  *reinterpret_cast<IoVec<T, 2>*>(p) = r;
-}
-
-__device__ __forceinline__ void scan_row8(const float* base, int half, int tl, float (&v)[SCAN_K]) {
-  const float4 a = *reinterpret_cast<const float4*>(base + tl * 4);
-  const float4 b = *reinterpret_cast<const float4*>(base + half + tl * 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-
-template <int LT>
-__device__ __forceinline__ u64 scan_up(u64 v, int off) { return __shfl_up_sync(0xffffffffu, v, off, LT); }
-template <int LT>
-__device__ __forceinline__ u64 scan_down(u64 v, int off) { return __shfl_down_sync(0xffffffffu, v, off, LT); }
-
-// Inclusive scan over the LT lanes of h <- p h_before + h, p being the lane's own
-// decay.  RESET: bit k of `block` stops what comes in step k, because a sequence starts in
-// the span on this side of it (selected away, not multiplied by zero: another
-// sequence's infinities and NaN stay its own).
-template <int LT, bool RESET>
-__device__ __forceinline__ void scan_lanes(u64& h, u64 p, int tl, unsigned block) {
-#pragma unroll
-  for (int off = 1, k = 0; off < LT; off <<= 1, ++k) {
-    const u64 hn = scan_up<LT>(h, off);
-    const bool take = tl >= off && !(RESET && (block >> k & 1));
-    if (off * 2 < LT) {
-      const u64 pn = scan_up<LT>(p, off);
-      if (take) {
-        h = fma2(p, hn, h);
-        p = mul2(p, pn);
-      }
-    } else if (take) {
-      h = fma2(p, hn, h);
-    }
+__device__ __forceinline__ void scan_put_pair(void* out, const ScanParams& P, const ScanBlock& s, int t, int c, float2 v) {
+  T* p = static_cast<T*>(out) + ((long long)s.b * P.T + t) * P.E + s.c0 + c;
+  if (P.vec && c + 1 < s.nc) {
+    const float f[2] = {v.x, v.y};
+    io_store<T, 2>(p, f);
+  } else {
+    if (c < s.nc) p[0] = io_from_f<T>(v.x);
+    if (c + 1 < s.nc) p[1] = io_from_f<T>(v.y);
   }
 }
-// The same towards lower lanes.
-template <int LT, bool RESET>
-__device__ __forceinline__ void scan_lanes_rev(u64& h, u64 p, int tl, unsigned block) {
+// Sum of a channel's L partial sums.
+template <int L>
+__device__ __forceinline__ float scan_join(const float* p) {
+  constexpr int V = L < 4 ? L : 4;
+  float acc = 0.f;
 #pragma unroll
-  for (int off = 1, k = 0; off < LT; off <<= 1, ++k) {
-    const u64 hn = scan_down<LT>(h, off);
-    const bool take = tl + off < LT && !(RESET && (block >> k & 1));
-    if (off * 2 < LT) {
-      const u64 pn = scan_down<LT>(p, off);
-      if (take) {
-        h = fma2(p, hn, h);
-        p = mul2(p, pn);
-      }
-    } else if (take) {
-      h = fma2(p, hn, h);
-    }
+  for (int q = 0; q < L / V; ++q) {
+    const IoVec<float, V> v = *reinterpret_cast<const IoVec<float, V>*>(p + q * V);
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc += v.v[k];
   }
+  return acc;
 }
 
-// Where sequences start and end among a lane's tokens (bit j: token j), and which
-// steps of the two lane scans that stops.
+// d of a token, 0 past the row's end.
+__device__ __forceinline__ float scan_d(const ScanParams& P, float raw, bool inside) {
+  const float d = P.softplus ? softplusf_(raw) : raw;
+  return inside ? d : 0.f;
+}
+
+// First and last tokens of sequences: thread tid < TT looks after token tid of the tiles, a
+// tile ahead of the place in shared memory ([TT] first, [TT] last) that it goes to.
+template <int TT>
 struct ScanFlags {
-  unsigned first, last, up, down;
-  bool any_first, any_last;  // anywhere in the tile
+  int f, l;
+  __device__ __forceinline__ void read(const ScanParams& P, int b, int t0, int tid) {
+    const int t = t0 + tid;
+    const bool in = tid < TT && t >= 0 && t < P.T;
+    f = in ? seq_start_at(P.seq, b, t) : -1;
+    l = in ? seq_end_at(P.seq, b, t) : -1;
+  }
+  __device__ __forceinline__ void write(int* flags, int tid) const {
+    if (tid < TT) {
+      flags[tid] = f;
+      flags[TT + tid] = l;
+    }
+  }
 };
-template <int LT>
-__device__ __forceinline__ ScanFlags scan_flags(const int* first, const int* last, int tl) {
-  ScanFlags f{};
+__device__ __forceinline__ bool scan_seg_flag(const int* first, const int* last) {
+  bool any = false;
 #pragma unroll
-  for (int j = 0; j < SCAN_K; ++j) {
-    f.first |= (unsigned)(first[tl * SCAN_K + j] >= 0) << j;
-    f.last |= (unsigned)(last[tl * SCAN_K + j] >= 0) << j;
+  for (int k = 0; k < SCAN_SEG; k += 4) {
+    const int4 f = *reinterpret_cast<const int4*>(first + k), l = *reinterpret_cast<const int4*>(last + k);
+    any |= (f.x & f.y & f.z & f.w & l.x & l.y & l.z & l.w) >= 0;  // -1 everywhere: no flag
   }
-  const unsigned starts = __ballot_sync(0xffffffffu, f.first != 0);
-  f.any_first = starts != 0;
-  f.any_last = __ballot_sync(0xffffffffu, f.last != 0) != 0;
-  const unsigned mine = LT == 32 ? starts : (starts >> ((threadIdx.x & 31) / LT * LT)) & ((1u << (LT & 31)) - 1u);
-#pragma unroll
-  for (int off = 1, k = 0; off < LT; off <<= 1, ++k) {
-    const unsigned span = (1u << off) - 1u;  // off <= 16
-    if (tl >= off && ((mine >> (tl - off + 1)) & span)) f.up |= 1u << k;
-    if ((mine >> tl) & span) f.down |= 1u << k;
-  }
-  return f;
+  return any;
 }
 
-// Sum over the LT lanes of a channel pair.
-template <int LT>
-__device__ __forceinline__ u64 scan_sum(u64 v) {
-#pragma unroll
-  for (int m = LT / 2; m >= 1; m >>= 1) v = add2(v, __shfl_xor_sync(0xffffffffu, v, m, LT));
-  return v;
+template <typename T, typename G>
+__host__ __device__ inline int scan_stage_elems(int N, int tensors) {
+  return tensors * G::RAW + 2 * G::TT * ((N + 7) / 8 * 8);
+}
+template <typename T, typename G>
+__host__ __device__ inline int scan_fwd_smem(int N) {
+  return SCAN_STAGES * scan_stage_elems<T, G>(N, 3) * (int)sizeof(T) +
+         2 * (G::TT * G::CPB * 8 + 2 * G::TT * G::NP * 4 + G::TT * G::CPB * G::L * 4 + 2 * G::TT * 4);
+}
+template <typename T, typename G>
+__host__ __device__ inline int scan_bwd_smem(int N) {
+  return SCAN_STAGES * scan_stage_elems<T, G>(N, 4) * (int)sizeof(T) +
+         3 * G::TT * G::CPB * 16 + 2 * (2 * G::TT * G::S * G::NP * 4 + 3 * G::TT * G::CPB * G::L * 4 +
+                                        SCAN_WARPS * G::TT * 2 * G::NP * 4 + 2 * G::TT * 4);
 }
 
-// A lane's steps d (0 past T), inputs d x, the sum of d, and the flags of its
-// tokens that are a sequence's first or last.
-template <typename T, int LT>
-__device__ __forceinline__ void scan_inputs(const ScanParams& P, const char* rx, const char* rdt, int t0, int tl, int c,
-                                            u64 bias, u64 (&d)[SCAN_K], u64 (&u)[SCAN_K], u64& sum) {
-  using G = ScanGeo<T, LT>;
-  sum = pk2(0.f, 0.f);
-#pragma unroll
-  for (int j = 0; j < SCAN_K; ++j) {
-    const int t = tl * SCAN_K + j;
-    const float2 r = upk2(add2(scan_pair<T>(rdt + G::raw_off(t, c)), bias));
-    u64 v = P.softplus ? pk2(softplusf_(r.x), softplusf_(r.y)) : pk2(r.x, r.y);
-    if (t0 + t >= P.T) v = pk2(0.f, 0.f);
-    d[j] = v;
-    u[j] = mul2(v, scan_pair<T>(rx + G::raw_off(t, c)));
-    sum = add2(sum, v);
-  }
+// A channel pair's values of a per-channel parameter (zeros without it or past the block).
+__device__ __forceinline__ float2 scan_param(const float* p, const ScanBlock& s, int c) {
+  return make_float2(p && c < s.nc ? p[s.c0 + c] : 0.f, p && c + 1 < s.nc ? p[s.c0 + c + 1] : 0.f);
 }
 
-// Shared memory: staged tensors, B, C, log2-scaled A, the carried states and the
-// sequence flags of the tile (packed).  The backward adds the carried gradients, the
-// dB and dC of the tile and the lanes' dA sums.
-template <typename T, int LT>
-__host__ __device__ inline int scan_smem_bytes(int N, int tensors, bool bwd) {
-  using G = ScanGeo<T, LT>;
-  int b = tensors * G::RAW + 2 * N * G::BCP * 4 + 2 * N * G::CPB * 4 + 2 * G::TL * 4;
-  if (bwd) b += N * G::CPB * 4 + 2 * N * G::TL * 4 + N * (LT == 32 ? SCAN_THREADS * 8 : G::CPB * 4);
-  return b;
-}
-
-__device__ __forceinline__ float2 scan_state2(const float* p, long long row, int E, int N, int c, int nc, int c0, int n) {
-  float2 v = make_float2(0.f, 0.f);
-  const float* q = p + (row * E + c0 + c) * (long long)N + n;
-  if (c < nc) v.x = __ldg(q);
-  if (c + 1 < nc) v.y = __ldg(q + N);
-  return v;
-}
-__device__ __forceinline__ void scan_put_state2(float* p, long long row, int E, int N, int c, int nc, int c0, int n,
-                                                float2 v) {
-  float* q = p + (row * E + c0 + c) * (long long)N + n;
-  if (c < nc) q[0] = v.x;
-  if (c + 1 < nc) q[N] = v.y;
-}
-
-template <typename T, int LT, bool PACKED>
-__global__ void __launch_bounds__(SCAN_THREADS) ssm_scan_fwd_kernel(ScanParams P, int np2) {
-  using G = ScanGeo<T, LT>;
+template <typename T, int L, int S, bool PAD>
+__global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParams P) {
+  using G = ScanFwdGeo<T, L, S>;
+  constexpr int TT = G::TT, CPB = G::CPB;
   extern __shared__ __align__(16) char scan_sm[];
-  char* rx = scan_sm;
-  char* rdt = rx + G::RAW;
-  char* rz = rdt + G::RAW;
-  float* Bs = reinterpret_cast<float*>(rz + (P.z.p ? G::RAW : 0));
-  float* Cs = Bs + P.N * G::BCP;
-  float* A2 = Cs + P.N * G::BCP;       // [N][CPB]
-  float* carry = A2 + P.N * G::CPB;    // [N][CPB]
-  int* first = reinterpret_cast<int*>(carry + P.N * G::CPB);  // [TL]
-  int* last = first + G::TL;
+  const int N = P.N, npad = (N + 7) / 8 * 8, stage = scan_stage_elems<T, G>(N, 3);
+  T* raw = reinterpret_cast<T*>(scan_sm);              // [STAGES]: x, dt, z, B rows, C rows
+  // double buffers:
+  float2* DU = reinterpret_cast<float2*>(raw + SCAN_STAGES * stage);  // [TT][CPB]: d, d x
+  float* Bs = reinterpret_cast<float*>(DU + 2 * TT * CPB);            // [TT][NP]
+  float* Cs = Bs + 2 * TT * G::NP;
+  float* YP = Cs + 2 * TT * G::NP;                                    // [TT][CPB][L]
+  int* flags = reinterpret_cast<int*>(YP + 2 * TT * CPB * L);         // first [TT], last [TT]
+  const ScanBlock s = scan_block<CPB>(P);
+  const int tiles = (P.T + TT - 1) / TT, segs = (P.T + SCAN_SEG - 1) / SCAN_SEG;
 
-  const ScanBlock s = scan_block<G::CPB>(P);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tl = lane % LT, c = warp * (2 * G::CL) + (lane / LT) * 2;
-  const int N = P.N;
-  for (int i = threadIdx.x; i < N * G::CPB; i += SCAN_THREADS) {
-    const int n = i / G::CPB, cc = i - n * G::CPB;
-    const bool ok = cc < s.nc;
-    A2[i] = ok ? P.A[(long long)(s.c0 + cc) * N + n] * LOG2E : 0.f;
-    carry[i] = !PACKED && P.h0 && ok ? P.h0[((long long)s.b * P.E + s.c0 + cc) * N + n] : 0.f;
-  }
-  const float2 zero2 = make_float2(0.f, 0.f);
-  float2 bias = zero2, dskip = zero2;
-  if (c < s.nc) {
-    if (P.dt_bias) bias.x = P.dt_bias[s.c0 + c];
-    if (P.D) dskip.x = P.D[s.c0 + c];
-  }
-  if (c + 1 < s.nc) {
-    if (P.dt_bias) bias.y = P.dt_bias[s.c0 + c + 1];
-    if (P.D) dskip.y = P.D[s.c0 + c + 1];
-  }
-  const u64 bias2 = pk2(bias.x, bias.y);
-
-  for (int tile = 0; tile < P.tiles; ++tile) {
-    const int t0 = tile * G::TL;
-    __syncthreads();  // the tile in front has left
-    scan_stage<T, LT>(rx, P.x, P, s, t0);
-    scan_stage<T, LT>(rdt, P.dt, P, s, t0);
-    if (P.z.p) scan_stage<T, LT>(rz, P.z, P, s, t0);
-    scan_stage_bc<T, LT>(Bs, P.Bm, P.b_sb, P.b_st, P.b_sg, P, s, t0, np2);
-    scan_stage_bc<T, LT>(Cs, P.Cm, P.c_sb, P.c_st, P.c_sg, P, s, t0, np2);
-    if (PACKED) {
-      for (int i = threadIdx.x; i < G::TL; i += SCAN_THREADS) {
-        first[i] = t0 + i < P.T ? __ldg(P.seq.start + t0 + i) : -1;
-        last[i] = t0 + i < P.T ? __ldg(P.seq.end + t0 + i) : -1;
+  if (threadIdx.x >= SCAN_MAIN) {  // tokens
+    const int tid = threadIdx.x - SCAN_MAIN;
+    const int pc = (tid % G::PAIRS) * 2, pt = tid / G::PAIRS;
+    const float2 bias = scan_param(P.dt_bias, s, pc), skip = scan_param(P.D, s, pc);
+    const RowView views[3] = {P.x, P.dt, P.z};
+    ScanFetch<T, G, 3> f;
+    f.init(P, s, views, tid, 3 * G::RAW, npad, 0, 1);
+    ScanFlags<TT> marks;
+    marks.read(P, s.b, 0, tid);
+    // (both passes: all reads of shared memory, then all writes)
+    constexpr int IT = TT / G::TSTEP;
+    const bool spare = G::SPARE && pt >= TT;
+    auto prepare = [&](int i) {
+      const int t0 = i * TT, q = i & 1;
+      const T* rx = raw + (i % SCAN_STAGES) * stage;
+      ScanBC<T, G, 1, PAD> bc;
+      float2 x[IT], dt[IT];
+      float4 du[IT];
+      if (!spare) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          x[k] = scan_pair(rx + (pt + k * G::TSTEP) * CPB + pc);
+          dt[k] = scan_pair(rx + G::RAW + (pt + k * G::TSTEP) * CPB + pc);
+        }
       }
-    }
-    if (P.ckpt) {
-      float* ck = P.ckpt + (((long long)s.b * P.tiles + tile) * gridDim.x + blockIdx.x) * (N * G::CPB);
-      for (int i = threadIdx.x; i < N * G::CPB; i += SCAN_THREADS) ck[i] = carry[i];
-    }
-    __syncthreads();
-
-    u64 d[SCAN_K], u[SCAN_K], y[SCAN_K], sum;
-    scan_inputs<T, LT>(P, rx, rdt, t0, tl, c, bias2, d, u, sum);
-    ScanFlags f{};
-    if (PACKED) f = scan_flags<LT>(first, last, tl);
+      bc.load(rx + 3 * G::RAW, npad, P, s, t0, tid);
+      if (!spare) {
 #pragma unroll
-    for (int j = 0; j < SCAN_K; ++j) y[j] = pk2(0.f, 0.f);
-
-    auto states = [&](auto reset) {
-      constexpr bool RESET = decltype(reset)::value;
-#pragma unroll 1
-      for (int n = 0; n < N; ++n) {
-        const u64 a2 = *reinterpret_cast<const u64*>(A2 + n * G::CPB + c);
-        const u64 h_in = *reinterpret_cast<const u64*>(carry + n * G::CPB + c);
-        float bv[SCAN_K], cv[SCAN_K];
-        scan_row8(Bs + n * G::BCP, G::TL / 2, tl, bv);
-        scan_row8(Cs + n * G::BCP, G::TL / 2, tl, cv);
-        u64 a[SCAN_K], b[SCAN_K];
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j) {
-          a[j] = ex2_2(mul2(d[j], a2));
-          b[j] = mul2(u[j], pk2(bv[j], bv[j]));
+        for (int k = 0; k < IT; ++k) {
+          const bool in = t0 + pt + k * G::TSTEP < P.T;
+          const float d0 = scan_d(P, dt[k].x + bias.x, in), d1 = scan_d(P, dt[k].y + bias.y, in);
+          du[k] = make_float4(d0, d0 * x[k].x, d1, d1 * x[k].y);
         }
-        if (RESET && P.h0) {  // a sequence's first token takes up its initial state
 #pragma unroll
-          for (int j = 0; j < SCAN_K; ++j)
-            if (f.first >> j & 1) {
-              const float2 h = scan_state2(P.h0, first[tl * SCAN_K + j], P.E, N, c, s.nc, s.c0, n);
-              b[j] = fma2(a[j], pk2(h.x, h.y), b[j]);
-            }
+        for (int k = 0; k < IT; ++k)
+          *reinterpret_cast<float4*>(DU + (q * TT + pt + k * G::TSTEP) * CPB + pc) = du[k];
+      }
+      bc.store(Bs + q * TT * G::NP, Cs + q * TT * G::NP, tid);
+      marks.write(flags + q * 2 * TT, tid);
+      marks.read(P, s.b, t0 + TT, tid);
+    };
+    auto finish = [&](int i) {
+      const int t0 = i * TT;
+      const T* rx = raw + (i % SCAN_STAGES) * stage;
+      const float* yp = YP + (i & 1) * TT * CPB * L;
+      if (spare) return;
+#pragma unroll
+      for (int k = 0; k < TT; k += G::TSTEP) {
+        const int t = pt + k;
+        const float2 x = scan_pair(rx + t * CPB + pc);
+        float2 v = make_float2(fmaf(skip.x, x.x, scan_join<L>(yp + (t * CPB + pc) * L)),
+                               fmaf(skip.y, x.y, scan_join<L>(yp + (t * CPB + pc + 1) * L)));
+        if (P.z.p) {
+          const float2 z = scan_pair(rx + 2 * G::RAW + t * CPB + pc);
+          v.x *= siluf_(z.x);
+          v.y *= siluf_(z.y);
         }
-        u64 h = b[0];
-#pragma unroll
-        for (int j = 1; j < SCAN_K; ++j) h = RESET && (f.first >> j & 1) ? b[j] : fma2(a[j], h, b[j]);
-        const u64 p = ex2_2(mul2(sum, a2));
-        if (tl == 0 && !(RESET && f.first)) h = fma2(p, h_in, h);
-        scan_lanes<LT, RESET>(h, p, tl, f.up);
-        __syncwarp();  // every lane has read the carried state
-        if (tl == LT - 1) *reinterpret_cast<u64*>(carry + n * G::CPB + c) = h;
-        h = scan_up<LT>(h, 1);
-        if (tl == 0) h = h_in;
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j) {
-          h = RESET && (f.first >> j & 1) ? b[j] : fma2(a[j], h, b[j]);
-          if (PACKED) b[j] = h;
-          y[j] = fma2(h, pk2(cv[j], cv[j]), y[j]);
-        }
-        if (PACKED && f.any_last && P.ht) {
-#pragma unroll
-          for (int j = 0; j < SCAN_K; ++j)
-            if (f.last >> j & 1)
-              scan_put_state2(P.ht, last[tl * SCAN_K + j], P.E, N, c, s.nc, s.c0, n, upk2(b[j]));
-        }
+        if (t0 + t < P.T) scan_put_pair<T>(P.y, P, s, t0 + t, pc, v);
       }
     };
-    if (PACKED && f.any_first) states(std::true_type{});
-    else states(std::false_type{});
-
-    const u64 skip2 = pk2(dskip.x, dskip.y);
-#pragma unroll
-    for (int j = 0; j < SCAN_K; ++j) {
-      const int off = G::raw_off(tl * SCAN_K + j, c);
-      float2 v = upk2(fma2(skip2, scan_pair<T>(rx + off), y[j]));
-      if (P.z.p) {
-        const float2 z = upk2(scan_pair<T>(rz + off));
-        v.x *= siluf_(z.x);
-        v.y *= siluf_(z.y);
-      }
-      scan_put<T>(rx + off, v);
-    }
+    f.fetch(P, s, views, raw, 0, tid);
+    if (tiles > 1) f.fetch(P, s, views, raw + stage, TT, tid);
+    cp_async_wait<0>();
+    asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");  // the first tiles have arrived, for the whole side
+    prepare(0);
     __syncthreads();
-    scan_unstage<T, LT>(rx, P.y, P, s, t0);
-  }
-  if (!PACKED && P.ht)
-    for (int i = threadIdx.x; i < N * G::CPB; i += SCAN_THREADS) {
-      const int n = i / G::CPB, cc = i - n * G::CPB;
-      if (cc < s.nc) P.ht[((long long)s.b * P.E + s.c0 + cc) * N + n] = carry[i];
-    }
-}
-
-// Backward: tiles from last to first; each rebuilds its states from the forward's
-// state at the tile's start.  The eight warps take the states n in an order of their
-// own (warp w starts at n = w), one barrier per step, so that no two add to the same dB
-// and dC rows at once and every sum has a fixed order.
-template <typename T, int LT, bool PACKED>
-__global__ void __launch_bounds__(SCAN_THREADS) ssm_scan_bwd_kernel(ScanParams P, int np2) {
-  using G = ScanGeo<T, LT>;
-  extern __shared__ __align__(16) char scan_sm[];
-  char* rx = scan_sm;
-  char* rdt = rx + G::RAW;
-  char* rdy = rdt + G::RAW;
-  char* rz = rdy + G::RAW;
-  float* Bs = reinterpret_cast<float*>(rz + (P.z.p ? G::RAW : 0));
-  float* Cs = Bs + P.N * G::BCP;
-  float* A2 = Cs + P.N * G::BCP;
-  float* hst = A2 + P.N * G::CPB;     // states at the tile's start
-  float* gcar = hst + P.N * G::CPB;   // gradient of the state in front of the tile behind
-  float* dBs = gcar + P.N * G::CPB;   // [2][N][TL], tokens in bc_off order
-  // dA: a sum per lane over the tiles with 32 lanes on time ([N][threads]), a sum per
-  // channel pair with fewer (three shuffles a state; [N][CPB])
-  constexpr int DAW = LT == 32 ? SCAN_THREADS : G::CPB / 2;
-  u64* dAs = reinterpret_cast<u64*>(dBs + 2 * P.N * G::TL);
-  int* first = reinterpret_cast<int*>(dAs + P.N * DAW);
-  int* last = first + G::TL;
-
-  const ScanBlock s = scan_block<G::CPB>(P);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int tl = lane % LT, c = warp * (2 * G::CL) + (lane / LT) * 2;
-  const int N = P.N, steps = max(N, SCAN_WARPS);
-  float* dCs = dBs + N * G::TL;
-  for (int i = threadIdx.x; i < N * G::CPB; i += SCAN_THREADS) {
-    const int n = i / G::CPB, cc = i - n * G::CPB;
-    const bool ok = cc < s.nc;
-    A2[i] = ok ? P.A[(long long)(s.c0 + cc) * N + n] * LOG2E : 0.f;
-    gcar[i] = !PACKED && P.dht && ok ? P.dht[((long long)s.b * P.E + s.c0 + cc) * N + n] : 0.f;
-  }
-  for (int i = threadIdx.x; i < N * DAW; i += SCAN_THREADS) dAs[i] = 0;
-  const float2 zero2 = make_float2(0.f, 0.f);
-  float2 bias = zero2, dskip = zero2;
-  if (c < s.nc) {
-    if (P.dt_bias) bias.x = P.dt_bias[s.c0 + c];
-    if (P.D) dskip.x = P.D[s.c0 + c];
-  }
-  if (c + 1 < s.nc) {
-    if (P.dt_bias) bias.y = P.dt_bias[s.c0 + c + 1];
-    if (P.D) dskip.y = P.D[s.c0 + c + 1];
-  }
-  const u64 bias2 = pk2(bias.x, bias.y), skip2 = pk2(dskip.x, dskip.y);
-  float2 sum_dD = zero2, sum_db = zero2;
-
-  for (int tile = P.tiles - 1; tile >= 0; --tile) {
-    const int t0 = tile * G::TL;
-    __syncthreads();
-    scan_stage<T, LT>(rx, P.x, P, s, t0);
-    scan_stage<T, LT>(rdt, P.dt, P, s, t0);
-    scan_stage<T, LT>(rdy, P.dy, P, s, t0);
-    if (P.z.p) scan_stage<T, LT>(rz, P.z, P, s, t0);
-    scan_stage_bc<T, LT>(Bs, P.Bm, P.b_sb, P.b_st, P.b_sg, P, s, t0, np2);
-    scan_stage_bc<T, LT>(Cs, P.Cm, P.c_sb, P.c_st, P.c_sg, P, s, t0, np2);
-    if (PACKED) {
-      for (int i = threadIdx.x; i < G::TL; i += SCAN_THREADS) {
-        first[i] = t0 + i < P.T ? __ldg(P.seq.start + t0 + i) : -1;
-        last[i] = t0 + i < P.T ? __ldg(P.seq.end + t0 + i) : -1;
-      }
-    }
-    {
-      const float* ck = P.ckpt + (((long long)s.b * P.tiles + tile) * gridDim.x + blockIdx.x) * (N * G::CPB);
-      for (int i = threadIdx.x; i < N * G::CPB; i += SCAN_THREADS) hst[i] = ck[i];
-    }
-    for (int i = threadIdx.x; i < 2 * N * G::TL; i += SCAN_THREADS) dBs[i] = 0.f;
-    __syncthreads();
-
-    u64 d[SCAN_K], u[SCAN_K], ds[SCAN_K], gb[SCAN_K], dd[SCAN_K], y[SCAN_K], sum;
-    scan_inputs<T, LT>(P, rx, rdt, t0, tl, c, bias2, d, u, sum);
-    ScanFlags f{};
-    if (PACKED) f = scan_flags<LT>(first, last, tl);
-#pragma unroll
-    for (int j = 0; j < SCAN_K; ++j) {
-      const int off = G::raw_off(tl * SCAN_K + j, c);
-      float2 v = upk2(scan_pair<T>(rdy + off));
-      if (P.z.p) {
-        const float2 z = upk2(scan_pair<T>(rz + off));
-        v.x *= siluf_(z.x);
-        v.y *= siluf_(z.y);
-      }
-      ds[j] = pk2(v.x, v.y);
-      gb[j] = dd[j] = y[j] = pk2(0.f, 0.f);
-    }
-
-    auto states = [&](auto reset) {
-      constexpr bool RESET = decltype(reset)::value;
-#pragma unroll 1
-      for (int step = 0; step < steps; ++step) {
-      const int n = step + warp < steps ? step + warp : step + warp - steps;
-      if (n < N) {
-        const u64 a2 = *reinterpret_cast<const u64*>(A2 + n * G::CPB + c);
-        const u64 h_in = *reinterpret_cast<const u64*>(hst + n * G::CPB + c);
-        const u64 g_in = *reinterpret_cast<const u64*>(gcar + n * G::CPB + c);
-        float bv[SCAN_K], cv[SCAN_K];
-        scan_row8(Bs + n * G::BCP, G::TL / 2, tl, bv);
-        scan_row8(Cs + n * G::BCP, G::TL / 2, tl, cv);
-        u64 a[SCAN_K], hh[SCAN_K];
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j) {
-          a[j] = ex2_2(mul2(d[j], a2));
-          hh[j] = mul2(u[j], pk2(bv[j], bv[j]));
-        }
-        if (RESET && P.h0) {
-#pragma unroll
-          for (int j = 0; j < SCAN_K; ++j)
-            if (f.first >> j & 1) {
-              const float2 h = scan_state2(P.h0, first[tl * SCAN_K + j], P.E, N, c, s.nc, s.c0, n);
-              hh[j] = fma2(a[j], pk2(h.x, h.y), hh[j]);
-            }
-        }
-        const u64 p = ex2_2(mul2(sum, a2));
-        // states of the tile
-        u64 h = hh[0];
-#pragma unroll
-        for (int j = 1; j < SCAN_K; ++j) h = RESET && (f.first >> j & 1) ? hh[j] : fma2(a[j], h, hh[j]);
-        if (tl == 0 && !(RESET && f.first)) h = fma2(p, h_in, h);
-        scan_lanes<LT, RESET>(h, p, tl, f.up);
-        h = scan_up<LT>(h, 1);
-        if (tl == 0) h = h_in;
-        const u64 h_first = h;
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j) {
-          h = RESET && (f.first >> j & 1) ? hh[j] : fma2(a[j], h, hh[j]);
-          hh[j] = h;
-        }
-        // gradients of the states, from the tile's end
-        u64 cg[SCAN_K];
-#pragma unroll
-        for (int j = 0; j < SCAN_K; ++j) cg[j] = mul2(ds[j], pk2(cv[j], cv[j]));
-        if (PACKED && f.any_last && P.dht) {
-#pragma unroll
-          for (int j = 0; j < SCAN_K; ++j)
-            if (f.last >> j & 1) {
-              const float2 v = scan_state2(P.dht, last[tl * SCAN_K + j], P.E, N, c, s.nc, s.c0, n);
-              cg[j] = add2(cg[j], pk2(v.x, v.y));
-            }
-        }
-        u64 r = pk2(0.f, 0.f);
-#pragma unroll
-        for (int j = SCAN_K - 1; j >= 0; --j) {
-          r = j == SCAN_K - 1 ? mul2(a[j], cg[j]) : mul2(a[j], add2(cg[j], r));
-          if (RESET && (f.first >> j & 1)) r = pk2(0.f, 0.f);  // nothing passes a sequence's start
-        }
-        if (tl == LT - 1 && !(RESET && f.first)) r = fma2(p, g_in, r);
-        scan_lanes_rev<LT, RESET>(r, p, tl, f.down);
-        __syncwarp();  // every lane has read the carried gradient
-        if (tl == 0) *reinterpret_cast<u64*>(gcar + n * G::CPB + c) = r;
-        r = scan_down<LT>(r, 1);
-        if (tl == LT - 1) r = g_in;
-        u64 sA = LT == 32 ? dAs[n * DAW + threadIdx.x] : pk2(0.f, 0.f);
-        const u64 an = mul2(a2, pk2(LN2, LN2));
-        float dB[SCAN_K], dC[SCAN_K];
-#pragma unroll
-        for (int j = SCAN_K - 1; j >= 0; --j) {
-          const u64 g = add2(cg[j], r);
-          r = mul2(a[j], g);
-          u64 q;
-          if (RESET && (f.first >> j & 1)) {  // what reaches the initial state
-            const int sq = first[tl * SCAN_K + j];
-            if (P.dh0) scan_put_state2(P.dh0, sq, P.E, N, c, s.nc, s.c0, n, upk2(r));
-            q = pk2(0.f, 0.f);
-            if (P.h0) {
-              const float2 h0 = scan_state2(P.h0, sq, P.E, N, c, s.nc, s.c0, n);
-              q = mul2(r, pk2(h0.x, h0.y));
-            }
-            r = pk2(0.f, 0.f);
-          } else {
-            q = mul2(r, j ? hh[j - 1] : h_first);
-          }
-          dd[j] = fma2(q, an, dd[j]);
-          sA = fma2(q, d[j], sA);
-          gb[j] = fma2(g, pk2(bv[j], bv[j]), gb[j]);
-          const float2 db = upk2(mul2(g, u[j])), dc = upk2(mul2(ds[j], hh[j]));
-          dB[j] = db.x + db.y;
-          dC[j] = dc.x + dc.y;
-          if (P.z.p) y[j] = fma2(hh[j], pk2(cv[j], cv[j]), y[j]);
-        }
-        if (LT == 32) {
-          dAs[n * DAW + threadIdx.x] = sA;
-        } else {
-          sA = scan_sum<LT>(sA);
-          if (tl == 0) dAs[n * DAW + c / 2] = add2(dAs[n * DAW + c / 2], sA);
-        }
-        // over the warp's channel pairs, then onto the tile's sums
-#pragma unroll
-        for (int m = LT; m < 32; m <<= 1) {
-#pragma unroll
-          for (int j = 0; j < SCAN_K; ++j) {
-            dB[j] += __shfl_xor_sync(0xffffffffu, dB[j], m);
-            dC[j] += __shfl_xor_sync(0xffffffffu, dC[j], m);
-          }
-        }
-        if (lane < LT) {
-#pragma unroll
-          for (int j = 0; j < SCAN_K; ++j) {
-            const int o = n * G::TL + G::bc_off(tl * SCAN_K + j);
-            dBs[o] += dB[j];
-            dCs[o] += dC[j];
-          }
-        }
-      }
+    for (int i = 0; i < tiles; ++i) {
+      // (stage of i + 2 held i - 2, which was finished before the last barrier)
+      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, (i + 2) * TT, tid);
+      if (i + 1 < tiles) prepare(i + 1);
+      if (i > 0) finish(i - 1);
+      cp_async_wait<0>();
       __syncthreads();
     }
-    };
-    if (PACKED && f.any_first) states(std::true_type{});
-    else states(std::false_type{});
+    finish(tiles - 1);
+    return;
+  }
 
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = lane / G::CH, c = warp * G::CH + lane % G::CH, n0 = l * S;
+  const unsigned ok = N - n0 >= S ? (1u << S) - 1u : N > n0 ? (1u << (N - n0)) - 1u : 0u;  // states that exist
+  const bool live = c < s.nc;
+  Lane<S> a2 = Lane<S>::all(0.f), h = a2;
+  const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
 #pragma unroll
-    for (int j = 0; j < SCAN_K; ++j) {
-      const int t = tl * SCAN_K + j, off = G::raw_off(t, c);
-      const u64 x2 = scan_pair<T>(rx + off);
-      const float2 raw = upk2(add2(scan_pair<T>(rdt + off), bias2));
-      if (P.z.p) {
-        const float2 z = upk2(scan_pair<T>(rz + off)), dy = upk2(scan_pair<T>(rdy + off));
-        const float2 v = upk2(fma2(skip2, x2, y[j]));
-        scan_put<T>(rz + off, make_float2(dy.x * v.x * silu_slopef_(z.x), dy.y * v.y * silu_slopef_(z.y)));
+  for (int i = 0; i < S; ++i)
+    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + i] * LOG2E);
+  __syncthreads();
+  for (int tile = 0; tile < tiles; ++tile) {
+    const int t0 = tile * TT, q = tile & 1;
+    const float2* du_ = DU + q * TT * CPB + c;
+    const float* b_ = Bs + q * TT * G::NP + n0;
+    const float* c_ = Cs + q * TT * G::NP + n0;
+    float* y_ = YP + q * TT * CPB * L + c * L + l;
+    const int* first = flags + q * 2 * TT;
+    const int* last = first + TT;
+    auto segment = [&](int t1, auto with_flags) {
+      constexpr bool FLAGS = decltype(with_flags)::value;
+      // all of the segment's reads in front of its stores, which the compiler must assume to alias
+      float2 du[SCAN_SEG];
+      Lane<S> bv[SCAN_SEG], cv[SCAN_SEG];
+      float y[SCAN_SEG];
+#pragma unroll
+      for (int k = 0; k < SCAN_SEG; ++k) {
+        du[k] = du_[(t1 + k) * CPB];
+        bv[k] = Lane<S>::load(b_ + (t1 + k) * G::NP);
+        cv[k] = Lane<S>::load(c_ + (t1 + k) * G::NP);
       }
-      const float2 px = upk2(mul2(ds[j], x2));
-      sum_dD.x += px.x;
-      sum_dD.y += px.y;
-      float2 v = upk2(fma2(gb[j], x2, dd[j]));
-      if (P.softplus) {
-        v.x *= sigmoidf_(raw.x);
-        v.y *= sigmoidf_(raw.y);
+#pragma unroll
+      for (int k = 0; k < SCAN_SEG; ++k) {
+        const int t = t1 + k;
+        if (FLAGS && first[t] >= 0) {
+#pragma unroll
+          for (int i = 0; i < S; ++i)
+            h.set(i, P.h0 && live && (ok >> i & 1) ? __ldg(P.h0 + (long long)first[t] * P.E * N + chan + i) : 0.f);
+        }
+        const Lane<S> a = lane_decay(a2, du[k].x);
+        h = lane_keep<PAD>(fma(a, h, bv[k] * Lane<S>::all(du[k].y)), ok);
+        y[k] = (h * cv[k]).sum();
+        if (FLAGS && last[t] >= 0 && P.ht) {
+#pragma unroll
+          for (int i = 0; i < S; ++i)
+            if (live && (ok >> i & 1)) P.ht[(long long)last[t] * P.E * N + chan + i] = h.get(i);
+        }
       }
-      if (t0 + t >= P.T) v = zero2;
-      sum_db.x += v.x;
-      sum_db.y += v.y;
-      scan_put<T>(rdt + off, v);
-      scan_put<T>(rx + off, upk2(fma2(gb[j], d[j], mul2(ds[j], skip2))));
+#pragma unroll
+      for (int k = 0; k < SCAN_SEG; ++k) y_[(t1 + k) * CPB * L] = y[k];
+    };
+#pragma unroll 1
+    for (int t1 = 0; t1 < TT && t0 + t1 < P.T; t1 += SCAN_SEG) {
+      if (P.ckpt && live) {
+        float* ck = P.ckpt + ((long long)s.b * segs + (t0 + t1) / SCAN_SEG) * P.E * N + chan;
+        if (!PAD) {
+          h.store(ck);
+        } else {
+#pragma unroll
+          for (int i = 0; i < S; ++i)
+            if (ok >> i & 1) ck[i] = h.get(i);
+        }
+      }
+      if (scan_seg_flag(first + t1, last + t1)) segment(t1, std::true_type{});
+      else segment(t1, std::false_type{});
     }
     __syncthreads();
-    scan_unstage<T, LT>(rx, P.dx, P, s, t0);
-    scan_unstage<T, LT>(rdt, P.ddt, P, s, t0);
-    if (P.z.p) scan_unstage<T, LT>(rz, P.dz, P, s, t0);
-    float* part = P.bc_part + ((((long long)s.b * P.tiles + tile) * P.G + s.g) * P.blocks + s.blk) * (2 * N * G::TL);
-    for (int i = threadIdx.x; i < 2 * N * G::TL; i += SCAN_THREADS) part[i] = dBs[i];
   }
-  if (!PACKED && P.dh0)
-    for (int i = threadIdx.x; i < N * G::CPB; i += SCAN_THREADS) {
-      const int n = i / G::CPB, cc = i - n * G::CPB;
-      if (cc < s.nc) P.dh0[((long long)s.b * P.E + s.c0 + cc) * N + n] = gcar[i];
-    }
-  // the row's dA, dD and d dt_bias: sums over the LT lanes of a channel pair
-  float* e0 = P.e_part + ((long long)s.b * P.E + s.c0 + c) * (N + 2);
-  float* e1 = e0 + N + 2;
-  for (int n = 0; n < N; ++n) {
-    const float2 v = upk2(LT == 32 ? scan_sum<LT>(dAs[n * DAW + threadIdx.x]) : dAs[n * DAW + c / 2]);
-    if (tl == 0 && c < s.nc) e0[n] = v.x;
-    if (tl == 0 && c + 1 < s.nc) e1[n] = v.y;
-  }
-  const float2 dD = upk2(scan_sum<LT>(pk2(sum_dD.x, sum_dD.y))), db = upk2(scan_sum<LT>(pk2(sum_db.x, sum_db.y)));
-  if (tl == 0 && c < s.nc) { e0[N] = dD.x; e0[N + 1] = db.x; }
-  if (tl == 0 && c + 1 < s.nc) { e1[N] = dD.y; e1[N + 1] = db.y; }
 }
 
-// dB and dC: the channel blocks' partial sums of a tile, summed in block order.
-// One CTA column per (row, tile, group); thread i takes element i of [2][N][TL].
+template <typename T, int L, int S, bool PAD>
+__global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParams P) {
+  using G = ScanBwdGeo<T, L, S>;
+  constexpr int TT = G::TT, CPB = G::CPB, CH = G::CH;
+  static_assert(TT == SCAN_SEG, "a tile of the backward is one segment");
+  // lane bits, from the top: XB channel bits that also order the lane's states, the L
+  // lanes of a channel, the other RB channel bits (so that lane pairs share B and C reads)
+  constexpr int CB = ilog2(CH), XB = CB < ilog2(S) ? CB : ilog2(S), RB = CB - XB, LB = ilog2(L);
+  extern __shared__ __align__(16) char scan_sm[];
+  const int N = P.N, npad = (N + 7) / 8 * 8, stage = scan_stage_elems<T, G>(N, 4);
+  T* raw = reinterpret_cast<T*>(scan_sm);  // [STAGES]: x, dt, dy, z, B rows, C rows
+  // three buffers (prepared, used by the recurrences, used to finish):
+  float2* DU = reinterpret_cast<float2*>(raw + SCAN_STAGES * stage);  // [TT][CPB]: d, d x
+  float* DS = reinterpret_cast<float*>(DU + 3 * TT * CPB);            // [TT][CPB]: dy silu(z)
+  float* DZ = DS + 3 * TT * CPB;                                      // [TT][CPB]: dy silu'(z)
+  // double buffers:
+  float* Bs = DZ + 3 * TT * CPB;                                      // [TT][S][NP]
+  float* Cs = Bs + 2 * TT * S * G::NP;
+  float* YP = Cs + 2 * TT * S * G::NP;       // [3][TT][CPB][L]: partial sums of y, dd / ln 2, sum g B
+  float* slots = YP + 2 * 3 * TT * CPB * L;  // [warps][TT][2][NP]: the warps' dB and dC
+  int* flags = reinterpret_cast<int*>(slots + 2 * SCAN_WARPS * TT * 2 * G::NP);  // first [TT], last [TT]
+  const ScanBlock s = scan_block<CPB>(P);
+  const int tiles = (P.T + TT - 1) / TT;  // step i takes tile tiles - 1 - i
+  float* e = P.e_part + (long long)s.b * P.E * (N + 2);
+
+  if (threadIdx.x >= SCAN_MAIN) {  // tokens
+    const int tid = threadIdx.x - SCAN_MAIN;
+    const int pc = (tid % G::PAIRS) * 2, pt = tid / G::PAIRS;
+    const float2 bias = scan_param(P.dt_bias, s, pc), skip = scan_param(P.D, s, pc);
+    const float2 zero = make_float2(0.f, 0.f);
+    float2 dD = zero, db = zero, dD_err = zero, db_err = zero;
+    const RowView views[4] = {P.x, P.dt, P.dy, P.z};
+    ScanFetch<T, G, 4> f;
+    f.init(P, s, views, tid, 4 * G::RAW, npad, tiles - 1, -1);
+    ScanFlags<TT> marks;
+    marks.read(P, s.b, (tiles - 1) * TT, tid);
+    // (both passes: all reads of shared memory, then all writes)
+    constexpr int IT = TT / G::TSTEP;
+    const bool spare = G::SPARE && pt >= TT;
+    auto prepare = [&](int i) {
+      const int t0 = (tiles - 1 - i) * TT, q = i & 1;
+      const T* rx = raw + (i % SCAN_STAGES) * stage;
+      ScanBC<T, G, S, PAD> bc;
+      float2 x[IT], dt[IT], ds[IT], z[IT];
+      if (!spare) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          const T* p = rx + (pt + k * G::TSTEP) * CPB + pc;
+          x[k] = scan_pair(p);
+          dt[k] = scan_pair(p + G::RAW);
+          ds[k] = scan_pair(p + 2 * G::RAW);
+          if (P.z.p) z[k] = scan_pair(p + 3 * G::RAW);
+        }
+      }
+      bc.load(rx + 4 * G::RAW, npad, P, s, t0, tid);
+      if (!spare) {
+        const int at = ((i % 3) * TT + pt) * CPB + pc;
+        float4 du[IT];
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          const bool in = t0 + pt + k * G::TSTEP < P.T;
+          const float d0 = scan_d(P, dt[k].x + bias.x, in), d1 = scan_d(P, dt[k].y + bias.y, in);
+          du[k] = make_float4(d0, d0 * x[k].x, d1, d1 * x[k].y);
+          if (P.z.p) {  // z becomes dy silu'(z)
+            const float p0 = sigmoidf_(z[k].x), p1 = sigmoidf_(z[k].y);
+            const float s0 = ds[k].x * z[k].x * p0, s1 = ds[k].y * z[k].y * p1;
+            z[k] = make_float2(ds[k].x * (p0 * fmaf(z[k].x, 1.f - p0, 1.f)), ds[k].y * (p1 * fmaf(z[k].y, 1.f - p1, 1.f)));
+            ds[k] = make_float2(s0, s1);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          *reinterpret_cast<float4*>(DU + at + k * G::TSTEP * CPB) = du[k];
+          *reinterpret_cast<float2*>(DS + at + k * G::TSTEP * CPB) = ds[k];
+          if (P.z.p) *reinterpret_cast<float2*>(DZ + at + k * G::TSTEP * CPB) = z[k];
+        }
+      }
+      bc.store(Bs + q * TT * S * G::NP, Cs + q * TT * S * G::NP, tid);
+      marks.write(flags + q * 2 * TT, tid);
+      marks.read(P, s.b, t0 - TT, tid);
+    };
+    auto finish = [&](int i) {
+      const int tile = tiles - 1 - i, t0 = tile * TT, q = i & 1, at = ((i % 3) * TT + pt) * CPB + pc;
+      const T* rx = raw + (i % SCAN_STAGES) * stage;
+      if (!spare) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          const int t = pt + k * G::TSTEP;
+          const T* p = rx + t * CPB + pc;
+          const float2 x = scan_pair(p), dt = scan_pair(p + G::RAW);
+          const float4 du = *reinterpret_cast<const float4*>(DU + at + k * G::TSTEP * CPB);
+          const float2 ds = *reinterpret_cast<const float2*>(DS + at + k * G::TSTEP * CPB);
+          float2 dz = make_float2(0.f, 0.f);
+          if (P.z.p) dz = *reinterpret_cast<const float2*>(DZ + at + k * G::TSTEP * CPB);
+          const float* y0 = YP + q * 3 * TT * CPB * L + (t * CPB + pc) * L;
+          const float* y1 = y0 + TT * CPB * L;
+          const float* y2 = y1 + TT * CPB * L;
+          const float s0 = scan_join<L>(y0), s1 = scan_join<L>(y0 + L), g0 = scan_join<L>(y2), g1 = scan_join<L>(y2 + L);
+          float2 dd = make_float2(fmaf(scan_join<L>(y1), LN2, g0 * x.x), fmaf(scan_join<L>(y1 + L), LN2, g1 * x.y));
+          if (P.softplus) {
+            dd.x *= sigmoidf_(dt.x + bias.x);
+            dd.y *= sigmoidf_(dt.y + bias.y);
+          }
+          if (t0 + t < P.T) {
+            if (P.z.p)
+              scan_put_pair<T>(P.dz, P, s, t0 + t, pc,
+                               make_float2(dz.x * fmaf(skip.x, x.x, s0), dz.y * fmaf(skip.y, x.y, s1)));
+            scan_put_pair<T>(P.ddt, P, s, t0 + t, pc, dd);
+            scan_put_pair<T>(P.dx, P, s, t0 + t, pc,
+                             make_float2(fmaf(g0, du.x, ds.x * skip.x), fmaf(g1, du.z, ds.y * skip.y)));
+            sum_add(db.x, db_err.x, dd.x);
+            sum_add(db.y, db_err.y, dd.y);
+            sum_add(dD.x, dD_err.x, ds.x * x.x);
+            sum_add(dD.y, dD_err.y, ds.y * x.y);
+          }
+        }
+      }
+      // the tile's dB and dC over the warps, [TT][2][N]
+      float* part = P.bc_part + ((((long long)s.b * tiles + tile) * P.G + s.g) * P.blocks + s.blk) * (TT * 2 * N);
+      const float* sl = slots + q * SCAN_WARPS * TT * 2 * G::NP;
+#pragma unroll
+      for (int i0 = 0; i0 < TT * 2 * G::NP; i0 += G::TOKENS) {
+        const int j = i0 + tid;
+        if (TT * 2 * G::NP % G::TOKENS != 0 && j >= TT * 2 * G::NP) break;
+        const int n = j % G::NP;
+        float o = 0.f;
+#pragma unroll
+        for (int w = 0; w < SCAN_WARPS; ++w) o += sl[w * TT * 2 * G::NP + j];
+        if (!PAD || n < N) part[j / G::NP * N + n] = o;
+      }
+    };
+    f.fetch(P, s, views, raw, (tiles - 1) * TT, tid);
+    if (tiles > 1) f.fetch(P, s, views, raw + stage, (tiles - 2) * TT, tid);
+    cp_async_wait<0>();
+    asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");  // the first tiles have arrived, for the whole side
+    prepare(0);
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, (tiles - 3 - i) * TT, tid);
+      if (i + 1 < tiles) prepare(i + 1);
+      if (i > 0) finish(i - 1);
+      cp_async_wait<0>();
+      __syncthreads();
+    }
+    finish(tiles - 1);
+    // the row's dD and d dt_bias: over the side's threads of a channel pair
+    asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");
+    float4* sums = reinterpret_cast<float4*>(scan_sm);
+    sums[tid] = make_float4(dD.x, dD.y, db.x, db.y);
+    asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");
+    if (tid < G::PAIRS) {
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = tid; k < G::TOKENS; k += G::PAIRS) {
+        const float4 v = sums[k];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+      }
+      float* p = e + (long long)(s.c0 + pc) * (N + 2) + N;
+      if (pc < s.nc) { p[0] = o.x; p[1] = o.z; }
+      if (pc + 1 < s.nc) { p[N + 2] = o.y; p[N + 3] = o.w; }
+    }
+    return;
+  }
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int mb = lane >> (RB + LB), l = (lane >> RB) & (L - 1), ch = (mb << RB) | (lane & ((1 << RB) - 1));
+  constexpr int LEFT = S >> XB;  // states of which a lane ends up with the sums
+  const int m = mb * LEFT;       // register i of the lane is state n0 + (i ^ m)
+  const int c = warp * CH + ch, n0 = l * S;
+  const bool live = c < s.nc;
+  const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
+  unsigned ok = 0;  // states that exist
+#pragma unroll
+  for (int i = 0; i < S; ++i) ok |= (unsigned)(n0 + (i ^ m) < N) << i;
+  float hs[S];  // the next tile's checkpoint (left alone until then: the load is on its way)
+  auto checkpoint = [&](int tile) {
+    const float* p = P.ckpt + ((long long)s.b * tiles + tile) * P.E * N + chan;
+#pragma unroll
+    for (int i = 0; i < S; ++i) hs[i] = live && (!PAD || (ok >> i & 1)) ? __ldg(p + (i ^ m)) : 0.f;
+  };
+  checkpoint(tiles - 1);
+  Lane<S> a2 = Lane<S>::all(0.f), r = a2;
+  float dA[S], dA_err[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    dA[i] = dA_err[i] = 0.f;
+    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + (i ^ m)] * LOG2E);
+  }
+  __syncthreads();
+  for (int step = 0; step < tiles; ++step) {
+    const int q = step & 1, q3 = step % 3;
+    const float2* du_ = DU + q3 * TT * CPB + c;
+    const float* ds_ = DS + q3 * TT * CPB + c;
+    const float* b_ = Bs + q * TT * S * G::NP + m * G::NP + n0;
+    const float* c_ = Cs + q * TT * S * G::NP + m * G::NP + n0;
+    float* y_ = YP + q * 3 * TT * CPB * L + c * L + l;
+    float* s_ = slots + (q * SCAN_WARPS + warp) * TT * 2 * G::NP + n0;
+    const int* first = flags + q * 2 * TT;
+    const int* last = first + TT;
+    Lane<S> h_in;
+#pragma unroll
+    for (int i = 0; i < S; ++i) h_in.set(i, hs[i]);
+    if (step + 1 < tiles) checkpoint(tiles - 2 - step);
+
+    auto segment = [&](auto with_flags) {
+      constexpr bool FLAGS = decltype(with_flags)::value;
+      auto start = [&](int k) {  // the state in front of a sequence's first token
+        Lane<S> v = Lane<S>::all(0.f);
+        if (P.h0 && live) {
+#pragma unroll
+          for (int i = 0; i < S; ++i)
+            if (ok >> i & 1) v.set(i, __ldg(P.h0 + (long long)first[k] * P.E * N + chan + (i ^ m)));
+        }
+        return v;
+      };
+      // The later half of the tokens first: its states are kept, those of the half before it only
+      // passed through, and rebuilt for their own turn.  Half a segment fits the registers of two CTAs
+      // per SM.  Reads come in front of stores, which the compiler must assume to alias.
+      constexpr int HALF = SCAN_SEG / 2;
+      Lane<S> mid = h_in;
+#pragma unroll
+      for (int k = 0; k < HALF; ++k) {
+        if (FLAGS && first[k] >= 0) mid = start(k);
+        const float2 u = du_[k * CPB];
+        mid = lane_keep<PAD>(fma(lane_decay(a2, u.x), mid, Lane<S>::load(b_ + k * S * G::NP) * Lane<S>::all(u.y)),
+                             ok);
+      }
+      Lane<S> h[HALF], a[HALF], bv[HALF], cv[HALF], dAs = Lane<S>::all(0.f);
+      float2 du[HALF];
+      float dsv[HALF];
+#pragma unroll
+      for (int k = SCAN_SEG - 1; k >= 0; --k) {
+        const int j = k % HALF;
+        const Lane<S>& front = k >= HALF ? mid : h_in;  // the state in front of the half
+        if (j == HALF - 1) {
+#pragma unroll
+          for (int o = 0; o < HALF; ++o) {
+            const int t = k - HALF + 1 + o;
+            du[o] = du_[t * CPB];
+            dsv[o] = ds_[t * CPB];
+            bv[o] = Lane<S>::load(b_ + t * S * G::NP);
+            cv[o] = Lane<S>::load(c_ + t * S * G::NP);
+          }
+#pragma unroll
+          for (int o = 0; o < HALF; ++o) {
+            const int t = k - HALF + 1 + o;
+            Lane<S> before = o ? h[o ? o - 1 : 0] : front;
+            if (FLAGS && first[t] >= 0) before = start(t);
+            a[o] = lane_decay(a2, du[o].x);
+            h[o] = lane_keep<PAD>(fma(a[o], before, bv[o] * Lane<S>::all(du[o].y)), ok);
+          }
+        }
+        if (FLAGS && last[k] >= 0 && P.dht && live) {
+#pragma unroll
+          for (int i = 0; i < S; ++i)
+            if (ok >> i & 1) r.set(i, r.get(i) + __ldg(P.dht + (long long)last[k] * P.E * N + chan + (i ^ m)));
+        }
+        const Lane<S> ds = Lane<S>::all(dsv[j]);
+        const Lane<S> g = lane_keep<PAD>(fma(cv[j], ds, r), ok);
+        r = a[j] * g;
+        Lane<S> before = j ? h[j ? j - 1 : 0] : front;
+        if (FLAGS && first[k] >= 0) before = start(k);
+        const Lane<S> w = lane_keep<PAD>(r * before, ok);
+        dAs = fma(w, Lane<S>::all(du[j].x), dAs);
+        const float y = (h[j] * cv[j]).sum(), dd = (w * a2).sum(), gb = (g * bv[j]).sum();
+        Lane<S> vb = g * Lane<S>::all(du[j].y), vc = ds * h[j];  // dB, dC of this channel
+        if (FLAGS && first[k] >= 0) {  // what reaches the initial state; nothing passes the start
+          if (P.dh0 && live) {
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+              if (ok >> i & 1) P.dh0[(long long)first[k] * P.E * N + chan + (i ^ m)] = r.get(i);
+          }
+          r = Lane<S>::all(0.f);
+        }
+        y_[k * CPB * L] = y;
+        y_[(TT + k) * CPB * L] = dd;
+        y_[(2 * TT + k) * CPB * L] = gb;
+        // over the warp's channels: states i < half stay, the others go to the lane that keeps them
+        float v[2][S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+          v[0][i] = vb.get(i);
+          v[1][i] = vc.get(i);
+        }
+#pragma unroll
+        for (int x = 0; x < XB; ++x) {
+          const int half = S >> (x + 1);
+#pragma unroll
+          for (int i = 0; i < half; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+              v[b][i] += __shfl_xor_sync(0xffffffffu, v[b][i + half], (half / LEFT) << (RB + LB));
+        }
+        float* slot = s_ + k * 2 * G::NP;
+        if (RB > 0) {  // one of the other channel bits decides between dB and dC, the rest just add
+          const bool odd = lane & 1;
+#pragma unroll
+          for (int i = 0; i < LEFT; ++i) {
+            const float give = odd ? v[0][i] : v[1][i], keep = odd ? v[1][i] : v[0][i];
+            float o = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+#pragma unroll
+            for (int x = 1; x < RB; ++x) o += __shfl_xor_sync(0xffffffffu, o, 1 << x);
+            if ((lane & ((1 << RB) - 1)) <= 1) slot[(odd ? G::NP : 0) + (i ^ m)] = o;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < LEFT; ++i) {
+            slot[i ^ m] = v[0][i];
+            slot[G::NP + (i ^ m)] = v[1][i];
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S; ++i) sum_add(dA[i], dA_err[i], dAs.get(i));
+    };
+    if (scan_seg_flag(first, last)) segment(std::true_type{});
+    else segment(std::false_type{});
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    if (live && (ok >> i & 1)) e[(long long)(s.c0 + c) * (N + 2) + n0 + (i ^ m)] = dA[i];
+}
+
+// dB and dC: the channel blocks' partial sums of a tile ([TT][2][N]), summed in block
+// order.  One CTA column per (row, tile, group).
 constexpr int SCAN_BC_THREADS = 256;
-template <typename T, int LT>
+template <typename T>
 __global__ void __launch_bounds__(SCAN_BC_THREADS) ssm_scan_bc_kernel(const float* part, int T_, int tiles, int Gr,
                                                                       int blocks, int N, T* dB, T* dC) {
-  using G = ScanGeo<T, LT>;
-  const int per = 2 * N * G::TL;
+  const int per = SCAN_TT_BWD * 2 * N;
   const int i = blockIdx.y * SCAN_BC_THREADS + threadIdx.x;
   if (i >= per) return;
   const long long w = blockIdx.x;  // (row, tile, group)
@@ -745,14 +950,11 @@ __global__ void __launch_bounds__(SCAN_BC_THREADS) ssm_scan_bc_kernel(const floa
   float acc = 0.f;
 #pragma unroll 8
   for (int k = 0; k < blocks; ++k) acc += p[(long long)k * per];
-  const int half = i / (N * G::TL), rest = i - half * (N * G::TL), n = rest / G::TL, o = rest - n * G::TL;
-  const int t = ((o & (G::TL / 2 - 1)) >> 2) * 8 + (o / (G::TL / 2)) * 4 + (o & 3);  // inverse of bc_off
+  const int t = i / (2 * N), rest = i - t * 2 * N, half = rest >= N, n = rest - half * N;
   const int g = (int)(w % Gr);
   const long long bt = w / Gr;
-  const int tile = (int)(bt % tiles);
-  const long long b = bt / tiles;
-  const int tok = tile * G::TL + t;
-  if (tok < T_) (half ? dC : dB)[((b * T_ + tok) * Gr + g) * N + n] = io_from_f<T>(acc);
+  const int tok = (int)(bt % tiles) * SCAN_TT_BWD + t;
+  if (tok < T_) (half ? dC : dB)[(((bt / tiles) * T_ + tok) * Gr + g) * N + n] = io_from_f<T>(acc);
 }
 
 // One token for each of `rows` requests: the slot's state [E][N] is read, stepped

@@ -138,10 +138,14 @@ SCAN = [  # dtype, B, T, E, N, G, gate, skip, bias, state, softplus, documents
     (torch.float32, 1, 256, 17, 8, 1, True, True, True, True, True, None),
     (torch.float32, 1, 257, 34, 5, 2, False, True, True, True, True, None),
     (torch.float32, 1, 600, 16, 16, 1, True, True, True, True, True, None),
-    (torch.float32, 2, 64, 70, 24, 1, True, True, True, True, True, None),   # more than 16 states: 8 lanes on time
+    (torch.float32, 2, 64, 70, 24, 1, True, True, True, True, True, None),   # padded states: 24 of 32
     (torch.float32, 1, 65, 64, 64, 1, False, True, True, True, True, None),
     (torch.float32, 1, 130, 40, 33, 2, True, True, False, True, True, None),
-    (torch.float32, 2, 70, 450, 3, 150, True, True, True, True, True, None),  # many groups: 8 lanes on time
+    (torch.float32, 2, 70, 450, 3, 150, True, True, True, True, True, None),  # many groups: four states a lane
+    (torch.float32, 2, 70, 448, 16, 64, True, True, True, True, True, None),
+    (torch.float32, 2, 37, 480, 32, 60, False, True, True, True, True, None),
+    (torch.float32, 1, 75, 320, 7, 80, True, True, True, True, True, (1, 2, 0, 7, 8, 9, 1, 47)),
+    (torch.bfloat16, 2, 61, 640, 16, 80, True, True, True, True, True, None),
     (torch.bfloat16, 2, 130, 32, 16, 1, True, True, True, True, True, None),
     (torch.bfloat16, 1, 300, 48, 16, 2, True, True, True, False, True, None),
     (torch.bfloat16, 1, 100, 64, 32, 1, True, True, True, True, True, None),
@@ -149,7 +153,7 @@ SCAN = [  # dtype, B, T, E, N, G, gate, skip, bias, state, softplus, documents
     (torch.float32, 1, 60, 18, 16, 1, True, True, True, True, True, (1, 2, 0, 7, 8, 9, 1, 32, 0)),
     (torch.float32, 1, 530, 16, 16, 1, True, True, True, True, True, (255, 1, 1, 200, 73)),
     (torch.float32, 1, 530, 16, 16, 1, False, False, True, False, True, (256, 0, 256, 18)),
-    (torch.float32, 1, 140, 66, 20, 1, True, True, True, True, True, (63, 1, 64, 0, 12)),  # 8 lanes, packed
+    (torch.float32, 1, 140, 66, 20, 1, True, True, True, True, True, (63, 1, 64, 0, 12)),
     (torch.bfloat16, 1, 290, 40, 16, 1, True, True, True, False, True, (0, 3, 100, 187)),
 ]
 
@@ -196,6 +200,15 @@ def test_scan_without_softplus_takes_positive_steps():
     close("final_state", ht, rht, torch.float32)
     for k in want:
         close("d_" + k, grads[k], want[k], torch.float32)
+
+
+@gpu
+def test_a_step_of_zero_leaves_the_state():
+    ts, _, _ = scan_tensors(torch.float32, 1, 40, 8, 16, 1, False, False, False, True, None)
+    zero = torch.zeros(1, 40, 8, device="cuda")
+    _, ht = sophia_b200.selective_scan(ts["x"].detach(), zero, ts["A"].detach(), ts["B"].detach(), ts["C"].detach(),
+                                       dt_softplus=False, initial_state=ts["h0"].detach(), output_final_state=True)
+    assert torch.equal(ht, ts["h0"].detach())
 
 
 @gpu
