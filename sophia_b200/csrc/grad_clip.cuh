@@ -6,10 +6,11 @@
 // scaling, which writes the output; a sum below the L2's size finds its second
 // read there, so the scaling walks the chunks backwards.  The tensors' addresses travel
 // as a kernel parameter (no copy, no host wait); each launch takes up to
-// GRAD_MAX_TENSORS of them.  A CTA strides over chunks of GRAD_CHUNK elements,
-// finding a chunk's tensor by a binary search of the chunk prefix.  Squares
+// GRAD_MAX_TENSORS of them.  A CTA takes a run of chunks of GRAD_CHUNK elements.  Squares
 // are summed in fp32 over at most GRAD_CHUNK / GRAD_THREADS elements of a thread
 // and in fp64 from there on, in an order that depends on the sizes alone.
+// Measured, 455 M elements of bf16 in 336 tensors to fp32: norm 152 us (6.0 TB/s), scaling
+// 487 us (5.6 TB/s); chunks of 4096 elements 178 and 479 us, of 8192 157 and 486 us.
 #pragma once
 
 #include "ssm_common.cuh"
@@ -17,7 +18,7 @@
 namespace kda {
 
 constexpr int GRAD_THREADS = 256;
-constexpr int GRAD_CHUNK = 8192;
+constexpr int GRAD_CHUNK = 16384;
 constexpr int GRAD_MAX_TENSORS = 1024;  // 30 KB of kernel parameters
 constexpr int GRAD_FEW_TENSORS = 64;    // the smaller table: 2 KB
 
@@ -31,32 +32,48 @@ struct GradTable {
   int n;
 };
 
+// The chunks of a CTA: a run of neighbours, so that the tensor of the next one is found by
+// walking on from the last (its table entry stays in registers meanwhile).
 template <int M>
-__device__ __forceinline__ int grad_find(const GradTable<M>& tab, int chunk) {
-  int lo = 0, hi = tab.n;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (tab.chunk0[mid] <= chunk) lo = mid; else hi = mid;
+struct GradWalk {
+  int first, end;  // chunks of this CTA
+  int i;           // tensor of the current chunk
+  __device__ __forceinline__ explicit GradWalk(const GradTable<M>& tab) {
+    const int chunks = tab.chunk0[tab.n], per = (chunks + gridDim.x - 1) / gridDim.x;
+    first = min((int)blockIdx.x * per, chunks);
+    end = min(first + per, chunks);
+    int lo = 0, hi = tab.n;
+    while (hi - lo > 1) {  // the last tensor that starts at or before the first chunk
+      const int mid = (lo + hi) >> 1;
+      if (tab.chunk0[mid] <= first) lo = mid; else hi = mid;
+    }
+    i = lo;
   }
-  return lo;
-}
+  __device__ __forceinline__ void to(const GradTable<M>& tab, int chunk) {
+    while (tab.chunk0[i + 1] <= chunk) ++i;
+    while (tab.chunk0[i] > chunk) --i;
+  }
+};
 
 // 16-byte vectors of T per thread and step when the address allows, else elements.
 template <typename T>
 __device__ __forceinline__ float grad_sumsq(const T* p, int n) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), U = 4;
   float acc = 0.f;
   if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
     const int nv = n / V;
     int i = threadIdx.x;
-    for (; i + 3 * GRAD_THREADS < nv; i += 4 * GRAD_THREADS) {
-      float f[4][V];
+    for (; i + (U - 1) * GRAD_THREADS < nv; i += U * GRAD_THREADS) {
+      IoVec<T, V> r[U];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) io_load<T, V>(p + (long long)(i + u * GRAD_THREADS) * V, f[u]);
+      for (int u = 0; u < U; ++u) r[u] = reinterpret_cast<const IoVec<T, V>*>(p)[i + u * GRAD_THREADS];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc = fmaf(f[u][k], f[u][k], acc);
+        for (int k = 0; k < V; ++k) {
+          const float f = io_to_f(r[u].v[k]);
+          acc = fmaf(f, f, acc);
+        }
     }
     for (; i < nv; i += GRAD_THREADS) {
       float f[V];
@@ -94,10 +111,11 @@ __device__ __forceinline__ double grad_block_sum(double v) {
 template <int M>
 __global__ void __launch_bounds__(GRAD_THREADS) grad_norm_kernel(const __grid_constant__ GradTable<M> tab,
                                                                  double* partial) {
-  const int chunks = tab.chunk0[tab.n];
+  GradWalk<M> walk(tab);
   double acc = 0;
-  for (int ch = blockIdx.x; ch < chunks; ch += gridDim.x) {
-    const int i = grad_find(tab, ch);
+  for (int ch = walk.first; ch < walk.end; ++ch) {
+    walk.to(tab, ch);
+    const int i = walk.i;
     const long long at = (long long)(ch - tab.chunk0[i]) * GRAD_CHUNK;
     const int n = (int)min((long long)GRAD_CHUNK, tab.numel[i] - at);
     float s;
@@ -110,17 +128,32 @@ __global__ void __launch_bounds__(GRAD_THREADS) grad_norm_kernel(const __grid_co
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
+// Pieces that take 16 bytes on the wider side, four in flight per thread, when both addresses
+// allow.
 template <typename TI, typename TO>
 __device__ __forceinline__ void grad_scale(const TI* p, TO* q, int n, float coef) {
-  constexpr int V = 16 / sizeof(TI);
-  if (((reinterpret_cast<uintptr_t>(p) & 15) | (reinterpret_cast<uintptr_t>(q) & (V * sizeof(TO) - 1))) == 0) {
+  constexpr int V = 16 / (sizeof(TI) > sizeof(TO) ? sizeof(TI) : sizeof(TO)), U = 4;
+  if (((reinterpret_cast<uintptr_t>(p) & (V * sizeof(TI) - 1)) | (reinterpret_cast<uintptr_t>(q) & (V * sizeof(TO) - 1))) ==
+      0) {
     const int nv = n / V;
-    for (int i = threadIdx.x; i < nv; i += GRAD_THREADS) {
+    int i = threadIdx.x;
+    for (; i + (U - 1) * GRAD_THREADS < nv; i += U * GRAD_THREADS) {
+      float f[U][V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) io_load<TI, V>(p + (i + u * GRAD_THREADS) * V, f[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) f[u][k] *= coef;
+        io_store<TO, V>(q + (i + u * GRAD_THREADS) * V, f[u]);
+      }
+    }
+    for (; i < nv; i += GRAD_THREADS) {
       float f[V];
-      io_load<TI, V>(p + (long long)i * V, f);
+      io_load<TI, V>(p + i * V, f);
 #pragma unroll
       for (int k = 0; k < V; ++k) f[k] *= coef;
-      io_store<TO, V>(q + (long long)i * V, f);
+      io_store<TO, V>(q + i * V, f);
     }
     for (int k = nv * V + threadIdx.x; k < n; k += GRAD_THREADS) q[k] = io_from_f<TO>(io_to_f(p[k]) * coef);
   } else {
@@ -162,9 +195,10 @@ __global__ void __launch_bounds__(GRAD_THREADS) grad_scale_kernel(const __grid_c
   }
   __syncthreads();
   const float coef = s_coef;
-  const int chunks = tab.chunk0[tab.n];
-  for (int ch = chunks - 1 - (int)blockIdx.x; ch >= 0; ch -= gridDim.x) {
-    const int i = grad_find(tab, ch);
+  GradWalk<M> walk(tab);
+  for (int ch = walk.end - 1; ch >= walk.first; --ch) {
+    walk.to(tab, ch);
+    const int i = walk.i;
     if (coef == 1.f && tab.in[i] == tab.out[i]) continue;  // a product by one, in place
     const long long at = (long long)(ch - tab.chunk0[i]) * GRAD_CHUNK;
     const int n = (int)min((long long)GRAD_CHUNK, tab.numel[i] - at);

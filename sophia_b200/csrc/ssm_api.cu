@@ -225,7 +225,7 @@ int scan_step(const ScanStepParams& p, cudaStream_t st) {
 
 // ---- gradient clipping
 
-int grad_ctas() { return 8 * sm_count(); }
+int grad_ctas() { return 16 * sm_count(); }
 
 template <int M>
 int grad_table(GradTable<M>& t, const kda_b200_grad_args* a, long long first, int n) {
