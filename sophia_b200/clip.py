@@ -16,23 +16,28 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import GradArgs
-from .ssm import _IO, _on, _stream
+from .ssm import _IO, _call
 
 __all__ = ["grad_norm", "clip_grad_norm_"]
 
 
-def _list(what: str, grads) -> list[Tensor]:
+def _list(what: str, grads) -> tuple[list[Tensor], torch.device | None, bytes]:
+    """The tensors, their one device and their types."""
     ts = [grads] if isinstance(grads, Tensor) else list(grads)
     for t in ts:
         if not isinstance(t, Tensor):
             raise ValueError(f"{what} takes gradient tensors, got {type(t).__name__}")
-        if t.dtype not in _IO:
-            raise NotImplementedError(f"{what}: gradients must be float32, bfloat16 or float16, got {t.dtype}")
-        if not t.is_cuda:
-            raise RuntimeError(f"{what} runs on the CUDA kernels only: gradients must be CUDA tensors")
-    if len({t.device for t in ts}) > 1:
+    try:
+        types = bytes([_IO[t.dtype] for t in ts])
+    except KeyError as e:
+        raise NotImplementedError(f"{what}: gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
+    devices = {t.device for t in ts}
+    if len(devices) > 1:
         raise RuntimeError(f"{what}: gradients are on several devices")
-    return ts
+    device = devices.pop() if devices else None
+    if device is not None and device.type != "cuda":
+        raise RuntimeError(f"{what} runs on the CUDA kernels only: gradients must be CUDA tensors")
+    return ts, device, types
 
 
 def _dense(t: Tensor) -> bool:
@@ -47,23 +52,16 @@ def _dense(t: Tensor) -> bool:
     return True
 
 
-def _addresses(ts: Sequence[Tensor]) -> array:
-    return array("Q", [t.data_ptr() for t in ts])
-
-
-def _types(ts: Sequence[Tensor]) -> bytes:
-    return bytes([_IO[t.dtype] for t in ts])
-
-
-def _call(ts: list[Tensor], out: list[Tensor] | None, max_norm: float, eps: float) -> Tensor:
-    norm = torch.empty((), device=ts[0].device, dtype=torch.float32)
+def _launch(ts: list[Tensor], types: bytes, out: list[Tensor] | None, out_types: bytes | None, max_norm: float,
+            eps: float) -> Tensor:
+    norm = ts[0].new_empty((), dtype=torch.float32)
     lib = _lib.load()
-    ws = torch.empty(lib.kda_b200_grad_workspace_bytes(len(ts)), device=ts[0].device, dtype=torch.uint8)
-    src, numel, tin = _addresses(ts), array("q", [t.numel() for t in ts]), _types(ts)
-    dst, tout = (None, None) if out is None else (_addresses(out), _types(out))
+    ws = norm.new_empty(lib.kda_b200_grad_workspace_bytes(len(ts)), dtype=torch.uint8)
+    src, numel = array("Q", map(Tensor.data_ptr, ts)), array("q", map(Tensor.numel, ts))
+    dst = None if out is None else src if out is ts else array("Q", map(Tensor.data_ptr, out))
     addr = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
-    args = GradArgs(len(ts), addr(src), addr(dst), addr(numel), tin, tout, max_norm, eps, norm.data_ptr())
-    _lib.check(lib.kda_b200_grad_clip(args, ws.data_ptr(), ws.numel(), _stream()))
+    args = GradArgs(len(ts), addr(src), addr(dst), addr(numel), types, out_types, max_norm, eps, norm.data_ptr())
+    _call(lib.kda_b200_grad_clip, norm.device, args, ws.data_ptr(), ws.numel())
     return norm
 
 
@@ -73,11 +71,10 @@ def grad_norm(grads: Tensor | Iterable[Tensor]) -> Tensor:
     current device.  No host wait.  The result does not depend on timing: sums have a
     fixed order."""
     with torch.no_grad():
-        ts = _list("grad_norm", grads)
+        ts, _, types = _list("grad_norm", grads)
         if not ts:
             return torch.zeros((), device="cuda", dtype=torch.float32)
-        with _on(ts[0]):
-            return _call([t if _dense(t) else t.contiguous() for t in ts], None, 0.0, 0.0)
+        return _launch([t if _dense(t) else t.contiguous() for t in ts], types, None, None, 0.0, 0.0)
 
 
 def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: float = 1e-6,
@@ -94,20 +91,23 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
     if math.isnan(max_norm) or max_norm < 0 or not eps >= 0:
         raise ValueError(f"{what}: max_norm and eps must be >= 0, got {max_norm} and {eps}")
     with torch.no_grad():
-        ts = _list(what, grads)
-        outs = ts if out is None else _list(what, out)
+        ts, device, types = _list(what, grads)
+        outs, out_device, out_types = (ts, device, types) if out is None else _list(what, out)
         if len(outs) != len(ts):
             raise ValueError(f"{what}: {len(ts)} gradients but {len(outs)} outputs")
         if not ts:
             return torch.zeros((), device="cuda", dtype=torch.float32)
-        for g, o in zip(ts, outs):
-            if g.shape != o.shape:
-                raise ValueError(f"{what}: an output of shape {list(o.shape)} for a gradient of {list(g.shape)}")
-        if outs[0].device != ts[0].device:
-            raise RuntimeError(f"{what}: gradients and outputs are on different devices")
+        if outs is not ts:
+            for g, o in zip(ts, outs):
+                if g.shape != o.shape:
+                    raise ValueError(f"{what}: an output of shape {list(o.shape)} for a gradient of {list(g.shape)}")
+            if out_device != device:
+                raise RuntimeError(f"{what}: gradients and outputs are on different devices")
         where = [o.data_ptr() for o in outs if o.numel()]
         if len(set(where)) != len(where):
             raise ValueError(f"{what}: one tensor is named twice")
+        if all(map(Tensor.is_contiguous, ts)) and (outs is ts or all(map(Tensor.is_contiguous, outs))):
+            return _launch(ts, types, outs, out_types, max_norm, eps)
         src, dst, back = list(ts), list(outs), []
         for i, (g, o) in enumerate(zip(ts, outs)):
             if g.is_contiguous() and o.is_contiguous():
@@ -118,8 +118,7 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
             if not o.is_contiguous():
                 dst[i] = torch.empty(o.shape, device=o.device, dtype=o.dtype)
                 back.append(i)
-        with _on(ts[0]):
-            norm = _call(src, dst, max_norm, eps)
+        norm = _launch(src, types, dst, out_types, max_norm, eps)
         for i in back:
             outs[i].copy_(dst[i])
         return norm

@@ -85,6 +85,8 @@ int check_conv(const void* x, const float* w, long long B, long long T, int C, i
   return KDA_OK;
 }
 
+constexpr int CONV_V = 2;  // channels per thread
+
 // Tokens per thread: long runs read the halo of three tokens less often, short ones
 // make enough threads for narrow or short problems.
 int conv_run(long long B, long long T, long long lanes) {
@@ -111,12 +113,10 @@ int launch_conv_fwd(ConvParams& p, cudaStream_t st) {
 
 template <typename T>
 int conv_fwd(ConvParams& p, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  const bool vec = p.C % V == 0 && aligned(p.y, 16) && vec_rows(p.x.p, p.x.sb, p.x.st, p.B, p.T, V, sizeof(T));
+  constexpr int V = CONV_V;
+  const bool vec = p.C % V == 0 && aligned(p.y, V * sizeof(T)) && vec_rows(p.x.p, p.x.sb, p.x.st, p.B, p.T, V, sizeof(T));
   return vec ? launch_conv_fwd<T, V>(p, st) : launch_conv_fwd<T, 1>(p, st);
 }
-
-constexpr int CONV_BWD_V = 4;
 
 template <typename T, int V>
 int launch_conv_bwd(ConvParams& p, float* dw, float* dbias, cudaStream_t st) {
@@ -133,11 +133,11 @@ int launch_conv_bwd(ConvParams& p, float* dw, float* dbias, cudaStream_t st) {
   return launch_check("short conv backward");
 }
 
-int conv_bwd_run(long long B, long long T, int C) { return conv_run(B, T, (C + CONV_BWD_V - 1) / CONV_BWD_V); }
+int conv_bwd_run(long long B, long long T, int C) { return conv_run(B, T, (C + CONV_V - 1) / CONV_V); }
 
 template <typename T>
 int conv_bwd(ConvParams& p, float* dw, float* dbias, cudaStream_t st) {
-  constexpr int V = CONV_BWD_V;
+  constexpr int V = CONV_V;
   const bool vec = p.C % V == 0 && aligned(p.dx, V * sizeof(T)) &&
                    vec_rows(p.x.p, p.x.sb, p.x.st, p.B, p.T, V, sizeof(T)) &&
                    vec_rows(p.dy.p, p.dy.sb, p.dy.st, p.B, p.T, V, sizeof(T));

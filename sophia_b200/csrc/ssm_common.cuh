@@ -40,6 +40,140 @@ __device__ __forceinline__ void io_store(T* p, const float (&f)[V]) {
   *reinterpret_cast<IoVec<T, V>*>(p) = r;
 }
 
+// S values of one kind that a thread owns, pairs in packed fp32 arithmetic.
+typedef unsigned long long u64;
+__device__ __forceinline__ u64 pk2(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 upk2(u64 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+template <int S>
+struct Lane {
+  static_assert(S % 2 == 0, "pairs");
+  u64 p[S / 2];
+  __device__ __forceinline__ float get(int i) const { return i & 1 ? upk2(p[i / 2]).y : upk2(p[i / 2]).x; }
+  __device__ __forceinline__ void set(int i, float v) {
+    const float2 o = upk2(p[i / 2]);
+    p[i / 2] = i & 1 ? pk2(o.x, v) : pk2(v, o.y);
+  }
+  __device__ __forceinline__ static Lane load(const float* q) {  // S * 4 bytes, aligned
+    Lane r;
+    if (S % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < S / 4; ++k) {
+        const ulonglong2 v = reinterpret_cast<const ulonglong2*>(q)[k];
+        r.p[2 * k] = v.x;
+        r.p[2 * k + 1] = v.y;
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < S / 2; ++k) r.p[k] = reinterpret_cast<const u64*>(q)[k];
+    }
+    return r;
+  }
+  __device__ __forceinline__ void store(float* q) const {
+    if (S % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < S / 4; ++k) reinterpret_cast<ulonglong2*>(q)[k] = make_ulonglong2(p[2 * k], p[2 * k + 1]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < S / 2; ++k) reinterpret_cast<u64*>(q)[k] = p[k];
+    }
+  }
+  __device__ __forceinline__ static Lane all(float v) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = pk2(v, v);
+    return r;
+  }
+  __device__ __forceinline__ float sum() const {
+    u64 t = p[0];
+#pragma unroll
+    for (int k = 1; k < S / 2; ++k) t = add2(t, p[k]);
+    const float2 f = upk2(t);
+    return f.x + f.y;
+  }
+  __device__ __forceinline__ Lane exp2() const {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) {
+      const float2 f = upk2(p[k]);
+      r.p[k] = pk2(ex2(f.x), ex2(f.y));
+    }
+    return r;
+  }
+  friend __device__ __forceinline__ Lane operator*(const Lane& a, const Lane& b) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = mul2(a.p[k], b.p[k]);
+    return r;
+  }
+  friend __device__ __forceinline__ Lane operator+(const Lane& a, const Lane& b) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = add2(a.p[k], b.p[k]);
+    return r;
+  }
+  friend __device__ __forceinline__ Lane fma(const Lane& a, const Lane& b, const Lane& c) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = fma2(a.p[k], b.p[k], c.p[k]);
+    return r;
+  }
+};
+template <>
+struct Lane<1> {
+  float f;
+  __device__ __forceinline__ float get(int) const { return f; }
+  __device__ __forceinline__ void set(int, float v) { f = v; }
+  __device__ __forceinline__ static Lane all(float v) { return {v}; }
+  __device__ __forceinline__ Lane exp2() const { return {ex2(f)}; }
+  friend __device__ __forceinline__ Lane operator*(const Lane& a, const Lane& b) { return {a.f * b.f}; }
+  friend __device__ __forceinline__ Lane operator+(const Lane& a, const Lane& b) { return {a.f + b.f}; }
+  friend __device__ __forceinline__ Lane fma(const Lane& a, const Lane& b, const Lane& c) { return {fmaf(a.f, b.f, c.f)}; }
+};
+template <int S>
+__device__ __forceinline__ Lane<S> lane_sigmoid(const Lane<S>& v) {
+  Lane<S> d = (v * Lane<S>::all(-LOG2E)).exp2() + Lane<S>::all(1.f);
+#pragma unroll
+  for (int i = 0; i < S; ++i) d.set(i, rcp(d.get(i)));
+  return d;
+}
+template <typename T, int S>
+__device__ __forceinline__ Lane<S> lane_from(const IoVec<T, S>& v) {
+  Lane<S> r = Lane<S>::all(0.f);
+#pragma unroll
+  for (int i = 0; i < S; ++i) r.set(i, io_to_f(v.v[i]));
+  return r;
+}
+template <typename T, int S>
+__device__ __forceinline__ void lane_store(T* p, const Lane<S>& v) {
+  float f[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) f[i] = v.get(i);
+  io_store<T, S>(p, f);
+}
+
 // A strided activation: element (b, t, c) at p + b*sb + t*st + c.
 struct RowView {
   const void* p;
@@ -95,6 +229,7 @@ __device__ __forceinline__ int step_slot(const int* slots, int r, int pool, int*
 }
 
 constexpr int SEQ_MAP_THREADS = 256;
+constexpr int SEQ_MAP_TABLE = 4096;
 
 struct SeqMapParams {
   const int* cu;  // [nseq + 1]
@@ -112,17 +247,24 @@ struct SeqMapParams {
 // that does not start at 0, decreases or does not end at T sets the device
 // error 3; the maps still hold only valid sequence numbers.
 static __global__ void __launch_bounds__(SEQ_MAP_THREADS) ssm_seq_map_kernel(SeqMapParams P) {
+  __shared__ int table[SEQ_MAP_TABLE];
   const int tok_blocks = (P.T + SEQ_MAP_THREADS - 1) / SEQ_MAP_THREADS;
   if ((int)blockIdx.x < tok_blocks) {
     const int t = blockIdx.x * SEQ_MAP_THREADS + threadIdx.x;
+    const int* cu = P.cu;
+    if (P.nseq < SEQ_MAP_TABLE) {  // one read of global memory in a row, not one per halving
+      for (int i = threadIdx.x; i <= P.nseq; i += SEQ_MAP_THREADS) table[i] = __ldg(P.cu + i);
+      __syncthreads();
+      cu = table;
+    }
     if (t >= P.T) return;
     int lo = 0, hi = P.nseq;  // the answer is in [lo, hi)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (__ldg(P.cu + mid) <= t) lo = mid; else hi = mid;
+      if (cu[mid] <= t) lo = mid; else hi = mid;
     }
-    P.start[t] = __ldg(P.cu + lo) == t ? lo : -1;
-    P.end[t] = __ldg(P.cu + lo + 1) == t + 1 ? lo : -1;
+    P.start[t] = cu[lo] == t ? lo : -1;
+    P.end[t] = cu[lo + 1] == t + 1 ? lo : -1;
     return;
   }
   const int first = (int)blockIdx.x - tok_blocks, step = (int)gridDim.x - tok_blocks;
@@ -148,6 +290,7 @@ static __global__ void __launch_bounds__(SSM_REDUCE_COLS * SSM_REDUCE_SLICES)
   const long long k = (long long)blockIdx.x * SSM_REDUCE_COLS + c;
   float acc = 0.f;
   if (k < cols)
+#pragma unroll 8
     for (long long b = sl; b < parts; b += SSM_REDUCE_SLICES) acc += partial[b * cols + k];
   part[sl][c] = acc;
   __syncthreads();

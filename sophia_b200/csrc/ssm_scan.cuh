@@ -98,101 +98,6 @@ __device__ __forceinline__ ScanBlock scan_block(const ScanParams& P) {
   return s;
 }
 
-// A lane's S values of one kind, pairs in packed fp32 arithmetic.
-typedef unsigned long long u64;
-__device__ __forceinline__ u64 pk2(float lo, float hi) {
-  u64 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 upk2(u64 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
-  u64 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-  u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-  u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-template <int S>
-struct Lane {
-  static_assert(S % 2 == 0, "pairs");
-  u64 p[S / 2];
-  __device__ __forceinline__ float get(int i) const { return i & 1 ? upk2(p[i / 2]).y : upk2(p[i / 2]).x; }
-  __device__ __forceinline__ void set(int i, float v) {
-    const float2 o = upk2(p[i / 2]);
-    p[i / 2] = i & 1 ? pk2(o.x, v) : pk2(v, o.y);
-  }
-  __device__ __forceinline__ static Lane load(const float* q) {  // S * 4 bytes, aligned
-    Lane r;
-    if (S % 4 == 0) {
-#pragma unroll
-      for (int k = 0; k < S / 4; ++k) {
-        const ulonglong2 v = reinterpret_cast<const ulonglong2*>(q)[k];
-        r.p[2 * k] = v.x;
-        r.p[2 * k + 1] = v.y;
-      }
-    } else {
-#pragma unroll
-      for (int k = 0; k < S / 2; ++k) r.p[k] = reinterpret_cast<const u64*>(q)[k];
-    }
-    return r;
-  }
-  __device__ __forceinline__ void store(float* q) const {
-    if (S % 4 == 0) {
-#pragma unroll
-      for (int k = 0; k < S / 4; ++k) reinterpret_cast<ulonglong2*>(q)[k] = make_ulonglong2(p[2 * k], p[2 * k + 1]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < S / 2; ++k) reinterpret_cast<u64*>(q)[k] = p[k];
-    }
-  }
-  __device__ __forceinline__ static Lane all(float v) {
-    Lane r;
-#pragma unroll
-    for (int k = 0; k < S / 2; ++k) r.p[k] = pk2(v, v);
-    return r;
-  }
-  __device__ __forceinline__ float sum() const {
-    u64 t = p[0];
-#pragma unroll
-    for (int k = 1; k < S / 2; ++k) t = add2(t, p[k]);
-    const float2 f = upk2(t);
-    return f.x + f.y;
-  }
-  __device__ __forceinline__ Lane exp2() const {
-    Lane r;
-#pragma unroll
-    for (int k = 0; k < S / 2; ++k) {
-      const float2 f = upk2(p[k]);
-      r.p[k] = pk2(ex2(f.x), ex2(f.y));
-    }
-    return r;
-  }
-  friend __device__ __forceinline__ Lane operator*(const Lane& a, const Lane& b) {
-    Lane r;
-#pragma unroll
-    for (int k = 0; k < S / 2; ++k) r.p[k] = mul2(a.p[k], b.p[k]);
-    return r;
-  }
-  friend __device__ __forceinline__ Lane fma(const Lane& a, const Lane& b, const Lane& c) {
-    Lane r;
-#pragma unroll
-    for (int k = 0; k < S / 2; ++k) r.p[k] = fma2(a.p[k], b.p[k], c.p[k]);
-    return r;
-  }
-};
 // The decays 2^(d a2).  ex2.approx is low by 0.5e-8 to 2.9e-8 on average where decays are close
 // to 1 (measured: 0.5e-8 for exponents of -3e-4 to -3e-3, 2.4e-8 for -0.005 to -0.08, 1.8e-8 for
 // -0.08 to -0.3), which adds up over the tokens that a state remembers.  An exponent

@@ -16,7 +16,6 @@ mixed types are promoted.  Arithmetic, parameters and states are float32.
 
 from __future__ import annotations
 
-import contextlib
 from typing import Optional
 
 import torch
@@ -33,30 +32,35 @@ MAX_TAPS = 4
 
 
 def _ptr(t: Tensor | None) -> int | None:
-    return None if t is None or t.numel() == 0 else t.data_ptr()
+    return None if t is None else t.data_ptr()  # 0 (NULL) where there is nothing
 
 
-def _on(t: Tensor):
-    """Kernels launch on the tensors' device; (stream handle, guard)."""
-    return torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else contextlib.nullcontext()
-
-
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+def _call(fn, device: torch.device, *args) -> None:
+    """A library call on the current stream of the tensors' device."""
+    if device.index == torch.cuda.current_device():
+        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def _rows(t: Tensor, dtype: torch.dtype) -> Tensor:
     """An activation as the kernels read it: its type, and a contiguous last dimension."""
-    t = t if t.dtype == dtype else t.to(dtype)
+    if t.dtype != dtype:
+        t = t.to(dtype)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _param(t: Tensor | None) -> Tensor | None:
-    return None if t is None else t.float().contiguous()
+    if t is None or (t.dtype == torch.float32 and t.is_contiguous()):
+        return t
+    return t.float().contiguous()
 
 
 def _cu(cu_seqlens: Tensor | None) -> Tensor | None:
-    return None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
+    if cu_seqlens is None or (cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous()):
+        return cu_seqlens
+    return cu_seqlens.to(torch.int32).contiguous()
 
 
 def _needs_grad(*tensors) -> bool:
@@ -65,18 +69,19 @@ def _needs_grad(*tensors) -> bool:
 
 def _check_activations(what: str, **tensors) -> torch.dtype:
     """All on one CUDA device and of supported types; returns the promoted type."""
-    dtype, device = None, None
+    first = tensors["x"]
+    dtype, device = first.dtype, first.device
+    if device.type != "cuda" and device.type != "meta":
+        raise RuntimeError(f"{what} runs on the CUDA kernels only: its tensors must be CUDA tensors")
     for name, t in tensors.items():
         if t is None:
             continue
         if t.dtype not in _IO:
             raise NotImplementedError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-        dtype = t.dtype if dtype is None or dtype == t.dtype else torch.promote_types(dtype, t.dtype)
-        if t.device.type not in ("cuda", "meta"):
-            raise RuntimeError(f"{what} runs on the CUDA kernels only: {name} must be a CUDA tensor")
-        if device is not None and t.device != device:
+        if t.dtype != dtype:
+            dtype = torch.promote_types(dtype, t.dtype)
+        if t.device != device:
             raise RuntimeError(f"{what}: tensors are on {device} and {t.device}")
-        device = t.device
     return dtype
 
 
@@ -138,44 +143,39 @@ def _conv_fwd_impl(x, weight, bias, h0, cu_seqlens, silu, want_final):
     B, T, C = x.shape
     W = weight.shape[1]
     N = B if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    with torch.autocast("cuda", enabled=False), _on(x):
-        lib = _lib.load()
-        xr = _rows(x, x.dtype)
-        w, b, h, cu = _param(weight), _param(bias), _param(h0), _cu(cu_seqlens)
-        y = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
-        ht = torch.empty((N, C, W - 1) if want_final else (0,), device=x.device, dtype=torch.float32)
-        ws = torch.empty(lib.kda_b200_short_conv_workspace_bytes(B, T, C, W, int(cu is not None), 0), device=x.device,
-                         dtype=torch.uint8)
-        if B:
-            _lib.check(lib.kda_b200_short_conv_fwd(
-                _ptr(xr), xr.stride(0), xr.stride(1), _ptr(w), _ptr(b), _ptr(h), _ptr(cu), B, T, C, W, N, _IO[x.dtype],
-                int(silu), _ptr(y), _ptr(ht), _ptr(ws), ws.numel(), _stream()))
-        return y, ht
+    lib = _lib.load()
+    xr = _rows(x, x.dtype)
+    w, b, h, cu = _param(weight), _param(bias), _param(h0), _cu(cu_seqlens)
+    y = x.new_empty((B, T, C))
+    ht = x.new_empty((N, C, W - 1) if want_final else 0, dtype=torch.float32)
+    ws = x.new_empty(lib.kda_b200_short_conv_workspace_bytes(B, T, C, W, int(cu is not None), 0), dtype=torch.uint8)
+    if B:
+        _call(lib.kda_b200_short_conv_fwd, x.device,
+              _ptr(xr), xr.stride(0), xr.stride(1), _ptr(w), _ptr(b), _ptr(h), _ptr(cu), B, T, C, W, N, _IO[x.dtype],
+              int(silu), _ptr(y), _ptr(ht), _ptr(ws), ws.numel())
+    return y, ht
 
 
 def _conv_bwd_impl(x, weight, bias, h0, cu_seqlens, dy, dht, silu, want_dh0):
     B, T, C = x.shape
     W = weight.shape[1]
     N = B if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    with torch.autocast("cuda", enabled=False), _on(x):
-        lib = _lib.load()
-        xr, dyr = _rows(x, x.dtype), _rows(dy, x.dtype)
-        w, b, h, cu, dh = _param(weight), _param(bias), _param(h0), _cu(cu_seqlens), _param(dht)
-        f32 = dict(device=x.device, dtype=torch.float32)
-        dx = torch.empty(B, T, C, device=x.device, dtype=x.dtype)
-        dw = torch.empty(C, W, **f32)
-        db = torch.empty((C,) if bias is not None else (0,), **f32)
-        dh0 = torch.empty((N, C, W - 1) if want_dh0 else (0,), **f32)
-        ws = torch.empty(lib.kda_b200_short_conv_workspace_bytes(B, T, C, W, int(cu is not None), 1), device=x.device,
-                         dtype=torch.uint8)
-        if B:
-            _lib.check(lib.kda_b200_short_conv_bwd(
-                _ptr(xr), xr.stride(0), xr.stride(1), _ptr(w), _ptr(b), _ptr(h), _ptr(cu), B, T, C, W, N, _IO[x.dtype],
-                int(silu), _ptr(dyr), dyr.stride(0), dyr.stride(1), _ptr(dh), _ptr(dx), _ptr(dw), _ptr(db), _ptr(dh0),
-                _ptr(ws), ws.numel(), _stream()))
-        else:
-            dw.zero_(), db.zero_()
-        return dx, dw, db, dh0
+    lib = _lib.load()
+    xr, dyr = _rows(x, x.dtype), _rows(dy, x.dtype)
+    w, b, h, cu, dh = _param(weight), _param(bias), _param(h0), _cu(cu_seqlens), _param(dht)
+    dx = x.new_empty((B, T, C))
+    dw = x.new_empty((C, W), dtype=torch.float32)
+    db = x.new_empty(C if bias is not None else 0, dtype=torch.float32)
+    dh0 = x.new_empty((N, C, W - 1) if want_dh0 else 0, dtype=torch.float32)
+    ws = x.new_empty(lib.kda_b200_short_conv_workspace_bytes(B, T, C, W, int(cu is not None), 1), dtype=torch.uint8)
+    if B:
+        _call(lib.kda_b200_short_conv_bwd, x.device,
+              _ptr(xr), xr.stride(0), xr.stride(1), _ptr(w), _ptr(b), _ptr(h), _ptr(cu), B, T, C, W, N, _IO[x.dtype],
+              int(silu), _ptr(dyr), dyr.stride(0), dyr.stride(1), _ptr(dh), _ptr(dx), _ptr(dw), _ptr(db), _ptr(dh0),
+              _ptr(ws), ws.numel())
+    else:
+        dw.zero_(), db.zero_()
+    return dx, dw, db, dh0
 
 
 @torch.library.custom_op("sophia_b200::short_conv_fwd", mutates_args=(), device_types="cuda")
@@ -283,14 +283,13 @@ def short_conv(x: Tensor, weight: Tensor, bias: Tensor | None = None, *, activat
 
 def _conv_step_impl(x, conv_state, weight, bias, slots, silu):
     rows, C = x.shape
-    with torch.autocast("cuda", enabled=False), _on(x):
-        xr = _rows(x, x.dtype)
-        w, b = _param(weight), _param(bias)
-        y = torch.empty(rows, C, device=x.device, dtype=x.dtype)
-        _lib.check(_lib.load().kda_b200_short_conv_step(
-            _ptr(xr), xr.stride(0), _ptr(w), _ptr(b), _ptr(conv_state), _ptr(slots), rows, C, weight.shape[1],
-            conv_state.shape[0], _IO[x.dtype], int(silu), _ptr(y), _stream()))
-        return y
+    xr = _rows(x, x.dtype)
+    w, b = _param(weight), _param(bias)
+    y = x.new_empty((rows, C))
+    _call(_lib.load().kda_b200_short_conv_step, x.device,
+          _ptr(xr), xr.stride(0), _ptr(w), _ptr(b), _ptr(conv_state), _ptr(slots), rows, C, weight.shape[1],
+          conv_state.shape[0], _IO[x.dtype], int(silu), _ptr(y))
+    return y
 
 
 @torch.library.custom_op("sophia_b200::short_conv_step", mutates_args=("conv_state",), device_types="cuda")
@@ -336,24 +335,21 @@ def _scan_fwd_impl(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want
     b, T, E = x.shape
     N, G = A.shape[1], B.shape[2]
     nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    with torch.autocast("cuda", enabled=False), _on(x):
-        lib = _lib.load()
-        xr, dtr, Br, Cr, zr = _scan_inputs(x.dtype, x, dt, B, C, z)
-        Af, Df, bf, h, cu = _param(A), _param(D), _param(dt_bias), _param(h0), _cu(cu_seqlens)
-        y = torch.empty(b, T, E, device=x.device, dtype=x.dtype)
-        ht = torch.empty((nseq, E, N) if want_final else (0,), device=x.device, dtype=torch.float32)
-        saved = torch.empty(lib.kda_b200_scan_saved_bytes(b, T, E, N, G) if training else 0, device=x.device,
-                            dtype=torch.uint8)
-        ws = torch.empty(lib.kda_b200_scan_workspace_bytes(b, T, E, N, G, int(cu is not None), 0), device=x.device,
-                         dtype=torch.uint8)
-        if b:
-            a = ScanArgs(b, T, E, N, G, nseq, _IO[x.dtype], int(softplus), _ptr(xr), _ptr(dtr), _ptr(zr), _ptr(Br),
-                         _ptr(Cr), xr.stride(0), xr.stride(1), dtr.stride(0), dtr.stride(1),
-                         *((zr.stride(0), zr.stride(1)) if zr is not None else (0, 0)),
-                         Br.stride(0), Br.stride(1), Br.stride(2), Cr.stride(0), Cr.stride(1), Cr.stride(2), _ptr(Af),
-                         _ptr(Df), _ptr(bf), _ptr(h), _ptr(cu), _ptr(y), _ptr(ht), _ptr(saved), saved.numel())
-            _lib.check(lib.kda_b200_selective_scan_fwd(a, _ptr(ws), ws.numel(), _stream()))
-        return y, ht, saved
+    lib = _lib.load()
+    xr, dtr, Br, Cr, zr = _scan_inputs(x.dtype, x, dt, B, C, z)
+    Af, Df, bf, h, cu = _param(A), _param(D), _param(dt_bias), _param(h0), _cu(cu_seqlens)
+    y = x.new_empty((b, T, E))
+    ht = x.new_empty((nseq, E, N) if want_final else 0, dtype=torch.float32)
+    saved = x.new_empty(lib.kda_b200_scan_saved_bytes(b, T, E, N, G) if training else 0, dtype=torch.uint8)
+    ws = x.new_empty(lib.kda_b200_scan_workspace_bytes(b, T, E, N, G, int(cu is not None), 0), dtype=torch.uint8)
+    if b:
+        a = ScanArgs(b, T, E, N, G, nseq, _IO[x.dtype], int(softplus), _ptr(xr), _ptr(dtr), _ptr(zr), _ptr(Br),
+                     _ptr(Cr), xr.stride(0), xr.stride(1), dtr.stride(0), dtr.stride(1),
+                     *((zr.stride(0), zr.stride(1)) if zr is not None else (0, 0)),
+                     Br.stride(0), Br.stride(1), Br.stride(2), Cr.stride(0), Cr.stride(1), Cr.stride(2), _ptr(Af),
+                     _ptr(Df), _ptr(bf), _ptr(h), _ptr(cu), _ptr(y), _ptr(ht), _ptr(saved), saved.numel())
+        _call(lib.kda_b200_selective_scan_fwd, x.device, a, _ptr(ws), ws.numel())
+    return y, ht, saved
 
 
 def _scan_bwd_impl(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, saved, dy, dht, softplus, want_dh0):
@@ -361,32 +357,30 @@ def _scan_bwd_impl(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, saved, dy, dht
     b, T, E = x.shape
     N, G = A.shape[1], B.shape[2]
     nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    with torch.autocast("cuda", enabled=False), _on(x):
-        lib = _lib.load()
-        io = x.dtype
-        xr, dtr, Br, Cr, zr = _scan_inputs(io, x, dt, B, C, z)
-        dyr = _rows(dy, io)
-        Af, Df, bf, h, cu, dh = _param(A), _param(D), _param(dt_bias), _param(h0), _cu(cu_seqlens), _param(dht)
-        new = lambda shape, dtype=torch.float32: torch.empty(shape, device=x.device, dtype=dtype)  # noqa: E731
-        dx, ddt = new((b, T, E), io), new((b, T, E), io)
-        dz = new((b, T, E) if z is not None else (0,), io)
-        dB, dC = new((b, T, G, N), io), new((b, T, G, N), io)
-        dA, dD, dbias = new((E, N)), new((E,) if D is not None else (0,)), new((E,) if dt_bias is not None else (0,))
-        dh0 = new((nseq, E, N) if want_dh0 else (0,))
-        ws = torch.empty(lib.kda_b200_scan_workspace_bytes(b, T, E, N, G, int(cu is not None), 1), device=x.device,
-                         dtype=torch.uint8)
-        if b:
-            a = ScanArgs(b, T, E, N, G, nseq, _IO[io], int(softplus), _ptr(xr), _ptr(dtr), _ptr(zr), _ptr(Br),
-                         _ptr(Cr), xr.stride(0), xr.stride(1), dtr.stride(0), dtr.stride(1),
-                         *((zr.stride(0), zr.stride(1)) if zr is not None else (0, 0)),
-                         Br.stride(0), Br.stride(1), Br.stride(2), Cr.stride(0), Cr.stride(1), Cr.stride(2), _ptr(Af),
-                         _ptr(Df), _ptr(bf), _ptr(h), _ptr(cu), None, None, _ptr(saved), saved.numel(),
-                         _ptr(dyr), dyr.stride(0), dyr.stride(1), _ptr(dh), _ptr(dx), _ptr(ddt), _ptr(dz), _ptr(dB),
-                         _ptr(dC), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dh0))
-            _lib.check(lib.kda_b200_selective_scan_bwd(a, _ptr(ws), ws.numel(), _stream()))
-        else:
-            dA.zero_(), dD.zero_(), dbias.zero_()
-        return dx, ddt, dA, dB, dC, dD, dz, dbias, dh0
+    lib = _lib.load()
+    io = x.dtype
+    xr, dtr, Br, Cr, zr = _scan_inputs(io, x, dt, B, C, z)
+    dyr = _rows(dy, io)
+    Af, Df, bf, h, cu, dh = _param(A), _param(D), _param(dt_bias), _param(h0), _cu(cu_seqlens), _param(dht)
+    new = lambda shape, dtype=torch.float32: x.new_empty(shape, dtype=dtype)  # noqa: E731
+    dx, ddt = new((b, T, E), io), new((b, T, E), io)
+    dz = new((b, T, E) if z is not None else (0,), io)
+    dB, dC = new((b, T, G, N), io), new((b, T, G, N), io)
+    dA, dD, dbias = new((E, N)), new((E,) if D is not None else (0,)), new((E,) if dt_bias is not None else (0,))
+    dh0 = new((nseq, E, N) if want_dh0 else (0,))
+    ws = x.new_empty(lib.kda_b200_scan_workspace_bytes(b, T, E, N, G, int(cu is not None), 1), dtype=torch.uint8)
+    if b:
+        a = ScanArgs(b, T, E, N, G, nseq, _IO[io], int(softplus), _ptr(xr), _ptr(dtr), _ptr(zr), _ptr(Br),
+                     _ptr(Cr), xr.stride(0), xr.stride(1), dtr.stride(0), dtr.stride(1),
+                     *((zr.stride(0), zr.stride(1)) if zr is not None else (0, 0)),
+                     Br.stride(0), Br.stride(1), Br.stride(2), Cr.stride(0), Cr.stride(1), Cr.stride(2), _ptr(Af),
+                     _ptr(Df), _ptr(bf), _ptr(h), _ptr(cu), None, None, _ptr(saved), saved.numel(),
+                     _ptr(dyr), dyr.stride(0), dyr.stride(1), _ptr(dh), _ptr(dx), _ptr(ddt), _ptr(dz), _ptr(dB),
+                     _ptr(dC), _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dh0))
+        _call(lib.kda_b200_selective_scan_bwd, x.device, a, _ptr(ws), ws.numel())
+    else:
+        dA.zero_(), dD.zero_(), dbias.zero_()
+    return dx, ddt, dA, dB, dC, dD, dz, dbias, dh0
 
 
 @torch.library.custom_op("sophia_b200::selective_scan_fwd", mutates_args=(), device_types="cuda")
@@ -525,16 +519,15 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Te
 def _scan_step_impl(x, dt, A, B, C, state, D, z, dt_bias, slots, softplus):
     rows, E = x.shape
     N, G = A.shape[1], B.shape[1]
-    with torch.autocast("cuda", enabled=False), _on(x):
-        xr, dtr, Br, Cr, zr = _scan_inputs(x.dtype, x, dt, B, C, z)
-        Af, Df, bf = _param(A), _param(D), _param(dt_bias)
-        y = torch.empty(rows, E, device=x.device, dtype=x.dtype)
-        a = ScanArgs(1, 1, E, N, G, 1, _IO[x.dtype], int(softplus), _ptr(xr), _ptr(dtr), _ptr(zr), _ptr(Br), _ptr(Cr),
-                     xr.stride(0), 0, dtr.stride(0), 0, zr.stride(0) if zr is not None else 0, 0,
-                     Br.stride(0), 0, Br.stride(1), Cr.stride(0), 0, Cr.stride(1), _ptr(Af), _ptr(Df), _ptr(bf))
-        a.y, a.state, a.slots, a.rows, a.pool = _ptr(y), _ptr(state), _ptr(slots), rows, state.shape[0]
-        _lib.check(_lib.load().kda_b200_selective_scan_step(a, _stream()))
-        return y
+    xr, dtr, Br, Cr, zr = _scan_inputs(x.dtype, x, dt, B, C, z)
+    Af, Df, bf = _param(A), _param(D), _param(dt_bias)
+    y = x.new_empty((rows, E))
+    a = ScanArgs(1, 1, E, N, G, 1, _IO[x.dtype], int(softplus), _ptr(xr), _ptr(dtr), _ptr(zr), _ptr(Br), _ptr(Cr),
+                 xr.stride(0), 0, dtr.stride(0), 0, zr.stride(0) if zr is not None else 0, 0,
+                 Br.stride(0), 0, Br.stride(1), Cr.stride(0), 0, Cr.stride(1), _ptr(Af), _ptr(Df), _ptr(bf))
+    a.y, a.state, a.slots, a.rows, a.pool = _ptr(y), _ptr(state), _ptr(slots), rows, state.shape[0]
+    _call(_lib.load().kda_b200_selective_scan_step, x.device, a)
+    return y
 
 
 @torch.library.custom_op("sophia_b200::selective_scan_step", mutates_args=("state",), device_types="cuda")
