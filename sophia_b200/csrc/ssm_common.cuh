@@ -76,6 +76,12 @@ struct Lane {
     const float2 o = upk2(p[i / 2]);
     p[i / 2] = i & 1 ? pk2(o.x, v) : pk2(v, o.y);
   }
+  __device__ __forceinline__ static Lane of(const float (&f)[S]) {
+    Lane r;
+#pragma unroll
+    for (int k = 0; k < S / 2; ++k) r.p[k] = pk2(f[2 * k], f[2 * k + 1]);
+    return r;
+  }
   __device__ __forceinline__ static Lane load(const float* q) {  // S * 4 bytes, aligned
     Lane r;
     if (S % 4 == 0) {

@@ -26,9 +26,13 @@
 // (i xor m), so that what a lane keeps sits in the same registers everywhere), the
 // warps' sums meet in shared memory and the CTAs' in a buffer that a last kernel sums in
 // block order.  No atomics: every sum has a fixed order.
+//
+// Few rows: the tokens are cut into spans with CTAs of their own.  As h is linear in the
+// state in front, a span's effect on it is h -> P h + c, P = e^(A sum d) and c the state that
+// the span makes of zeros; a first kernel finds P and c of every span (the recurrence
+// alone: no C, no output), and a CTA of the scan itself composes those in front of its own.
+// Backward the same with g, from behind.
 #pragma once
-
-#include <type_traits>
 
 #include "ssm_common.cuh"
 
@@ -71,6 +75,8 @@ struct ScanParams {
   SeqMap seq;
   int B, T, E, N, G;
   int blocks;                      // channel blocks per group
+  int spans, span;                 // of `span` tokens (a multiple of 32)
+  float2* carry;                   // [B][spans][E][N]: c and P (negative: nothing passes) of the spans; null = one span
   bool softplus, vec, vec_bc;      // vec: x, dt, z, dy and the outputs allow 16-byte pieces; vec_bc: B and C
   void* y;                         // [B, T, E] contiguous
   float* ht;                       // [nseq][E][N] or null
@@ -80,14 +86,16 @@ struct ScanParams {
   void *dx, *ddt, *dz;
   float* dh0;
   float* bc_part;                  // [B][tiles][G][blocks][TT][2][N]
-  float* e_part;                   // [B][E][N + 2]: dA, dD, d dt_bias
+  float* e_part;                   // [B][spans][E][N + 2]: dA, dD, d dt_bias
 };
 
 struct ScanBlock {
   int g, blk, c0, nc, b;  // group, block in it, first channel, channels, row
+  int k;                  // span
+  int tile0, tiles;       // its tiles
 };
-template <int CPB>
-__device__ __forceinline__ ScanBlock scan_block(const ScanParams& P) {
+template <int CPB, int TT>
+__device__ __forceinline__ ScanBlock scan_block(const ScanParams& P, int span) {
   ScanBlock s;
   const int eg = P.E / P.G;
   s.g = blockIdx.x / P.blocks;
@@ -95,6 +103,9 @@ __device__ __forceinline__ ScanBlock scan_block(const ScanParams& P) {
   s.c0 = s.g * eg + s.blk * CPB;
   s.nc = min(CPB, eg - s.blk * CPB);
   s.b = blockIdx.y;
+  s.k = span;
+  s.tile0 = span * (P.span / TT);
+  s.tiles = (min(P.span, P.T - span * P.span) + TT - 1) / TT;
   return s;
 }
 
@@ -350,9 +361,204 @@ __host__ __device__ inline int scan_bwd_smem(int N) {
                                         SCAN_WARPS * G::TT * 2 * G::NP * 4 + 2 * G::TT * 4);
 }
 
+template <typename T, typename G>
+__host__ __device__ inline int scan_carry_smem(int N, int tensors) {
+  return SCAN_STAGES * scan_stage_elems<T, G>(N, tensors) * (int)sizeof(T) +
+         2 * (G::TT * G::CPB * 8 + 2 * G::TT * G::NP * 4 + 2 * G::TT * 4);
+}
+
 // A channel pair's values of a per-channel parameter (zeros without it or past the block).
 __device__ __forceinline__ float2 scan_param(const float* p, const ScanBlock& s, int c) {
   return make_float2(p && c < s.nc ? p[s.c0 + c] : 0.f, p && c + 1 < s.nc ? p[s.c0 + c + 1] : 0.f);
+}
+
+// A lane's states of sequence q, register i being state i ^ m of the lane's (zeros where `ok` has no
+// bit, and without the tensor).
+template <int S>
+__device__ __forceinline__ Lane<S> scan_state(const float* states, int q, long long per, long long chan, unsigned ok, int m) {
+  float f[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) f[i] = 0.f;
+  if (states && ok) {
+    const float* p = states + q * per + chan;
+#pragma unroll
+    for (int i = 0; i < S; ++i)
+      if (ok >> i & 1) f[i] = p[i ^ m];
+  }
+  return Lane<S>::of(f);
+}
+
+// What the spans in front of span k (REV: behind it) hand over: state n of a lane's register i
+// at chan + (i ^ m).  A product with a zero is left out, so that P may be infinite.
+template <int S, bool REV>
+__device__ __forceinline__ Lane<S> scan_enter(const ScanParams& P, const ScanBlock& s, long long chan, unsigned ok, int m) {
+  constexpr int U = 4;  // loads of four spans at once
+  const long long per = (long long)P.E * P.N, step = REV ? -per : per;
+  const int n = REV ? P.spans - 1 - s.k : s.k;
+  const float2* p = P.carry + ((long long)s.b * P.spans + (REV ? P.spans - 1 : 0)) * per + chan;
+  float v[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) v[i] = 0.f;
+  for (int j = 0; j < n; j += U, p += U * step) {
+    float2 c[U][S];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        c[u][i] = j + u < n && (ok >> i & 1) ? __ldg(p + u * step + (i ^ m)) : make_float2(0.f, 1.f);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < S; ++i) v[i] = c[u][i].y < 0.f || v[i] == 0.f ? c[u][i].x : fmaf(c[u][i].y, v[i], c[u][i].x);
+  }
+  return Lane<S>::of(v);
+}
+
+// P and c of the spans that have one behind them (REV: in front, for the backward's g, where
+// u = dy silu(z) and C stand for d x and B).  The same layout as the scan's, without its outputs.
+template <typename T, int L, int S, bool PAD, bool REV>
+__global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_carry_kernel(ScanParams P) {
+  using G = ScanFwdGeo<T, L, S>;
+  constexpr int TT = G::TT, CPB = G::CPB, TENSORS = REV ? 3 : 2;
+  extern __shared__ __align__(16) char scan_sm[];
+  const int N = P.N, npad = (N + 7) / 8 * 8, stage = scan_stage_elems<T, G>(N, TENSORS);
+  T* raw = reinterpret_cast<T*>(scan_sm);                             // [STAGES]: dt, x or (dy, z), B rows, C rows
+  float2* DU = reinterpret_cast<float2*>(raw + SCAN_STAGES * stage);  // double buffers: [TT][CPB]: d, u
+  float* Bs = reinterpret_cast<float*>(DU + 2 * TT * CPB);            // [TT][NP]
+  float* Cs = Bs + 2 * TT * G::NP;
+  int* flags = reinterpret_cast<int*>(Cs + 2 * TT * G::NP);           // first [TT], last [TT]
+  const ScanBlock s = scan_block<CPB, TT>(P, blockIdx.z + (REV ? 1 : 0));
+  const int tiles = s.tiles, dir = REV ? -1 : 1, tile0 = REV ? s.tile0 + tiles - 1 : s.tile0;  // step i takes tile0 + i dir
+
+  if (threadIdx.x >= SCAN_MAIN) {  // tokens
+    const int tid = threadIdx.x - SCAN_MAIN;
+    const int pc = (tid % G::PAIRS) * 2, pt = tid / G::PAIRS;
+    const float2 bias = scan_param(P.dt_bias, s, pc);
+    RowView views[TENSORS];
+    views[0] = P.dt;
+    views[1] = REV ? P.dy : P.x;
+    if (REV) views[TENSORS - 1] = P.z;
+    ScanFetch<T, G, TENSORS> f;
+    f.init(P, s, views, tid, TENSORS * G::RAW, npad, tile0, dir);
+    ScanFlags<TT> marks;
+    marks.read(P, s.b, tile0 * TT, tid);
+    constexpr int IT = TT / G::TSTEP;
+    const bool spare = G::SPARE && pt >= TT;
+    auto prepare = [&](int i) {
+      const int t0 = (tile0 + i * dir) * TT, q = i & 1;
+      const T* rx = raw + (i % SCAN_STAGES) * stage;
+      ScanBC<T, G, 1, PAD> bc;
+      float4 du[IT];
+      if (!spare) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k) {
+          const int t = pt + k * G::TSTEP;
+          const T* p = rx + t * CPB + pc;
+          const float2 dt = scan_pair(p);
+          float2 u = scan_pair(p + G::RAW);
+          const bool in = t0 + t < P.T;
+          const float d0 = scan_d(P, dt.x + bias.x, in), d1 = scan_d(P, dt.y + bias.y, in);
+          if (!REV) {
+            u.x *= d0;
+            u.y *= d1;
+          } else if (P.z.p) {
+            const float2 z = scan_pair(p + 2 * G::RAW);
+            u.x *= z.x * sigmoidf_(z.x);
+            u.y *= z.y * sigmoidf_(z.y);
+          }
+          du[k] = make_float4(d0, u.x, d1, u.y);
+        }
+      }
+      bc.load(rx + TENSORS * G::RAW, npad, P, s, t0, tid);
+      if (!spare) {
+#pragma unroll
+        for (int k = 0; k < IT; ++k)
+          *reinterpret_cast<float4*>(DU + (q * TT + pt + k * G::TSTEP) * CPB + pc) = du[k];
+      }
+      bc.store(Bs + q * TT * G::NP, Cs + q * TT * G::NP, tid);
+      marks.write(flags + q * 2 * TT, tid);
+      marks.read(P, s.b, t0 + dir * TT, tid);
+    };
+    f.fetch(P, s, views, raw, tile0 * TT, tid);
+    if (tiles > 1) f.fetch(P, s, views, raw + stage, (tile0 + dir) * TT, tid);
+    cp_async_wait<0>();
+    asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");  // the first tiles have arrived, for the whole side
+    prepare(0);
+    __syncthreads();
+    for (int i = 0; i < tiles; ++i) {
+      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, (tile0 + (i + 2) * dir) * TT, tid);
+      if (i + 1 < tiles) prepare(i + 1);
+      cp_async_wait<0>();
+      __syncthreads();
+    }
+    return;
+  }
+
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int l = lane / G::CH, c = warp * G::CH + lane % G::CH, n0 = l * S;
+  const unsigned ok = N - n0 >= S ? (1u << S) - 1u : N > n0 ? (1u << (N - n0)) - 1u : 0u;  // states that exist
+  const bool live = c < s.nc;
+  Lane<S> a2 = Lane<S>::all(0.f), h = a2;
+  const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + i] * LOG2E);
+  float dsum = 0.f, dsum_err = 0.f;
+  bool cut = false;  // a sequence starts in the span: nothing passes it
+  __syncthreads();
+  for (int step = 0; step < tiles; ++step) {
+    const int t0 = (tile0 + step * dir) * TT, q = step & 1;
+    const float2* du_ = DU + q * TT * CPB + c;
+    const float* v_ = (REV ? Cs : Bs) + q * TT * G::NP + n0;
+    const int* first = flags + q * 2 * TT;
+    const int* last = first + TT;
+    float d;
+    auto token = [&](float2 u, const Lane<S>& v) {
+      const Lane<S> a = lane_decay(a2, u.x);
+      d += u.x;
+      if (!REV) h = lane_keep<PAD>(fma(a, h, v * Lane<S>::all(u.y)), ok);
+      else h = a * lane_keep<PAD>(fma(v, Lane<S>::all(u.y), h), ok);
+    };
+    auto segment = [&](int t1) {
+      float2 du[SCAN_SEG];
+      Lane<S> v[SCAN_SEG];
+#pragma unroll
+      for (int k = 0; k < SCAN_SEG; ++k) {
+        du[k] = du_[(t1 + k) * CPB];
+        v[k] = Lane<S>::load(v_ + (t1 + k) * G::NP);
+      }
+#pragma unroll
+      for (int o = 0; o < SCAN_SEG; ++o) token(du[REV ? SCAN_SEG - 1 - o : o], v[REV ? SCAN_SEG - 1 - o : o]);
+    };
+    auto flagged = [&](int t1) {  // sequences start or end among the tokens
+      const long long per = (long long)P.E * N;
+#pragma unroll 1
+      for (int o = 0; o < SCAN_SEG; ++o) {
+        const int t = t1 + (REV ? SCAN_SEG - 1 - o : o);
+        const bool starts = first[t] >= 0;
+        cut |= starts;
+        if (!REV && starts) h = scan_state<S>(P.h0, first[t], per, chan, live ? ok : 0u, 0);
+        if (REV && last[t] >= 0) h = h + scan_state<S>(P.dht, last[t], per, chan, live ? ok : 0u, 0);
+        token(du_[t * CPB], Lane<S>::load(v_ + t * G::NP));
+        if (REV && starts) h = Lane<S>::all(0.f);
+      }
+    };
+    const int segs = (min(TT, P.T - t0) + SCAN_SEG - 1) / SCAN_SEG;
+#pragma unroll 1
+    for (int j = 0; j < segs; ++j) {
+      const int t1 = (REV ? segs - 1 - j : j) * SCAN_SEG;
+      d = 0.f;
+      if (scan_seg_flag(first + t1, last + t1)) flagged(t1);
+      else segment(t1);
+      sum_add(dsum, dsum_err, d);
+    }
+    __syncthreads();
+  }
+  const Lane<S> pass = (a2 * Lane<S>::all(dsum)).exp2();
+  float2* out = P.carry + ((long long)s.b * P.spans + s.k) * P.E * N + chan;
+#pragma unroll
+  for (int i = 0; i < S; ++i)
+    if (live && (ok >> i & 1)) out[i] = make_float2(h.get(i), cut ? -1.f : pass.get(i));
 }
 
 template <typename T, int L, int S, bool PAD>
@@ -368,8 +574,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
   float* Cs = Bs + 2 * TT * G::NP;
   float* YP = Cs + 2 * TT * G::NP;                                    // [TT][CPB][L]
   int* flags = reinterpret_cast<int*>(YP + 2 * TT * CPB * L);         // first [TT], last [TT]
-  const ScanBlock s = scan_block<CPB>(P);
-  const int tiles = (P.T + TT - 1) / TT, segs = (P.T + SCAN_SEG - 1) / SCAN_SEG;
+  const ScanBlock s = scan_block<CPB, TT>(P, blockIdx.z);
+  const int tiles = s.tiles, first_t = s.tile0 * TT, segs = (P.T + SCAN_SEG - 1) / SCAN_SEG;
 
   if (threadIdx.x >= SCAN_MAIN) {  // tokens
     const int tid = threadIdx.x - SCAN_MAIN;
@@ -377,14 +583,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
     const float2 bias = scan_param(P.dt_bias, s, pc), skip = scan_param(P.D, s, pc);
     const RowView views[3] = {P.x, P.dt, P.z};
     ScanFetch<T, G, 3> f;
-    f.init(P, s, views, tid, 3 * G::RAW, npad, 0, 1);
+    f.init(P, s, views, tid, 3 * G::RAW, npad, s.tile0, 1);
     ScanFlags<TT> marks;
-    marks.read(P, s.b, 0, tid);
+    marks.read(P, s.b, first_t, tid);
     // (both passes: all reads of shared memory, then all writes)
     constexpr int IT = TT / G::TSTEP;
     const bool spare = G::SPARE && pt >= TT;
     auto prepare = [&](int i) {
-      const int t0 = i * TT, q = i & 1;
+      const int t0 = first_t + i * TT, q = i & 1;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
       ScanBC<T, G, 1, PAD> bc;
       float2 x[IT], dt[IT];
@@ -413,7 +619,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
       marks.read(P, s.b, t0 + TT, tid);
     };
     auto finish = [&](int i) {
-      const int t0 = i * TT;
+      const int t0 = first_t + i * TT;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
       const float* yp = YP + (i & 1) * TT * CPB * L;
       if (spare) return;
@@ -431,15 +637,15 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
         if (t0 + t < P.T) scan_put_pair<T>(P.y, P, s, t0 + t, pc, v);
       }
     };
-    f.fetch(P, s, views, raw, 0, tid);
-    if (tiles > 1) f.fetch(P, s, views, raw + stage, TT, tid);
+    f.fetch(P, s, views, raw, first_t, tid);
+    if (tiles > 1) f.fetch(P, s, views, raw + stage, first_t + TT, tid);
     cp_async_wait<0>();
     asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");  // the first tiles have arrived, for the whole side
     prepare(0);
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
       // (stage of i + 2 held i - 2, which was finished before the last barrier)
-      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, (i + 2) * TT, tid);
+      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, first_t + (i + 2) * TT, tid);
       if (i + 1 < tiles) prepare(i + 1);
       if (i > 0) finish(i - 1);
       cp_async_wait<0>();
@@ -458,17 +664,17 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
 #pragma unroll
   for (int i = 0; i < S; ++i)
     if (live && (ok >> i & 1)) a2.set(i, P.A[chan + i] * LOG2E);
+  if (s.k > 0 && live) h = scan_enter<S, false>(P, s, chan, ok, 0);
   __syncthreads();
   for (int tile = 0; tile < tiles; ++tile) {
-    const int t0 = tile * TT, q = tile & 1;
+    const int t0 = first_t + tile * TT, q = tile & 1;
     const float2* du_ = DU + q * TT * CPB + c;
     const float* b_ = Bs + q * TT * G::NP + n0;
     const float* c_ = Cs + q * TT * G::NP + n0;
     float* y_ = YP + q * TT * CPB * L + c * L + l;
     const int* first = flags + q * 2 * TT;
     const int* last = first + TT;
-    auto segment = [&](int t1, auto with_flags) {
-      constexpr bool FLAGS = decltype(with_flags)::value;
+    auto segment = [&](int t1) {
       // all of the segment's reads in front of its stores, which the compiler must assume to alias
       float2 du[SCAN_SEG];
       Lane<S> bv[SCAN_SEG], cv[SCAN_SEG];
@@ -481,23 +687,26 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
       }
 #pragma unroll
       for (int k = 0; k < SCAN_SEG; ++k) {
-        const int t = t1 + k;
-        if (FLAGS && first[t] >= 0) {
-#pragma unroll
-          for (int i = 0; i < S; ++i)
-            h.set(i, P.h0 && live && (ok >> i & 1) ? __ldg(P.h0 + (long long)first[t] * P.E * N + chan + i) : 0.f);
-        }
-        const Lane<S> a = lane_decay(a2, du[k].x);
-        h = lane_keep<PAD>(fma(a, h, bv[k] * Lane<S>::all(du[k].y)), ok);
+        h = lane_keep<PAD>(fma(lane_decay(a2, du[k].x), h, bv[k] * Lane<S>::all(du[k].y)), ok);
         y[k] = (h * cv[k]).sum();
-        if (FLAGS && last[t] >= 0 && P.ht) {
-#pragma unroll
-          for (int i = 0; i < S; ++i)
-            if (live && (ok >> i & 1)) P.ht[(long long)last[t] * P.E * N + chan + i] = h.get(i);
-        }
       }
 #pragma unroll
       for (int k = 0; k < SCAN_SEG; ++k) y_[(t1 + k) * CPB * L] = y[k];
+    };
+    auto flagged = [&](int t1) {  // sequences start or end among the tokens
+      const long long per = (long long)P.E * N;
+#pragma unroll 1
+      for (int t = t1; t < t1 + SCAN_SEG; ++t) {
+        if (first[t] >= 0) h = scan_state<S>(P.h0, first[t], per, chan, live ? ok : 0u, 0);
+        const float2 u = du_[t * CPB];
+        h = lane_keep<PAD>(fma(lane_decay(a2, u.x), h, Lane<S>::load(b_ + t * G::NP) * Lane<S>::all(u.y)), ok);
+        if (last[t] >= 0 && P.ht) {
+#pragma unroll
+          for (int i = 0; i < S; ++i)
+            if (live && (ok >> i & 1)) P.ht[last[t] * per + chan + i] = h.get(i);
+        }
+        y_[t * CPB * L] = (h * Lane<S>::load(c_ + t * G::NP)).sum();
+      }
     };
 #pragma unroll 1
     for (int t1 = 0; t1 < TT && t0 + t1 < P.T; t1 += SCAN_SEG) {
@@ -511,8 +720,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
             if (ok >> i & 1) ck[i] = h.get(i);
         }
       }
-      if (scan_seg_flag(first + t1, last + t1)) segment(t1, std::true_type{});
-      else segment(t1, std::false_type{});
+      if (scan_seg_flag(first + t1, last + t1)) flagged(t1);
+      else segment(t1);
     }
     __syncthreads();
   }
@@ -539,9 +748,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
   float* YP = Cs + 2 * TT * S * G::NP;       // [3][TT][CPB][L]: partial sums of y, dd / ln 2, sum g B
   float* slots = YP + 2 * 3 * TT * CPB * L;  // [warps][TT][2][NP]: the warps' dB and dC
   int* flags = reinterpret_cast<int*>(slots + 2 * SCAN_WARPS * TT * 2 * G::NP);  // first [TT], last [TT]
-  const ScanBlock s = scan_block<CPB>(P);
-  const int tiles = (P.T + TT - 1) / TT;  // step i takes tile tiles - 1 - i
-  float* e = P.e_part + (long long)s.b * P.E * (N + 2);
+  const ScanBlock s = scan_block<CPB, TT>(P, blockIdx.z);
+  const int tiles = s.tiles, tile_z = s.tile0 + tiles - 1;  // step i takes tile tile_z - i
+  const int all = (P.T + TT - 1) / TT;                      // tiles of the row
+  float* e = P.e_part + ((long long)s.b * P.spans + s.k) * P.E * (N + 2);
 
   if (threadIdx.x >= SCAN_MAIN) {  // tokens
     const int tid = threadIdx.x - SCAN_MAIN;
@@ -551,14 +761,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     float2 dD = zero, db = zero, dD_err = zero, db_err = zero;
     const RowView views[4] = {P.x, P.dt, P.dy, P.z};
     ScanFetch<T, G, 4> f;
-    f.init(P, s, views, tid, 4 * G::RAW, npad, tiles - 1, -1);
+    f.init(P, s, views, tid, 4 * G::RAW, npad, tile_z, -1);
     ScanFlags<TT> marks;
-    marks.read(P, s.b, (tiles - 1) * TT, tid);
+    marks.read(P, s.b, tile_z * TT, tid);
     // (both passes: all reads of shared memory, then all writes)
     constexpr int IT = TT / G::TSTEP;
     const bool spare = G::SPARE && pt >= TT;
     auto prepare = [&](int i) {
-      const int t0 = (tiles - 1 - i) * TT, q = i & 1;
+      const int t0 = (tile_z - i) * TT, q = i & 1;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
       ScanBC<T, G, S, PAD> bc;
       float2 x[IT], dt[IT], ds[IT], z[IT];
@@ -600,7 +810,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
       marks.read(P, s.b, t0 - TT, tid);
     };
     auto finish = [&](int i) {
-      const int tile = tiles - 1 - i, t0 = tile * TT, q = i & 1, at = ((i % 3) * TT + pt) * CPB + pc;
+      const int tile = tile_z - i, t0 = tile * TT, q = i & 1, at = ((i % 3) * TT + pt) * CPB + pc;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
       if (!spare) {
 #pragma unroll
@@ -636,7 +846,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
         }
       }
       // the tile's dB and dC over the warps, [TT][2][N]
-      float* part = P.bc_part + ((((long long)s.b * tiles + tile) * P.G + s.g) * P.blocks + s.blk) * (TT * 2 * N);
+      float* part = P.bc_part + ((((long long)s.b * all + tile) * P.G + s.g) * P.blocks + s.blk) * (TT * 2 * N);
       const float* sl = slots + q * SCAN_WARPS * TT * 2 * G::NP;
 #pragma unroll
       for (int i0 = 0; i0 < TT * 2 * G::NP; i0 += G::TOKENS) {
@@ -649,14 +859,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
         if (!PAD || n < N) part[j / G::NP * N + n] = o;
       }
     };
-    f.fetch(P, s, views, raw, (tiles - 1) * TT, tid);
-    if (tiles > 1) f.fetch(P, s, views, raw + stage, (tiles - 2) * TT, tid);
+    f.fetch(P, s, views, raw, tile_z * TT, tid);
+    if (tiles > 1) f.fetch(P, s, views, raw + stage, (tile_z - 1) * TT, tid);
     cp_async_wait<0>();
     asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");  // the first tiles have arrived, for the whole side
     prepare(0);
     __syncthreads();
     for (int i = 0; i < tiles; ++i) {
-      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, (tiles - 3 - i) * TT, tid);
+      if (i + 2 < tiles) f.fetch(P, s, views, raw + ((i + 2) % SCAN_STAGES) * stage, (tile_z - 2 - i) * TT, tid);
       if (i + 1 < tiles) prepare(i + 1);
       if (i > 0) finish(i - 1);
       cp_async_wait<0>();
@@ -693,11 +903,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
   for (int i = 0; i < S; ++i) ok |= (unsigned)(n0 + (i ^ m) < N) << i;
   float hs[S];  // the next tile's checkpoint (left alone until then: the load is on its way)
   auto checkpoint = [&](int tile) {
-    const float* p = P.ckpt + ((long long)s.b * tiles + tile) * P.E * N + chan;
+    const float* p = P.ckpt + ((long long)s.b * all + tile) * P.E * N + chan;
 #pragma unroll
     for (int i = 0; i < S; ++i) hs[i] = live && (!PAD || (ok >> i & 1)) ? __ldg(p + (i ^ m)) : 0.f;
   };
-  checkpoint(tiles - 1);
+  checkpoint(tile_z);
   Lane<S> a2 = Lane<S>::all(0.f), r = a2;
   float dA[S], dA_err[S];
 #pragma unroll
@@ -705,6 +915,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     dA[i] = dA_err[i] = 0.f;
     if (live && (ok >> i & 1)) a2.set(i, P.A[chan + (i ^ m)] * LOG2E);
   }
+  if (s.k + 1 < P.spans && live) r = scan_enter<S, true>(P, s, chan, ok, m);
   __syncthreads();
   for (int step = 0; step < tiles; ++step) {
     const int q = step & 1, q3 = step % 3;
@@ -716,22 +927,64 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     float* s_ = slots + (q * SCAN_WARPS + warp) * TT * 2 * G::NP + n0;
     const int* first = flags + q * 2 * TT;
     const int* last = first + TT;
-    Lane<S> h_in;
-#pragma unroll
-    for (int i = 0; i < S; ++i) h_in.set(i, hs[i]);
-    if (step + 1 < tiles) checkpoint(tiles - 2 - step);
+    const Lane<S> h_in = Lane<S>::of(hs);
+    if (step + 1 < tiles) checkpoint(tile_z - 1 - step);
 
-    auto segment = [&](auto with_flags) {
-      constexpr bool FLAGS = decltype(with_flags)::value;
-      auto start = [&](int k) {  // the state in front of a sequence's first token
-        Lane<S> v = Lane<S>::all(0.f);
-        if (P.h0 && live) {
+    Lane<S> dAs = Lane<S>::all(0.f);
+    // Token k backwards: a, h its decay and state, `before` the state in front of it.  r leaves as what
+    // passes to the token in front.
+    auto token = [&](int k, const Lane<S>& a, const Lane<S>& h, const Lane<S>& before, const Lane<S>& bv,
+                     const Lane<S>& cv, float2 u, float dy) {
+      const Lane<S> ds = Lane<S>::all(dy);
+      const Lane<S> g = lane_keep<PAD>(fma(cv, ds, r), ok);
+      r = a * g;
+      const Lane<S> w = lane_keep<PAD>(r * before, ok);
+      dAs = fma(w, Lane<S>::all(u.x), dAs);
+      const float y = (h * cv).sum(), dd = (w * a2).sum(), gb = (g * bv).sum();
+      const Lane<S> vb = g * Lane<S>::all(u.y), vc = ds * h;  // dB, dC of this channel
+      y_[k * CPB * L] = y;
+      y_[(TT + k) * CPB * L] = dd;
+      y_[(2 * TT + k) * CPB * L] = gb;
+      // over the warp's channels: states i < half stay, the others go to the lane that keeps them
+      float v[2][S];
 #pragma unroll
-          for (int i = 0; i < S; ++i)
-            if (ok >> i & 1) v.set(i, __ldg(P.h0 + (long long)first[k] * P.E * N + chan + (i ^ m)));
+      for (int i = 0; i < S; ++i) {
+        v[0][i] = vb.get(i);
+        v[1][i] = vc.get(i);
+      }
+#pragma unroll
+      for (int x = 0; x < XB; ++x) {
+        const int half = S >> (x + 1);
+#pragma unroll
+        for (int i = 0; i < half; ++i)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            v[b][i] += __shfl_xor_sync(0xffffffffu, v[b][i + half], (half / LEFT) << (RB + LB));
+      }
+      float* slot = s_ + k * 2 * G::NP;
+      if (RB > 0) {  // one of the other channel bits decides between dB and dC, the rest just add
+        const bool odd = lane & 1;
+#pragma unroll
+        for (int i = 0; i < LEFT; ++i) {
+          const float give = odd ? v[0][i] : v[1][i], keep = odd ? v[1][i] : v[0][i];
+          float o = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+#pragma unroll
+          for (int x = 1; x < RB; ++x) o += __shfl_xor_sync(0xffffffffu, o, 1 << x);
+          if ((lane & ((1 << RB) - 1)) <= 1) slot[(odd ? G::NP : 0) + (i ^ m)] = o;
         }
-        return v;
-      };
+      } else {
+#pragma unroll
+        for (int i = 0; i < LEFT; ++i) {
+          slot[i ^ m] = v[0][i];
+          slot[G::NP + (i ^ m)] = v[1][i];
+        }
+      }
+    };
+    auto step_h = [&](const Lane<S>& a, const Lane<S>& before, const Lane<S>& bv, float2 u) {
+      return lane_keep<PAD>(fma(a, before, bv * Lane<S>::all(u.y)), ok);
+    };
+    auto at = [&](const float* rows, int t) { return Lane<S>::load(rows + t * S * G::NP); };  // of B or C
+    if (!scan_seg_flag(first, last)) {
       // The later half of the tokens first: its states are kept, those of the half before it only
       // passed through, and rebuilt for their own turn.  Half a segment fits the registers of two CTAs
       // per SM.  Reads come in front of stores, which the compiler must assume to alias.
@@ -739,12 +992,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
       Lane<S> mid = h_in;
 #pragma unroll
       for (int k = 0; k < HALF; ++k) {
-        if (FLAGS && first[k] >= 0) mid = start(k);
         const float2 u = du_[k * CPB];
-        mid = lane_keep<PAD>(fma(lane_decay(a2, u.x), mid, Lane<S>::load(b_ + k * S * G::NP) * Lane<S>::all(u.y)),
-                             ok);
+        mid = step_h(lane_decay(a2, u.x), mid, at(b_, k), u);
       }
-      Lane<S> h[HALF], a[HALF], bv[HALF], cv[HALF], dAs = Lane<S>::all(0.f);
+      Lane<S> h[HALF], a[HALF], bv[HALF], cv[HALF];
       float2 du[HALF];
       float dsv[HALF];
 #pragma unroll
@@ -757,83 +1008,46 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
             const int t = k - HALF + 1 + o;
             du[o] = du_[t * CPB];
             dsv[o] = ds_[t * CPB];
-            bv[o] = Lane<S>::load(b_ + t * S * G::NP);
-            cv[o] = Lane<S>::load(c_ + t * S * G::NP);
+            bv[o] = at(b_, t);
+            cv[o] = at(c_, t);
           }
 #pragma unroll
           for (int o = 0; o < HALF; ++o) {
-            const int t = k - HALF + 1 + o;
-            Lane<S> before = o ? h[o ? o - 1 : 0] : front;
-            if (FLAGS && first[t] >= 0) before = start(t);
             a[o] = lane_decay(a2, du[o].x);
-            h[o] = lane_keep<PAD>(fma(a[o], before, bv[o] * Lane<S>::all(du[o].y)), ok);
+            h[o] = step_h(a[o], o ? h[o ? o - 1 : 0] : front, bv[o], du[o]);
           }
         }
-        if (FLAGS && last[k] >= 0 && P.dht && live) {
-#pragma unroll
-          for (int i = 0; i < S; ++i)
-            if (ok >> i & 1) r.set(i, r.get(i) + __ldg(P.dht + (long long)last[k] * P.E * N + chan + (i ^ m)));
-        }
-        const Lane<S> ds = Lane<S>::all(dsv[j]);
-        const Lane<S> g = lane_keep<PAD>(fma(cv[j], ds, r), ok);
-        r = a[j] * g;
-        Lane<S> before = j ? h[j ? j - 1 : 0] : front;
-        if (FLAGS && first[k] >= 0) before = start(k);
-        const Lane<S> w = lane_keep<PAD>(r * before, ok);
-        dAs = fma(w, Lane<S>::all(du[j].x), dAs);
-        const float y = (h[j] * cv[j]).sum(), dd = (w * a2).sum(), gb = (g * bv[j]).sum();
-        Lane<S> vb = g * Lane<S>::all(du[j].y), vc = ds * h[j];  // dB, dC of this channel
-        if (FLAGS && first[k] >= 0) {  // what reaches the initial state; nothing passes the start
+        token(k, a[j], h[j], j ? h[j ? j - 1 : 0] : front, bv[j], cv[j], du[j], dsv[j]);
+      }
+    } else {
+      // a sequence starts or ends here: token by token, the states in front of them kept in local memory
+      const long long per = (long long)P.E * N;
+      Lane<S> front[SCAN_SEG], h = h_in;
+#pragma unroll 1
+      for (int k = 0; k < SCAN_SEG; ++k) {
+        if (first[k] >= 0) h = scan_state<S>(P.h0, first[k], per, chan, live ? ok : 0u, m);
+        front[k] = h;
+        const float2 u = du_[k * CPB];
+        h = step_h(lane_decay(a2, u.x), h, at(b_, k), u);
+      }
+#pragma unroll 1
+      for (int k = SCAN_SEG - 1; k >= 0; --k) {
+        if (last[k] >= 0) r = r + scan_state<S>(P.dht, last[k], per, chan, live ? ok : 0u, m);
+        const float2 u = du_[k * CPB];
+        const Lane<S> a = lane_decay(a2, u.x), bv = at(b_, k), before = front[k];
+        token(k, a, step_h(a, before, bv, u), before, bv, at(c_, k), u, ds_[k * CPB]);
+        if (first[k] >= 0) {  // what reaches the initial state; nothing passes the start
           if (P.dh0 && live) {
 #pragma unroll
             for (int i = 0; i < S; ++i)
-              if (ok >> i & 1) P.dh0[(long long)first[k] * P.E * N + chan + (i ^ m)] = r.get(i);
+              if (ok >> i & 1) P.dh0[first[k] * per + chan + (i ^ m)] = r.get(i);
           }
           r = Lane<S>::all(0.f);
         }
-        y_[k * CPB * L] = y;
-        y_[(TT + k) * CPB * L] = dd;
-        y_[(2 * TT + k) * CPB * L] = gb;
-        // over the warp's channels: states i < half stay, the others go to the lane that keeps them
-        float v[2][S];
-#pragma unroll
-        for (int i = 0; i < S; ++i) {
-          v[0][i] = vb.get(i);
-          v[1][i] = vc.get(i);
-        }
-#pragma unroll
-        for (int x = 0; x < XB; ++x) {
-          const int half = S >> (x + 1);
-#pragma unroll
-          for (int i = 0; i < half; ++i)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-              v[b][i] += __shfl_xor_sync(0xffffffffu, v[b][i + half], (half / LEFT) << (RB + LB));
-        }
-        float* slot = s_ + k * 2 * G::NP;
-        if (RB > 0) {  // one of the other channel bits decides between dB and dC, the rest just add
-          const bool odd = lane & 1;
-#pragma unroll
-          for (int i = 0; i < LEFT; ++i) {
-            const float give = odd ? v[0][i] : v[1][i], keep = odd ? v[1][i] : v[0][i];
-            float o = keep + __shfl_xor_sync(0xffffffffu, give, 1);
-#pragma unroll
-            for (int x = 1; x < RB; ++x) o += __shfl_xor_sync(0xffffffffu, o, 1 << x);
-            if ((lane & ((1 << RB) - 1)) <= 1) slot[(odd ? G::NP : 0) + (i ^ m)] = o;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < LEFT; ++i) {
-            slot[i ^ m] = v[0][i];
-            slot[G::NP + (i ^ m)] = v[1][i];
-          }
-        }
       }
+    }
 #pragma unroll
-      for (int i = 0; i < S; ++i) sum_add(dA[i], dA_err[i], dAs.get(i));
-    };
-    if (scan_seg_flag(first, last)) segment(std::true_type{});
-    else segment(std::false_type{});
+    for (int i = 0; i < S; ++i) sum_add(dA[i], dA_err[i], dAs.get(i));
     __syncthreads();
   }
 #pragma unroll

@@ -17,51 +17,103 @@ struct ScanGrads {  // outputs of the backward's reductions
 template <typename T> int scan_fwd(const ScanParams& p, cudaStream_t st);
 template <typename T> int scan_bwd(const ScanParams& p, const ScanGrads& g, cudaStream_t st);
 
-// Lanes per channel for S states a lane.
-inline int scan_lanes(int N, int S) {
-  int l = S == 4 ? 2 : 4;
-  while (l * S < N) l <<= 1;
+// States per lane.  Four do the most work per value read from shared memory and per token that is
+// passed between the two sides; two give twice the CTAs, but spans give more of them for less (1 x 8192
+// tokens x 2048 channels, N = 16: forward and backward 374 + 1147 us with two states, one span).
+constexpr int SCAN_S = 4;
+
+// Lanes per channel.
+inline int scan_lanes(int N) {
+  int l = 2;
+  while (l * SCAN_S < N) l <<= 1;
   return l;
 }
 inline int scan_blocks(int E, int G, int L) {
   const int cpb = SCAN_WARPS * (32 / L);
   return (E / G + cpb - 1) / cpb;
 }
-// States per lane.  Four keep the most work per value read from shared memory; where they
-// leave more than half of the SMs without a CTA, two make twice the CTAs.  Measured (bf16, N = 16,
-// forward and backward, us): 4 x 4096 tokens x 2048 channels (256 CTAs of four states) 319 + 992
-// against 527 + 1537 with two; 1 x 8192 x 2048 (64 CTAs) 450 + 1453 against 377 + 1211.
-// More than 32 states run with four in any case.
-inline int scan_states(long long B, int E, int N, int G) {
-  if (N > 32) return 4;
-  return 2 * B * G * scan_blocks(E, G, scan_lanes(N, 4)) >= sm_count() ? 4 : 2;
+// Tokens of a span.  The cost of k spans, in tokens of a CTA that shares its SM with another one: the
+// scan's rounds of 2 CTAs per SM, and those of the carries, which weigh 0.75 of the forward's
+// time or 0.27 of the backward's (0.058 of 0.078 and of 0.217 us a token, measured: bf16, N = 16); a
+// round of one CTA per SM takes 0.68 of the time; a CTA's start and a launch count 40 tokens each, composing a
+// span's carry half a token of every CTA, on average.
+inline int scan_span(long long B, long long T, int E, int N, int G, bool backward) {
+  const long long ctas = B * G * scan_blocks(E, G, scan_lanes(N));
+  const int sms = sm_count();
+  const float weight = backward ? 0.27f : 0.75f;
+  auto rounds = [&](long long n) {
+    const long long full = n / (2 * sms), rest = n - full * 2 * sms;
+    return (float)full + (rest > sms ? 1.f : rest > 0 ? 0.68f : 0.f);
+  };
+  long long best = T;
+  float least = 0.f;
+  const long long most = std::min<long long>(64, T / 64);
+  for (long long k = 1; k == 1 || k <= most; ++k) {
+    const long long span = ((T + k - 1) / k + 31) / 32 * 32;
+    if (k > 1 && (T + span - 1) / span != k) continue;
+    const float t = (float)span + 40.f;
+    const float cost = rounds(ctas * k) * (t + 0.5f * k) + (k > 1 ? rounds(ctas * (k - 1)) * weight * t + 40.f : 0.f);
+    if (k == 1 || cost < least) {
+      least = cost;
+      best = span;
+    }
+  }
+  return (int)best;
+}
+inline int scan_spans(long long B, long long T, int E, int N, int G, bool backward) {
+  const int span = scan_span(B, T, E, N, G, backward);
+  return (int)((T + span - 1) / span);
+}
+// Bytes of the spans' carries (none for one span).
+inline size_t scan_carry_bytes(long long B, int spans, int E, int N) {
+  return spans > 1 ? (size_t)B * spans * E * N * 8 : 0;
 }
 // Floats of the backward's dB / dC partial sums.
 inline long long scan_part_floats(long long B, long long T, int E, int N, int G) {
-  const int L = scan_lanes(N, scan_states(B, E, N, G));
-  return B * ((T + SCAN_TT_BWD - 1) / SCAN_TT_BWD) * G * scan_blocks(E, G, L) * SCAN_TT_BWD * 2 * N;
+  return B * ((T + SCAN_TT_BWD - 1) / SCAN_TT_BWD) * G * scan_blocks(E, G, scan_lanes(N)) * SCAN_TT_BWD * 2 * N;
 }
 
 #ifdef SSM_SCAN_INSTANTIATE
-template <typename T, int L, int S, bool PAD>
+// P and c of the spans, if there are several.
+template <typename T, int L, bool PAD, bool REV>
+int launch_scan_carry(const ScanParams& p, cudaStream_t st) {
+  if (p.spans == 1) return KDA_OK;
+  const int smem = scan_carry_smem<T, ScanFwdGeo<T, L, SCAN_S>>(p.N, REV ? 3 : 2);
+  auto kernel = ssm_scan_carry_kernel<T, L, SCAN_S, PAD, REV>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan carry smem: ") + cudaGetErrorString(e));
+  {
+    TimedLaunch tl(REV ? K_SCAN_BWD : K_SCAN_FWD, st);
+    kernel<<<dim3(p.G * p.blocks, p.B, p.spans - 1), SCAN_THREADS, smem, st>>>(p);
+  }
+  return launch_check("scan carry");
+}
+
+template <typename T, int L, bool PAD>
 int launch_scan_fwd(ScanParams p, cudaStream_t st) {
+  constexpr int S = SCAN_S;
   using G = ScanFwdGeo<T, L, S>;
   p.blocks = scan_blocks(p.E, p.G, L);
+  const int rc = launch_scan_carry<T, L, PAD, false>(p, st);
+  if (rc) return rc;
   const int smem = scan_fwd_smem<T, G>(p.N);
   auto kernel = ssm_scan_fwd_kernel<T, L, S, PAD>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan forward smem: ") + cudaGetErrorString(e));
   {
     TimedLaunch tl(K_SCAN_FWD, st);
-    kernel<<<dim3(p.G * p.blocks, p.B), SCAN_THREADS, smem, st>>>(p);
+    kernel<<<dim3(p.G * p.blocks, p.B, p.spans), SCAN_THREADS, smem, st>>>(p);
   }
   return launch_check("scan forward");
 }
 
-template <typename T, int L, int S, bool PAD>
+template <typename T, int L, bool PAD>
 int launch_scan_bwd(ScanParams p, const ScanGrads& g, cudaStream_t st) {
+  constexpr int S = SCAN_S;
   using G = ScanBwdGeo<T, L, S>;
   p.blocks = scan_blocks(p.E, p.G, L);
+  const int rc = launch_scan_carry<T, L, PAD, true>(p, st);
+  if (rc) return rc;
   const int smem = scan_bwd_smem<T, G>(p.N);
   auto kernel = ssm_scan_bwd_kernel<T, L, S, PAD>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -70,35 +122,33 @@ int launch_scan_bwd(ScanParams p, const ScanGrads& g, cudaStream_t st) {
   const long long cols = (long long)p.E * (p.N + 2);
   {
     TimedLaunch tl(K_SCAN_BWD, st);
-    kernel<<<dim3(p.G * p.blocks, p.B), SCAN_THREADS, smem, st>>>(p);
+    kernel<<<dim3(p.G * p.blocks, p.B, p.spans), SCAN_THREADS, smem, st>>>(p);
     ssm_scan_bc_kernel<T><<<dim3((unsigned)((long long)p.B * tiles * p.G), (per + SCAN_BC_THREADS - 1) / SCAN_BC_THREADS),
                             SCAN_BC_THREADS, 0, st>>>(p.bc_part, p.T, tiles, p.G, p.blocks, p.N, static_cast<T*>(g.dB),
                                                       static_cast<T*>(g.dC));
     ssm_reduce_kernel<<<(unsigned)((cols + SSM_REDUCE_COLS - 1) / SSM_REDUCE_COLS), SSM_REDUCE_COLS * SSM_REDUCE_SLICES,
-                        0, st>>>(p.e_part, p.B, cols, p.N, p.N + 2, g.dA, g.dD, g.ddt_bias);
+                        0, st>>>(p.e_part, (long long)p.B * p.spans, cols, p.N, p.N + 2, g.dA, g.dD, g.ddt_bias);
   }
   return launch_check("scan backward");
 }
 
 template <typename T>
 int scan_fwd(const ScanParams& p, cudaStream_t st) {
-  const int S = scan_states(p.B, p.E, p.N, p.G), L = scan_lanes(p.N, S);
-  const bool pad = p.N != L * S;
-#define SCAN_CASE(l, s) \
-  if (L == l && S == s) return pad ? launch_scan_fwd<T, l, s, true>(p, st) : launch_scan_fwd<T, l, s, false>(p, st);
-  SCAN_CASE(2, 4) SCAN_CASE(4, 4) SCAN_CASE(8, 4) SCAN_CASE(16, 4)
-  SCAN_CASE(4, 2) SCAN_CASE(8, 2) SCAN_CASE(16, 2)
+  const int L = scan_lanes(p.N);
+  const bool pad = p.N != L * SCAN_S;
+#define SCAN_CASE(l) \
+  if (L == l) return pad ? launch_scan_fwd<T, l, true>(p, st) : launch_scan_fwd<T, l, false>(p, st);
+  SCAN_CASE(2) SCAN_CASE(4) SCAN_CASE(8) SCAN_CASE(16)
 #undef SCAN_CASE
   return fail(KDA_ERR_UNSUPPORTED, "no scan kernel for this state size");
 }
 template <typename T>
 int scan_bwd(const ScanParams& p, const ScanGrads& g, cudaStream_t st) {
-  const int S = scan_states(p.B, p.E, p.N, p.G), L = scan_lanes(p.N, S);
-  const bool pad = p.N != L * S;
-#define SCAN_CASE(l, s) \
-  if (L == l && S == s) return pad ? launch_scan_bwd<T, l, s, true>(p, g, st) : launch_scan_bwd<T, l, s, false>(p, g, st);
-  SCAN_CASE(2, 4) SCAN_CASE(4, 4) SCAN_CASE(8, 4) SCAN_CASE(16, 4)
-  SCAN_CASE(4, 2) SCAN_CASE(8, 2) SCAN_CASE(16, 2)
+  const int L = scan_lanes(p.N);
+  const bool pad = p.N != L * SCAN_S;
+#define SCAN_CASE(l) \
+  if (L == l) return pad ? launch_scan_bwd<T, l, true>(p, g, st) : launch_scan_bwd<T, l, false>(p, g, st);
+  SCAN_CASE(2) SCAN_CASE(4) SCAN_CASE(8) SCAN_CASE(16)
 #undef SCAN_CASE
   return fail(KDA_ERR_UNSUPPORTED, "no scan kernel for this state size");
 }

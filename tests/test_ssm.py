@@ -23,7 +23,8 @@ ROUND = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -1
 gpu = pytest.mark.gpu
 
 
-def close(name, got, want, dtype):
+def close_each(name, got, want, dtype):
+    """Every value within its rounding and the arithmetic's error."""
     got, want = got.detach().double(), want.detach().double()
     assert got.shape == want.shape, name
     if not want.numel():
@@ -34,6 +35,11 @@ def close(name, got, want, dtype):
     tol = tol + (2.0 ** -24 if dtype == torch.float16 else 0.0)  # fp16 subnormals
     worst = ((got - want).abs() - tol).max()
     assert worst <= 0, f"{name}: {float((got - want).abs().max())} off, rms {float(rms)}"
+
+
+def close(name, got, want, dtype):
+    close_each(name, got, want, dtype)
+    got, want = got.detach().double(), want.detach().double()
     assert (got - want).norm() <= (1e-5 + ROUND[dtype] / 2) * want.norm() + 1e-30, name
 
 
@@ -188,6 +194,71 @@ def test_scan_forward_and_gradients(case):
     for k in want:
         close("d_" + k, grads[k], want[k], ts[k].dtype)
     assert sophia_b200._lib.device_error(reset=True) == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N", [4, 16, 5, 48])
+def test_sequences_start_and_end_at_every_place_of_a_segment(dtype, N):
+    """Value by value: a few dozen outputs are too few for a bound on their mean rounding."""
+    for tail in [(1,), (2,), (3,), (4,), (5,), (6,), (7,), (8,), (1, 1), (1, 1, 1), (2, 3, 1), (1, 0, 8)]:
+        for T in (8, 21, 56):
+            docs = (T - sum(tail), *tail) if T > sum(tail) else tail
+            ts, dy, dht = scan_tensors(dtype, 1, sum(docs), 12, N, 1, True, True, True, True, docs)
+            cu = cu_of(docs)
+            y, ht, grads = run_scan(ts, cu, True, dy, dht)
+            ry, rht, want = reference_scan(ts, cu, True, dy, dht)
+            close_each("y", y, ry, dtype)
+            close_each("final_state", ht, rht, torch.float32)
+            for k in want:
+                close_each("d_" + k, grads[k], want[k], ts[k].dtype)
+
+
+SPANS = [  # few channels and many tokens: the tokens are cut into spans
+    (torch.float32, 1, 1500, 8, 16, 1, True, None),
+    (torch.float32, 2, 1111, 40, 5, 2, True, None),
+    (torch.bfloat16, 1, 2049, 24, 16, 1, False, None),
+    (torch.float32, 1, 1400, 8, 16, 1, True, (64, 1, 63, 127, 1, 0, 500, 2, 642)),
+    (torch.bfloat16, 1, 1030, 16, 32, 1, True, (1, 1028, 1)),
+    (torch.float16, 1, 777, 20, 8, 1, False, (255, 1, 521)),
+    (torch.float32, 3, 600, 72, 64, 1, True, None),
+]
+
+
+@gpu
+@pytest.mark.parametrize("case", SPANS, ids=lambda c: "-".join(str(v).replace("torch.", "").replace(" ", "") for v in c))
+def test_scan_of_few_rows(case):
+    dtype, B, T, E, N, G, state, docs = case
+    ts, dy, dht = scan_tensors(dtype, B, T, E, N, G, True, True, True, state, docs)
+    cu = cu_of(docs)
+    y, ht, grads = run_scan(ts, cu, True, dy, dht)
+    ry, rht, want = reference_scan(ts, cu, True, dy, dht)
+    close("y", y, ry, dtype)
+    close("final_state", ht, rht, torch.float32)
+    for k in want:
+        close("d_" + k, grads[k], want[k], ts[k].dtype)
+
+
+@gpu
+def test_spans_keep_infinities_and_growing_states():
+    """A state that grows (positive rates) and one that is infinite cross the spans; a document behind
+    them sees neither."""
+    E, N, T = 8, 4, 1000
+    rn = gen(5)
+    x, Bm, Cm = rn(1, T, E), rn(1, T, N), rn(1, T, N)
+    dt = torch.full((1, T, E), 0.02, device="cuda")
+    A = torch.full((E, N), 0.5, device="cuda")
+    y, _ = sophia_b200.selective_scan(x, dt, A, Bm, Cm, dt_softplus=False)
+    want, _ = ref.scan(x.double(), dt.double(), A.double(), Bm[:, :, None].double(), Cm[:, :, None].double(), None, None,
+                       None, None, None, False)
+    assert torch.isfinite(y).all()
+    assert ((y.double() - want).norm() <= 1e-4 * want.norm())
+    x[:, 100, 3] = float("inf")
+    cu = cu_of((700, 300))
+    y, ht = sophia_b200.selective_scan(x, dt, -A, Bm, Cm, dt_softplus=False, cu_seqlens=cu, output_final_state=True)
+    assert not torch.isfinite(y[:, 100:700, 3]).any() and not torch.isfinite(ht[0, 3]).any()
+    assert torch.isfinite(y[:, :100]).all() and torch.isfinite(y[:, 700:]).all() and torch.isfinite(ht[1]).all()
+    assert torch.isfinite(y[:, :, [0, 1, 2, 4, 5, 6, 7]]).all()
 
 
 @gpu
