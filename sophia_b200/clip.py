@@ -81,7 +81,8 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
                     out: Sequence[Tensor] | Tensor | None = None) -> Tensor:
     """Scales the gradients by ``min(1, max_norm / (norm + eps))``, ``norm``
     their global 2-norm, and returns the norm (0-d float32 CUDA tensor, before
-    clipping).  In place by default; with ``out``, tensors of the gradients' shapes and of any
+    clipping).  It takes the gradients themselves, not the parameters that hold them.  In place
+    by default; with ``out``, tensors of the gradients' shapes and of any
     supported type (an optimizer's float32 gradients), every element of which is
     written, the gradients stay as they are.  ``out[i] is grads[i]`` is allowed; otherwise no two
     tensors may overlap.  A NaN norm makes the scaled gradients NaN, an infinite one 0 (and
@@ -106,6 +107,8 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
         where = [o.data_ptr() for o in outs if o.numel()]
         if len(set(where)) != len(where):
             raise ValueError(f"{what}: one tensor is named twice")
+        if any(o.requires_grad for o in outs):
+            raise ValueError(f"{what} scales gradients; a tensor that requires grad (a parameter?) is not one")
         if all(map(Tensor.is_contiguous, ts)) and (outs is ts or all(map(Tensor.is_contiguous, outs))):
             return _launch(ts, types, outs, out_types, max_norm, eps)
         src, dst, back = list(ts), list(outs), []

@@ -146,3 +146,7 @@ def test_refusals_of_outputs():
         sophia_b200.clip_grad_norm_([t], 1.0, out=[])
     with pytest.raises(ValueError):
         sophia_b200.clip_grad_norm_([t], 1.0, out=[torch.zeros(4, device="cuda")])
+    w = torch.nn.Parameter(torch.ones(3, device="cuda"))
+    with pytest.raises(ValueError):
+        sophia_b200.clip_grad_norm_([w], 1.0)
+    assert (w == 1).all()
