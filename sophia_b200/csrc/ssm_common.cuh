@@ -112,13 +112,6 @@ struct Lane {
     for (int k = 0; k < S / 2; ++k) r.p[k] = pk2(v, v);
     return r;
   }
-  __device__ __forceinline__ float sum() const {
-    u64 t = p[0];
-#pragma unroll
-    for (int k = 1; k < S / 2; ++k) t = add2(t, p[k]);
-    const float2 f = upk2(t);
-    return f.x + f.y;
-  }
   __device__ __forceinline__ Lane exp2() const {
     Lane r;
 #pragma unroll
@@ -158,6 +151,15 @@ struct Lane<1> {
   friend __device__ __forceinline__ Lane operator+(const Lane& a, const Lane& b) { return {a.f + b.f}; }
   friend __device__ __forceinline__ Lane fma(const Lane& a, const Lane& b, const Lane& c) { return {fmaf(a.f, b.f, c.f)}; }
 };
+// sum of a b over a lane's states
+template <int S>
+__device__ __forceinline__ float lane_dot(const Lane<S>& a, const Lane<S>& b) {
+  u64 t = mul2(a.p[0], b.p[0]);
+#pragma unroll
+  for (int k = 1; k < S / 2; ++k) t = fma2(a.p[k], b.p[k], t);
+  const float2 f = upk2(t);
+  return f.x + f.y;
+}
 template <int S>
 __device__ __forceinline__ Lane<S> lane_sigmoid(const Lane<S>& v) {
   Lane<S> d = (v * Lane<S>::all(-LOG2E)).exp2() + Lane<S>::all(1.f);

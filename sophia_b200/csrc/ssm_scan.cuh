@@ -285,17 +285,21 @@ __device__ __forceinline__ float2 scan_pair(const T* p) {
   io_load<T, 2>(p, f);
   return make_float2(f[0], f[1]);
 }
-// Stores a pair of a row's channels c, c+1 (of nc).
+// Stores a pair of channels of a [B, T, E] output at element `at`: how is 2 for both at once, 1 one by one,
+// bit 2 without the first and bit 3 without the second.
 template <typename T>
-__device__ __forceinline__ void scan_put_pair(void* out, const ScanParams& P, const ScanBlock& s, int t, int c, float2 v) {
-  T* p = static_cast<T*>(out) + ((long long)s.b * P.T + t) * P.E + s.c0 + c;
-  if (P.vec && c + 1 < s.nc) {
+__device__ __forceinline__ void scan_put_pair(void* out, long long at, int how, float2 v) {
+  T* p = static_cast<T*>(out) + at;
+  if (how == 2) {
     const float f[2] = {v.x, v.y};
     io_store<T, 2>(p, f);
   } else {
-    if (c < s.nc) p[0] = io_from_f<T>(v.x);
-    if (c + 1 < s.nc) p[1] = io_from_f<T>(v.y);
+    if (!(how & 4)) p[0] = io_from_f<T>(v.x);
+    if (!(how & 8)) p[1] = io_from_f<T>(v.y);
   }
+}
+__device__ __forceinline__ int scan_how(const ScanParams& P, const ScanBlock& s, int c) {
+  return P.vec && c + 1 < s.nc ? 2 : 1 | (c < s.nc ? 0 : 4) | (c + 1 < s.nc ? 0 : 8);
 }
 // Sum of a channel's L partial sums.
 template <int L>
@@ -323,6 +327,7 @@ template <int TT>
 struct ScanFlags {
   int f, l;
   __device__ __forceinline__ void read(const ScanParams& P, int b, int t0, int tid) {
+    if (tid >= 32) return;  // (TT <= 32: the first warp's)
     const int t = t0 + tid;
     const bool in = tid < TT && t >= 0 && t < P.T;
     f = in ? seq_start_at(P.seq, b, t) : -1;
@@ -417,7 +422,7 @@ __device__ __forceinline__ Lane<S> scan_enter(const ScanParams& P, const ScanBlo
 // P and c of the spans that have one behind them (REV: in front, for the backward's g, where
 // u = dy silu(z) and C stand for d x and B).  The same layout as the scan's, without its outputs.
 template <typename T, int L, int S, bool PAD, bool REV>
-__global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_carry_kernel(ScanParams P) {
+__global__ void __launch_bounds__(SCAN_THREADS, 3) ssm_scan_carry_kernel(ScanParams P) {
   using G = ScanFwdGeo<T, L, S>;
   constexpr int TT = G::TT, CPB = G::CPB, TENSORS = REV ? 3 : 2;
   extern __shared__ __align__(16) char scan_sm[];
@@ -618,6 +623,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
       marks.write(flags + q * 2 * TT, tid);
       marks.read(P, s.b, t0 + TT, tid);
     };
+    const int how = scan_how(P, s, pc);
+    long long at = ((long long)s.b * P.T + first_t + pt) * P.E + s.c0 + pc;  // of the tile to finish
+    const long long row_step = (long long)G::TSTEP * P.E;
     auto finish = [&](int i) {
       const int t0 = first_t + i * TT;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
@@ -634,7 +642,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
           v.x *= siluf_(z.x);
           v.y *= siluf_(z.y);
         }
-        if (t0 + t < P.T) scan_put_pair<T>(P.y, P, s, t0 + t, pc, v);
+        if (t0 + t < P.T) scan_put_pair<T>(P.y, at, how, v);
+        at += row_step;
       }
     };
     f.fetch(P, s, views, raw, first_t, tid);
@@ -688,7 +697,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
 #pragma unroll
       for (int k = 0; k < SCAN_SEG; ++k) {
         h = lane_keep<PAD>(fma(lane_decay(a2, du[k].x), h, bv[k] * Lane<S>::all(du[k].y)), ok);
-        y[k] = (h * cv[k]).sum();
+        y[k] = lane_dot(h, cv[k]);
       }
 #pragma unroll
       for (int k = 0; k < SCAN_SEG; ++k) y_[(t1 + k) * CPB * L] = y[k];
@@ -705,7 +714,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
           for (int i = 0; i < S; ++i)
             if (live && (ok >> i & 1)) P.ht[last[t] * per + chan + i] = h.get(i);
         }
-        y_[t * CPB * L] = (h * Lane<S>::load(c_ + t * G::NP)).sum();
+        y_[t * CPB * L] = lane_dot(h, Lane<S>::load(c_ + t * G::NP));
       }
     };
 #pragma unroll 1
@@ -767,6 +776,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     // (both passes: all reads of shared memory, then all writes)
     constexpr int IT = TT / G::TSTEP;
     const bool spare = G::SPARE && pt >= TT;
+    int p3 = 0, q3 = 0;  // buffers of the next tile to prepare and to finish
     auto prepare = [&](int i) {
       const int t0 = (tile_z - i) * TT, q = i & 1;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
@@ -784,7 +794,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
       }
       bc.load(rx + 4 * G::RAW, npad, P, s, t0, tid);
       if (!spare) {
-        const int at = ((i % 3) * TT + pt) * CPB + pc;
+        const int at = (p3 * TT + pt) * CPB + pc;
         float4 du[IT];
 #pragma unroll
         for (int k = 0; k < IT; ++k) {
@@ -805,12 +815,20 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
           if (P.z.p) *reinterpret_cast<float2*>(DZ + at + k * G::TSTEP * CPB) = z[k];
         }
       }
+      p3 = p3 == 2 ? 0 : p3 + 1;
       bc.store(Bs + q * TT * S * G::NP, Cs + q * TT * S * G::NP, tid);
       marks.write(flags + q * 2 * TT, tid);
       marks.read(P, s.b, t0 - TT, tid);
     };
+    const int how = scan_how(P, s, pc);
+    long long to = ((long long)s.b * P.T + tile_z * TT + pt) * P.E + s.c0 + pc;  // of the tile to finish
+    const long long to_step = (long long)TT * P.E, row_step = (long long)G::TSTEP * P.E;
+    // the tile's dB and dC over the warps, [TT][2][N], and the step to the tile in front
+    const long long part_step = (long long)P.G * P.blocks * (TT * 2 * N);
+    float* part = P.bc_part + ((long long)s.b * all + tile_z) * part_step + (s.g * P.blocks + s.blk) * (TT * 2 * N);
     auto finish = [&](int i) {
-      const int tile = tile_z - i, t0 = tile * TT, q = i & 1, at = ((i % 3) * TT + pt) * CPB + pc;
+      const int t0 = (tile_z - i) * TT, q = i & 1, at = (q3 * TT + pt) * CPB + pc;
+      q3 = q3 == 2 ? 0 : q3 + 1;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
       if (!spare) {
 #pragma unroll
@@ -832,12 +850,11 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
             dd.y *= sigmoidf_(dt.y + bias.y);
           }
           if (t0 + t < P.T) {
+            const long long o = to + k * row_step;
             if (P.z.p)
-              scan_put_pair<T>(P.dz, P, s, t0 + t, pc,
-                               make_float2(dz.x * fmaf(skip.x, x.x, s0), dz.y * fmaf(skip.y, x.y, s1)));
-            scan_put_pair<T>(P.ddt, P, s, t0 + t, pc, dd);
-            scan_put_pair<T>(P.dx, P, s, t0 + t, pc,
-                             make_float2(fmaf(g0, du.x, ds.x * skip.x), fmaf(g1, du.z, ds.y * skip.y)));
+              scan_put_pair<T>(P.dz, o, how, make_float2(dz.x * fmaf(skip.x, x.x, s0), dz.y * fmaf(skip.y, x.y, s1)));
+            scan_put_pair<T>(P.ddt, o, how, dd);
+            scan_put_pair<T>(P.dx, o, how, make_float2(fmaf(g0, du.x, ds.x * skip.x), fmaf(g1, du.z, ds.y * skip.y)));
             sum_add(db.x, db_err.x, dd.x);
             sum_add(db.y, db_err.y, dd.y);
             sum_add(dD.x, dD_err.x, ds.x * x.x);
@@ -845,8 +862,6 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
           }
         }
       }
-      // the tile's dB and dC over the warps, [TT][2][N]
-      float* part = P.bc_part + ((((long long)s.b * all + tile) * P.G + s.g) * P.blocks + s.blk) * (TT * 2 * N);
       const float* sl = slots + q * SCAN_WARPS * TT * 2 * G::NP;
 #pragma unroll
       for (int i0 = 0; i0 < TT * 2 * G::NP; i0 += G::TOKENS) {
@@ -858,6 +873,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
         for (int w = 0; w < SCAN_WARPS; ++w) o += sl[w * TT * 2 * G::NP + j];
         if (!PAD || n < N) part[j / G::NP * N + n] = o;
       }
+      to -= to_step;
+      part -= part_step;
     };
     f.fetch(P, s, views, raw, tile_z * TT, tid);
     if (tiles > 1) f.fetch(P, s, views, raw + stage, (tile_z - 1) * TT, tid);
@@ -940,7 +957,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
       r = a * g;
       const Lane<S> w = lane_keep<PAD>(r * before, ok);
       dAs = fma(w, Lane<S>::all(u.x), dAs);
-      const float y = (h * cv).sum(), dd = (w * a2).sum(), gb = (g * bv).sum();
+      const float y = lane_dot(h, cv), dd = lane_dot(w, a2), gb = lane_dot(g, bv);
       const Lane<S> vb = g * Lane<S>::all(u.y), vc = ds * h;  // dB, dC of this channel
       y_[k * CPB * L] = y;
       y_[(TT + k) * CPB * L] = dd;

@@ -32,19 +32,18 @@ inline int scan_blocks(int E, int G, int L) {
   const int cpb = SCAN_WARPS * (32 / L);
   return (E / G + cpb - 1) / cpb;
 }
-// Tokens of a span.  The cost of k spans, in tokens of a CTA that shares its SM with another one: the
-// scan's rounds of 2 CTAs per SM, and those of the carries, which weigh 0.75 of the forward's
-// time or 0.27 of the backward's (0.058 of 0.078 and of 0.217 us a token, measured: bf16, N = 16); a
-// round of one CTA per SM takes 0.68 of the time; a CTA's start and a launch count 40 tokens each, composing a
-// span's carry half a token of every CTA, on average.
+// Tokens of a span: of the numbers k of spans the one that costs least, in tokens of a CTA of the scan that shares
+// its SM with another.  An SM takes its CTAs two at a time, three at a time in the carries' kernel; a
+// lone CTA takes 0.68 (there 0.5, two 0.71) of a full SM's time; the carries' token costs
+// 1.04 of the forward's, 0.37 of the backward's (0.081 us of 0.078 and 0.217, measured: bf16, N = 16); a
+// CTA's start and a launch count 40 tokens each, composing a span's carry half a token of every
+// CTA, on average.
 inline int scan_span(long long B, long long T, int E, int N, int G, bool backward) {
   const long long ctas = B * G * scan_blocks(E, G, scan_lanes(N));
   const int sms = sm_count();
-  const float weight = backward ? 0.27f : 0.75f;
-  auto rounds = [&](long long n) {
-    const long long full = n / (2 * sms), rest = n - full * 2 * sms;
-    return (float)full + (rest > sms ? 1.f : rest > 0 ? 0.68f : 0.f);
-  };
+  const float weight = backward ? 0.37f : 1.04f;
+  auto two = [&](long long n) { return (float)(n / 2) + (n % 2 ? 0.68f : 0.f); };
+  auto three = [&](long long n) { return (float)(n / 3) + (n % 3 == 2 ? 0.71f : n % 3 ? 0.5f : 0.f); };
   long long best = T;
   float least = 0.f;
   const long long most = std::min<long long>(64, T / 64);
@@ -52,7 +51,8 @@ inline int scan_span(long long B, long long T, int E, int N, int G, bool backwar
     const long long span = ((T + k - 1) / k + 31) / 32 * 32;
     if (k > 1 && (T + span - 1) / span != k) continue;
     const float t = (float)span + 40.f;
-    const float cost = rounds(ctas * k) * (t + 0.5f * k) + (k > 1 ? rounds(ctas * (k - 1)) * weight * t + 40.f : 0.f);
+    const float cost = two((ctas * k + sms - 1) / sms) * (t + 0.5f * k) +
+                       (k > 1 ? three((ctas * (k - 1) + sms - 1) / sms) * weight * t + 40.f : 0.f);
     if (k == 1 || cost < least) {
       least = cost;
       best = span;
