@@ -167,6 +167,7 @@ int check_scan(const kda_b200_scan_args* a, bool step) {
   if (a->E % a->G) return fail(KDA_ERR_INVALID, "the groups must divide the channels");
   if (a->N > SCAN_MAX_N) return fail(KDA_ERR_UNSUPPORTED, "more than 64 states per channel");
   if (step) {
+    if ((long long)a->E * a->N > INT32_MAX) return fail(KDA_ERR_UNSUPPORTED, "too many channels");
     if (a->rows < 0 || a->pool < 0) return fail(KDA_ERR_INVALID, "rows >= 0 and pool >= 0 are required");
     if (!a->slots && a->rows > a->pool) return fail(KDA_ERR_INVALID, "more rows than states");
     if (a->rows > 0 && (!a->x || !a->dt || !a->A || !a->B_ || !a->C_ || !a->state || !a->y))
@@ -207,15 +208,19 @@ void scan_cut(ScanParams& p, Carver& cv, bool backward) {
   p.carry = p.spans > 1 ? cv.take<float2>(scan_carry_bytes(p.B, p.spans, p.E, p.N)) : nullptr;
 }
 
-template <typename T, int LP>
+template <typename T, int LP, int Q>
 int launch_scan_step(const ScanStepParams& p, cudaStream_t st) {
   const long long gx = ((long long)p.E * LP + STEP_THREADS - 1) / STEP_THREADS;
-  const int gy = (int)std::max(1LL, std::min((long long)p.rows, (16LL * sm_count() + gx - 1) / gx));
-  const bool vec = p.N % 4 == 0 && aligned(p.state, 16);
+  const int gy = (int)std::max(1LL, std::min((long long)p.rows, (8LL * sm_count() + gx - 1) / gx));
+  const size_t piece = 4 * sizeof(T);
+  auto fours = [&](const void* q, long long sb, long long sg) {
+    return aligned(q, piece) && (p.rows == 1 || sb % 4 == 0) && (p.G == 1 || sg % 4 == 0);
+  };
+  const bool vec = p.N % 4 == 0 && aligned(p.state, 16) && fours(p.Bm, p.b_sb, p.b_sg) && fours(p.Cm, p.c_sb, p.c_sg);
   {
     TimedLaunch tl(K_SCAN_STEP, st);
-    if (vec) ssm_scan_step_kernel<T, LP, true><<<dim3((unsigned)gx, gy), STEP_THREADS, 0, st>>>(p);
-    else ssm_scan_step_kernel<T, LP, false><<<dim3((unsigned)gx, gy), STEP_THREADS, 0, st>>>(p);
+    if (vec) ssm_scan_step_kernel<T, LP, Q, true><<<dim3((unsigned)gx, gy), STEP_THREADS, 0, st>>>(p);
+    else ssm_scan_step_kernel<T, LP, Q, false><<<dim3((unsigned)gx, gy), STEP_THREADS, 0, st>>>(p);
   }
   return launch_check("scan step");
 }
@@ -223,11 +228,11 @@ int launch_scan_step(const ScanStepParams& p, cudaStream_t st) {
 template <typename T>
 int scan_step(const ScanStepParams& p, cudaStream_t st) {
   const int quads = (p.N + 3) / 4;
-  if (quads <= 1) return launch_scan_step<T, 1>(p, st);
-  if (quads <= 2) return launch_scan_step<T, 2>(p, st);
-  if (quads <= 4) return launch_scan_step<T, 4>(p, st);
-  if (quads <= 8) return launch_scan_step<T, 8>(p, st);
-  return launch_scan_step<T, 16>(p, st);
+  if (quads <= 1) return launch_scan_step<T, 1, 1>(p, st);
+  if (quads <= 2) return launch_scan_step<T, 1, 2>(p, st);
+  if (quads <= 4) return launch_scan_step<T, 2, 2>(p, st);
+  if (quads <= 8) return launch_scan_step<T, 4, 2>(p, st);
+  return launch_scan_step<T, 8, 2>(p, st);
 }
 
 // ---- gradient clipping
