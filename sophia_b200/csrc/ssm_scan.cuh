@@ -67,6 +67,11 @@ struct ScanGeo {
   static constexpr int TSTEP = TOKENS / PAIRS < TT ? TOKENS / PAIRS : TT;  // tokens per pass of the side
   static constexpr bool SPARE = TOKENS / PAIRS > TT;  // threads without a token
   static constexpr int V = 16 / (int)sizeof(T), NV = CPB / V;  // 16-byte pieces of a row
+  // partial sums over the lanes, [TT][L][CPB and a pad]: neither the lanes' stores nor the reads of channel
+  // pairs share a bank
+  static constexpr int YS = CPB + CH, YT = L * YS;
+  // the backward's S versions of B and C, [TT][S and a pad][NP], likewise
+  static constexpr int BS = (S + 1) * NP;
 };
 template <typename T, int L, int S>
 using ScanFwdGeo = ScanGeo<T, L, S, sizeof(T) == 2 ? 32 : 16>;
@@ -279,7 +284,7 @@ struct ScanBC {
         IoVec<float, G::S> o;
 #pragma unroll
         for (int q = 0; q < G::S; ++q) o.v[q] = v[k][q ^ w];
-        *reinterpret_cast<IoVec<float, G::S>*>(dst + (t * VERS + w) * G::NP + n0) = o;
+        *reinterpret_cast<IoVec<float, G::S>*>(dst + t * (VERS == 1 ? G::NP : G::BS) + w * G::NP + n0) = o;
       }
     }
   }
@@ -308,18 +313,13 @@ __device__ __forceinline__ void scan_put_pair(void* out, long long at, int how, 
 __device__ __forceinline__ int scan_how(const ScanParams& P, const ScanBlock& s, int c) {
   return P.vec && c + 1 < s.nc ? 2 : 1 | (c < s.nc ? 0 : 4) | (c + 1 < s.nc ? 0 : 8);
 }
-// Sum of a channel's L partial sums.
-template <int L>
-__device__ __forceinline__ float scan_join(const float* p) {
-  constexpr int V = L < 4 ? L : 4;
-  float acc = 0.f;
+// Sums of a channel pair's L partial sums.
+template <typename G>
+__device__ __forceinline__ float2 scan_join(const float* p) {
+  u64 acc = *reinterpret_cast<const u64*>(p);
 #pragma unroll
-  for (int q = 0; q < L / V; ++q) {
-    const IoVec<float, V> v = *reinterpret_cast<const IoVec<float, V>*>(p + q * V);
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc += v.v[k];
-  }
-  return acc;
+  for (int l = 1; l < G::L; ++l) acc = add2(acc, *reinterpret_cast<const u64*>(p + l * G::YS));
+  return upk2(acc);
 }
 
 // d of a token, 0 past the row's end.
@@ -364,12 +364,12 @@ __host__ __device__ inline int scan_stage_elems(int N, int tensors) {
 template <typename T, typename G>
 __host__ __device__ inline int scan_fwd_smem(int N) {
   return SCAN_STAGES * scan_stage_elems<T, G>(N, 3) * (int)sizeof(T) +
-         2 * (G::TT * G::CPB * 8 + 2 * G::TT * G::NP * 4 + G::TT * G::CPB * G::L * 4 + 2 * G::TT * 4);
+         2 * (G::TT * G::CPB * 8 + 2 * G::TT * G::NP * 4 + G::TT * G::YT * 4 + 2 * G::TT * 4);
 }
 template <typename T, typename G>
 __host__ __device__ inline int scan_bwd_smem(int N) {
   return SCAN_STAGES * scan_stage_elems<T, G>(N, 4) * (int)sizeof(T) +
-         3 * G::TT * G::CPB * 16 + 2 * (2 * G::TT * G::S * G::NP * 4 + 3 * G::TT * G::CPB * G::L * 4 +
+         3 * G::TT * G::CPB * 16 + 2 * (2 * G::TT * G::BS * 4 + 3 * G::TT * G::YT * 4 +
                                         SCAN_WARPS * G::TT * 2 * G::NP * 4 + 2 * G::TT * 4);
 }
 
@@ -584,8 +584,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
   float2* DU = reinterpret_cast<float2*>(raw + SCAN_STAGES * stage);  // [TT][CPB]: d, d x
   float* Bs = reinterpret_cast<float*>(DU + 2 * TT * CPB);            // [TT][NP]
   float* Cs = Bs + 2 * TT * G::NP;
-  float* YP = Cs + 2 * TT * G::NP;                                    // [TT][CPB][L]
-  int* flags = reinterpret_cast<int*>(YP + 2 * TT * CPB * L);         // first [TT], last [TT]
+  float* YP = Cs + 2 * TT * G::NP;                                    // [TT][L][YS]
+  int* flags = reinterpret_cast<int*>(YP + 2 * TT * G::YT);           // first [TT], last [TT]
   const ScanBlock s = scan_block<CPB, TT>(P, blockIdx.z);
   const int tiles = s.tiles, first_t = s.tile0 * TT, segs = (P.T + SCAN_SEG - 1) / SCAN_SEG;
 
@@ -636,14 +636,14 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
     auto finish = [&](int i) {
       const int t0 = first_t + i * TT;
       const T* rx = raw + (i % SCAN_STAGES) * stage;
-      const float* yp = YP + (i & 1) * TT * CPB * L;
+      const float* yp = YP + (i & 1) * TT * G::YT;
       if (spare) return;
 #pragma unroll
       for (int k = 0; k < TT; k += G::TSTEP) {
         const int t = pt + k;
         const float2 x = scan_pair(rx + t * CPB + pc);
-        float2 v = make_float2(fmaf(skip.x, x.x, scan_join<L>(yp + (t * CPB + pc) * L)),
-                               fmaf(skip.y, x.y, scan_join<L>(yp + (t * CPB + pc + 1) * L)));
+        const float2 sum = scan_join<G>(yp + t * G::YT + pc);
+        float2 v = make_float2(fmaf(skip.x, x.x, sum.x), fmaf(skip.y, x.y, sum.y));
         if (P.z.p) {
           const float2 z = scan_pair(rx + 2 * G::RAW + t * CPB + pc);
           v.x *= siluf_(z.x);
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
     const float2* du_ = DU + q * TT * CPB + c;
     const float* b_ = Bs + q * TT * G::NP + n0;
     const float* c_ = Cs + q * TT * G::NP + n0;
-    float* y_ = YP + q * TT * CPB * L + c * L + l;
+    float* y_ = YP + q * TT * G::YT + l * G::YS + c;
     const int* first = flags + q * 2 * TT;
     const int* last = first + TT;
     auto segment = [&](int t1) {
@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
         y[k] = lane_dot(h, cv[k]);
       }
 #pragma unroll
-      for (int k = 0; k < SCAN_SEG; ++k) y_[(t1 + k) * CPB * L] = y[k];
+      for (int k = 0; k < SCAN_SEG; ++k) y_[(t1 + k) * G::YT] = y[k];
     };
     auto flagged = [&](int t1) {  // sequences start or end among the tokens
       const long long per = (long long)P.E * N;
@@ -721,7 +721,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
           for (int i = 0; i < S; ++i)
             if (live && (ok >> i & 1)) P.ht[last[t] * per + chan + i] = h.get(i);
         }
-        y_[t * CPB * L] = lane_dot(h, Lane<S>::load(c_ + t * G::NP));
+        y_[t * G::YT] = lane_dot(h, Lane<S>::load(c_ + t * G::NP));
       }
     };
 #pragma unroll 1
@@ -759,10 +759,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
   float* DS = reinterpret_cast<float*>(DU + 3 * TT * CPB);            // [TT][CPB]: dy silu(z)
   float* DZ = DS + 3 * TT * CPB;                                      // [TT][CPB]: dy silu'(z)
   // double buffers:
-  float* Bs = DZ + 3 * TT * CPB;                                      // [TT][S][NP]
-  float* Cs = Bs + 2 * TT * S * G::NP;
-  float* YP = Cs + 2 * TT * S * G::NP;       // [3][TT][CPB][L]: partial sums of y, dd / ln 2, sum g B
-  float* slots = YP + 2 * 3 * TT * CPB * L;  // [warps][TT][2][NP]: the warps' dB and dC
+  float* Bs = DZ + 3 * TT * CPB;                                      // [TT][S + 1][NP]
+  float* Cs = Bs + 2 * TT * G::BS;
+  float* YP = Cs + 2 * TT * G::BS;           // [3][TT][L][YS]: partial sums of y, dd / ln 2, sum g B
+  float* slots = YP + 2 * 3 * TT * G::YT;    // [warps][TT][2][NP]: the warps' dB and dC
   int* flags = reinterpret_cast<int*>(slots + 2 * SCAN_WARPS * TT * 2 * G::NP);  // first [TT], last [TT]
   const ScanBlock s = scan_block<CPB, TT>(P, blockIdx.z);
   const int tiles = s.tiles, tile_z = s.tile0 + tiles - 1;  // step i takes tile tile_z - i
@@ -823,7 +823,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
         }
       }
       p3 = p3 == 2 ? 0 : p3 + 1;
-      bc.store(Bs + q * TT * S * G::NP, Cs + q * TT * S * G::NP, tid);
+      bc.store(Bs + q * TT * G::BS, Cs + q * TT * G::BS, tid);
       marks.write(flags + q * 2 * TT, tid);
       marks.read(P, s.b, t0 - TT, tid);
     };
@@ -847,11 +847,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
           const float2 ds = *reinterpret_cast<const float2*>(DS + at + k * G::TSTEP * CPB);
           float2 dz = make_float2(0.f, 0.f);
           if (P.z.p) dz = *reinterpret_cast<const float2*>(DZ + at + k * G::TSTEP * CPB);
-          const float* y0 = YP + q * 3 * TT * CPB * L + (t * CPB + pc) * L;
-          const float* y1 = y0 + TT * CPB * L;
-          const float* y2 = y1 + TT * CPB * L;
-          const float s0 = scan_join<L>(y0), s1 = scan_join<L>(y0 + L), g0 = scan_join<L>(y2), g1 = scan_join<L>(y2 + L);
-          float2 dd = make_float2(fmaf(scan_join<L>(y1), LN2, g0 * x.x), fmaf(scan_join<L>(y1 + L), LN2, g1 * x.y));
+          const float* sums = YP + (q * 3 * TT + t) * G::YT + pc;
+          const float2 s0 = scan_join<G>(sums), q0 = scan_join<G>(sums + TT * G::YT), g0 = scan_join<G>(sums + 2 * TT * G::YT);
+          float2 dd = make_float2(fmaf(q0.x, LN2, g0.x * x.x), fmaf(q0.y, LN2, g0.y * x.y));
           if (P.softplus) {
             dd.x *= sigmoidf_(dt.x + bias.x);
             dd.y *= sigmoidf_(dt.y + bias.y);
@@ -859,9 +857,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
           if (t0 + t < P.T) {
             const long long o = to + k * row_step;
             if (P.z.p)
-              scan_put_pair<T>(P.dz, o, how, make_float2(dz.x * fmaf(skip.x, x.x, s0), dz.y * fmaf(skip.y, x.y, s1)));
+              scan_put_pair<T>(P.dz, o, how, make_float2(dz.x * fmaf(skip.x, x.x, s0.x), dz.y * fmaf(skip.y, x.y, s0.y)));
             scan_put_pair<T>(P.ddt, o, how, dd);
-            scan_put_pair<T>(P.dx, o, how, make_float2(fmaf(g0, du.x, ds.x * skip.x), fmaf(g1, du.z, ds.y * skip.y)));
+            scan_put_pair<T>(P.dx, o, how, make_float2(fmaf(g0.x, du.x, ds.x * skip.x), fmaf(g0.y, du.z, ds.y * skip.y)));
             sum_add(db.x, db_err.x, dd.x);
             sum_add(db.y, db_err.y, dd.y);
             sum_add(dD.x, dD_err.x, ds.x * x.x);
@@ -945,9 +943,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     const int q = step & 1, q3 = step % 3;
     const float2* du_ = DU + q3 * TT * CPB + c;
     const float* ds_ = DS + q3 * TT * CPB + c;
-    const float* b_ = Bs + q * TT * S * G::NP + m * G::NP + n0;
-    const float* c_ = Cs + q * TT * S * G::NP + m * G::NP + n0;
-    float* y_ = YP + q * 3 * TT * CPB * L + c * L + l;
+    const float* b_ = Bs + q * TT * G::BS + m * G::NP + n0;
+    const float* c_ = Cs + q * TT * G::BS + m * G::NP + n0;
+    float* y_ = YP + q * 3 * TT * G::YT + l * G::YS + c;
     float* s_ = slots + (q * SCAN_WARPS + warp) * TT * 2 * G::NP + n0;
     const int* first = flags + q * 2 * TT;
     const int* last = first + TT;
@@ -966,9 +964,9 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
       dAs = fma(w, Lane<S>::all(u.x), dAs);
       const float y = lane_dot(h, cv), dd = lane_dot(w, a2), gb = lane_dot(g, bv);
       const Lane<S> vb = g * Lane<S>::all(u.y), vc = ds * h;  // dB, dC of this channel
-      y_[k * CPB * L] = y;
-      y_[(TT + k) * CPB * L] = dd;
-      y_[(2 * TT + k) * CPB * L] = gb;
+      y_[k * G::YT] = y;
+      y_[(TT + k) * G::YT] = dd;
+      y_[(2 * TT + k) * G::YT] = gb;
       // over the warp's channels: states i < half stay, the others go to the lane that keeps them
       float v[2][S];
 #pragma unroll
@@ -1007,7 +1005,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     auto step_h = [&](const Lane<S>& a, const Lane<S>& before, const Lane<S>& bv, float2 u) {
       return lane_keep<PAD>(fma(a, before, bv * Lane<S>::all(u.y)), ok);
     };
-    auto at = [&](const float* rows, int t) { return Lane<S>::load(rows + t * S * G::NP); };  // of B or C
+    auto at = [&](const float* rows, int t) { return Lane<S>::load(rows + t * G::BS); };  // of B or C
     if (!scan_seg_flag(first, last)) {
       // The later half of the tokens first: its states are kept, those of the half before it only
       // passed through, and rebuilt for their own turn.  Half a segment fits the registers of two CTAs
