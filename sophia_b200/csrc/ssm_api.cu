@@ -199,8 +199,10 @@ ScanParams scan_params(const kda_b200_scan_args* a) {
   p.vec = a->E % V == 0 && (a->G == 1 || (a->E / a->G) % V == 0) &&
           vec_rows(a->x, a->x_sb, a->x_st, a->B, a->T, V, esz) && vec_rows(a->dt, a->dt_sb, a->dt_st, a->B, a->T, V, esz) &&
           (!a->z || vec_rows(a->z, a->z_sb, a->z_st, a->B, a->T, V, esz));
-  p.vec_bc = a->N % V == 0 && vec_rows(a->B_, a->B_sb, a->B_st, a->B, a->T, V, esz) &&
-             vec_rows(a->C_, a->C_sb, a->C_st, a->B, a->T, V, esz) && (a->G == 1 || (a->B_sg % V == 0 && a->C_sg % V == 0));
+  const int VB = std::min(V, a->N);  // elements of a piece of B and C
+  p.vec_bc = (a->N % V == 0 || a->N == 4) && vec_rows(a->B_, a->B_sb, a->B_st, a->B, a->T, VB, esz) &&
+             vec_rows(a->C_, a->C_sb, a->C_st, a->B, a->T, VB, esz) &&
+             (a->G == 1 || (a->B_sg % VB == 0 && a->C_sg % VB == 0));
   return p;
 }
 

@@ -34,11 +34,10 @@
 // Backward the same with g, from behind.
 //
 // What bounds it: instruction issue and shared memory, not HBM.  For 32 states' tokens (N = 16) the
-// forward issues 10 instructions and holds the shared-memory pipe for 3.5 cycles and the exponential's
-// for 2.5; the backward 33, 8.8 and 4.3, half of them on the token side.  Measured, bf16,
-// 2048 channels, N = 16: 4 x 4096 tokens forward 314 us (0.86 TB/s), backward 845 + 31 us for dB and dC;
-// 8192 packed tokens in 9 spans 155 + 114 (carries) forward, 416 + 114 backward; a prompt of 16384
-// tokens 271 + 194.
+// forward issues 10 instructions and holds the exponential's pipe for 2.5 cycles of 4.2; the backward 32
+// and 4.3 of 11, half of the instructions on the token side.  Measured, bf16, 2048 channels, N = 16:
+// 4 x 4096 tokens forward 302 us (0.9 TB/s), backward 796 + 31 us for dB and dC; 8192 packed tokens in
+// 9 spans 150 + 114 (carries) forward, 392 + 114 backward; a prompt of 16384 tokens 262 + 193.
 #pragma once
 
 #include "ssm_common.cuh"
@@ -73,8 +72,11 @@ struct ScanGeo {
   // the backward's S versions of B and C, [TT][S and a pad][NP], likewise
   static constexpr int BS = (S + 1) * NP;
 };
+// Forward tiles: 32 tokens, or 16 where two CTAs of 32 would not fit an SM (fp32; 64 channels a CTA, up to 8
+// states).  Measured for 8 states, 2048 channels, us with 16 and with 32: 1 x 8192 fp16 tokens 108 and 153; 4 x 4096
+// bf16 tokens, one CTA per SM either way, 368 (two spans) and 330.
 template <typename T, int L, int S>
-using ScanFwdGeo = ScanGeo<T, L, S, sizeof(T) == 2 ? 32 : 16>;
+using ScanFwdGeo = ScanGeo<T, L, S, (sizeof(T) == 2 && L > 2) ? 32 : 16>;
 template <typename T, int L, int S>
 using ScanBwdGeo = ScanGeo<T, L, S, SCAN_TT_BWD>;
 
@@ -149,6 +151,10 @@ __device__ __forceinline__ Lane<S> lane_keep(Lane<S> v, unsigned ok) {
   return v;
 }
 
+__device__ __forceinline__ void cp_async8(void* smem, const void* gmem, bool pred) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(pred ? 8 : 0));
+}
+
 // The token side's fetches.  Every thread keeps where its pieces of a tile come from
 // (the aligned case: 16-byte pieces by cp.async, zeros past T and, whole pieces, past the
 // block's channels); else elements are copied one by one.  Rows of B and C likewise.
@@ -189,7 +195,7 @@ struct ScanFetch {
       }
     }
     if (P.vec_bc) {
-      const int nv = P.N / G::V, per = G::TT * nv;
+      const int nv = P.N < G::V ? 1 : P.N / G::V, per = G::TT * nv;
 #pragma unroll
       for (int k = 0; k < BC_SLOTS; ++k) {
         const int i = k * G::TOKENS + tid, w = i / per, j = i - w * per;
@@ -228,13 +234,16 @@ struct ScanFetch {
       for (int k = 0; k < BC_SLOTS; ++k)
         if (bc_src[k]) {
           const bool in = bc_row[k] < P.T - t0;
-          cp_async16(stage + bc_dst[k], in ? bc_src[k] : static_cast<const T*>(P.Bm), in);
+          const T* src_bc = in ? bc_src[k] : static_cast<const T*>(P.Bm);
+          if (P.N < G::V) cp_async8(stage + bc_dst[k], src_bc, in);
+          else cp_async16(stage + bc_dst[k], src_bc, in);
           bc_src[k] += bc_step[k];
         }
     }
     cp_async_commit();
   }
 };
+// vec_bc: rows of B and C are whole 16-byte pieces, or the 8 bytes of four 16-bit states.
 // vec: a block's channels are whole 16-byte pieces, or end with the tensor's row
 // (E a multiple of the piece), so a piece never mixes two blocks' channels.
 

@@ -34,7 +34,7 @@ inline int scan_blocks(int E, int G, int L) {
 }
 // Tokens of a span: of the numbers k of spans the one that costs least, in tokens of a CTA of the scan that shares
 // its SM with another.  An SM takes its CTAs two at a time, three at a time in the carries' kernel; a
-// lone CTA takes 0.68 (there 0.5, two 0.71) of a full SM's time; the carries' token costs
+// lone CTA takes 0.68 (up to 8 states: 0.83; there 0.5, two 0.71) of a full SM's time; the carries' token costs
 // 1.04 of the forward's, 0.37 of the backward's (0.081 us of 0.078 and 0.217, measured: bf16, N = 16); a
 // CTA's start and a launch count 40 tokens each, composing a span's carry half a token of every
 // CTA, on average.
@@ -42,7 +42,8 @@ inline int scan_span(long long B, long long T, int E, int N, int G, bool backwar
   const long long ctas = B * G * scan_blocks(E, G, scan_lanes(N));
   const int sms = sm_count();
   const float weight = backward ? 0.37f : 1.04f;
-  auto two = [&](long long n) { return (float)(n / 2) + (n % 2 ? 0.68f : 0.f); };
+  const float lone = scan_lanes(N) == 2 ? 0.83f : 0.68f;
+  auto two = [&](long long n) { return (float)(n / 2) + (n % 2 ? lone : 0.f); };
   auto three = [&](long long n) { return (float)(n / 3) + (n % 3 == 2 ? 0.71f : n % 3 ? 0.5f : 0.f); };
   long long best = T;
   float least = 0.f;
