@@ -445,8 +445,9 @@ class _ScanEager(torch.autograd.Function):
     """The eager path: the custom ops' implementation without their dispatch."""
 
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want_final):
-        training = any(ctx.needs_input_grad)
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want_final, training):
+        # `training` is the caller's: grad mode is off in here, and ctx.needs_input_grad follows requires_grad
+        # alone, so that it would keep states for a backward under no_grad as well
         y, ht, saved = _scan_fwd_impl(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want_final, training)
         if training:
             ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, saved)
@@ -456,7 +457,7 @@ class _ScanEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dht):
-        return (*_scan_grads(ctx, dy, dht, _scan_bwd_impl), None, None, None)
+        return (*_scan_grads(ctx, dy, dht, _scan_bwd_impl), None, None, None, None)
 
 
 def _check_scan(what, x, dt, A, B, C, D, z, dt_bias):
@@ -508,9 +509,10 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Te
     like = x.dtype
     x, dt, B, C = (t if t.dtype == io else t.to(io) for t in (x, dt, B, C))
     z = z if z is None or z.dtype == io else z.to(io)
-    args = (x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, bool(dt_softplus), bool(output_final_state))
+    args = (x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, bool(dt_softplus), bool(output_final_state),
+            _needs_grad(x, dt, A, B, C, D, z, dt_bias, initial_state))
     if torch.compiler.is_compiling():
-        y, ht, _ = _scan_fwd(*args, _needs_grad(x, dt, A, B, C, D, z, dt_bias, initial_state))
+        y, ht, _ = _scan_fwd(*args)
     else:
         y, ht = _ScanEager.apply(*args)
     return (y if y.dtype == like else y.to(like)), (ht if output_final_state else None)

@@ -1,0 +1,77 @@
+"""How the state-space operators are called: grad modes, derivatives that they do not have, compilation
+for changing lengths, and single tokens after long prompts."""
+
+from __future__ import annotations
+
+import contextlib
+
+import pytest
+import torch
+
+import sophia_b200
+from sophia_b200 import ssm
+
+gpu = pytest.mark.gpu
+
+
+def _meta(*s, dtype=torch.float32):
+    return torch.empty(*s, device="meta", dtype=dtype)
+
+
+def gen(seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return lambda *s, scale=1.0, dtype=torch.float32: (torch.randn(*s, device="cuda", generator=g) * scale).to(dtype)
+
+
+MODES = {"grad": contextlib.nullcontext, "no_grad": torch.no_grad, "inference": torch.inference_mode}
+
+
+@pytest.mark.parametrize("mode", list(MODES))
+@pytest.mark.parametrize("parameters", [False, True])
+def test_states_are_kept_for_a_backward_alone(monkeypatch, mode, parameters):
+    """Parameters among the inputs are no reason to keep states where no graph is built."""
+    asked = []
+
+    def forward(x, dt, A, B, C, D, z, dt_bias, h0, cu, softplus, want_final, training):
+        asked.append(training)
+        return x.new_empty(x.shape), x.new_empty(0, dtype=torch.float32), x.new_empty(0, dtype=torch.uint8)
+
+    monkeypatch.setattr(ssm, "_scan_fwd_impl", forward)
+    leaf = (lambda t: torch.nn.Parameter(t)) if parameters else (lambda t: t)
+    A, D, bias = leaf(_meta(8, 16)), leaf(_meta(8)), leaf(_meta(8))
+    with MODES[mode]():
+        x, b = _meta(2, 40, 8), _meta(2, 40, 16)
+        y, _ = sophia_b200.selective_scan(x, x, A, b, b, D, None, bias)
+    assert asked == [mode == "grad" and parameters]
+    assert y.requires_grad == asked[0]
+
+
+@gpu
+@pytest.mark.parametrize("mode", ["no_grad", "inference"])
+def test_a_prompt_allocates_no_checkpoints(mode):
+    """The memory of a call with Parameters under no_grad: y, the final state and the spans' workspace,
+    far less than the checkpoints of a training call."""
+    B, T, E, N = 1, 2048, 512, 16
+    rn = gen(1)
+    x, z, dt, Bm, Cm = rn(B, T, E), rn(B, T, E), rn(B, T, E), rn(B, T, N), rn(B, T, N)
+    A, D, bias = (torch.nn.Parameter(t) for t in (-torch.exp(rn(E, N)), rn(E), rn(E)))
+    lib = sophia_b200._lib.load()
+    saved = lib.kda_b200_scan_saved_bytes(B, T, E, N, 1)
+    ws = lib.kda_b200_scan_workspace_bytes(B, T, E, N, 1, 0, 0)
+
+    def peak(context):
+        with context():
+            torch.cuda.synchronize()
+            torch.cuda.reset_peak_memory_stats()
+            before = torch.cuda.memory_allocated()
+            y, ht = sophia_b200.selective_scan(x, dt, A, Bm, Cm, D, z, bias, output_final_state=True)
+            torch.cuda.synchronize()
+            return torch.cuda.max_memory_allocated() - before, y.detach().clone(), ht.detach().clone()
+
+    want = B * T * E * 4 + B * E * N * 4 + ws
+    got, y, ht = peak(MODES[mode])
+    # the allocator may hand out up to 1 MB more than each of the three large buffers needs
+    assert got <= want + (3 << 20) < want + saved, (got, want, saved)
+    trained, y1, h1 = peak(MODES["grad"])
+    assert trained >= got + saved // 2
+    assert torch.equal(y, y1) and torch.equal(ht, h1)
