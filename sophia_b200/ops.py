@@ -226,8 +226,8 @@ class _KdaEager(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0, cu_seqlens, scale, lower_bound,
-                output_final_state):
-        training = any(ctx.needs_input_grad)
+                output_final_state, training):
+        # `training` is the caller's: ctx.needs_input_grad follows requires_grad alone, under no_grad too
         o, ht, saved = _kda_fwd_impl(q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0, cu_seqlens,
                                      scale, lower_bound, output_final_state, training)
         if training:
@@ -238,7 +238,7 @@ class _KdaEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, do, dht):
-        return _kda_grads(ctx, do, dht, _kda_bwd_impl)[:15]
+        return _kda_grads(ctx, do, dht, _kda_bwd_impl)
 
 
 def _needs_grad(*tensors) -> bool:
@@ -247,13 +247,13 @@ def _needs_grad(*tensors) -> bool:
 
 def _layer(q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0, cu_seqlens, scale, lower_bound,
            output_final_state):
+    training = _needs_grad(q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0)
     if torch.compiler.is_compiling():  # traced: the custom op, an opaque node with a fake
-        training = _needs_grad(q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0)
         o, ht, _ = _kda_fwd(q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0, cu_seqlens, float(scale),
                             float(lower_bound), bool(output_final_state), training)
     else:
         o, ht = _KdaEager.apply(q, k, v, g, beta, A_log, dt_bias, conv_q, conv_k, conv_v, h0, cu_seqlens,
-                                float(scale), float(lower_bound), bool(output_final_state))
+                                float(scale), float(lower_bound), bool(output_final_state), training)
     return o.to(q.dtype), (ht if output_final_state else None)
 
 
