@@ -33,6 +33,23 @@ class SSMPool(NamedTuple):
     scan: torch.Tensor  # [slots, inner, state] float32
 
 
+def write_slots(pool: SSMPool, slots: torch.Tensor, conv: torch.Tensor, scan: torch.Tensor) -> None:
+    """Row r of the states to slots[r] of the pool, rows with a slot outside the pool nowhere.  An index outside
+    would fault the device, and dropping the rows by a mask would wait for it: such a row repeats the copy of
+    the first row with a slot, or, where no row has one, writes an entry's own state to it."""
+    n, rows = pool.scan.shape[0], slots.shape[0]
+    if n == 0 or rows == 0:
+        return
+    at = slots.long()
+    inside = at.clamp(0, n - 1)
+    ok = inside == at
+    some = ok.any()
+    row = torch.where(ok, torch.arange(rows, device=slots.device), ok.byte().argmax())
+    at = inside[row]
+    for states, new in ((pool.conv, conv), (pool.scan, scan)):
+        states.index_copy_(0, at, torch.where(some, new[row], states[at]))
+
+
 class SSMMixerBlock(nn.Module):
     def __init__(self, dim: int = 1536, inner: int = 2048, state: int = 16, dt_rank: int = 128, conv_kernel: int = 4,
                  eps: float = 1e-5, dt_min: float = 1e-3, dt_max: float = 1e-1, dt_floor: float = 1e-4,
@@ -86,10 +103,12 @@ class SSMMixerBlock(nn.Module):
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cu_seqlens: torch.Tensor, pool: SSMPool, slots: torch.Tensor) -> torch.Tensor:
         """Prompts packed along T: x [1, T, dim], cu_seqlens [R + 1], slots [R]; the requests' states go
-        to their slots of the pool.  Returns [1, T, dim]."""
+        to their slots of the pool.  A negative slot marks a padding request (as in ``step``, and so does one past
+        the pool): its state goes nowhere.  Returns [1, T, dim]."""
+        if tuple(slots.shape) != (cu_seqlens.shape[0] - 1,):
+            raise ValueError(f"prefill: {cu_seqlens.shape[0] - 1} prompts but slots of shape {list(slots.shape)}")
         y, conv, scan = self._mix(x, cu_seqlens, want_state=True)
-        pool.conv.index_copy_(0, slots.long(), conv)
-        pool.scan.index_copy_(0, slots.long(), scan)
+        write_slots(pool, slots, conv, scan)
         return y
 
     @torch.no_grad()
