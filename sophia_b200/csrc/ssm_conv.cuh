@@ -145,8 +145,8 @@ struct ConvRing {
         if (ASYNC && next + u < last) {
           const uint32_t d = smem_u32(&sm.p[put][q][u][threadIdx.x]);
           const void* g = src[q] + u * st[q];
-          if (sizeof(Piece) == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(g));
-          else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(g));
+          if (sizeof(Piece) == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(g) : "memory");
+          else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(d), "l"(g) : "memory");
         }
       if (ASYNC) src[q] += GROUP * st[q];
     }

@@ -152,7 +152,8 @@ __device__ __forceinline__ Lane<S> lane_keep(Lane<S> v, unsigned ok) {
 }
 
 __device__ __forceinline__ void cp_async8(void* smem, const void* gmem, bool pred) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(pred ? 8 : 0));
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(pred ? 8 : 0)
+               : "memory");
 }
 
 // The token side's fetches.  Every thread keeps where its pieces of a tile come from
