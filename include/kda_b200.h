@@ -346,6 +346,13 @@ int kda_b200_short_conv_step(const void* x, int64_t x_sr, const float* w, const 
                              void* stream);
 
 /*
+ * After a prompt: row r of `src` ([rows][per], final states) to entry slots[r] of a pool ([pool][per]).
+ * Slots (not NULL) as in kda_b200_short_conv_step: a row with a negative one goes nowhere, one past the
+ * pool neither and sets kda_b200_device_error() to 11.
+ */
+int kda_b200_put_states(const float* src, const int32_t* slots, int rows, int64_t per, int pool, float* dst, void* stream);
+
+/*
  * Selective state space scan.  Per sequence, channel e and state n, with
  * d = softplus(dt + dt_bias) (or dt + dt_bias, softplus = 0):
  *     h[t] = exp(d A[e][n]) h[t-1] + d x[t] B[t][n]

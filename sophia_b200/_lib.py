@@ -82,6 +82,7 @@ SIGNATURES = {
     "kda_b200_short_conv_bwd": ([c_void_p, c_int64, c_int64] + [c_void_p] * 4 + [c_int64, c_int64] + [c_int] * 5
                                 + [c_void_p, c_int64, c_int64] + [c_void_p] * 5 + [c_void_p, c_size_t, c_void_p], c_int),
     "kda_b200_short_conv_step": ([c_void_p, c_int64] + [c_void_p] * 4 + [c_int] * 6 + [c_void_p, c_void_p], c_int),
+    "kda_b200_put_states": ([c_void_p, c_void_p, c_int, c_int64, c_int, c_void_p, c_void_p], c_int),
     "kda_b200_scan_saved_bytes": ([c_int64, c_int64] + [c_int] * 3, c_size_t),
     "kda_b200_scan_workspace_bytes": ([c_int64, c_int64] + [c_int] * 5, c_size_t),
     "kda_b200_selective_scan_fwd": ([ctypes.POINTER(ScanArgs), c_void_p, c_size_t, c_void_p], c_int),

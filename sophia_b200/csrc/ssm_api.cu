@@ -379,6 +379,24 @@ int kda_b200_short_conv_step(const void* x, int64_t x_sr, const float* w, const 
   return SSM_DISPATCH(dtype, conv_step, p, static_cast<cudaStream_t>(stream));
 }
 
+int kda_b200_put_states(const float* src, const int32_t* slots, int rows, int64_t per, int pool, float* dst, void* stream) {
+  if (rows < 0 || per < 0 || pool < 0) return fail(KDA_ERR_INVALID, "rows >= 0, per >= 0 and pool >= 0 are required");
+  if (rows == 0 || per == 0) return KDA_OK;
+  if (!src || !slots || (!dst && pool > 0)) return fail(KDA_ERR_INVALID, "null pointer");
+  int* err = device_error_flag();
+  if (!err) return fail(KDA_ERR_CUDA, "the device error flag has no address");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool vec = per % 4 == 0 && aligned(src, 16) && aligned(dst, 16);
+  const long long elems = vec ? per / 4 : per;
+  const dim3 grid((unsigned)std::min<long long>((elems + 255) / 256, 1024), std::min(rows, 65535));
+  if (vec)
+    ssm_put_states_kernel<<<grid, 256, 0, st>>>(reinterpret_cast<const float4*>(src), slots, rows, elems, pool,
+                                                reinterpret_cast<float4*>(dst), err);
+  else
+    ssm_put_states_kernel<<<grid, 256, 0, st>>>(src, slots, rows, elems, pool, dst, err);
+  return launch_check("states to their slots");
+}
+
 size_t kda_b200_scan_saved_bytes(int64_t B, int64_t T, int E, int N, int G) {
   if (B < 1 || T < 0 || E < 1 || N < 1 || N > SCAN_MAX_N || G < 1 || E % G) return 0;
   return std::max<size_t>(16, (size_t)B * ((T + SCAN_SEG - 1) / SCAN_SEG) * E * N * 4);

@@ -285,6 +285,19 @@ static __global__ void __launch_bounds__(SEQ_MAP_THREADS) ssm_seq_map_kernel(Seq
   }
 }
 
+// Rows of new states to their pool entries (elements of V floats, `per` of them a row); padding rows and rows past the
+// pool as in the single-token calls.
+template <typename V>
+static __global__ void __launch_bounds__(256) ssm_put_states_kernel(const V* src, const int* slots, int rows, long long per,
+                                                                    int pool, V* dst, int* err) {
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    const int s = step_slot(slots, r, pool, err);
+    if (s < 0) continue;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < per; i += (long long)gridDim.x * blockDim.x)
+      dst[s * per + i] = src[r * per + i];
+  }
+}
+
 // Sums `parts` rows of `cols` = q * w1 columns, w1 = w0 + 1 or w0 + 2: 8 strided slices
 // of the rows in order, then the slices in order -- a fixed order for a given
 // number of rows.  Columns r < w0 of item q go to out0[q * w0 + r], the next to

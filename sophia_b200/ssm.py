@@ -136,6 +136,24 @@ def _check_pool(what: str, state: Tensor, inner: tuple, device: torch.device, ro
         raise RuntimeError(f"{what}: slots are on {slots.device}, the activations on {device}")
 
 
+def _put_states_impl(new, pool, slots):
+    rows = new.shape[0]
+    _call(_lib.load().kda_b200_put_states, new.device,
+          _ptr(new), _ptr(slots), rows, new.numel() // max(1, rows), pool.shape[0], _ptr(pool))
+
+
+@torch.library.custom_op("sophia_b200::put_states", mutates_args=("pool",), device_types="cuda")
+def _put_states(new: Tensor, pool: Tensor, slots: Tensor) -> None:
+    _put_states_impl(new, pool, slots)
+
+
+def put_states(new: Tensor, pool: Tensor, slots: Tensor) -> None:
+    """Row r of ``new``, final states of a prompt call, to ``pool[slots[r]]``; padding rows as in the single-token
+    calls, with their states nowhere."""
+    _check_pool("put_states", pool, tuple(new.shape[1:]), new.device, new.shape[0], slots)
+    (_put_states if torch.compiler.is_compiling() else _put_states_impl)(_param(new), pool, slots)
+
+
 # --------------------------------------------------------------------------- convolution
 
 

@@ -23,7 +23,7 @@ from torch.nn import functional as F
 
 from .clip import clip_grad_norm_
 from .mixer import _inverse_softplus
-from .ssm import selective_scan, selective_scan_step, short_conv, short_conv_step
+from .ssm import put_states, selective_scan, selective_scan_step, short_conv, short_conv_step
 
 
 class SSMPool(NamedTuple):
@@ -31,23 +31,6 @@ class SSMPool(NamedTuple):
 
     conv: torch.Tensor  # [slots, inner, taps - 1] float32
     scan: torch.Tensor  # [slots, inner, state] float32
-
-
-def write_slots(pool: SSMPool, slots: torch.Tensor, conv: torch.Tensor, scan: torch.Tensor) -> None:
-    """Row r of the states to slots[r] of the pool, rows with a slot outside the pool nowhere.  An index outside
-    would fault the device, and dropping the rows by a mask would wait for it: such a row repeats the copy of
-    the first row with a slot, or, where no row has one, writes an entry's own state to it."""
-    n, rows = pool.scan.shape[0], slots.shape[0]
-    if n == 0 or rows == 0:
-        return
-    at = slots.long()
-    inside = at.clamp(0, n - 1)
-    ok = inside == at
-    some = ok.any()
-    row = torch.where(ok, torch.arange(rows, device=slots.device), ok.byte().argmax())
-    at = inside[row]
-    for states, new in ((pool.conv, conv), (pool.scan, scan)):
-        states.index_copy_(0, at, torch.where(some, new[row], states[at]))
 
 
 class SSMMixerBlock(nn.Module):
@@ -103,12 +86,13 @@ class SSMMixerBlock(nn.Module):
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cu_seqlens: torch.Tensor, pool: SSMPool, slots: torch.Tensor) -> torch.Tensor:
         """Prompts packed along T: x [1, T, dim], cu_seqlens [R + 1], slots [R]; the requests' states go
-        to their slots of the pool.  A negative slot marks a padding request (as in ``step``, and so does one past
-        the pool): its state goes nowhere.  Returns [1, T, dim]."""
-        if tuple(slots.shape) != (cu_seqlens.shape[0] - 1,):
-            raise ValueError(f"prefill: {cu_seqlens.shape[0] - 1} prompts but slots of shape {list(slots.shape)}")
+        to their slots of the pool.  A negative slot marks a padding request, as in ``step``.  Returns [1, T, dim]."""
         y, conv, scan = self._mix(x, cu_seqlens, want_state=True)
-        write_slots(pool, slots, conv, scan)
+        if slots.dtype != torch.int32:
+            slots = slots.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+        slots = slots.contiguous()
+        put_states(conv, pool.conv, slots)
+        put_states(scan, pool.scan, slots)
         return y
 
     @torch.no_grad()
