@@ -403,8 +403,10 @@ int kda_b200_selective_scan_step(const kda_b200_scan_args* args, void* stream);
  * counts and KDA_IO_* types, read during the call; out NULL computes the norm
  * alone.  out[i] == in[i] clips in place (nothing is written when the factor is 1); a
  * tensor and an output must not overlap otherwise.  norm: device fp32 [1].  Squares are summed
- * in an order that the sizes alone decide.  A non-finite norm leaves as it is: with it
- * the outputs are NaN (norm NaN) or 0 and NaN (norm infinite).
+ * in an order that depends on the sizes, the addresses modulo 16 bytes and the GPU's number of SMs, never on
+ * timing, and over the whole range of fp32 (values around 1e20 or 1e-30 have a finite norm that is not zero).
+ * A norm past fp32's range is infinite.  A non-finite norm leaves as it is: with it the outputs are NaN (norm NaN) or
+ * 0 and NaN (norm infinite).
  */
 typedef struct kda_b200_grad_args {
   int64_t count;

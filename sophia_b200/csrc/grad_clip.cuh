@@ -8,7 +8,9 @@
 // as a kernel parameter (no copy, no host wait); each launch takes up to
 // GRAD_MAX_TENSORS of them.  A CTA takes a run of chunks of GRAD_CHUNK elements.  Squares
 // are summed in fp32 over at most GRAD_CHUNK / GRAD_THREADS elements of a thread
-// and in fp64 from there on, in an order that depends on the sizes alone.
+// and in fp64 from there on, in an order that depends on the sizes, on the addresses modulo 16
+// bytes and on the number of SMs, never on timing.  Where fp32 squares would overflow or vanish the thread sums its
+// elements again in fp64, so the norm is right over the whole range of fp32.
 // Measured, 455 M elements of bf16 in 336 tensors to fp32: norm 152 us (6.0 TB/s), scaling
 // 487 us (5.6 TB/s); chunks of 4096 elements 178 and 479 us, of 8192 157 and 486 us.
 #pragma once
@@ -55,43 +57,63 @@ struct GradWalk {
   }
 };
 
-// 16-byte vectors of T per thread and step when the address allows, else elements.
-template <typename T>
-__device__ __forceinline__ float grad_sumsq(const T* p, int n) {
+// A thread's share of a chunk in pieces, fn(piece): 16 bytes each when the address allows, else elements.
+template <typename T, typename F>
+__device__ __forceinline__ void grad_each(const T* p, int n, F fn) {
   constexpr int V = 16 / sizeof(T), U = 4;
-  float acc = 0.f;
+  int k = threadIdx.x;
   if ((reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+    const IoVec<T, V>* q = reinterpret_cast<const IoVec<T, V>*>(p);
     const int nv = n / V;
     int i = threadIdx.x;
     for (; i + (U - 1) * GRAD_THREADS < nv; i += U * GRAD_THREADS) {
       IoVec<T, V> r[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) r[u] = reinterpret_cast<const IoVec<T, V>*>(p)[i + u * GRAD_THREADS];
+      for (int u = 0; u < U; ++u) r[u] = q[i + u * GRAD_THREADS];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < V; ++k) {
-          const float f = io_to_f(r[u].v[k]);
-          acc = fmaf(f, f, acc);
-        }
+      for (int u = 0; u < U; ++u) fn(r[u]);
     }
-    for (; i < nv; i += GRAD_THREADS) {
-      float f[V];
-      io_load<T, V>(p + (long long)i * V, f);
-#pragma unroll
-      for (int k = 0; k < V; ++k) acc = fmaf(f[k], f[k], acc);
-    }
-    for (int k = nv * V + threadIdx.x; k < n; k += GRAD_THREADS) {
-      const float v = io_to_f(p[k]);
-      acc = fmaf(v, v, acc);
-    }
-  } else {
-    for (int k = threadIdx.x; k < n; k += GRAD_THREADS) {
-      const float v = io_to_f(p[k]);
-      acc = fmaf(v, v, acc);
-    }
+    for (; i < nv; i += GRAD_THREADS) fn(q[i]);
+    k += nv * V;
   }
-  return acc;
+  for (; k < n; k += GRAD_THREADS) fn(*reinterpret_cast<const IoVec<T, 1>*>(p + k));
+}
+// The bits of a piece's elements, joined: zero where all of them are (signs stay in).
+template <typename T, int V>
+__device__ __forceinline__ uint32_t grad_bits(const IoVec<T, V>& r) {
+  if (sizeof(T) * V < 4) return *reinterpret_cast<const unsigned short*>(&r);
+  uint32_t b = 0;
+#pragma unroll
+  for (int w = 0; w < (int)sizeof(T) * V / 4; ++w) b |= reinterpret_cast<const uint32_t*>(&r)[w];
+  return b;
+}
+
+// Sum of squares of a thread's elements: in fp32, and again in fp64 where fp32 squares leave their range -- the
+// sum is not finite (one element above 1.8e19 is enough), or so small that squares below 2^-126 may have lost
+// their digits in it (64 of them, each off by 2^-150, are 2^-44 of a sum of 2^-100).  `bits` tells small elements from
+// zeros.
+template <typename T>
+__device__ __forceinline__ double grad_sumsq(const T* p, int n) {
+  float acc = 0.f;
+  uint32_t bits = 0;
+  grad_each(p, n, [&](const auto& r) {
+#pragma unroll
+    for (const T v : r.v) {
+      const float f = io_to_f(v);
+      acc = fmaf(f, f, acc);
+    }
+    bits |= grad_bits(r);
+  });
+  if (acc >= 0x1p-100f && acc < INFINITY) return acc;
+  if ((bits & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu)) == 0) return 0;
+  double wide = 0;
+  grad_each(p, n, [&](const auto& r) {
+    for (const T v : r.v) {
+      const double f = io_to_f(v);
+      wide = fma(f, f, wide);
+    }
+  });
+  return wide;
 }
 
 // Sum over the CTA in a fixed order; valid in thread 0.
@@ -118,7 +140,7 @@ __global__ void __launch_bounds__(GRAD_THREADS) grad_norm_kernel(const __grid_co
     const int i = walk.i;
     const long long at = (long long)(ch - tab.chunk0[i]) * GRAD_CHUNK;
     const int n = (int)min((long long)GRAD_CHUNK, tab.numel[i] - at);
-    float s;
+    double s;
     if (tab.tin[i] == 0) s = grad_sumsq(static_cast<const float*>(tab.in[i]) + at, n);
     else if (tab.tin[i] == 1) s = grad_sumsq(static_cast<const bf16*>(tab.in[i]) + at, n);
     else s = grad_sumsq(static_cast<const f16*>(tab.in[i]) + at, n);
