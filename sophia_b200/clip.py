@@ -118,6 +118,8 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
                 continue
             if g.stride() == o.stride() and _dense(g):  # the same order of elements in both
                 continue
+            if any(st == 0 and n > 1 for st, n in zip(o.stride(), o.shape)):  # an expanded tensor
+                raise ValueError(f"{what}: an output of shape {list(o.shape)} holds several elements in one place")
             src[i] = g.contiguous()
             if not o.is_contiguous():
                 dst[i] = torch.empty(o.shape, device=o.device, dtype=o.dtype)

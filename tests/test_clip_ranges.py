@@ -94,3 +94,19 @@ def test_chunk_ends_at_any_address(dtype, n, offset):
     for t, o in zip(ts, outs):
         exact = t.double() * min(1.0, float(factor))
         assert ((o.double() - exact).abs() <= 1.2e-7 * exact.abs() + 1e-37).all()  # one rounding
+
+
+def test_an_expanded_output_is_refused_before_anything_is_scaled():
+    """autograd.grad of a sum returns a broadcast tensor: its elements share a place."""
+    whole, base = torch.ones(10, device="cuda"), torch.ones(1, device="cuda")
+    with pytest.raises(ValueError):
+        sophia_b200.clip_grad_norm_([whole, base.expand(5)], 0.1)
+    with pytest.raises(ValueError):
+        sophia_b200.clip_grad_norm_([whole, torch.ones(4, 3, device="cuda")], 0.1,
+                                    out=[whole, torch.ones(4, 1, device="cuda").expand(4, 3)])
+    assert (whole == 1).all() and float(base) == 1
+    # as an input it is read like any other
+    out = [torch.empty(10, device="cuda"), torch.empty(5, device="cuda")]
+    norm = sophia_b200.clip_grad_norm_([whole, base.expand(5)], 0.1, out=out)
+    assert abs(float(norm) - math.sqrt(15)) <= 2e-6 * math.sqrt(15)
+    assert torch.equal(torch.cat(out), torch.ones(15, device="cuda") * (torch.tensor(0.1, device="cuda") / (norm + 1e-6)))
