@@ -13,6 +13,7 @@ from typing import Iterable, Sequence
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import GradArgs
@@ -111,7 +112,9 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
         if any(o.requires_grad for o in outs):
             raise ValueError(f"{what} scales gradients; a tensor that requires grad (a parameter?) is not one")
         if all(map(Tensor.is_contiguous, ts)) and (outs is ts or all(map(Tensor.is_contiguous, outs))):
-            return _launch(ts, types, outs, out_types, max_norm, eps)
+            norm = _launch(ts, types, outs, out_types, max_norm, eps)
+            increment_version(outs)  # written in place: a graph that saved one has to notice
+            return norm
         src, dst, back = list(ts), list(outs), []
         for i, (g, o) in enumerate(zip(ts, outs)):
             if g.is_contiguous() and o.is_contiguous():
@@ -125,6 +128,7 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
                 dst[i] = torch.empty(o.shape, device=o.device, dtype=o.dtype)
                 back.append(i)
         norm = _launch(src, types, dst, out_types, max_norm, eps)
+        increment_version(outs)
         for i in back:
             outs[i].copy_(dst[i])
         return norm

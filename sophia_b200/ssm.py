@@ -20,6 +20,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import ScanArgs
@@ -151,7 +152,11 @@ def put_states(new: Tensor, pool: Tensor, slots: Tensor) -> None:
     """Row r of ``new``, final states of a prompt call, to ``pool[slots[r]]``; padding rows as in the single-token
     calls, with their states nowhere."""
     _check_pool("put_states", pool, tuple(new.shape[1:]), new.device, new.shape[0], slots)
-    (_put_states if torch.compiler.is_compiling() else _put_states_impl)(_param(new), pool, slots)
+    if torch.compiler.is_compiling():
+        _put_states(_param(new), pool, slots)
+    else:
+        _put_states_impl(_param(new), pool, slots)
+        increment_version(pool)
 
 
 # --------------------------------------------------------------------------- convolution
@@ -337,8 +342,11 @@ def short_conv_step(x: Tensor, conv_state: Tensor, weight: Tensor, bias: Tensor 
     _check_pool("short_conv_step", conv_state, (x.shape[1], W - 1), x.device, x.shape[0], slots)
     if _needs_grad(x, weight, bias, conv_state):
         raise NotImplementedError("short_conv_step has no backward; use short_conv for training")
-    fn = _conv_step if torch.compiler.is_compiling() else _conv_step_impl
-    return fn(x, conv_state, weight, bias, slots, silu)
+    if torch.compiler.is_compiling():
+        return _conv_step(x, conv_state, weight, bias, slots, silu)
+    y = _conv_step_impl(x, conv_state, weight, bias, slots, silu)
+    increment_version(conv_state)  # written in place: a graph that saved it has to notice
+    return y
 
 
 # --------------------------------------------------------------------------- scan
@@ -583,6 +591,9 @@ def selective_scan_step(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, 
     like = x.dtype
     x, dt, B, C = (t if t.dtype == io else t.to(io) for t in (x, dt, B, C))
     z = z if z is None or z.dtype == io else z.to(io)
-    fn = _scan_step if torch.compiler.is_compiling() else _scan_step_impl
-    y = fn(x, dt, A, B, C, state, D, z, dt_bias, slots, bool(dt_softplus))
+    if torch.compiler.is_compiling():
+        y = _scan_step(x, dt, A, B, C, state, D, z, dt_bias, slots, bool(dt_softplus))
+    else:
+        y = _scan_step_impl(x, dt, A, B, C, state, D, z, dt_bias, slots, bool(dt_softplus))
+        increment_version(state)
     return y if y.dtype == like else y.to(like)

@@ -75,3 +75,39 @@ def test_a_prompt_allocates_no_checkpoints(mode):
     trained, y1, h1 = peak(MODES["grad"])
     assert trained >= got + saved // 2
     assert torch.equal(y, y1) and torch.equal(ht, h1)
+
+
+@gpu
+@pytest.mark.parametrize("call", ["conv_step", "scan_step", "put_states", "clip", "clip_out", "clip_copy"])
+def test_a_graph_notices_what_is_written_in_place(call):
+    """A tensor that a graph saved and a call then rewrote: backward refuses, as behind torch's own in-place operations."""
+    rn = gen(3)
+    written = rn(4, 6, 3)
+    w = rn(4, 6, 3).requires_grad_()
+    loss = (w * written).sum()  # saves `written`
+    x, slots = rn(4, 6), torch.arange(4, device="cuda", dtype=torch.int32)
+    if call == "conv_step":
+        sophia_b200.short_conv_step(x, written, rn(6, 4))
+    elif call == "scan_step":
+        sophia_b200.selective_scan_step(x, x, -torch.ones(6, 3, device="cuda"), rn(4, 3), rn(4, 3), written)
+    elif call == "put_states":
+        ssm.put_states(rn(4, 6, 3), written, slots)
+    elif call == "clip":
+        sophia_b200.clip_grad_norm_([written], 0.1)
+    elif call == "clip_out":
+        sophia_b200.clip_grad_norm_([rn(4, 6, 3)], 0.1, out=[written])
+    else:
+        sophia_b200.clip_grad_norm_([rn(4, 6, 3)], 0.1, out=[written.transpose(0, 1).contiguous().transpose(0, 1), ])
+        sophia_b200.clip_grad_norm_([written, rn(6, 8)[:, ::2]], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@gpu
+def test_inference_tensors_are_written():
+    rn = gen(3)
+    with torch.inference_mode():
+        pool, grad = torch.zeros(4, 6, 3, device="cuda"), torch.ones(6, device="cuda")
+        sophia_b200.short_conv_step(rn(4, 6), pool, rn(6, 4))
+        sophia_b200.clip_grad_norm_([grad], 0.1)
+        assert pool[:, :, 2].any() and float(grad[0]) < 0.1
