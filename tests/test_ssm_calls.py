@@ -111,3 +111,35 @@ def test_inference_tensors_are_written():
         sophia_b200.short_conv_step(rn(4, 6), pool, rn(6, 4))
         sophia_b200.clip_grad_norm_([grad], 0.1)
         assert pool[:, :, 2].any() and float(grad[0]) < 0.1
+
+
+def test_kept_states_have_the_size_that_the_library_asks_for():
+    """What the traced form allocates is what the library computes, at every size."""
+    lib = sophia_b200._lib.load()
+    op = torch.ops.sophia_b200.selective_scan_fwd
+    for b, T, E, N, G in [(1, 1, 1, 1, 1), (1, 0, 4, 4, 1), (2, 7, 3, 16, 1), (1, 8, 6, 5, 2), (3, 9, 8, 64, 4), (1, 257, 34, 33, 2)]:
+        with torch._subclasses.FakeTensorMode():
+            y, _, saved = op(torch.empty(b, T, E, device="cuda"), torch.empty(b, T, E, device="cuda"),
+                             torch.empty(E, N, device="cuda"), torch.empty(b, T, G, N, device="cuda"),
+                             torch.empty(b, T, G, N, device="cuda"), None, None, None, None, None, True, False, True)
+        assert saved.numel() == lib.kda_b200_scan_saved_bytes(b, T, E, N, G) and y.shape == (b, T, E)
+
+
+def test_changing_lengths_compile_once():
+    """Training steps of other token counts run the code that the first ones compiled."""
+    from torch._dynamo.testing import CompileCounterWithBackend
+
+    counter = CompileCounterWithBackend("aot_eager")
+
+    def step(x, w, dt, A, B, C):
+        c, _ = sophia_b200.short_conv(x, w)
+        return sophia_b200.selective_scan(c, dt, A, B, C)[0]
+
+    run = torch.compile(step, backend=counter, fullgraph=True, dynamic=True)
+    w, A = _meta(32, 4).requires_grad_(), _meta(32, 16).requires_grad_()
+    for T in (70, 91, 128, 260, 33, 1000):
+        x, dt, bc = _meta(2, T, 32).requires_grad_(), _meta(2, T, 32).requires_grad_(), _meta(2, T, 16).requires_grad_()
+        y = run(x, w, dt, A, bc, bc)
+        y.sum().backward()
+        assert x.grad.shape == x.shape and bc.grad.shape == bc.shape
+    assert counter.frame_count == 1
