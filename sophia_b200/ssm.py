@@ -69,6 +69,28 @@ def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+class _FirstOrder(torch.autograd.Function):
+    """Gradients of a backward under ``create_graph``: they depend on the inputs, but how is not provided."""
+
+    @staticmethod
+    def forward(ctx, what, count, *tensors):
+        ctx.what = what
+        return tuple(None if t is None else t.view_as(t) for t in tensors[:count])
+
+    @staticmethod
+    def backward(ctx, *_):
+        raise NotImplementedError(f"{ctx.what} has no second derivative")
+
+
+def _first_order(what: str, ctx, grads: tuple, *dys: Tensor | None) -> tuple:
+    """The gradients as they are, or, where a graph of them is built, so that differentiating them is refused; they
+    would count as constants otherwise."""
+    if not torch.is_grad_enabled():
+        return grads
+    depend = (*dys, *ctx.saved_tensors)
+    return _FirstOrder.apply(what, len(grads), *grads, *depend)
+
+
 def _check_activations(what: str, **tensors) -> torch.dtype:
     """All on one CUDA device and of supported types; returns the promoted type."""
     first = tensors["x"]
@@ -261,7 +283,7 @@ class _ConvEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dht):
-        return _conv_grads(ctx, dy, dht, _conv_bwd_impl)
+        return _first_order("short_conv", ctx, _conv_grads(ctx, dy, dht, _conv_bwd_impl), dy, dht)
 
 
 def _check_taps(what: str, weight: Tensor, C: int) -> int:
@@ -485,7 +507,8 @@ class _ScanEager(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, dht):
-        return (*_scan_grads(ctx, dy, dht, _scan_bwd_impl), None, None, None, None)
+        grads = _first_order("selective_scan", ctx, _scan_grads(ctx, dy, dht, _scan_bwd_impl), dy, dht)
+        return (*grads, None, None, None, None)
 
 
 def _check_scan(what, x, dt, A, B, C, D, z, dt_bias):

@@ -143,3 +143,39 @@ def test_changing_lengths_compile_once():
         y.sum().backward()
         assert x.grad.shape == x.shape and bc.grad.shape == bc.shape
     assert counter.frame_count == 1
+
+
+def _without_kernels(monkeypatch):
+    """Both operators on meta tensors, their kernels replaced by allocations."""
+    empty = lambda t, dtype=None: None if t is None else t.new_empty(t.shape, dtype=dtype or t.dtype)  # noqa: E731
+    none = lambda x: x.new_empty(0, dtype=torch.float32)  # noqa: E731
+    monkeypatch.setattr(ssm, "_conv_fwd_impl", lambda x, *r: (empty(x), none(x)))
+    monkeypatch.setattr(ssm, "_conv_bwd_impl", lambda x, w, b, h0, cu, dy, dht, silu, want: (
+        empty(x), empty(w), empty(b), none(x)))
+    monkeypatch.setattr(ssm, "_scan_fwd_impl", lambda x, *r: (empty(x), none(x), x.new_empty(0, dtype=torch.uint8)))
+    monkeypatch.setattr(ssm, "_scan_bwd_impl", lambda x, dt, A, B, C, D, z, bias, h0, cu, saved, dy, dht, sp, want: (
+        empty(x), empty(dt), empty(A), empty(B), empty(C), empty(D), empty(z), empty(bias), none(x)))
+
+
+@pytest.mark.parametrize("leaf", ["x", "weight", "dy"])
+def test_second_derivatives_are_refused(monkeypatch, leaf):
+    """A gradient penalty would count the gradient as a constant and lose its part of the loss silently."""
+    _without_kernels(monkeypatch)
+    g = {k: _meta(2, 9, 8) for k in ("x", "dy")}
+    g["weight"] = _meta(8, 4)
+    g[leaf].requires_grad_()
+    for call in (lambda: sophia_b200.short_conv(g["x"] + 0, g["weight"], g["bias"])[0],
+                 lambda: sophia_b200.selective_scan(g["x"] + 0, g["x"] + 0, -g["weight"], g["b"], g["b"], g["bias"])[0]):
+        g["bias"], g["b"] = _meta(8).requires_grad_(), _meta(2, 9, 4)
+        (db,) = torch.autograd.grad(call(), g["bias"], g["dy"], create_graph=True)
+        assert db.requires_grad
+        with pytest.raises(NotImplementedError, match="no second derivative"):
+            (db.square().sum() + g[leaf].sum()).backward()
+
+
+def test_first_derivatives_take_no_detour(monkeypatch):
+    _without_kernels(monkeypatch)
+    x, w, b = _meta(2, 9, 8).requires_grad_(), _meta(8, 4).requires_grad_(), _meta(2, 9, 4).requires_grad_()
+    y = sophia_b200.selective_scan(sophia_b200.short_conv(x, w)[0], x, -w, b, b)[0]
+    y.sum().backward()
+    assert not any(t.grad.requires_grad for t in (x, w, b))
