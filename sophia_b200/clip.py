@@ -17,7 +17,7 @@ from torch.autograd.graph import increment_version
 
 from . import _lib
 from ._lib import GradArgs
-from .ssm import _IO, _call
+from .ssm import _IO, _call, _check_no_tangents
 
 __all__ = ["grad_norm", "clip_grad_norm_"]
 
@@ -32,6 +32,7 @@ def _list(what: str, grads) -> tuple[list[Tensor], torch.device | None, bytes]:
         types = bytes([_IO[t.dtype] for t in ts])
     except KeyError as e:
         raise NotImplementedError(f"{what}: gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
+    _check_no_tangents(what, *ts)
     devices = {t.device for t in ts}
     if len(devices) > 1:
         raise RuntimeError(f"{what}: gradients are on several devices")

@@ -20,6 +20,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -67,6 +68,14 @@ def _cu(cu_seqlens: Tensor | None) -> Tensor | None:
 
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _check_no_tangents(what: str, *tensors: Tensor | None) -> None:
+    """Refuses forward-mode differentiation, whose tangents a kernel called directly would drop."""
+    if forward_ad._current_level < 0:  # no dual numbers anywhere
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 class _FirstOrder(torch.autograd.Function):
@@ -175,6 +184,9 @@ def put_states(new: Tensor, pool: Tensor, slots: Tensor) -> None:
     """Row r of ``new``, final states of a prompt call, to ``pool[slots[r]]``; padding rows as in the single-token
     calls, with their states nowhere."""
     _check_pool("put_states", pool, tuple(new.shape[1:]), new.device, new.shape[0], slots)
+    if _needs_grad(new, pool):
+        raise NotImplementedError("put_states has no backward")
+    _check_no_tangents("put_states", new, pool)
     if torch.compiler.is_compiling():
         _put_states(_param(new), pool, slots)
     else:
@@ -365,6 +377,7 @@ def short_conv_step(x: Tensor, conv_state: Tensor, weight: Tensor, bias: Tensor 
     _check_pool("short_conv_step", conv_state, (x.shape[1], W - 1), x.device, x.shape[0], slots)
     if _needs_grad(x, weight, bias, conv_state):
         raise NotImplementedError("short_conv_step has no backward; use short_conv for training")
+    _check_no_tangents("short_conv_step", x, conv_state, weight, bias)
     if torch.compiler.is_compiling():
         return _conv_step(x, conv_state, weight, bias, slots, silu)
     y = _conv_step_impl(x, conv_state, weight, bias, slots, silu)
@@ -613,6 +626,7 @@ def selective_scan_step(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, 
     _check_pool(what, state, (E, N), x.device, x.shape[0], slots)
     if _needs_grad(x, dt, A, B, C, D, z, dt_bias, state):
         raise NotImplementedError(f"{what} has no backward; use selective_scan for training")
+    _check_no_tangents(what, x, dt, A, B, C, state, D, z, dt_bias)
     like = x.dtype
     x, dt, B, C = (t if t.dtype == io else t.to(io) for t in (x, dt, B, C))
     z = z if z is None or z.dtype == io else z.to(io)

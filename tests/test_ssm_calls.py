@@ -179,3 +179,46 @@ def test_first_derivatives_take_no_detour(monkeypatch):
     y = sophia_b200.selective_scan(sophia_b200.short_conv(x, w)[0], x, -w, b, b)[0]
     y.sum().backward()
     assert not any(t.grad.requires_grad for t in (x, w, b))
+
+
+def test_forward_mode_is_refused():
+    """Calls that go straight to a kernel would drop a dual number's tangent."""
+    from torch.autograd import forward_ad
+
+    x, w, pool, b = _meta(3, 8), _meta(8, 4), _meta(3, 8, 3), _meta(3, 16)
+    scan = dict(x=x, dt=x, A=_meta(8, 16), B=b, C=b, state=_meta(3, 8, 16), D=_meta(8), z=x, dt_bias=_meta(8))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        calls = [lambda: sophia_b200.short_conv_step(dual(x), pool, w), lambda: sophia_b200.short_conv_step(x, dual(pool), w),
+                 lambda: sophia_b200.short_conv_step(x, pool, dual(w)),
+                 lambda: sophia_b200.short_conv_step(x, pool, w, dual(_meta(8))),
+                 lambda: ssm.put_states(dual(pool), pool, _meta(3, dtype=torch.int32)),
+                 lambda: sophia_b200.grad_norm([dual(torch.ones(3))]),
+                 lambda: sophia_b200.clip_grad_norm_([torch.ones(3), dual(torch.ones(3))], 1.0)]
+        calls += [lambda k=k: sophia_b200.selective_scan_step(**{**scan, k: dual(scan[k])}) for k in scan]
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError):  # CUDA tensors only: plain ones in a dual level are not refused for it
+            sophia_b200.grad_norm([torch.ones(3)])
+
+
+@pytest.mark.parametrize("op", ["conv", "scan"])
+def test_forward_mode_of_the_prompt_calls_is_refused(monkeypatch, op):
+    from torch.autograd import forward_ad
+
+    _without_kernels(monkeypatch)
+    x, w, b = _meta(2, 9, 8), _meta(8, 4), _meta(2, 9, 4)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            sophia_b200.short_conv(d, w) if op == "conv" else sophia_b200.selective_scan(d, x, -w, b, b)
+
+
+def test_single_tokens_compile():
+    def step(x, pool, w, A, b, state):
+        y = sophia_b200.short_conv_step(x, pool, w)
+        return sophia_b200.selective_scan_step(y, x, A, b, b, state)
+
+    args = (_meta(3, 8), _meta(4, 8, 3), _meta(8, 4), _meta(8, 16), _meta(3, 16), _meta(4, 8, 16))
+    assert torch.compile(step, backend="aot_eager", fullgraph=True)(*args).shape == (3, 8)
