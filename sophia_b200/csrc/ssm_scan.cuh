@@ -1109,7 +1109,9 @@ __global__ void __launch_bounds__(SCAN_BC_THREADS) ssm_scan_bc_kernel(const floa
 }
 
 // One token for each of `rows` requests: the slot's state [E][N] is read, stepped
-// and rewritten; every other input is a row.  Memory bound on the states.
+// and rewritten; every other input is a row.  Memory bound on the states.  A state's arithmetic is the scan's,
+// operation by operation (lane_decay's centred exponential too): decoded token by token it has the bits that a
+// prompt of one span gives it.
 // A thread owns 4 Q states of a channel (LP lanes per channel, y summed by shuffles) and
 // walks the rows with its A in registers; the grid is twice what the GPU holds.  Eight states
 // a thread rather than four halve the work per state on softplus and addresses, which
@@ -1192,7 +1194,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) ssm_scan_step_kernel(ScanStep
         for (int k = 0; k < 4; ++k)
           if (VEC || n0 + o + k < N) {
             float& v = h[4 * q + k];
-            v = fmaf(ex2(d * a[4 * q + k]), v, u * io_to_f(B[q].v[k]));
+            v = fmaf(ex2(fmaf(a[4 * q + k], d, SCAN_EXP_SHIFT)), v, u * io_to_f(B[q].v[k]));
             y = fmaf(v, io_to_f(C[q].v[k]), y);
             if (!VEC) st[o + k] = v;
           }

@@ -222,3 +222,40 @@ def test_single_tokens_compile():
 
     args = (_meta(3, 8), _meta(4, 8, 3), _meta(8, 4), _meta(8, 16), _meta(3, 16), _meta(4, 8, 16))
     assert torch.compile(step, backend="aot_eager", fullgraph=True)(*args).shape == (3, 8)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,G", [(16, 1), (4, 1), (5, 2), (24, 1), (40, 1), (64, 2)])
+def test_decoded_states_have_the_prompts_bits(dtype, N, G):
+    """A hundred tokens one by one and in one call (too few for spans): the same arithmetic for every state, so
+    the same bits, with slow decays, whose errors a state would gather over the tokens, among them."""
+    T, E, rows = 100, 26, 3
+    rn = gen(12)
+    x, z, dt = rn(rows, T, E, dtype=dtype), rn(rows, T, E, dtype=dtype), rn(rows, T, E, scale=0.5, dtype=dtype)
+    Bm, Cm = rn(rows, T, G, N, dtype=dtype), rn(rows, T, G, N, dtype=dtype)
+    A, D, bias, h0 = -torch.exp(rn(E, N) - 1.0), rn(E), rn(E) - 4.0, rn(rows, E, N)
+    y, want = sophia_b200.selective_scan(x, dt, A, Bm, Cm, D, z, bias, initial_state=h0, output_final_state=True)
+    pool, slots = torch.zeros(5, E, N, device="cuda"), torch.tensor([4, 0, 2], device="cuda", dtype=torch.int32)
+    pool[slots.long()] = h0
+    round_ = {torch.float32: 0.0, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype]
+    for t in range(T):
+        out = sophia_b200.selective_scan_step(x[:, t], dt[:, t], A, Bm[:, t], Cm[:, t], pool, D, z[:, t], bias, slots=slots)
+        # y sums the same 64 products at most in another order: 64 roundings of 2^-24 of their sizes' sum
+        size = (Cm[:, t].double().abs().repeat_interleave(E // G, 1) * pool[slots.long()].double().abs()).sum(-1)
+        size = (size + (D * x[:, t]).double().abs()) * z[:, t].double().abs()
+        tol = 64 * 2.0 ** -24 * size + 2 * round_ * y[:, t].double().abs() + 2.0 ** -24
+        assert ((out.double() - y[:, t].double()).abs() <= tol).all()
+    assert torch.equal(pool[slots.long()], want) and not pool[[1, 3]].any()
+
+
+@gpu
+@pytest.mark.parametrize("W", [1, 2, 3, 4])
+def test_fp16_convolution_steps_continue_a_prompt(W):
+    rn = gen(6)
+    x, w, b = rn(3, 30, 50, dtype=torch.float16), rn(50, W, scale=0.5), rn(50)
+    whole, final = sophia_b200.short_conv(x, w, b, output_final_state=True)
+    _, pool = sophia_b200.short_conv(x[:, :11], w, b, output_final_state=True)
+    for t in range(11, 30):
+        assert torch.equal(sophia_b200.short_conv_step(x[:, t], pool, w, b), whole[:, t])
+    assert torch.equal(pool, final)
