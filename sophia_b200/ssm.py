@@ -372,9 +372,11 @@ def short_conv_step(x: Tensor, conv_state: Tensor, weight: Tensor, bias: Tensor 
     _check_activations("short_conv_step", x=x)
     if x.dim() != 2:
         raise ValueError(f"short_conv_step: x must have shape [B, C], got {list(x.shape)}")
-    W = _check_taps("short_conv_step", weight, x.shape[1])
-    _check_params("short_conv_step", x.device, weight=(weight, (x.shape[1], W)), bias=(bias, (x.shape[1],)))
-    _check_pool("short_conv_step", conv_state, (x.shape[1], W - 1), x.device, x.shape[0], slots)
+    rows, C = x.shape
+    W = _check_taps("short_conv_step", weight, C)
+    device = x.device
+    _check_params("short_conv_step", device, weight=(weight, (C, W)), bias=(bias, (C,)))
+    _check_pool("short_conv_step", conv_state, (C, W - 1), device, rows, slots)
     if _needs_grad(x, weight, bias, conv_state):
         raise NotImplementedError("short_conv_step has no backward; use short_conv for training")
     _check_no_tangents("short_conv_step", x, conv_state, weight, bias)
@@ -508,9 +510,9 @@ class _ScanEager(torch.autograd.Function):
     """The eager path: the custom ops' implementation without their dispatch."""
 
     @staticmethod
-    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want_final, training):
-        # `training` is the caller's: grad mode is off in here, and ctx.needs_input_grad follows requires_grad
-        # alone, so that it would keep states for a backward under no_grad as well
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want_final, grad_mode):
+        # (the caller's grad mode: it is off in here, and ctx.needs_input_grad follows requires_grad alone)
+        training = grad_mode and any(ctx.needs_input_grad)
         y, ht, saved = _scan_fwd_impl(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, softplus, want_final, training)
         if training:
             ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, h0, cu_seqlens, saved)
@@ -571,14 +573,13 @@ def selective_scan(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Te
     nseq = _num_seqs(what, x, cu_seqlens)
     _check_state(what, initial_state, (nseq, E, N), x.device)
     like = x.dtype
-    x, dt, B, C = (t if t.dtype == io else t.to(io) for t in (x, dt, B, C))
-    z = z if z is None or z.dtype == io else z.to(io)
-    args = (x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, bool(dt_softplus), bool(output_final_state),
-            _needs_grad(x, dt, A, B, C, D, z, dt_bias, initial_state))
+    if x.dtype != io or dt.dtype != io or B.dtype != io or C.dtype != io or (z is not None and z.dtype != io):
+        x, dt, B, C, z = (t if t is None else t.to(io) for t in (x, dt, B, C, z))
+    args = (x, dt, A, B, C, D, z, dt_bias, initial_state, cu_seqlens, bool(dt_softplus), bool(output_final_state))
     if torch.compiler.is_compiling():
-        y, ht, _ = _scan_fwd(*args)
+        y, ht, _ = _scan_fwd(*args, _needs_grad(x, dt, A, B, C, D, z, dt_bias, initial_state))
     else:
-        y, ht = _ScanEager.apply(*args)
+        y, ht = _ScanEager.apply(*args, torch.is_grad_enabled())
     return (y if y.dtype == like else y.to(like)), (ht if output_final_state else None)
 
 
@@ -628,8 +629,8 @@ def selective_scan_step(x: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, 
         raise NotImplementedError(f"{what} has no backward; use selective_scan for training")
     _check_no_tangents(what, x, dt, A, B, C, state, D, z, dt_bias)
     like = x.dtype
-    x, dt, B, C = (t if t.dtype == io else t.to(io) for t in (x, dt, B, C))
-    z = z if z is None or z.dtype == io else z.to(io)
+    if x.dtype != io or dt.dtype != io or B.dtype != io or C.dtype != io or (z is not None and z.dtype != io):
+        x, dt, B, C, z = (t if t is None else t.to(io) for t in (x, dt, B, C, z))
     if torch.compiler.is_compiling():
         y = _scan_step(x, dt, A, B, C, state, D, z, dt_bias, slots, bool(dt_softplus))
     else:
