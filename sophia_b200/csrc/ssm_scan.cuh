@@ -842,7 +842,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     const long long to_step = (long long)TT * P.E, row_step = (long long)G::TSTEP * P.E;
     // the tile's dB and dC over the warps, [TT][2][N], and the step to the tile in front
     const long long part_step = (long long)P.G * P.blocks * (TT * 2 * N);
-    float* part = P.bc_part + ((long long)s.b * all + tile_z) * part_step + (s.g * P.blocks + s.blk) * (TT * 2 * N);
+    float* part = P.bc_part + ((long long)s.b * all + tile_z) * part_step + (long long)blockIdx.x * (TT * 2 * N);
     auto finish = [&](int i) {
       const int t0 = (tile_z - i) * TT, q = i & 1, at = (q3 * TT + pt) * CPB + pc;
       q3 = q3 == 2 ? 0 : q3 + 1;
