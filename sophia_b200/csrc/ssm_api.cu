@@ -207,9 +207,11 @@ ScanParams scan_params(const kda_b200_scan_args* a) {
 }
 
 // The spans, and the room of their carries.
-void scan_cut(ScanParams& p, Carver& cv, bool backward) {
-  p.span = scan_span(p.B, p.T, p.E, p.N, p.G, backward);
-  p.spans = (p.T + p.span - 1) / p.span;
+void cut_scan(ScanParams& p, Carver& cv, int dtype, bool backward) {
+  const ScanCut cut = scan_cut(p.B, p.T, p.E, p.N, p.G, dtype != KDA_IO_F32, backward);
+  p.span = cut.span;
+  p.spans = cut.spans(p.T);
+  p.tile = cut.tile;
   p.carry = p.spans > 1 ? cv.take<float2>(scan_carry_bytes(p.B, p.spans, p.E, p.N)) : nullptr;
 }
 
@@ -405,7 +407,7 @@ size_t kda_b200_scan_saved_bytes(int64_t B, int64_t T, int E, int N, int G) {
 size_t kda_b200_scan_workspace_bytes(int64_t B, int64_t T, int E, int N, int G, int packed, int backward) {
   if (B < 1 || T < 0 || E < 1 || N < 1 || N > SCAN_MAX_N || G < 1 || E % G) return 0;
   size_t b = map_bytes(T, packed != 0);
-  const int spans = T ? scan_spans(B, T, E, N, G, backward != 0) : 0;
+  const int spans = T ? scan_most_spans(B, T, E, N, G, backward != 0) : 0;
   b += align256(scan_carry_bytes(B, spans, E, N));
   if (backward)
     b += align256((size_t)scan_part_floats(B, T, E, N, G) * 4) + align256((size_t)B * spans * E * (N + 2) * 4);
@@ -430,7 +432,7 @@ int kda_b200_selective_scan_fwd(const kda_b200_scan_args* a, void* workspace, si
   p.vec = p.vec && aligned(a->y, 16);
   Carver cv(workspace);
   if ((rc = build_map(p.seq, cv, a->cu_seqlens, p.T, a->nseq, a->h0, a->ht, (long long)a->E * a->N, st))) return rc;
-  scan_cut(p, cv, false);
+  cut_scan(p, cv, a->dtype, false);
   return SSM_DISPATCH(a->dtype, scan_fwd, p, st);
 }
 
@@ -462,7 +464,7 @@ int kda_b200_selective_scan_bwd(const kda_b200_scan_args* a, void* workspace, si
           aligned(a->ddt, 16) && (!a->z || aligned(a->dz, 16));
   Carver cv(workspace);
   if ((rc = build_map(p.seq, cv, a->cu_seqlens, p.T, a->nseq, a->dht, a->dh0, (long long)a->E * a->N, st))) return rc;
-  scan_cut(p, cv, true);
+  cut_scan(p, cv, a->dtype, true);
   p.bc_part = cv.take<float>((size_t)scan_part_floats(p.B, p.T, p.E, p.N, p.G) * 4);
   p.e_part = cv.take<float>((size_t)p.B * p.spans * p.E * (p.N + 2) * 4);
   const ScanGrads g{a->dA, a->dD, a->ddt_bias, a->dB, a->dC};

@@ -72,11 +72,9 @@ struct ScanGeo {
   // the backward's S versions of B and C, [TT][S and a pad][NP], likewise
   static constexpr int BS = (S + 1) * NP;
 };
-// Forward tiles: 32 tokens, or 16 where two CTAs of 32 would not fit an SM (fp32; 64 channels a CTA, up to 8
-// states).  Measured for 8 states, 2048 channels, us with 16 and with 32: 1 x 8192 fp16 tokens 108 and 153; 4 x 4096
-// bf16 tokens, one CTA per SM either way, 368 (two spans) and 330.
+// Tiles of the carries' kernel; the forward's are scan_cut's choice.
 template <typename T, int L, int S>
-using ScanFwdGeo = ScanGeo<T, L, S, (sizeof(T) == 2 && L > 2) ? 32 : 16>;
+using ScanCarryGeo = ScanGeo<T, L, S, (sizeof(T) == 2 && L > 2) ? 32 : 16>;
 template <typename T, int L, int S>
 using ScanBwdGeo = ScanGeo<T, L, S, SCAN_TT_BWD>;
 
@@ -90,6 +88,7 @@ struct ScanParams {
   int B, T, E, N, G;
   int blocks;                      // channel blocks per group
   int spans, span;                 // of `span` tokens (a multiple of 32)
+  int tile;                        // tokens of a forward tile
   float2* carry;                   // [B][spans][E][N]: c and P (negative: nothing passes) of the spans; null = one span
   bool softplus, vec, vec_bc;      // vec: x, dt, z, dy and the outputs allow 16-byte pieces; vec_bc: B and C
   void* y;                         // [B, T, E] contiguous
@@ -440,7 +439,7 @@ __device__ __forceinline__ Lane<S> scan_enter(const ScanParams& P, const ScanBlo
 // u = dy silu(z) and C stand for d x and B).  The same layout as the scan's, without its outputs.
 template <typename T, int L, int S, bool PAD, bool REV>
 __global__ void __launch_bounds__(SCAN_THREADS, 3) ssm_scan_carry_kernel(ScanParams P) {
-  using G = ScanFwdGeo<T, L, S>;
+  using G = ScanCarryGeo<T, L, S>;
   constexpr int TT = G::TT, CPB = G::CPB, TENSORS = REV ? 3 : 2;
   extern __shared__ __align__(16) char scan_sm[];
   const int N = P.N, npad = (N + 7) / 8 * 8, stage = scan_stage_elems<T, G>(N, TENSORS);
@@ -583,10 +582,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) ssm_scan_carry_kernel(ScanPar
     if (live && (ok >> i & 1)) out[i] = make_float2(h.get(i), cut ? -1.f : pass.get(i));
 }
 
-template <typename T, int L, int S, bool PAD>
+template <typename T, int L, int S, int TT, bool PAD>
 __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParams P) {
-  using G = ScanFwdGeo<T, L, S>;
-  constexpr int TT = G::TT, CPB = G::CPB;
+  using G = ScanGeo<T, L, S, TT>;
+  constexpr int CPB = G::CPB;
   extern __shared__ __align__(16) char scan_sm[];
   const int N = P.N, npad = (N + 7) / 8 * 8, stage = scan_stage_elems<T, G>(N, 3);
   T* raw = reinterpret_cast<T*>(scan_sm);              // [STAGES]: x, dt, z, B rows, C rows

@@ -32,38 +32,56 @@ inline int scan_blocks(int E, int G, int L) {
   const int cpb = SCAN_WARPS * (32 / L);
   return (E / G + cpb - 1) / cpb;
 }
-// Tokens of a span: of the numbers k of spans the one that costs least, in tokens of a CTA of the scan that shares
-// its SM with another.  An SM takes its CTAs two at a time, three at a time in the carries' kernel; a
-// lone CTA takes 0.68 (up to 8 states: 0.83; there 0.5, two 0.71) of a full SM's time; the carries' token costs
-// 1.04 of the forward's, 0.37 of the backward's (0.081 us of 0.078 and 0.217, measured: bf16, N = 16); a
-// CTA's start and a launch count 40 tokens each, composing a span's carry half a token of every
-// CTA, on average.
-inline int scan_span(long long B, long long T, int E, int N, int G, bool backward) {
-  const long long ctas = B * G * scan_blocks(E, G, scan_lanes(N));
+// How a pass is cut: spans of `span` tokens, forward tiles of `tile` tokens.
+struct ScanCut {
+  int span, tile;
+  int spans(long long T) const { return (int)((T + span - 1) / span); }
+};
+// Of the numbers k of spans (and of the tiles) the one that costs least, in tokens of a CTA of the scan that shares
+// its SM with another.  An SM takes its CTAs two at a time, three at a time in the carries' kernel, one at a time
+// in the backward of more than 40 states (fp32: more than 32; 117 KB of shared memory and more).  A lone CTA takes 0.68 (up to 8 states: 0.83; more
+// than 56 in 16 bits: 0.81; there, in the carries' kernel, 0.5, two 0.71) of a full SM's time; the carries' token costs
+// 1.04 of the forward's, 0.37 of the backward's (0.081 us of 0.078 and 0.217, measured: bf16, N = 16; 0.24 of 0.34 us
+// for the backward's lone CTA of 64 states); a CTA's start and a launch count 40 tokens each, composing a span's
+// carry half a token of every CTA, on average.
+//
+// Tiles of the forward: 32 tokens in 16 bits, 16 in fp32 (two CTAs of 32 would not fit an SM).  In 16 bits two CTAs
+// of 32 do not fit either with up to 8 states (64 channels a CTA) and with more than 56 (rows of B and C).  There 16
+// tokens bring the second CTA, and 32 are the faster for one alone: 0.71 and 0.67 of a full SM's time.  So 32 where
+// the grid gives no SM a second one.  Measured, bf16, 8 and 64 states, us with 16 and with 32 (one span): one CTA per
+// SM, 148 x 2048 tokens, 207 and 170, 141 and 117; two, 240 and 334, 174 and 226.  4 x 4096 x 2048, 8 states:
+// 372 (two spans) and 330.
+inline ScanCut scan_cut(long long B, long long T, int E, int N, int G, bool half, bool backward) {
+  const int L = scan_lanes(N);
+  const long long ctas = B * G * scan_blocks(E, G, L);
   const int sms = sm_count();
-  const float weight = backward ? 0.37f : 1.04f;
-  const float lone = scan_lanes(N) == 2 ? 0.83f : 0.68f;
-  auto two = [&](long long n) { return (float)(n / 2) + (n % 2 ? lone : 0.f); };
+  const bool one = backward && N > (half ? 40 : 32);
+  const bool pick = half && !backward && (L == 2 || N > 56);  // the tiles are chosen by the grid
+  const float weight = !backward ? 1.04f : one ? 0.24f : 0.37f;
+  const float lone = L == 2 ? 0.83f : pick ? 0.81f : 0.68f, lone32 = L == 2 ? 0.71f : 0.67f;
+  auto two = [&](long long n) { return one ? (float)n : (float)(n / 2) + (n % 2 ? lone : 0.f); };
   auto three = [&](long long n) { return (float)(n / 3) + (n % 3 == 2 ? 0.71f : n % 3 ? 0.5f : 0.f); };
-  long long best = T;
+  ScanCut best{(int)T, 16};
   float least = 0.f;
   const long long most = std::min<long long>(64, T / 64);
   for (long long k = 1; k == 1 || k <= most; ++k) {
     const long long span = ((T + k - 1) / k + 31) / 32 * 32;
     if (k > 1 && (T + span - 1) / span != k) continue;
     const float t = (float)span + 40.f;
-    const float cost = two((ctas * k + sms - 1) / sms) * (t + 0.5f * k) +
+    const bool wide = half && (!pick || ctas * k <= sms);
+    const float per_sm = pick && wide ? lone32 : two((ctas * k + sms - 1) / sms);
+    const float cost = per_sm * (t + 0.5f * k) +
                        (k > 1 ? three((ctas * (k - 1) + sms - 1) / sms) * weight * t + 40.f : 0.f);
     if (k == 1 || cost < least) {
       least = cost;
-      best = span;
+      best = {(int)span, wide ? 32 : 16};
     }
   }
-  return (int)best;
+  return best;
 }
-inline int scan_spans(long long B, long long T, int E, int N, int G, bool backward) {
-  const int span = scan_span(B, T, E, N, G, backward);
-  return (int)((T + span - 1) / span);
+// Spans of a pass, whatever its type (for the size of its workspace).
+inline int scan_most_spans(long long B, long long T, int E, int N, int G, bool backward) {
+  return std::max(scan_cut(B, T, E, N, G, false, backward).spans(T), scan_cut(B, T, E, N, G, true, backward).spans(T));
 }
 // Bytes of the spans' carries (none for one span).
 inline size_t scan_carry_bytes(long long B, int spans, int E, int N) {
@@ -79,7 +97,7 @@ inline long long scan_part_floats(long long B, long long T, int E, int N, int G)
 template <typename T, int L, bool PAD, bool REV>
 int launch_scan_carry(const ScanParams& p, cudaStream_t st) {
   if (p.spans == 1) return KDA_OK;
-  const int smem = scan_carry_smem<T, ScanFwdGeo<T, L, SCAN_S>>(p.N, REV ? 3 : 2);
+  const int smem = scan_carry_smem<T, ScanCarryGeo<T, L, SCAN_S>>(p.N, REV ? 3 : 2);
   auto kernel = ssm_scan_carry_kernel<T, L, SCAN_S, PAD, REV>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan carry smem: ") + cudaGetErrorString(e));
@@ -90,15 +108,12 @@ int launch_scan_carry(const ScanParams& p, cudaStream_t st) {
   return launch_check("scan carry");
 }
 
-template <typename T, int L, bool PAD>
-int launch_scan_fwd(ScanParams p, cudaStream_t st) {
+template <typename T, int L, int TT, bool PAD>
+int launch_scan_fwd_tile(const ScanParams& p, cudaStream_t st) {
   constexpr int S = SCAN_S;
-  using G = ScanFwdGeo<T, L, S>;
-  p.blocks = scan_blocks(p.E, p.G, L);
-  const int rc = launch_scan_carry<T, L, PAD, false>(p, st);
-  if (rc) return rc;
+  using G = ScanGeo<T, L, S, TT>;
   const int smem = scan_fwd_smem<T, G>(p.N);
-  auto kernel = ssm_scan_fwd_kernel<T, L, S, PAD>;
+  auto kernel = ssm_scan_fwd_kernel<T, L, S, TT, PAD>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan forward smem: ") + cudaGetErrorString(e));
   {
@@ -106,6 +121,17 @@ int launch_scan_fwd(ScanParams p, cudaStream_t st) {
     kernel<<<dim3(p.G * p.blocks, p.B, p.spans), SCAN_THREADS, smem, st>>>(p);
   }
   return launch_check("scan forward");
+}
+
+template <typename T, int L, bool PAD>
+int launch_scan_fwd(ScanParams p, cudaStream_t st) {
+  p.blocks = scan_blocks(p.E, p.G, L);
+  const int rc = launch_scan_carry<T, L, PAD, false>(p, st);
+  if (rc) return rc;
+  if constexpr (sizeof(T) == 4) return launch_scan_fwd_tile<T, L, 16, PAD>(p, st);
+  else if constexpr (L == 2 || L == 16)
+    return p.tile == 32 ? launch_scan_fwd_tile<T, L, 32, PAD>(p, st) : launch_scan_fwd_tile<T, L, 16, PAD>(p, st);
+  else return launch_scan_fwd_tile<T, L, 32, PAD>(p, st);
 }
 
 template <typename T, int L, bool PAD>
