@@ -40,6 +40,8 @@
 // 9 spans 150 + 114 (carries) forward, 392 + 114 backward; a prompt of 16384 tokens 262 + 193.
 #pragma once
 
+#include <cfloat>
+
 #include "ssm_common.cuh"
 
 namespace kda {
@@ -131,6 +133,13 @@ constexpr float SCAN_EXP_SHIFT = 1.44e-8f;
 template <int S>
 __device__ __forceinline__ Lane<S> lane_decay(const Lane<S>& a2, float d) {
   return fma(a2, Lane<S>::all(d), Lane<S>::all(SCAN_EXP_SHIFT)).exp2();
+}
+// A decay rate in powers of two.  A state that forgets at once (a rate of -inf) has the lowest finite one: 2^(d a2) is
+// 0 for every d above 1e-36 all the same, and 1 for the d = 0 of the places past a row's end, where 0 x inf would
+// make NaN of the gradients that the backward carries on from there.
+__device__ __forceinline__ float scan_rate(float a) {
+  const float v = a * LOG2E;
+  return v == -INFINITY ? -FLT_MAX : v;
 }
 // sum += v with the rounding errors carried along (a compensated sum: its error does not
 // grow with the number of tokens).
@@ -523,7 +532,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) ssm_scan_carry_kernel(ScanPar
   const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
 #pragma unroll
   for (int i = 0; i < S; ++i)
-    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + i] * LOG2E);
+    if (live && (ok >> i & 1)) a2.set(i, scan_rate(P.A[chan + i]));
   float dsum = 0.f, dsum_err = 0.f;
   bool cut = false;  // a sequence starts in the span: nothing passes it
   __syncthreads();
@@ -688,7 +697,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
   const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
 #pragma unroll
   for (int i = 0; i < S; ++i)
-    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + i] * LOG2E);
+    if (live && (ok >> i & 1)) a2.set(i, scan_rate(P.A[chan + i]));
   if (s.k > 0 && live) h = scan_enter<S, false>(P, s, chan, ok, 0);
   __syncthreads();
   for (int tile = 0; tile < tiles; ++tile) {
@@ -944,7 +953,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
 #pragma unroll
   for (int i = 0; i < S; ++i) {
     dA[i] = dA_err[i] = 0.f;
-    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + (i ^ m)] * LOG2E);
+    if (live && (ok >> i & 1)) a2.set(i, scan_rate(P.A[chan + (i ^ m)]));
   }
   if (s.k + 1 < P.spans && live) r = scan_enter<S, true>(P, s, chan, ok, m);
   __syncthreads();
@@ -1151,7 +1160,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) ssm_scan_step_kernel(ScanStep
   int s = step_slot(P.slots, r, P.pool, P.err);
   float a[S];
 #pragma unroll
-  for (int i = 0; i < S; ++i) a[i] = n0 + at(i) < N ? __ldg(P.A + (long long)ec * N + n0 + at(i)) * LOG2E : 0.f;
+  for (int i = 0; i < S; ++i) a[i] = n0 + at(i) < N ? scan_rate(__ldg(P.A + (long long)ec * N + n0 + at(i))) : 0.f;
   const float D = P.D ? __ldg(P.D + ec) : 0.f, bias = P.dt_bias ? __ldg(P.dt_bias + ec) : 0.f;
   while (true) {
     const int after = r + step < P.rows ? step_slot(P.slots, r + step, P.pool, P.err) : -1;

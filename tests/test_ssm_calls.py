@@ -259,3 +259,41 @@ def test_fp16_convolution_steps_continue_a_prompt(W):
     for t in range(11, 30):
         assert torch.equal(sophia_b200.short_conv_step(x[:, t], pool, w, b), whole[:, t])
     assert torch.equal(pool, final)
+
+
+@gpu
+@pytest.mark.parametrize("T,B", [(5, 2), (16, 1), (43, 2), (1203, 1)])  # ends inside a tile and at one; spans
+def test_states_that_forget_at_once(T, B):
+    """A rate of -inf: its decay is 0 for every step, so everything is as with a rate of -1e30, bit for bit; the
+    places past a row's end (steps of 0) add nothing."""
+    E, N = 20, 5
+    rn = gen(8)
+    x, dt, z, bc = rn(B, T, E), rn(B, T, E), rn(B, T, E), rn(B, T, 2 * N)
+    dy, h0 = rn(B, T, E), rn(B, E, N)
+
+    def run(rate):
+        A = -torch.exp(gen(4)(E, N))
+        A[::3, 1] = rate
+        A[4] = rate
+        ts = [t.detach().clone().requires_grad_() for t in (x, dt, A, bc[..., :N], bc[..., N:], z, h0)]
+        y, ht = sophia_b200.selective_scan(*ts[:5], None, ts[5], initial_state=ts[6], output_final_state=True)
+        return [y, ht, *torch.autograd.grad((y, ht), ts, (dy, torch.ones_like(ht)))], A, ts
+
+    got, A, _ = run(float("-inf"))
+    want, _, _ = run(-1e30)
+    for a, b in zip(got, want):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    pool = h0.clone()
+    for t in range(min(T, 5)):
+        sophia_b200.selective_scan_step(x[:, t], dt[:, t], A, bc[:, t, :N], bc[:, t, N:], pool, None, z[:, t])
+    assert torch.isfinite(pool).all()
+
+
+@gpu
+def test_a_rate_that_is_not_a_number_shows():
+    A = -torch.ones(4, 3, device="cuda")
+    A[1, 2] = float("nan")
+    rn = gen(1)
+    x, b = rn(1, 9, 4), rn(1, 9, 3)
+    y, _ = sophia_b200.selective_scan(x, x, A, b, b)
+    assert torch.isnan(y[0, :, 1]).all() and torch.isfinite(y[0, :, [0, 2, 3]]).all()
