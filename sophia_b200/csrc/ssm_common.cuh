@@ -218,12 +218,7 @@ __device__ __forceinline__ float softplusf_(float x) {
   q = fmaf(q, v, 1.f);
   return fmaf(2.f * s, q, fmaxf(x, 0.f));
 }
-// silu(v) and its derivative p (1 + v (1 - p)), p = logistic(v)
 __device__ __forceinline__ float siluf_(float v) { return v * sigmoidf_(v); }
-__device__ __forceinline__ float silu_slopef_(float v) {
-  const float p = sigmoidf_(v);
-  return p * fmaf(v, 1.f - p, 1.f);
-}
 
 // The pool entry of a single-token call's row: negative for a padding row; an entry past the pool is
 // reported (device error 11) and treated as one.

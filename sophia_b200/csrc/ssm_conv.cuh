@@ -7,17 +7,20 @@
 //   dbias = sum_t dc[t],
 // the terms of positions before the first token going to the initial state.
 //
-// Memory bound: x is read once and y written once (forward), x and dy read and
+// Memory bound by its bytes: x is read once and y written once (forward), x and dy read and
 // dx written once (backward, c is recomputed).  A thread owns V = 2 neighbouring
 // channels (1 where rows are not aligned for that) and walks a run of tokens with the last
-// three inputs (and the three pending dx) in registers, rows loaded 8 ahead; runs re-read a
-// halo of three tokens.  Two channels a thread rather than eight: the same bytes in flight from four
-// times the threads at a third of the registers.  W < 4 runs as
+// three inputs (and the three pending dx) in registers, rows fetched groups ahead through a ring in
+// shared memory; runs re-read a halo of three tokens.  Two channels a thread rather than eight: the same bytes in
+// flight from four times the threads at a third of the registers.  W < 4 runs as
 // four taps whose leading ones are left out (FULL = false): not multiplied by zero, so that
 // an infinity beyond the taps' reach stays out of the sum.
 // Measured, bf16 [4, 4096, 2048] with SiLU: forward 36 us (3.7 TB/s of 134 MB), backward
-// 64 us (3.2 TB/s of 201 MB) and 3 us to join dw; the issue of instructions, half of the
-// backward's for the gradient of SiLU, bounds both by then.
+// 64 us (3.2 TB/s of 201 MB) and 3 us to join dw.  No pipe is full by the counters of that size; warps wait for their
+// own results.  Forward: 58 % of issue slots, 49 % of the pipe of ex2 and rcp, 31 % of HBM's time, 6.7 warps per
+// scheduler of which 1.8 can issue, 1024 CTAs in 1.7 waves.  Backward: 53 %, 26 %, 31 %, 3.4 warps (114 registers) of
+// which 1.0 can issue; of the 6.4 cycles between a warp's instructions 2.0 are fixed latency, 0.8 shared memory
+// and special functions, 0.7 the fp32 pipe.
 #pragma once
 
 #include <type_traits>
@@ -28,7 +31,7 @@ namespace kda {
 
 constexpr int CONV_THREADS = 256;
 constexpr int CONV_BWD_GROUP = 4;
-constexpr int CONV_GROUP = 8;  // rows loaded ahead: 8 x 4 bytes of 1500 threads per SM keep HBM busy
+constexpr int CONV_GROUP = 8;  // rows a forward group (the ring holds four groups of 4-byte pieces, two of 8 bytes)
 
 struct ConvParams {
   RowView x, dy;        // [B, T, C]

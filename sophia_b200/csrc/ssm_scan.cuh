@@ -33,10 +33,14 @@
 // alone: no C, no output), and a CTA of the scan itself composes those in front of its own.
 // Backward the same with g, from behind.
 //
-// What bounds it: instruction issue and shared memory, not HBM.  For 32 states' tokens (N = 16) the
-// forward issues 10 instructions and holds the exponential's pipe for 2.5 cycles of 4.2; the backward 32
-// and 4.3 of 11, half of the instructions on the token side.  Measured, bf16, 2048 channels, N = 16:
-// 4 x 4096 tokens forward 302 us (0.9 TB/s), backward 796 + 31 us for dB and dC; 8192 packed tokens in
+// What bounds it: latency, neither HBM nor a pipe.  For 32 states' tokens (N = 16) the forward issues 10
+// instructions and holds the exponentials' pipe for 2.5 cycles of 4.2; the backward 32 and 4.3 of 11, half of
+// the instructions on the token side.  Counters, bf16, 4 x 4096 tokens x 2048 channels, N = 16 (256 CTAs: 108 SMs with
+// two, 40 with one): forward 53 % of issue slots, 53 % of that pipe, 71 % of shared memory, 3.4 warps per
+// scheduler of which 0.8 can issue, none in 47 % of cycles; backward 62 %, 30 %, 60 %, 3.3 warps, 1.1, 38 %.  Of the
+// 6.4 and 5.4 cycles between a warp's instructions 1.9 and 1.3 are fixed latency, 1.3 and 0.5 shared memory and
+// special functions, 0.5 and 0.7 the barrier of the tile.
+// Measured there: forward 285 us (0.9 TB/s), backward 796 + 31 us for dB and dC; 8192 packed tokens in
 // 9 spans 150 + 114 (carries) forward, 392 + 114 backward; a prompt of 16384 tokens 262 + 193.
 #pragma once
 
