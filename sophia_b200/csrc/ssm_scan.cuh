@@ -152,6 +152,11 @@ __device__ __forceinline__ void sum_add(float& sum, float& err, float v) {
   err = __fadd_rn(__fadd_rn(t, -sum), -y);
   sum = t;
 }
+// The same for sums that an infinity has to leave infinite (inf - inf would make NaN of the error).
+__device__ __forceinline__ void sum_add_inf(float& sum, float& err, float v) {
+  sum_add(sum, err, v);
+  err = fabsf(sum) <= FLT_MAX ? err : 0.f;
+}
 
 // Zero in the states that do not exist (PAD: N < L S), whatever arithmetic made of them.
 template <bool PAD, int S>
@@ -882,10 +887,10 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
               scan_put_pair<T>(P.dz, o, how, make_float2(dz.x * fmaf(skip.x, x.x, s0.x), dz.y * fmaf(skip.y, x.y, s0.y)));
             scan_put_pair<T>(P.ddt, o, how, dd);
             scan_put_pair<T>(P.dx, o, how, make_float2(fmaf(g0.x, du.x, ds.x * skip.x), fmaf(g0.y, du.z, ds.y * skip.y)));
-            sum_add(db.x, db_err.x, dd.x);
-            sum_add(db.y, db_err.y, dd.y);
-            sum_add(dD.x, dD_err.x, ds.x * x.x);
-            sum_add(dD.y, dD_err.y, ds.y * x.y);
+            sum_add_inf(db.x, db_err.x, dd.x);
+            sum_add_inf(db.y, db_err.y, dd.y);
+            sum_add_inf(dD.x, dD_err.x, ds.x * x.x);
+            sum_add_inf(dD.y, dD_err.y, ds.y * x.y);
           }
         }
       }

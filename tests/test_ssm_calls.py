@@ -297,3 +297,24 @@ def test_a_rate_that_is_not_a_number_shows():
     x, b = rn(1, 9, 4), rn(1, 9, 3)
     y, _ = sophia_b200.selective_scan(x, x, A, b, b)
     assert torch.isnan(y[0, :, 1]).all() and torch.isfinite(y[0, :, [0, 2, 3]]).all()
+
+
+@gpu
+def test_an_infinite_gradient_leaves_infinite_sums():
+    """dD = sum ds x and d dt_bias = sum d dt over the tokens: one infinite term makes them infinite, as the plain sum,
+    where it is the only one; other channels stay finite."""
+    E, N, T = 12, 4, 75
+    rn = gen(2)
+    x, dt, b, dy = rn(2, T, E), rn(2, T, E), rn(2, T, N), rn(2, T, E)
+    z = rn(2, T, E)
+    for at in (0, 33, T - 1):
+        for value in (float("inf"), -float("inf")):
+            bad = dy.clone()
+            bad[1, at, 5] = value
+            D, bias = rn(E).requires_grad_(), rn(E).requires_grad_()
+            y, _ = sophia_b200.selective_scan(x, dt, -torch.ones(E, N, device="cuda"), b, b, D, z, bias)
+            dD, dbias = torch.autograd.grad(y, (D, bias), bad)
+            want = value * torch.sign(x[1, at, 5] * z[1, at, 5])
+            assert dD[5] == want and not torch.isfinite(dbias[5])
+            rest = [k for k in range(E) if k != 5]
+            assert torch.isfinite(dD[rest]).all() and torch.isfinite(dbias[rest]).all()
