@@ -208,7 +208,7 @@ ScanParams scan_params(const kda_b200_scan_args* a) {
 
 // The spans, and the room of their carries.
 void cut_scan(ScanParams& p, Carver& cv, int dtype, bool backward) {
-  const ScanCut cut = scan_cut(p.B, p.T, p.E, p.N, p.G, dtype != KDA_IO_F32, backward);
+  const ScanCut cut = scan_cut(p.B, p.T, p.E, p.N, p.G, dtype != KDA_IO_F32, p.vec, backward);
   p.span = cut.span;
   p.spans = cut.spans(p.T);
   p.tile = cut.tile;

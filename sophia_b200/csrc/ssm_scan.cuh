@@ -138,9 +138,10 @@ template <int S>
 __device__ __forceinline__ Lane<S> lane_decay(const Lane<S>& a2, float d) {
   return fma(a2, Lane<S>::all(d), Lane<S>::all(SCAN_EXP_SHIFT)).exp2();
 }
-// A decay rate in powers of two.  A state that forgets at once (a rate of -inf) has the lowest finite one: 2^(d a2) is
-// 0 for every d above 1e-36 all the same, and 1 for the d = 0 of the places past a row's end, where 0 x inf would
-// make NaN of the gradients that the backward carries on from there.
+// A decay rate in powers of two, for the backward.  A state that forgets at once (a rate of -inf) has the lowest finite
+// one: 2^(d a2) is 0 for every d above 1e-36 all the same, and 1 for the d = 0 of the places past a row's end,
+// where 0 x inf would make NaN of the gradients that the backward carries on from there (nothing is carried from
+// there forward).
 __device__ __forceinline__ float scan_rate(float a) {
   const float v = a * LOG2E;
   return v == -INFINITY ? -FLT_MAX : v;
@@ -151,11 +152,6 @@ __device__ __forceinline__ void sum_add(float& sum, float& err, float v) {
   const float y = __fadd_rn(v, -err), t = __fadd_rn(sum, y);
   err = __fadd_rn(__fadd_rn(t, -sum), -y);
   sum = t;
-}
-// The same for sums that an infinity has to leave infinite (inf - inf would make NaN of the error).
-__device__ __forceinline__ void sum_add_inf(float& sum, float& err, float v) {
-  sum_add(sum, err, v);
-  err = fabsf(sum) <= FLT_MAX ? err : 0.f;
 }
 
 // Zero in the states that do not exist (PAD: N < L S), whatever arithmetic made of them.
@@ -541,7 +537,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 3) ssm_scan_carry_kernel(ScanPar
   const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
 #pragma unroll
   for (int i = 0; i < S; ++i)
-    if (live && (ok >> i & 1)) a2.set(i, scan_rate(P.A[chan + i]));
+    if (live && (ok >> i & 1)) a2.set(i, REV ? scan_rate(P.A[chan + i]) : P.A[chan + i] * LOG2E);
   float dsum = 0.f, dsum_err = 0.f;
   bool cut = false;  // a sequence starts in the span: nothing passes it
   __syncthreads();
@@ -706,7 +702,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_fwd_kernel(ScanParam
   const long long chan = (long long)(s.c0 + (live ? c : 0)) * N + n0;
 #pragma unroll
   for (int i = 0; i < S; ++i)
-    if (live && (ok >> i & 1)) a2.set(i, scan_rate(P.A[chan + i]));
+    if (live && (ok >> i & 1)) a2.set(i, P.A[chan + i] * LOG2E);
   if (s.k > 0 && live) h = scan_enter<S, false>(P, s, chan, ok, 0);
   __syncthreads();
   for (int tile = 0; tile < tiles; ++tile) {
@@ -801,7 +797,8 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     const int pc = (tid % G::PAIRS) * 2, pt = tid / G::PAIRS;
     const float2 bias = scan_param(P.dt_bias, s, pc), skip = scan_param(P.D, s, pc);
     const float2 zero = make_float2(0.f, 0.f);
-    float2 dD = zero, db = zero, dD_err = zero, db_err = zero;
+    // (dD_plain: what dD is where a term is infinite, of which a compensated sum makes NaN, inf - inf)
+    float2 dD = zero, db = zero, dD_err = zero, db_err = zero, dD_plain = zero;
     const RowView views[4] = {P.x, P.dt, P.dy, P.z};
     ScanFetch<T, G, 4> f;
     f.init(P, s, views, tid, 4 * G::RAW, npad, tile_z, -1);
@@ -887,10 +884,13 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
               scan_put_pair<T>(P.dz, o, how, make_float2(dz.x * fmaf(skip.x, x.x, s0.x), dz.y * fmaf(skip.y, x.y, s0.y)));
             scan_put_pair<T>(P.ddt, o, how, dd);
             scan_put_pair<T>(P.dx, o, how, make_float2(fmaf(g0.x, du.x, ds.x * skip.x), fmaf(g0.y, du.z, ds.y * skip.y)));
-            sum_add_inf(db.x, db_err.x, dd.x);
-            sum_add_inf(db.y, db_err.y, dd.y);
-            sum_add_inf(dD.x, dD_err.x, ds.x * x.x);
-            sum_add_inf(dD.y, dD_err.y, ds.y * x.y);
+            sum_add(db.x, db_err.x, dd.x);
+            sum_add(db.y, db_err.y, dd.y);
+            const float2 v = make_float2(ds.x * x.x, ds.y * x.y);
+            sum_add(dD.x, dD_err.x, v.x);
+            sum_add(dD.y, dD_err.y, v.y);
+            dD_plain.x += v.x;
+            dD_plain.y += v.y;
           }
         }
       }
@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(SCAN_THREADS, 2) ssm_scan_bwd_kernel(ScanParam
     // the row's dD and d dt_bias: over the side's threads of a channel pair
     asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");
     float4* sums = reinterpret_cast<float4*>(scan_sm);
-    sums[tid] = make_float4(dD.x, dD.y, db.x, db.y);
+    sums[tid] = make_float4(isnan(dD.x) ? dD_plain.x : dD.x, isnan(dD.y) ? dD_plain.y : dD.y, db.x, db.y);
     asm volatile("bar.sync 1, %0;" ::"n"(G::TOKENS) : "memory");
     if (tid < G::PAIRS) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -1169,7 +1169,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 4) ssm_scan_step_kernel(ScanStep
   int s = step_slot(P.slots, r, P.pool, P.err);
   float a[S];
 #pragma unroll
-  for (int i = 0; i < S; ++i) a[i] = n0 + at(i) < N ? scan_rate(__ldg(P.A + (long long)ec * N + n0 + at(i))) : 0.f;
+  for (int i = 0; i < S; ++i) a[i] = n0 + at(i) < N ? __ldg(P.A + (long long)ec * N + n0 + at(i)) * LOG2E : 0.f;
   const float D = P.D ? __ldg(P.D + ec) : 0.f, bias = P.dt_bias ? __ldg(P.dt_bias + ec) : 0.f;
   while (true) {
     const int after = r + step < P.rows ? step_slot(P.slots, r + step, P.pool, P.err) : -1;

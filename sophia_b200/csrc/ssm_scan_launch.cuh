@@ -39,28 +39,34 @@ struct ScanCut {
 };
 // Of the numbers k of spans (and of the tiles) the one that costs least, in tokens of a CTA of the scan that shares
 // its SM with another.  An SM takes its CTAs two at a time, three at a time in the carries' kernel, one at a time
-// in the backward of more than 40 states (fp32: more than 32; 117 KB of shared memory and more).  A lone CTA takes 0.68 (up to 8 states: 0.83; more
-// than 56 in 16 bits: 0.81; there, in the carries' kernel, 0.5, two 0.71) of a full SM's time; the carries' token costs
-// 1.04 of the forward's, 0.37 of the backward's (0.081 us of 0.078 and 0.217, measured: bf16, N = 16; 0.24 of 0.34 us
-// for the backward's lone CTA of 64 states); a CTA's start and a launch count 40 tokens each, composing a span's
-// carry half a token of every CTA, on average.
+// in the backward of more than 40 states (fp32: more than 32; 117 KB of shared memory and more).  A lone CTA takes
+// 0.68 (up to 8 states: 0.83; more than 56 in 16 bits: 0.81; in the carries' kernel 0.5, two 0.71) of a full SM's time;
+// the carries' token costs 1.04 of the forward's, 0.37 of the backward's (0.081 us of 0.078 and 0.217, measured:
+// bf16, N = 16; 0.24 of 0.34 us for the backward's lone CTA of 64 states).  Up to 8 states forward, rows in 16-byte
+// pieces: 0.66 of 0.117 us, there a lone CTA 0.75, two 0.8 (3 x 8021 x 2520 tokens and channels in 4, 6, 8, 12 spans:
+// 645, 656, 648, 590 us by this, 669, 661, 634, 591 measured).  A CTA's start and a launch count 40 tokens each,
+// composing a span's carry half a token of every CTA, on average.
 //
 // Tiles of the forward: 32 tokens in 16 bits, 16 in fp32 (two CTAs of 32 would not fit an SM).  In 16 bits two CTAs
 // of 32 do not fit either with up to 8 states (64 channels a CTA) and with more than 56 (rows of B and C).  There 16
-// tokens bring the second CTA, and 32 are the faster for one alone: 0.71 and 0.67 of a full SM's time.  So 32 where
-// the grid gives no SM a second one.  Measured, bf16, 8 and 64 states, us with 16 and with 32 (one span): one CTA per
-// SM, 148 x 2048 tokens, 207 and 170, 141 and 117; two, 240 and 334, 174 and 226.  4 x 4096 x 2048, 8 states:
-// 372 (two spans) and 330.
-inline ScanCut scan_cut(long long B, long long T, int E, int N, int G, bool half, bool backward) {
+// tokens bring the second CTA, and 32 are the faster for one alone: 0.69 and 0.67 of a full SM's time.  So 32 where
+// the grid gives no SM a second one, from 64 tokens on (one CTA per SM, 3 states, us with 16 and with 32: 16 tokens
+// 10.2 and 11.0, 33 tokens 13.2 and 13.2, 64 tokens 15.3 and 13.3); with up to 8 states only where rows are read in
+// 16-byte pieces (element by element, 120 x 2048 x 61: 429 us with 16 and spans, 609 with 32).  Measured, bf16, 8 and 64
+// states, us with 16 and with 32 (one span): one CTA per SM, 148 x 2048 tokens, 207 and 170, 141 and 117; two, 240
+// and 334, 174 and 226.  4 x 4096 x 2048, 8 states: 343 (four spans) and 330.
+inline ScanCut scan_cut(long long B, long long T, int E, int N, int G, bool half, bool vec, bool backward) {
   const int L = scan_lanes(N);
   const long long ctas = B * G * scan_blocks(E, G, L);
   const int sms = sm_count();
   const bool one = backward && N > (half ? 40 : 32);
+  const bool few = !backward && L == 2 && vec;
   const bool pick = half && !backward && (L == 2 || N > 56);  // the tiles are chosen by the grid
-  const float weight = !backward ? 1.04f : one ? 0.24f : 0.37f;
-  const float lone = L == 2 ? 0.83f : pick ? 0.81f : 0.68f, lone32 = L == 2 ? 0.71f : 0.67f;
+  const float weight = backward ? (one ? 0.24f : 0.37f) : few ? 0.66f : 1.04f;
+  const float lone = L == 2 ? 0.83f : pick ? 0.81f : 0.68f, lone32 = few ? 0.69f : 0.67f;
   auto two = [&](long long n) { return one ? (float)n : (float)(n / 2) + (n % 2 ? lone : 0.f); };
-  auto three = [&](long long n) { return (float)(n / 3) + (n % 3 == 2 ? 0.71f : n % 3 ? 0.5f : 0.f); };
+  const float carry1 = few ? 0.75f : 0.5f, carry2 = few ? 0.8f : 0.71f;
+  auto three = [&](long long n) { return (float)(n / 3) + (n % 3 == 2 ? carry2 : n % 3 ? carry1 : 0.f); };
   ScanCut best{(int)T, 16};
   float least = 0.f;
   const long long most = std::min<long long>(64, T / 64);
@@ -68,7 +74,7 @@ inline ScanCut scan_cut(long long B, long long T, int E, int N, int G, bool half
     const long long span = ((T + k - 1) / k + 31) / 32 * 32;
     if (k > 1 && (T + span - 1) / span != k) continue;
     const float t = (float)span + 40.f;
-    const bool wide = half && (!pick || ctas * k <= sms);
+    const bool wide = half && (!pick || ((few || N > 56) && ctas * k <= sms && T >= 64));
     const float per_sm = pick && wide ? lone32 : two((ctas * k + sms - 1) / sms);
     const float cost = per_sm * (t + 0.5f * k) +
                        (k > 1 ? three((ctas * (k - 1) + sms - 1) / sms) * weight * t + 40.f : 0.f);
@@ -79,9 +85,13 @@ inline ScanCut scan_cut(long long B, long long T, int E, int N, int G, bool half
   }
   return best;
 }
-// Spans of a pass, whatever its type (for the size of its workspace).
+// The most spans that a pass of any type and alignment is cut into (its workspace has room for them).
 inline int scan_most_spans(long long B, long long T, int E, int N, int G, bool backward) {
-  return std::max(scan_cut(B, T, E, N, G, false, backward).spans(T), scan_cut(B, T, E, N, G, true, backward).spans(T));
+  auto spans = [&](bool half, bool vec) { return scan_cut(B, T, E, N, G, half, vec, backward).spans(T); };
+  int n = spans(true, true);
+  if (backward ? N > 32 && N <= 40 : N <= 8 || N > 56) n = std::max(n, spans(false, true));
+  if (!backward && N <= 8) n = std::max(n, spans(false, false));  // (as in 16 bits)
+  return n;
 }
 // Bytes of the spans' carries (none for one span).
 inline size_t scan_carry_bytes(long long B, int spans, int E, int N) {
