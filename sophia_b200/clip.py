@@ -25,18 +25,17 @@ __all__ = ["grad_norm", "clip_grad_norm_"]
 def _list(what: str, grads) -> tuple[list[Tensor], torch.device | None, bytes]:
     """The tensors, their one device and their types."""
     ts = [grads] if isinstance(grads, Tensor) else list(grads)
-    for t in ts:
-        if not isinstance(t, Tensor):
-            raise ValueError(f"{what} takes gradient tensors, got {type(t).__name__}")
+    for kind in set(map(type, ts)):
+        if not issubclass(kind, Tensor):
+            raise ValueError(f"{what} takes gradient tensors, got {kind.__name__}")
     try:
         types = bytes([_IO[t.dtype] for t in ts])
     except KeyError as e:
         raise NotImplementedError(f"{what}: gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
     _check_no_tangents(what, *ts)
-    devices = {t.device for t in ts}
-    if len(devices) > 1:
+    if len(set(map(Tensor.get_device, ts))) > 1:
         raise RuntimeError(f"{what}: gradients are on several devices")
-    device = devices.pop() if devices else None
+    device = ts[0].device if ts else None
     if device is not None and device.type != "cuda":
         raise RuntimeError(f"{what} runs on the CUDA kernels only: gradients must be CUDA tensors")
     return ts, device, types
@@ -55,12 +54,14 @@ def _dense(t: Tensor) -> bool:
 
 
 def _launch(ts: list[Tensor], types: bytes, out: list[Tensor] | None, out_types: bytes | None, max_norm: float,
-            eps: float) -> Tensor:
+            eps: float, at: list[int] | None = None, sizes: list[int] | None = None) -> Tensor:
+    """``at``, ``sizes``: the outputs' addresses and element counts, where the caller has them."""
     norm = ts[0].new_empty((), dtype=torch.float32)
     lib = _lib.load()
     ws = norm.new_empty(lib.kda_b200_grad_workspace_bytes(len(ts)), dtype=torch.uint8)
-    src, numel = array("Q", map(Tensor.data_ptr, ts)), array("q", map(Tensor.numel, ts))
-    dst = None if out is None else src if out is ts else array("Q", map(Tensor.data_ptr, out))
+    numel = array("q", map(Tensor.numel, ts) if sizes is None else sizes)
+    dst = None if out is None else array("Q", map(Tensor.data_ptr, out) if at is None else at)
+    src = dst if dst is not None and out is ts else array("Q", map(Tensor.data_ptr, ts))
     addr = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
     args = GradArgs(len(ts), addr(src), addr(dst), addr(numel), types, out_types, max_norm, eps, norm.data_ptr())
     _call(lib.kda_b200_grad_clip, norm.device, args, ws.data_ptr(), ws.numel())
@@ -107,13 +108,13 @@ def clip_grad_norm_(grads: Tensor | Iterable[Tensor], max_norm: float, *, eps: f
                     raise ValueError(f"{what}: an output of shape {list(o.shape)} for a gradient of {list(g.shape)}")
             if out_device != device:
                 raise RuntimeError(f"{what}: gradients and outputs are on different devices")
-        where = [o.data_ptr() for o in outs if o.numel()]
-        if len(set(where)) != len(where):
+        at, sizes = list(map(Tensor.data_ptr, outs)), list(map(Tensor.numel, outs))
+        if len(set(at)) != len(at) and len({a for a, n in zip(at, sizes) if n}) != len(sizes) - sizes.count(0):
             raise ValueError(f"{what}: one tensor is named twice")
         if any(o.requires_grad for o in outs):
             raise ValueError(f"{what} scales gradients; a tensor that requires grad (a parameter?) is not one")
         if all(map(Tensor.is_contiguous, ts)) and (outs is ts or all(map(Tensor.is_contiguous, outs))):
-            norm = _launch(ts, types, outs, out_types, max_norm, eps)
+            norm = _launch(ts, types, outs, out_types, max_norm, eps, at, sizes)
             increment_version(outs)  # written in place: a graph that saved one has to notice
             return norm
         src, dst, back = list(ts), list(outs), []
