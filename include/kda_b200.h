@@ -309,7 +309,7 @@ int kda_b200_gated_norm_bwd(const void* dy, const void* o, const void* g, const 
  * gradients are fp32.  cu_seqlens (int32 [N+1], device; then B == 1) packs N
  * sequences along T; every sequence starts from its own initial state.  An
  * empty sequence's final state is its initial state.  A malformed table sets
- * kda_b200_device_error() to 3.  Every element of every output is written.
+ * kda_b200_device_error() to 3.  Every element of every output is written.  B <= 65535.
  */
 #define KDA_IO_F32 0
 #define KDA_IO_BF16 1

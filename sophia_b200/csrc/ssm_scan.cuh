@@ -40,7 +40,7 @@
 // scheduler of which 0.8 can issue, none in 47 % of cycles; backward 62 %, 30 %, 60 %, 3.3 warps, 1.1, 38 %.  Of the
 // 6.4 and 5.4 cycles between a warp's instructions 1.9 and 1.3 are fixed latency, 1.3 and 0.5 shared memory and
 // special functions, 0.5 and 0.7 the barrier of the tile.
-// Measured there: forward 285 us (0.9 TB/s), backward 796 + 31 us for dB and dC; 8192 packed tokens in
+// Measured there: forward 302 us (0.9 TB/s; 285 without checkpoints), backward 796 + 31 us for dB and dC; 8192 packed tokens in
 // 9 spans 150 + 114 (carries) forward, 392 + 114 backward; a prompt of 16384 tokens 262 + 193.
 #pragma once
 
