@@ -73,7 +73,8 @@ def grad_norm(grads: Tensor | Iterable[Tensor]) -> Tensor:
     float16, any mix), as a 0-d float32 CUDA tensor; 0 on an empty list is on the
     current device.  No host wait.  The result does not depend on timing: sums have a
     fixed order (which the sizes, the addresses modulo 16 bytes and the number of SMs decide).  Squares do not
-    overflow or vanish: the norm is right wherever float32 can hold it."""
+    overflow or vanish: the norm is right wherever float32 can hold it.  Not differentiable: the norm has no
+    graph."""
     with torch.no_grad():
         ts, _, types = _list("grad_norm", grads)
         if not ts:
