@@ -397,6 +397,48 @@ int kda_b200_selective_scan_bwd(const kda_b200_scan_args* args, void* workspace,
 int kda_b200_selective_scan_step(const kda_b200_scan_args* args, void* stream);
 
 /*
+ * Gated linear recurrence.  Per sequence and channel e, with r = sigmoid(decay + decay_bias) and
+ * i = sigmoid(gate + gate_bias):
+ *     a = exp(A[e] r),   h[t] = a h[t-1] + sqrt(1 - a^2) i x[t],   y[t] = h[t] silu(z[t])  (or h[t])
+ * A: [E], not positive (a positive rate has no real normaliser: its outputs are NaN).  One state per
+ * channel: h0, ht, dht, dh0: [nseq][E].  Unused pointers are NULL: z, decay_bias, gate_bias, h0, ht, dht, dh0,
+ * cu_seqlens; saved (kda_b200_recurrence_saved_bytes() bytes) is NULL for inference.
+ * kda_b200_recurrence_bwd takes the same inputs, the saved buffer of the forward, dy and dht, and writes dx, ddecay,
+ * dgate, dz [B, T, E] in the activations' type and dA, ddecay_bias, dgate_bias [E] (the last two may be
+ * NULL) and dh0 in fp32; all sums have a fixed order.  Where nothing decays (a = 1 to the last bit) the input's part of
+ * ddecay and dA, which has no limit for A = 0, counts as 0.
+ * kda_b200_recurrence_step takes `rows` single tokens: x, decay, gate, z [rows, E] (*_sb: row strides), a pool of
+ * states [pool][E] rewritten in place, and slots as kda_b200_short_conv_step; y [rows, E].
+ */
+typedef struct kda_b200_recurrence_args {
+  int64_t B, T;
+  int32_t E, nseq, dtype, rows;
+  const void *x, *decay, *gate, *z;
+  int64_t x_sb, x_st, decay_sb, decay_st, gate_sb, gate_st, z_sb, z_st;
+  const float *A, *decay_bias, *gate_bias, *h0;
+  const int32_t* cu_seqlens;
+  void* y;
+  float* ht;
+  void* saved;
+  size_t saved_bytes;
+  /* backward */
+  const void* dy;
+  int64_t dy_sb, dy_st;
+  const float* dht;
+  void *dx, *ddecay, *dgate, *dz;
+  float *dA, *ddecay_bias, *dgate_bias, *dh0;
+  /* single tokens */
+  float* state;
+  const int32_t* slots;
+  int32_t pool;
+} kda_b200_recurrence_args;
+size_t kda_b200_recurrence_saved_bytes(int64_t B, int64_t T, int E, int dtype);
+size_t kda_b200_recurrence_workspace_bytes(int64_t B, int64_t T, int E, int dtype, int packed, int backward);
+int kda_b200_recurrence_fwd(const kda_b200_recurrence_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int kda_b200_recurrence_bwd(const kda_b200_recurrence_args* args, void* workspace, size_t workspace_bytes, void* stream);
+int kda_b200_recurrence_step(const kda_b200_recurrence_args* args, void* stream);
+
+/*
  * Global gradient norm over `count` tensors, and clipping:
  *     norm = sqrt(sum g^2);   out = g * min(1, max_norm / (norm + eps))
  * in, numel, in_type (and out, out_type): HOST arrays of device addresses, element

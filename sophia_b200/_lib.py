@@ -34,6 +34,20 @@ class ScanArgs(ctypes.Structure):
                 + [("rows", ctypes.c_int32), ("pool", ctypes.c_int32)])
 
 
+class RecArgs(ctypes.Structure):
+    """``kda_b200_recurrence_args``."""
+
+    _fields_ = ([(n, c_int64) for n in ("B", "T")]
+                + [(n, ctypes.c_int32) for n in ("E", "nseq", "dtype", "rows")]
+                + [(n, c_void_p) for n in ("x", "decay", "gate", "z")]
+                + [(n, c_int64) for n in ("x_sb", "x_st", "decay_sb", "decay_st", "gate_sb", "gate_st", "z_sb", "z_st")]
+                + [(n, c_void_p) for n in ("A", "decay_bias", "gate_bias", "h0", "cu_seqlens", "y", "ht", "saved")]
+                + [("saved_bytes", c_size_t), ("dy", c_void_p), ("dy_sb", c_int64), ("dy_st", c_int64)]
+                + [(n, c_void_p) for n in ("dht", "dx", "ddecay", "dgate", "dz", "dA", "ddecay_bias", "dgate_bias", "dh0",
+                                           "state", "slots")]
+                + [("pool", ctypes.c_int32)])
+
+
 class GradArgs(ctypes.Structure):
     """``kda_b200_grad_args`` (host arrays; the types as bytes objects)."""
 
@@ -88,6 +102,11 @@ SIGNATURES = {
     "kda_b200_selective_scan_fwd": ([ctypes.POINTER(ScanArgs), c_void_p, c_size_t, c_void_p], c_int),
     "kda_b200_selective_scan_bwd": ([ctypes.POINTER(ScanArgs), c_void_p, c_size_t, c_void_p], c_int),
     "kda_b200_selective_scan_step": ([ctypes.POINTER(ScanArgs), c_void_p], c_int),
+    "kda_b200_recurrence_saved_bytes": ([c_int64, c_int64] + [c_int] * 2, c_size_t),
+    "kda_b200_recurrence_workspace_bytes": ([c_int64, c_int64] + [c_int] * 4, c_size_t),
+    "kda_b200_recurrence_fwd": ([ctypes.POINTER(RecArgs), c_void_p, c_size_t, c_void_p], c_int),
+    "kda_b200_recurrence_bwd": ([ctypes.POINTER(RecArgs), c_void_p, c_size_t, c_void_p], c_int),
+    "kda_b200_recurrence_step": ([ctypes.POINTER(RecArgs), c_void_p], c_int),
     "kda_b200_grad_workspace_bytes": ([c_int64], c_size_t),
     "kda_b200_grad_clip": ([ctypes.POINTER(GradArgs), c_void_p, c_size_t, c_void_p], c_int),
 }

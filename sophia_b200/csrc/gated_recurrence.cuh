@@ -1,0 +1,696 @@
+// Gated linear recurrence (one state per channel, gates per token and channel):
+//   r = sigmoid(decay + decay_bias),  i = sigmoid(gate + gate_bias)
+//   a = exp(A r)  (A <= 0),           b = sqrt(1 - a^2) i x
+//   h[t] = a h[t-1] + b,              y = h silu(z)  (or h)
+// forward, backward and single tokens.
+//
+// A CTA owns 64 channels of a row and goes through the tokens in order, a tile of
+// 8 S tokens at a time: warp w has the w-th S tokens, a lane two channels.  A thread
+// maps the state in front of its tokens to the one behind them, h -> P h + c;
+// the maps of the warps in front, composed on the state that the tile starts
+// from, give its own start.  So nothing is read twice and no state leaves the
+// SM between tiles.  Few rows: a cluster of CTAs takes the tiles in turn and
+// exchanges their maps through distributed shared memory, in the order of the
+// tiles -- one pass over the data at any number of rows.
+//
+// 10 bytes an element (bf16, with z) against seven special functions (ex2 and rcp
+// of three sigmoids, rsqrt), which the SM makes at 16 a clock: both take about as long
+// (50 us per 4 x 4096 x 2048 elements), so the decay's exponential is a polynomial on
+// packed fp32 arithmetic, which also gives 1 - a^2 without cancellation.
+#pragma once
+
+#include <cooperative_groups.h>
+
+#include "ssm_common.cuh"
+
+namespace kda {
+
+namespace cg = cooperative_groups;
+
+constexpr int REC_THREADS = 256;
+constexpr int REC_WARPS = REC_THREADS / 32;
+constexpr int REC_CH = 64;           // channels of a CTA, two a lane
+constexpr int REC_MAX_CLUSTER = 8;   // the portable limit
+// Tokens of a thread: a tile of 8 S tokens of one tensor is 8 KB in every type.
+template <typename T>
+__host__ __device__ constexpr int rec_s() { return sizeof(T) == 2 ? 8 : 4; }
+template <typename T>
+__host__ __device__ constexpr int rec_tile() { return REC_WARPS * rec_s<T>(); }
+// Rows of a staged tile: 64 channels; without 16-byte alignment 16-bit rows are copied in
+// words from the word that holds their first element, which takes one more.
+template <typename T, bool VEC>
+__host__ __device__ constexpr int rec_pitch() { return REC_CH * (int)sizeof(T) + (!VEC && sizeof(T) == 2 ? 4 : 0); }
+template <typename T, bool VEC>
+__host__ __device__ constexpr int rec_tensor_bytes() { return rec_tile<T>() * rec_pitch<T, VEC>(); }
+// Tiles in flight or in use: two CTAs of an SM share its 227 KB.
+template <bool VEC>
+__host__ __device__ constexpr int rec_fwd_stages() { return VEC ? 3 : 2; }
+constexpr int REC_BWD_STAGES = 2;
+
+struct RecParams {
+  RowView x, decay, gate, z, dy;  // z.p null = no output gate
+  const float *A, *decay_bias, *gate_bias, *h0, *dht;
+  void *y, *dx, *ddecay, *dgate, *dz;
+  float *ht, *dh0;
+  float* ckpt;     // [B][tiles][E] states in front of every tile
+  float* partial;  // [B * cluster][E][3]: dA, ddecay_bias, dgate_bias
+  int B, T, E, tiles, cluster;
+  SeqMap seq;
+};
+
+// ---------------------------------------------------------------- arithmetic on two channels
+
+__device__ __forceinline__ u64 ex2_2(u64 v) {
+  const float2 f = upk2(v);
+  return pk2(ex2(f.x), ex2(f.y));
+}
+__device__ __forceinline__ u64 rcp_2(u64 v) {
+  const float2 f = upk2(v);
+  return pk2(rcp(f.x), rcp(f.y));
+}
+__device__ __forceinline__ u64 all2(float v) { return pk2(v, v); }
+__device__ __forceinline__ u64 neg2(u64 v) { return v ^ 0x8000000080000000ull; }
+// e = exp(-(v + bias)) from v and nb = -bias log2 e
+__device__ __forceinline__ u64 rec_expneg(u64 v, u64 nb) { return ex2_2(fma2(v, all2(-LOG2E), nb)); }
+__device__ __forceinline__ u64 rec_sig(u64 e) { return rcp_2(add2(e, all2(1.f))); }
+// 1 - sigmoid without cancellation: 1 - r below one half, e r above (e is finite there)
+__device__ __forceinline__ u64 rec_one_minus(u64 r, u64 e) {
+  const float2 p = upk2(fma2(r, all2(-1.f), all2(1.f))), q = upk2(mul2(e, r)), f = upk2(r);
+  return pk2(f.x < 0.5f ? p.x : q.x, f.y < 0.5f ? p.y : q.y);
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float rsq(float v) {
+  float r;
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+// a = 2^l and w = 1 - a^2 for l <= 0, both with fp32 relative accuracy.  l = n + f, n the nearest whole
+// number; q = 2^f - 1 is a polynomial (a fit of (2^f - 1) / f, relative error 1.1e-8, which keeps q exact in relative
+// terms next to 0); a = 2^n (1 + q), m = a - 1 = 2^n q + (2^n - 1) cancels nowhere, w = -m (2 + m).
+__device__ __forceinline__ void rec_decay(u64 l, u64& a, u64& w) {
+  float2 lf = upk2(l);
+  lf.x = max_nan(lf.x, -126.f);
+  lf.y = max_nan(lf.y, -126.f);
+  l = pk2(lf.x, lf.y);
+  const u64 t = add2(l, all2(12582912.f));  // 1.5 2^23: the sum's low bits are n
+  const u64 f = add2(l, neg2(add2(t, all2(-12582912.f))));
+  u64 p = all2(0.000154035122f);
+  p = fma2(p, f, all2(0.00133907353f));
+  p = fma2(p, f, all2(0.00961823761f));
+  p = fma2(p, f, all2(0.0555035733f));
+  p = fma2(p, f, all2(0.240226492f));
+  p = fma2(p, f, all2(0.693147182f));
+  const float2 tf = upk2(t);
+  const u64 s = pk2(__int_as_float((__float_as_int(tf.x) << 23) + 0x3f800000),
+                    __int_as_float((__float_as_int(tf.y) << 23) + 0x3f800000));
+  const u64 q = mul2(p, f);
+  a = fma2(s, q, s);
+  const u64 m = fma2(s, q, add2(s, all2(-1.f)));
+  w = mul2(neg2(m), add2(m, all2(2.f)));
+}
+// 1 / sqrt(w), 0 for w = 0: no decay, so nothing enters.  (A denormal w counts as 0; a negative one, of a positive
+// rate, gives NaN.)
+__device__ __forceinline__ u64 rec_rsqrt(u64 w) {
+  const float2 f = upk2(w);
+  return pk2(fabsf(f.x) < 1.17549435e-38f ? 0.f : rsq(f.x), fabsf(f.y) < 1.17549435e-38f ? 0.f : rsq(f.y));
+}
+
+// ---------------------------------------------------------------- staged tiles
+
+// Four bytes into shared memory, of which the first n are read and the others zero.
+__device__ __forceinline__ void cp_async4n(void* smem, const void* gmem, int n) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(n) : "memory");
+}
+
+// One tensor's tile from `base` (the CTA's first channel of its row).  Rows past T and channels past the width
+// are not copied; what is computed from them is not used.
+template <typename T, bool VEC>
+__device__ __forceinline__ void rec_copy(char* dst, const T* base, long long st, int t0, int tokens, int nch) {
+  constexpr int TILE = rec_tile<T>(), PITCH = rec_pitch<T, VEC>();
+  if (VEC) {
+    constexpr int V = 16 / sizeof(T), PIECES = REC_CH / V, ROWS = REC_THREADS / PIECES;
+    const int row = threadIdx.x / PIECES, col = threadIdx.x % PIECES;
+    if (col * V >= nch) return;
+    const T* src = base + (long long)(t0 + row) * st + col * V;
+    char* d = dst + row * PITCH + col * 16;
+#pragma unroll
+    for (int k = 0; k < TILE / ROWS; ++k)
+      if (t0 + row + k * ROWS < tokens) cp_async16(d + k * ROWS * PITCH, src + (long long)(k * ROWS) * st, true);
+  } else {
+    constexpr int WORDS = PITCH / 4;
+    for (int q = threadIdx.x; q < TILE * WORDS; q += REC_THREADS) {
+      const int row = q / WORDS, word = q - row * WORDS;
+      if (t0 + row >= tokens) break;
+      const uintptr_t at = reinterpret_cast<uintptr_t>(base + (long long)(t0 + row) * st);
+      const uintptr_t src = (at & ~uintptr_t(3)) + 4 * word, end = at + nch * sizeof(T);
+      if (src < end)  // (a last word may be half inside: only its valid bytes are read)
+        cp_async4n(dst + row * PITCH + word * 4, reinterpret_cast<const void*>(src), (int)min((unsigned long long)(end - src), 4ull));
+    }
+  }
+}
+
+// A thread's two channels of a staged row: neighbours (VEC), or 32 apart.
+template <typename T, bool VEC>
+__device__ __forceinline__ u64 rec_get(const char* tile, int row, int odd) {
+  const int lane = threadIdx.x & 31;
+  const char* p = tile + row * rec_pitch<T, VEC>();
+  if (VEC) {
+    if (sizeof(T) == 4) return *reinterpret_cast<const u64*>(p + lane * 8);
+    const IoVec<T, 2> v = *reinterpret_cast<const IoVec<T, 2>*>(p + lane * 4);
+    return pk2(io_to_f(v.v[0]), io_to_f(v.v[1]));
+  }
+  const T* e = reinterpret_cast<const T*>(p) + odd + lane;
+  return pk2(io_to_f(e[0]), io_to_f(e[32]));
+}
+__device__ __forceinline__ int rec_lane_ch(bool vec, int k) {
+  const int lane = threadIdx.x & 31;
+  return vec ? 2 * lane + k : lane + 32 * k;
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void rec_put(T* row, u64 v, int nch) {
+  const float2 f = upk2(v);
+  const int c0 = rec_lane_ch(VEC, 0), c1 = rec_lane_ch(VEC, 1);
+  if (VEC) {
+    if (c0 < nch) {  // nch is a multiple of 16 bytes' elements
+      const float o[2] = {f.x, f.y};
+      io_store<T, 2>(row + c0, o);
+    }
+  } else {
+    if (c0 < nch) row[c0] = io_from_f<T>(f.x);
+    if (c1 < nch) row[c1] = io_from_f<T>(f.y);
+  }
+}
+// fp32 vectors over the channels
+__device__ __forceinline__ u64 rec_vec(const float* p, bool vec, int nch, float none) {
+  const int c0 = rec_lane_ch(vec, 0), c1 = rec_lane_ch(vec, 1);
+  return pk2(p && c0 < nch ? p[c0] : none, p && c1 < nch ? p[c1] : none);
+}
+__device__ __forceinline__ void rec_put_vec(float* p, u64 v, bool vec, int nch) {
+  const float2 f = upk2(v);
+  const int c0 = rec_lane_ch(vec, 0), c1 = rec_lane_ch(vec, 1);
+  if (c0 < nch) p[c0] = f.x;
+  if (c1 < nch) p[c1] = f.y;
+}
+
+// Where a staged 16-bit row starts inside its first word (0 or 1 elements).
+template <typename T, bool VEC>
+__device__ __forceinline__ int rec_odd(const T* base, long long st, int t) {
+  if (VEC || sizeof(T) == 4) return 0;
+  return (int)((reinterpret_cast<uintptr_t>(base) >> 1) + (unsigned long long)t * (unsigned long long)st) & 1;
+}
+
+// The starts and ends of sequences among a warp's S tokens, as masks; lane j < 8 holds the sequence that starts at token
+// j, lane 8 + j the one that ends there (S <= 8).
+struct RecMarks {
+  int mine;
+  unsigned starts, ends;
+};
+template <int S>
+__device__ __forceinline__ RecMarks rec_marks(const SeqMap& m, int t0) {
+  RecMarks r{-1, 0u, 0u};
+  if (!m.start) return r;
+  const int lane = threadIdx.x & 31, t = t0 + (lane & 7);
+  if (lane < 16 && (lane & 7) < S && t < m.T) r.mine = __ldg((lane < 8 ? m.start : m.end) + t);
+  const unsigned b = __ballot_sync(0xffffffffu, r.mine >= 0);
+  r.starts = b & 0xff;
+  r.ends = (b >> 8) & 0xff;
+  return r;
+}
+
+// Maps of the warps (and of the CTAs of a cluster): h -> P h + c per channel; `cut` (a bit per warp or CTA):
+// a sequence starts (backward: ends) inside, so the result is c alone.  A map is P, P, c, c of a lane's channels.
+__device__ __forceinline__ u64 rec_step_map(const float4& m, bool cut, u64 h) {
+  const u64 c = pk2(m.z, m.w), n = fma2(pk2(m.x, m.y), h, c);
+  return cut ? c : n;
+}
+
+// Composes the maps m[0..7] of the warps in order (`mask`: their cuts).
+__device__ __forceinline__ void rec_compose(const float4 (*m)[32], unsigned mask, bool reverse, float4& out) {
+  const int lane = threadIdx.x & 31;
+  u64 p = all2(1.f), c = 0ull;
+#pragma unroll
+  for (int k = 0; k < REC_WARPS; ++k) {
+    const int w = reverse ? REC_WARPS - 1 - k : k;
+    const float4 v = m[w][lane];
+    c = rec_step_map(v, mask >> w & 1, c);
+    p = mul2(p, pk2(v.x, v.y));
+  }
+  const float2 pf = upk2(p), cf = upk2(c);
+  out = make_float4(pf.x, pf.y, cf.x, cf.y);
+}
+
+// ---------------------------------------------------------------- forward
+
+struct RecFwdSmem {
+  float4 maps[2][REC_WARPS][32];
+  float4 cta[2][REC_MAX_CLUSTER][32];
+  unsigned cuts[2][REC_WARPS];
+  unsigned cta_cut[2][REC_MAX_CLUSTER];
+};
+
+__device__ __forceinline__ unsigned rec_cuts(const unsigned (&c)[REC_WARPS]) {
+  unsigned m = 0;
+#pragma unroll
+  for (int w = 0; w < REC_WARPS; ++w) m |= c[w] ? 1u << w : 0u;
+  return m;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(RecParams P) {
+  constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>(), STAGES = rec_fwd_stages<VEC>();
+  extern __shared__ __align__(16) char stages[];
+  __shared__ RecFwdSmem sm;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nc = P.cluster, rank = nc > 1 ? (int)blockIdx.x % nc : 0;
+  const int b = blockIdx.y, ch0 = (int)blockIdx.x / nc * REC_CH, nch = min(REC_CH, P.E - ch0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool has_z = P.z.p != nullptr, packed = P.seq.start != nullptr;
+  const T* px = row_ptr<T>(P.x, b, 0) + ch0;
+  const T* pd = row_ptr<T>(P.decay, b, 0) + ch0;
+  const T* pg = row_ptr<T>(P.gate, b, 0) + ch0;
+  const T* pz = has_z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
+  T* py = static_cast<T*>(P.y) + (long long)b * P.T * P.E + ch0;
+  const int stage_bytes = (has_z ? 4 : 3) * TB;
+  const int iters = (P.tiles + nc - 1) / nc;
+
+  auto fetch = [&](int it) {
+    if (it < iters) {
+      const int t0 = (it * nc + rank) * TILE;
+      char* s = stages + (it % STAGES) * stage_bytes;
+      rec_copy<T, VEC>(s, pd, P.decay.st, t0, P.T, nch);
+      rec_copy<T, VEC>(s + TB, px, P.x.st, t0, P.T, nch);
+      rec_copy<T, VEC>(s + 2 * TB, pg, P.gate.st, t0, P.T, nch);
+      if (has_z) rec_copy<T, VEC>(s + 3 * TB, pz, P.z.st, t0, P.T, nch);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) fetch(k);
+
+  const u64 A2 = mul2(rec_vec(P.A + ch0, VEC, nch, 0.f), all2(LOG2E));
+  const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  u64 carry = packed ? 0ull : rec_vec(P.h0 ? P.h0 + (long long)b * P.E + ch0 : nullptr, VEC, nch, 0.f);
+
+  for (int it = 0; it < iters; ++it) {
+    const int tile = it * nc + rank, t0 = tile * TILE + warp * S, par = it & 1;
+    const char* s = stages + (it % STAGES) * stage_bytes;
+    cp_async_wait<STAGES - 2>();
+    __syncthreads();
+    fetch(it + STAGES - 1);
+    const int n = min(S, P.T - t0);  // tokens of this warp (may be <= 0)
+    const RecMarks marks = rec_marks<S>(P.seq, t0);
+
+    // gates, and the map of this warp's tokens
+    u64 a[S], bb[S], sz[S];
+    u64 p = all2(1.f), c = 0ull;
+#pragma unroll
+    for (int j = 0; j < S; ++j) {
+      a[j] = all2(1.f);
+      bb[j] = 0ull;
+      if (j < n) {
+        const int row = warp * S + j, t = t0 + j;
+        const u64 r = rec_sig(rec_expneg(rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
+        u64 w;
+        rec_decay(mul2(A2, r), a[j], w);
+        const u64 g = rec_sig(rec_expneg(rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng));
+        const u64 x = rec_get<T, VEC>(s + TB, row, rec_odd<T, VEC>(px, P.x.st, t));
+        bb[j] = mul2(mul2(mul2(w, rec_rsqrt(w)), g), x);
+        if (has_z) {
+          const u64 z = rec_get<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t));
+          sz[j] = mul2(z, rec_sig(rec_expneg(z, 0ull)));
+        }
+        if (marks.starts >> j & 1) {
+          const int q = __shfl_sync(0xffffffffu, marks.mine, j);
+          c = rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+        }
+        c = fma2(a[j], c, bb[j]);
+        p = mul2(p, a[j]);
+      }
+    }
+    {
+      const float2 pf = upk2(p), cf = upk2(c);
+      sm.maps[par][warp][lane] = make_float4(pf.x, pf.y, cf.x, cf.y);
+      if (lane == 0) sm.cuts[par][warp] = marks.starts;
+    }
+    __syncthreads();
+    const unsigned cuts = packed ? rec_cuts(sm.cuts[par]) : 0u;
+
+    if (nc > 1) {  // the tiles of the cluster's other CTAs: their maps, in order
+      if (warp == 0) {
+        float4 m;
+        rec_compose(sm.maps[par], cuts, false, m);
+        for (int q = 0; q < nc; ++q) {
+          cluster.map_shared_rank(&sm.cta[par][rank][0], q)[lane] = m;
+          if (lane == 0) *cluster.map_shared_rank(&sm.cta_cut[par][rank], q) = cuts;
+        }
+      }
+      cluster.sync();
+    }
+    u64 h = carry;
+    if (nc > 1) {
+      u64 next = carry;
+      for (int q = 0; q < nc; ++q) {
+        if (q == rank) h = next;
+        next = rec_step_map(sm.cta[par][q][lane], packed && sm.cta_cut[par][q] != 0, next);
+      }
+      carry = next;
+    }
+    if (P.ckpt && warp == 0 && tile < P.tiles)
+      rec_put_vec(P.ckpt + ((long long)b * P.tiles + tile) * P.E + ch0, h, VEC, nch);
+    {
+      u64 v = h;
+#pragma unroll
+      for (int w = 0; w < REC_WARPS; ++w) {
+        if (w == warp) h = v;
+        v = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, v);
+      }
+      if (nc == 1) carry = v;
+    }
+
+    // the states, and what leaves
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (j < n) {
+        if (marks.starts >> j & 1) {
+          const int q = __shfl_sync(0xffffffffu, marks.mine, j);
+          h = rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+        }
+        h = fma2(a[j], h, bb[j]);
+        rec_put<T, VEC>(py + (long long)(t0 + j) * P.E, has_z ? mul2(h, sz[j]) : h, nch);
+        if (P.ht && (marks.ends >> j & 1)) {
+          const int q = __shfl_sync(0xffffffffu, marks.mine, 8 + j);
+          rec_put_vec(P.ht + (long long)q * P.E + ch0, h, VEC, nch);
+        }
+      }
+  }
+  if (!packed && P.ht && rank == 0 && warp == 0) rec_put_vec(P.ht + (long long)b * P.E + ch0, carry, VEC, nch);
+  cp_async_wait<0>();
+  if (nc > 1) cluster.sync();  // no CTA leaves while another may still write its maps here
+}
+
+// ---------------------------------------------------------------- backward
+
+// With G[t] the gradient of h[t], from the last token to the first:
+//   G[t] = dy silu(z) + a[t+1] G[t+1]   (at a sequence's last token: + dht instead)
+//   dx = G n i,  dgate = G n x i (1 - i),  n = sqrt(1 - a^2);   dz = dy h silu'(z)
+//   d(A r) = G (a h[t-1] - (a^2 / n) i x),  ddecay = d(A r) A r (1 - r),  dA = sum d(A r) r
+// A warp's tokens map what comes from behind, U = a[t+1] G[t+1], to what they hand on: U -> P U + d with the same P
+// as the states, so both directions meet in one exchange.  The states start from the tile's checkpoint.
+struct RecBwdSmem {
+  float4 maps[2][REC_WARPS][32];  // states: P, P, c, c
+  float2 back[2][REC_WARPS][32];  // gradients: d, d (P as above)
+  float4 cta[2][REC_MAX_CLUSTER][32];
+  unsigned cuts[2][REC_WARPS], ends[2][REC_WARPS];
+  unsigned cta_cut[2][REC_MAX_CLUSTER];
+};
+
+// Adds v to a compensated sum (s, c).
+__device__ __forceinline__ void rec_add(u64& s, u64& c, u64 v) {
+  const u64 y = add2(v, neg2(c)), t = add2(s, y);
+  c = add2(add2(t, neg2(s)), neg2(y));
+  s = t;
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(RecParams P) {
+  constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>();
+  extern __shared__ __align__(16) char stages[];
+  __shared__ RecBwdSmem sm;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int nc = P.cluster, rank = nc > 1 ? (int)blockIdx.x % nc : 0;
+  const int b = blockIdx.y, ch0 = (int)blockIdx.x / nc * REC_CH, nch = min(REC_CH, P.E - ch0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool has_z = P.z.p != nullptr, packed = P.seq.start != nullptr;
+  const T* px = row_ptr<T>(P.x, b, 0) + ch0;
+  const T* pd = row_ptr<T>(P.decay, b, 0) + ch0;
+  const T* pg = row_ptr<T>(P.gate, b, 0) + ch0;
+  const T* pz = has_z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
+  const T* pdy = row_ptr<T>(P.dy, b, 0) + ch0;
+  const long long out0 = (long long)b * P.T * P.E + ch0;
+  const int stage_bytes = (has_z ? 5 : 4) * TB;
+  const int iters = (P.tiles + nc - 1) / nc;
+
+  auto fetch = [&](int k) {  // the k-th tile from the end
+    if (k < iters) {
+      const int t0 = ((iters - 1 - k) * nc + rank) * TILE;
+      char* s = stages + (k % REC_BWD_STAGES) * stage_bytes;
+      rec_copy<T, VEC>(s, pd, P.decay.st, t0, P.T, nch);
+      rec_copy<T, VEC>(s + TB, px, P.x.st, t0, P.T, nch);
+      rec_copy<T, VEC>(s + 2 * TB, pg, P.gate.st, t0, P.T, nch);
+      rec_copy<T, VEC>(s + 3 * TB, pdy, P.dy.st, t0, P.T, nch);
+      if (has_z) rec_copy<T, VEC>(s + 4 * TB, pz, P.z.st, t0, P.T, nch);
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < REC_BWD_STAGES - 1; ++k) fetch(k);
+
+  const u64 A1 = rec_vec(P.A + ch0, VEC, nch, 0.f), A2 = mul2(A1, all2(LOG2E));
+  const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  u64 carry = packed ? 0ull : rec_vec(P.dht ? P.dht + (long long)b * P.E + ch0 : nullptr, VEC, nch, 0.f);
+  u64 sumA = 0ull, lowA = 0ull, sumD = 0ull, lowD = 0ull, sumG = 0ull, lowG = 0ull;
+
+  for (int k = 0; k < iters; ++k) {
+    const int tile = (iters - 1 - k) * nc + rank, t0 = tile * TILE + warp * S, par = k & 1;
+    const char* s = stages + (k % REC_BWD_STAGES) * stage_bytes;
+    u64 h = tile < P.tiles ? rec_vec(P.ckpt + ((long long)b * P.tiles + tile) * P.E + ch0, VEC, nch, 0.f) : 0ull;
+    cp_async_wait<REC_BWD_STAGES - 2>();
+    __syncthreads();
+    fetch(k + REC_BWD_STAGES - 1);
+    const int n = min(S, P.T - t0);
+    const RecMarks marks = rec_marks<S>(P.seq, t0);
+
+    auto get = [&](int which, const T* base, long long st, int j) {
+      return rec_get<T, VEC>(s + which * TB, warp * S + j, rec_odd<T, VEC>(base, st, t0 + j));
+    };
+    auto h0_of = [&](int j) {
+      const int q = __shfl_sync(0xffffffffu, marks.mine, j);
+      return rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+    };
+    auto dht_of = [&](int j) {
+      const int q = __shfl_sync(0xffffffffu, marks.mine, 8 + j);
+      return rec_vec(P.dht ? P.dht + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+    };
+
+    u64 a[S], hs[S], rr[S], ii[S], zz[S];  // decay; b, then the state; the sigmoids
+    {
+      u64 p = all2(1.f), c = 0ull, d = 0ull;
+      bool open = true;  // no end among the tokens so far
+#pragma unroll
+      for (int j = 0; j < S; ++j)
+        if (j < n) {
+          rr[j] = rec_sig(rec_expneg(get(0, pd, P.decay.st, j), nd));
+          u64 w;
+          rec_decay(mul2(A2, rr[j]), a[j], w);
+          ii[j] = rec_sig(rec_expneg(get(2, pg, P.gate.st, j), ng));
+          hs[j] = mul2(mul2(mul2(w, rec_rsqrt(w)), ii[j]), get(1, px, P.x.st, j));
+          u64 g = get(3, pdy, P.dy.st, j);
+          if (has_z) {
+            const u64 z = get(4, pz, P.z.st, j);
+            zz[j] = rec_sig(rec_expneg(z, 0ull));
+            g = mul2(g, mul2(z, zz[j]));
+          }
+          if (marks.starts >> j & 1) c = h0_of(j);
+          c = fma2(a[j], c, hs[j]);
+          p = mul2(p, a[j]);
+          if (open) {
+            if (marks.ends >> j & 1) {
+              g = add2(g, dht_of(j));
+              open = false;
+            }
+            d = fma2(p, g, d);
+          }
+        }
+      const float2 pf = upk2(p), cf = upk2(c);
+      sm.maps[par][warp][lane] = make_float4(pf.x, pf.y, cf.x, cf.y);
+      sm.back[par][warp][lane] = upk2(d);
+      if (lane == 0) {
+        sm.cuts[par][warp] = marks.starts;
+        sm.ends[par][warp] = marks.ends;
+      }
+    }
+    __syncthreads();
+    const unsigned cuts = packed ? rec_cuts(sm.cuts[par]) : 0u, ends = packed ? rec_cuts(sm.ends[par]) : 0u;
+    auto back = [&](int w) {
+      const float4 m = sm.maps[par][w][lane];
+      const float2 d = sm.back[par][w][lane];
+      return make_float4(m.x, m.y, d.x, d.y);
+    };
+    if (nc > 1) {
+      if (warp == 0) {
+        u64 p = all2(1.f), d = 0ull;
+#pragma unroll
+        for (int w = REC_WARPS - 1; w >= 0; --w) {
+          const float4 m = back(w);
+          d = rec_step_map(m, ends >> w & 1, d);
+          p = mul2(p, pk2(m.x, m.y));
+        }
+        const float2 pf = upk2(p), df = upk2(d);
+        for (int q = 0; q < nc; ++q) {
+          cluster.map_shared_rank(&sm.cta[par][rank][0], q)[lane] = make_float4(pf.x, pf.y, df.x, df.y);
+          if (lane == 0) *cluster.map_shared_rank(&sm.cta_cut[par][rank], q) = ends;
+        }
+      }
+      cluster.sync();
+    }
+    u64 U = carry;
+    if (nc > 1) {
+      u64 next = carry;
+      for (int q = nc - 1; q >= 0; --q) {
+        if (q == rank) U = next;
+        next = rec_step_map(sm.cta[par][q][lane], packed && sm.cta_cut[par][q] != 0, next);
+      }
+      carry = next;
+    }
+    {
+      u64 v = U;
+#pragma unroll
+      for (int w = REC_WARPS - 1; w >= 0; --w) {
+        if (w == warp) U = v;
+        v = rec_step_map(back(w), ends >> w & 1, v);
+      }
+      if (nc == 1) carry = v;
+      for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
+    }
+
+    const u64 h_in = h;
+#pragma unroll
+    for (int j = 0; j < S; ++j)
+      if (j < n) {
+        if (marks.starts >> j & 1) h = h0_of(j);
+        h = fma2(a[j], h, hs[j]);
+        hs[j] = h;
+      }
+
+    u64 tA = 0ull, tD = 0ull, tG = 0ull;
+#pragma unroll
+    for (int j = S - 1; j >= 0; --j)
+      if (j < n) {
+        const long long at = out0 + (long long)(t0 + j) * P.E;
+        u64 prev = j > 0 ? hs[j > 0 ? j - 1 : 0] : h_in;
+        if (marks.starts >> j & 1) prev = h0_of(j);
+        u64 G = get(3, pdy, P.dy.st, j);
+        if (has_z) {
+          const u64 z = get(4, pz, P.z.st, j), dyh = mul2(G, hs[j]);
+          G = mul2(G, mul2(z, zz[j]));
+          // silu' = s (1 + z (1 - s))
+          const u64 one = fma2(zz[j], all2(-1.f), all2(1.f));
+          rec_put<T, VEC>(static_cast<T*>(P.dz) + at, mul2(dyh, mul2(zz[j], fma2(z, one, all2(1.f)))), nch);
+        }
+        if (marks.ends >> j & 1) U = dht_of(j);
+        G = add2(G, U);
+        U = mul2(a[j], G);
+        if ((marks.starts >> j & 1) && P.dh0) {
+          const int q = __shfl_sync(0xffffffffu, marks.mine, j);
+          rec_put_vec(P.dh0 + (long long)q * P.E + ch0, U, VEC, nch);
+        }
+        const u64 x = get(1, px, P.x.st, j);
+        const u64 er = rec_expneg(get(0, pd, P.decay.st, j), nd), ei = rec_expneg(get(2, pg, P.gate.st, j), ng);
+        u64 aa, w;
+        rec_decay(mul2(A2, rr[j]), aa, w);
+        const u64 rs = rec_rsqrt(w), norm = mul2(w, rs);
+        const u64 Gn = mul2(G, norm), ix = mul2(ii[j], x);
+        rec_put<T, VEC>(static_cast<T*>(P.dx) + at, mul2(Gn, ii[j]), nch);
+        const u64 dg = mul2(mul2(Gn, ix), rec_one_minus(ii[j], ei));
+        rec_put<T, VEC>(static_cast<T*>(P.dgate) + at, dg, nch);
+        tG = add2(tG, dg);
+        // d(A r) r = G (a h' r - a^2 i x r / n): the small factors first, so that nothing overflows
+        const u64 ar = mul2(a[j], rr[j]);
+        const u64 q = mul2(mul2(ar, rs), mul2(a[j], ix));
+        const u64 dAr = mul2(G, fma2(ar, prev, neg2(q)));
+        tA = add2(tA, dAr);
+        const u64 dd = mul2(mul2(dAr, A1), rec_one_minus(rr[j], er));
+        rec_put<T, VEC>(static_cast<T*>(P.ddecay) + at, dd, nch);
+        tD = add2(tD, dd);
+      }
+    rec_add(sumA, lowA, tA);
+    rec_add(sumD, lowD, tD);
+    rec_add(sumG, lowG, tG);
+  }
+  if (!packed && P.dh0 && rank == 0 && warp == 0) rec_put_vec(P.dh0 + (long long)b * P.E + ch0, carry, VEC, nch);
+  cp_async_wait<0>();
+  __syncthreads();
+  // the CTA's sums: the warps in order
+  float* red = reinterpret_cast<float*>(stages);  // [warps][3][64]
+  const u64 sums[3] = {add2(sumA, neg2(lowA)), add2(sumD, neg2(lowD)), add2(sumG, neg2(lowG))};
+#pragma unroll
+  for (int q = 0; q < 3; ++q) rec_put_vec(red + (warp * 3 + q) * REC_CH, sums[q], VEC, REC_CH);
+  __syncthreads();
+  for (int i = threadIdx.x; i < 3 * REC_CH; i += REC_THREADS) {
+    const int c = i / 3, q = i - 3 * c;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < REC_WARPS; ++w) t += red[(w * 3 + q) * REC_CH + c];
+    if (c < nch) P.partial[(((long long)b * nc + rank) * P.E + ch0 + c) * 3 + q] = t;
+  }
+  if (nc > 1) cluster.sync();
+}
+
+// ---------------------------------------------------------------- single tokens
+
+struct RecStepParams {
+  const void *x, *decay, *gate, *z;
+  long long sx, sd, sg, sz;
+  const float *A, *decay_bias, *gate_bias;
+  float* state;
+  const int* slots;
+  int rows, E, pool;
+  void* y;
+  int* err;
+};
+
+constexpr int REC_STEP_THREADS = 128;
+
+// A thread has two neighbouring channels (VEC) or one, and strides over the rows: latency, not
+// bandwidth, bounds every size that a decoding batch has.  The arithmetic is the prompt's, operation by operation.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(RecStepParams P) {
+  constexpr int V = VEC ? 2 : 1;
+  const int c = (blockIdx.x * REC_STEP_THREADS + threadIdx.x) * V;
+  if (c >= P.E) return;
+  auto vec = [&](const float* p) { return p ? pk2(__ldg(p + c), VEC ? __ldg(p + c + 1) : 0.f) : 0ull; };
+  const u64 A2 = mul2(vec(P.A), all2(LOG2E));
+  const u64 nd = mul2(vec(P.decay_bias), all2(-LOG2E)), ng = mul2(vec(P.gate_bias), all2(-LOG2E));
+  for (int r = blockIdx.y; r < P.rows; r += gridDim.y) {
+    const int slot = step_slot(P.slots, r, P.pool, P.err);
+    T* y = static_cast<T*>(P.y) + (long long)r * P.E + c;
+    if (slot < 0) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) y[k] = io_from_f<T>(0.f);
+      continue;
+    }
+    auto in = [&](const void* p, long long st) {
+      float f[V];
+      io_load<T, V>(static_cast<const T*>(p) + r * st + c, f);
+      return pk2(f[0], f[V - 1]);
+    };
+    float* sp = P.state + (long long)slot * P.E + c;
+    float hf[V];
+    io_load<float, V>(sp, hf);
+    const u64 rd = rec_sig(rec_expneg(in(P.decay, P.sd), nd)), gi = rec_sig(rec_expneg(in(P.gate, P.sg), ng));
+    u64 a, w;
+    rec_decay(mul2(A2, rd), a, w);
+    const u64 b = mul2(mul2(mul2(w, rec_rsqrt(w)), gi), in(P.x, P.sx));
+    const u64 h = fma2(a, pk2(hf[0], hf[V - 1]), b);
+    u64 o = h;
+    if (P.z) {
+      const u64 z = in(P.z, P.sz);
+      o = mul2(h, mul2(z, rec_sig(rec_expneg(z, 0ull))));
+    }
+    const float2 hn = upk2(h), on = upk2(o);
+    const float h2[2] = {hn.x, hn.y}, o2[2] = {on.x, on.y};
+    float hv[V], ov[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) hv[k] = h2[k], ov[k] = o2[k];
+    io_store<float, V>(sp, hv);
+    io_store<T, V>(y, ov);
+  }
+}
+
+}  // namespace kda
