@@ -20,6 +20,9 @@
 #pragma once
 
 #include <cooperative_groups.h>
+#include <cuda.h>  // CUtensorMap
+
+#include <cstring>
 
 #include "ssm_common.cuh"
 
@@ -47,7 +50,27 @@ template <bool VEC>
 __host__ __device__ constexpr int rec_fwd_stages() { return VEC ? 3 : 2; }
 constexpr int REC_BWD_STAGES = 2;
 
+// The packed arithmetic's constants, as kernel parameters: operands from the constant bank or uniform registers
+// where literals would be moved into a pair of registers at every use (28 of 141 instructions a pair of elements).
+struct RecConst {
+  u64 one, two, log2e, round, poly[6];
+};
+inline RecConst rec_const() {
+  auto two = [](float v) {
+    unsigned u;
+    std::memcpy(&u, &v, 4);
+    return (u64)u << 32 | u;
+  };
+  // a fit of (1 - 2^f) / f on [-1/2, 1/2], relative error 1.1e-8, highest power first; 1.5 2^23
+  return {two(1.f), two(2.f), two(-LOG2E), two(12582912.f),
+          {two(-0.000154035122f), two(-0.00133907353f), two(-0.00961823761f), two(-0.0555035733f), two(-0.240226492f),
+           two(-0.693147182f)}};
+}
+
 struct RecParams {
+  RecConst k;
+  CUtensorMap map[5];  // decay, x, gate, then forward z, backward dy and z: [B][T][E], boxes of a tile (16-byte pieces only)
+  int* err;
   RowView x, decay, gate, z, dy;  // z.p null = no output gate
   const float *A, *decay_bias, *gate_bias, *h0, *dht;
   void *y, *dx, *ddecay, *dgate, *dz;
@@ -69,13 +92,19 @@ __device__ __forceinline__ u64 rcp_2(u64 v) {
   return pk2(rcp(f.x), rcp(f.y));
 }
 __device__ __forceinline__ u64 all2(float v) { return pk2(v, v); }
-__device__ __forceinline__ u64 neg2(u64 v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ u64 sub2(u64 a, u64 b) {
+  u64 r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // e = exp(-(v + bias)) from v and nb = -bias log2 e
-__device__ __forceinline__ u64 rec_expneg(u64 v, u64 nb) { return ex2_2(fma2(v, all2(-LOG2E), nb)); }
-__device__ __forceinline__ u64 rec_sig(u64 e) { return rcp_2(add2(e, all2(1.f))); }
+__device__ __forceinline__ u64 rec_expneg(const RecConst& k, u64 v, u64 nb) { return ex2_2(fma2(v, k.log2e, nb)); }
+__device__ __forceinline__ u64 rec_sig(const RecConst& k, u64 e) { return rcp_2(add2(e, k.one)); }
+// v sigmoid(v)
+__device__ __forceinline__ u64 rec_silu(const RecConst& k, u64 v) { return mul2(v, rec_sig(k, ex2_2(mul2(v, k.log2e)))); }
 // 1 - sigmoid without cancellation: 1 - r below one half, e r above (e is finite there)
-__device__ __forceinline__ u64 rec_one_minus(u64 r, u64 e) {
-  const float2 p = upk2(fma2(r, all2(-1.f), all2(1.f))), q = upk2(mul2(e, r)), f = upk2(r);
+__device__ __forceinline__ u64 rec_one_minus(const RecConst& k, u64 r, u64 e) {
+  const float2 p = upk2(sub2(k.one, r)), q = upk2(mul2(e, r)), f = upk2(r);
   return pk2(f.x < 0.5f ? p.x : q.x, f.y < 0.5f ? p.y : q.y);
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -89,67 +118,94 @@ __device__ __forceinline__ float rsq(float v) {
   return r;
 }
 // a = 2^l and w = 1 - a^2 for l <= 0, both with fp32 relative accuracy.  l = n + f, n the nearest whole
-// number; q = 2^f - 1 is a polynomial (a fit of (2^f - 1) / f, relative error 1.1e-8, which keeps q exact in relative
-// terms next to 0); a = 2^n (1 + q), m = a - 1 = 2^n q + (2^n - 1) cancels nowhere, w = -m (2 + m).
-__device__ __forceinline__ void rec_decay(u64 l, u64& a, u64& w) {
+// number; q = 1 - 2^f is a polynomial times f, which keeps q accurate in relative terms next to 0;
+// a = 2^n (1 - q), m = 1 - a = 2^n q + (1 - 2^n) cancels nowhere, w = m (2 - m).
+__device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64& w) {
   float2 lf = upk2(l);
   lf.x = max_nan(lf.x, -126.f);
   lf.y = max_nan(lf.y, -126.f);
   l = pk2(lf.x, lf.y);
-  const u64 t = add2(l, all2(12582912.f));  // 1.5 2^23: the sum's low bits are n
-  const u64 f = add2(l, neg2(add2(t, all2(-12582912.f))));
-  u64 p = all2(0.000154035122f);
-  p = fma2(p, f, all2(0.00133907353f));
-  p = fma2(p, f, all2(0.00961823761f));
-  p = fma2(p, f, all2(0.0555035733f));
-  p = fma2(p, f, all2(0.240226492f));
-  p = fma2(p, f, all2(0.693147182f));
+  const u64 t = add2(l, k.round);  // the sum's low bits are n
+  const u64 f = sub2(l, sub2(t, k.round));
+  u64 p = fma2(k.poly[0], f, k.poly[1]);
+#pragma unroll
+  for (int i = 2; i < 6; ++i) p = fma2(p, f, k.poly[i]);
   const float2 tf = upk2(t);
   const u64 s = pk2(__int_as_float((__float_as_int(tf.x) << 23) + 0x3f800000),
                     __int_as_float((__float_as_int(tf.y) << 23) + 0x3f800000));
   const u64 q = mul2(p, f);
-  a = fma2(s, q, s);
-  const u64 m = fma2(s, q, add2(s, all2(-1.f)));
-  w = mul2(neg2(m), add2(m, all2(2.f)));
+  a = mul2(s, sub2(k.one, q));
+  const u64 m = fma2(s, q, sub2(k.one, s));
+  w = mul2(m, sub2(k.two, m));
 }
-// 1 / sqrt(w), 0 for w = 0: no decay, so nothing enters.  (A denormal w counts as 0; a negative one, of a positive
-// rate, gives NaN.)
+// sqrt(w) as w / sqrt(w): 0 for w = 0, NaN for NaN (a denormal w counts as 0).
+__device__ __forceinline__ u64 rec_root(u64 w) {
+  const float2 f = upk2(w);
+  return mul2(w, pk2(rsq(fmaxf(f.x, 1.17549435e-38f)), rsq(fmaxf(f.y, 1.17549435e-38f))));
+}
+// 1 / sqrt(w), but 0 for w = 0: nothing decays, so nothing enters.
 __device__ __forceinline__ u64 rec_rsqrt(u64 w) {
   const float2 f = upk2(w);
-  return pk2(fabsf(f.x) < 1.17549435e-38f ? 0.f : rsq(f.x), fabsf(f.y) < 1.17549435e-38f ? 0.f : rsq(f.y));
+  return pk2(f.x < 1.17549435e-38f ? 0.f : rsq(f.x), f.y < 1.17549435e-38f ? 0.f : rsq(f.y));
 }
 
 // ---------------------------------------------------------------- staged tiles
+
+__device__ __forceinline__ void rec_bar_init(uint64_t* bar) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void rec_bar_expect(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+constexpr uint32_t REC_POLLS = 1u << 26;
+__device__ __forceinline__ bool rec_bar_wait(uint64_t* bar, uint32_t parity) {
+  for (uint32_t i = 0; i < REC_POLLS; ++i) {
+    uint32_t done;
+    asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(done)
+                 : "r"(smem_u32(bar)), "r"(parity)
+                 : "memory");
+    if (done) return true;
+  }
+  return false;
+}
+// Sixteen bytes to the same place of a CTA of the cluster, counted by its mbarrier at the place of `bar`.
+__device__ __forceinline__ void rec_send(const void* slot, const void* bar, int cta, const float4& v) {
+  uint32_t to, sig;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(slot)), "r"(cta));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(sig) : "r"(smem_u32(bar)), "r"(cta));
+  asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
+               "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(sig)
+               : "memory");
+}
+// A tile's box into shared memory; tokens and channels past the tensor arrive as zeros.  (ch is a multiple of 64.)
+__device__ __forceinline__ void rec_tma(char* dst, const CUtensorMap* map, int ch, int t, int b, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(ch), "r"(t), "r"(b), "r"(smem_u32(bar))
+      : "memory");
+}
 
 // Four bytes into shared memory, of which the first n are read and the others zero.
 __device__ __forceinline__ void cp_async4n(void* smem, const void* gmem, int n) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(smem_u32(smem)), "l"(gmem), "r"(n) : "memory");
 }
 
-// One tensor's tile from `base` (the CTA's first channel of its row).  Rows past T and channels past the width
-// are not copied; what is computed from them is not used.
-template <typename T, bool VEC>
+// One tensor's tile from `base` (the CTA's first channel of its row), in words.  Rows past T and channels past the
+// width are not copied; what is computed from them is not used.  (A first or last word may be half inside.  Of the last
+// one only the valid bytes are read; the first one's other half is the element in front of an odd address, which shares
+// its aligned word.)
+template <typename T>
 __device__ __forceinline__ void rec_copy(char* dst, const T* base, long long st, int t0, int tokens, int nch) {
-  constexpr int TILE = rec_tile<T>(), PITCH = rec_pitch<T, VEC>();
-  if (VEC) {
-    constexpr int V = 16 / sizeof(T), PIECES = REC_CH / V, ROWS = REC_THREADS / PIECES;
-    const int row = threadIdx.x / PIECES, col = threadIdx.x % PIECES;
-    if (col * V >= nch) return;
-    const T* src = base + (long long)(t0 + row) * st + col * V;
-    char* d = dst + row * PITCH + col * 16;
-#pragma unroll
-    for (int k = 0; k < TILE / ROWS; ++k)
-      if (t0 + row + k * ROWS < tokens) cp_async16(d + k * ROWS * PITCH, src + (long long)(k * ROWS) * st, true);
-  } else {
-    constexpr int WORDS = PITCH / 4;
-    for (int q = threadIdx.x; q < TILE * WORDS; q += REC_THREADS) {
-      const int row = q / WORDS, word = q - row * WORDS;
-      if (t0 + row >= tokens) break;
-      const uintptr_t at = reinterpret_cast<uintptr_t>(base + (long long)(t0 + row) * st);
-      const uintptr_t src = (at & ~uintptr_t(3)) + 4 * word, end = at + nch * sizeof(T);
-      if (src < end)  // (a last word may be half inside: only its valid bytes are read)
-        cp_async4n(dst + row * PITCH + word * 4, reinterpret_cast<const void*>(src), (int)min((unsigned long long)(end - src), 4ull));
-    }
+  constexpr int TILE = rec_tile<T>(), PITCH = rec_pitch<T, false>(), WORDS = PITCH / 4;
+  for (int q = threadIdx.x; q < TILE * WORDS; q += REC_THREADS) {
+    const int row = q / WORDS, word = q - row * WORDS;
+    if (t0 + row >= tokens) break;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(base + (long long)(t0 + row) * st);
+    const uintptr_t src = (at & ~uintptr_t(3)) + 4 * word, end = at + nch * sizeof(T);
+    if (src < end)
+      cp_async4n(dst + row * PITCH + word * 4, reinterpret_cast<const void*>(src), (int)min((unsigned long long)(end - src), 4ull));
   }
 }
 
@@ -174,10 +230,18 @@ template <typename T, bool VEC>
 __device__ __forceinline__ void rec_put(T* row, u64 v, int nch) {
   const float2 f = upk2(v);
   const int c0 = rec_lane_ch(VEC, 0), c1 = rec_lane_ch(VEC, 1);
-  if (VEC) {
-    if (c0 < nch) {  // nch is a multiple of 16 bytes' elements
-      const float o[2] = {f.x, f.y};
-      io_store<T, 2>(row + c0, o);
+  if (VEC) {  // nch is a multiple of 16 bytes' elements; a predicate, where a branch would cost three instructions
+    if (sizeof(T) == 4) {
+      asm volatile("{ .reg .pred p; setp.lt.s32 p, %2, %3; @p st.global.b64 [%0], %1; }" ::"l"(row + c0), "l"(v), "r"(c0),
+                   "r"(nch)
+                   : "memory");
+    } else {
+      IoVec<T, 2> o;
+      o.v[0] = io_from_f<T>(f.x);
+      o.v[1] = io_from_f<T>(f.y);
+      asm volatile("{ .reg .pred p; setp.lt.s32 p, %2, %3; @p st.global.b32 [%0], %1; }" ::"l"(row + c0),
+                   "r"(*reinterpret_cast<const uint32_t*>(&o)), "r"(c0), "r"(nch)
+                   : "memory");
     }
   } else {
     if (c0 < nch) row[c0] = io_from_f<T>(f.x);
@@ -228,28 +292,33 @@ __device__ __forceinline__ u64 rec_step_map(const float4& m, bool cut, u64 h) {
   return cut ? c : n;
 }
 
-// Composes the maps m[0..7] of the warps in order (`mask`: their cuts).
-__device__ __forceinline__ void rec_compose(const float4 (*m)[32], unsigned mask, bool reverse, float4& out) {
-  const int lane = threadIdx.x & 31;
+// The whole CTA's map: the warps' maps m[0..7] in order (reverse: last first; `mask`: their cuts).  P < 0 stands for a
+// cut inside (a product of decays is not negative).
+template <typename Get>
+__device__ __forceinline__ float4 rec_compose(Get get, unsigned mask, bool reverse) {
   u64 p = all2(1.f), c = 0ull;
 #pragma unroll
   for (int k = 0; k < REC_WARPS; ++k) {
     const int w = reverse ? REC_WARPS - 1 - k : k;
-    const float4 v = m[w][lane];
+    const float4 v = get(w);
     c = rec_step_map(v, mask >> w & 1, c);
     p = mul2(p, pk2(v.x, v.y));
   }
   const float2 pf = upk2(p), cf = upk2(c);
-  out = make_float4(pf.x, pf.y, cf.x, cf.y);
+  return make_float4(mask ? -1.f : pf.x, mask ? -1.f : pf.y, cf.x, cf.y);
 }
 
 // ---------------------------------------------------------------- forward
 
+struct RecTrue { static constexpr bool value = true; };
+struct RecFalse { static constexpr bool value = false; };
+
 struct RecFwdSmem {
   float4 maps[2][REC_WARPS][32];
   float4 cta[2][REC_MAX_CLUSTER][32];
+  u64 carry[2][32];
+  uint64_t full[3], peers[2];
   unsigned cuts[2][REC_WARPS];
-  unsigned cta_cut[2][REC_MAX_CLUSTER];
 };
 
 __device__ __forceinline__ unsigned rec_cuts(const unsigned (&c)[REC_WARPS]) {
@@ -259,137 +328,163 @@ __device__ __forceinline__ unsigned rec_cuts(const unsigned (&c)[REC_WARPS]) {
   return m;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(RecParams P) {
+template <typename T, bool VEC, bool Z>
+__global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_constant__ RecParams P) {
   constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>(), STAGES = rec_fwd_stages<VEC>();
-  extern __shared__ __align__(16) char stages[];
+  constexpr int STAGE_BYTES = (Z ? 4 : 3) * TB;
+  extern __shared__ __align__(128) char stages[];
   __shared__ RecFwdSmem sm;
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = P.cluster, rank = nc > 1 ? (int)blockIdx.x % nc : 0;
   const int b = blockIdx.y, ch0 = (int)blockIdx.x / nc * REC_CH, nch = min(REC_CH, P.E - ch0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool has_z = P.z.p != nullptr, packed = P.seq.start != nullptr;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const bool packed = P.seq.start != nullptr;
   const T* px = row_ptr<T>(P.x, b, 0) + ch0;
   const T* pd = row_ptr<T>(P.decay, b, 0) + ch0;
   const T* pg = row_ptr<T>(P.gate, b, 0) + ch0;
-  const T* pz = has_z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
+  const T* pz = Z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
   T* py = static_cast<T*>(P.y) + (long long)b * P.T * P.E + ch0;
-  const int stage_bytes = (has_z ? 4 : 3) * TB;
   const int iters = (P.tiles + nc - 1) / nc;
+  bool alive = true;
 
   auto fetch = [&](int it) {
-    if (it < iters) {
-      const int t0 = (it * nc + rank) * TILE;
-      char* s = stages + (it % STAGES) * stage_bytes;
-      rec_copy<T, VEC>(s, pd, P.decay.st, t0, P.T, nch);
-      rec_copy<T, VEC>(s + TB, px, P.x.st, t0, P.T, nch);
-      rec_copy<T, VEC>(s + 2 * TB, pg, P.gate.st, t0, P.T, nch);
-      if (has_z) rec_copy<T, VEC>(s + 3 * TB, pz, P.z.st, t0, P.T, nch);
+    char* s = stages + (it % STAGES) * STAGE_BYTES;
+    const int t0 = (it * nc + rank) * TILE;
+    if (VEC) {
+      if (threadIdx.x == 0 && it < iters && alive) {
+        uint64_t* bar = &sm.full[it % STAGES];
+        rec_bar_expect(bar, STAGE_BYTES);
+#pragma unroll
+        for (int q = 0; q < (Z ? 4 : 3); ++q) rec_tma(s + q * TB, &P.map[q], ch0, t0, b, bar);
+      }
+    } else {
+      if (it < iters) {
+        rec_copy<T>(s, pd, P.decay.st, t0, P.T, nch);
+        rec_copy<T>(s + TB, px, P.x.st, t0, P.T, nch);
+        rec_copy<T>(s + 2 * TB, pg, P.gate.st, t0, P.T, nch);
+        if (Z) rec_copy<T>(s + 3 * TB, pz, P.z.st, t0, P.T, nch);
+      }
+      cp_async_commit();
     }
-    cp_async_commit();
   };
+  if (threadIdx.x == 0) {
+    for (int q = 0; q < STAGES; ++q) rec_bar_init(&sm.full[q]);
+    rec_bar_init(&sm.peers[0]);
+    rec_bar_init(&sm.peers[1]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (nc > 1) cluster.sync();  // before any other CTA sends here
+  else __syncthreads();
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
   const u64 A2 = mul2(rec_vec(P.A + ch0, VEC, nch, 0.f), all2(LOG2E));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  // the state in front of the cluster's first tile; then (one CTA) in shared memory, (several) composed by everyone
   u64 carry = packed ? 0ull : rec_vec(P.h0 ? P.h0 + (long long)b * P.E + ch0 : nullptr, VEC, nch, 0.f);
+  auto h0_of = [&](const RecMarks& m, int j) {  // the state that the sequence starting at a warp's token j starts from
+    const int q = __shfl_sync(0xffffffffu, m.mine, j);
+    return rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+  };
 
   for (int it = 0; it < iters; ++it) {
     const int tile = it * nc + rank, t0 = tile * TILE + warp * S, par = it & 1;
-    const char* s = stages + (it % STAGES) * stage_bytes;
-    cp_async_wait<STAGES - 2>();
-    __syncthreads();
-    fetch(it + STAGES - 1);
+    const char* s = stages + (it % STAGES) * STAGE_BYTES;
     const int n = min(S, P.T - t0);  // tokens of this warp (may be <= 0)
     const RecMarks marks = rec_marks<S>(P.seq, t0);
+    if (VEC) {
+      if (alive) alive = rec_bar_wait(&sm.full[it % STAGES], (it / STAGES) & 1);
+    } else {
+      cp_async_wait<STAGES - 2>();
+      __syncthreads();
+    }
 
     // gates, and the map of this warp's tokens
+    const bool whole = n == S && !(marks.starts | marks.ends);  // all there, no sequence starts or ends among them
     u64 a[S], bb[S], sz[S];
     u64 p = all2(1.f), c = 0ull;
+    auto gates = [&](auto all) {
 #pragma unroll
-    for (int j = 0; j < S; ++j) {
-      a[j] = all2(1.f);
-      bb[j] = 0ull;
-      if (j < n) {
+      for (int j = 0; j < S; ++j) {
+        if (!all.value && j >= n) break;
         const int row = warp * S + j, t = t0 + j;
-        const u64 r = rec_sig(rec_expneg(rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
+        const u64 r = rec_sig(P.k, rec_expneg(P.k, rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
         u64 w;
-        rec_decay(mul2(A2, r), a[j], w);
-        const u64 g = rec_sig(rec_expneg(rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng));
+        rec_decay(P.k, mul2(A2, r), a[j], w);
+        const u64 g = rec_sig(P.k, rec_expneg(P.k, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng));
         const u64 x = rec_get<T, VEC>(s + TB, row, rec_odd<T, VEC>(px, P.x.st, t));
-        bb[j] = mul2(mul2(mul2(w, rec_rsqrt(w)), g), x);
-        if (has_z) {
-          const u64 z = rec_get<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t));
-          sz[j] = mul2(z, rec_sig(rec_expneg(z, 0ull)));
-        }
-        if (marks.starts >> j & 1) {
-          const int q = __shfl_sync(0xffffffffu, marks.mine, j);
-          c = rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
-        }
+        bb[j] = mul2(mul2(rec_root(w), g), x);
+        if (Z) sz[j] = rec_silu(P.k, rec_get<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t)));
+        if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
         c = fma2(a[j], c, bb[j]);
         p = mul2(p, a[j]);
       }
-    }
+    };
+    if (whole) gates(RecTrue{});
+    else gates(RecFalse{});
     {
       const float2 pf = upk2(p), cf = upk2(c);
       sm.maps[par][warp][lane] = make_float4(pf.x, pf.y, cf.x, cf.y);
       if (lane == 0) sm.cuts[par][warp] = marks.starts;
     }
-    __syncthreads();
+    __syncthreads();  // the maps are there, and nobody reads the staged tile any more
+    fetch(it + STAGES - 1);
     const unsigned cuts = packed ? rec_cuts(sm.cuts[par]) : 0u;
 
+    u64 h;
     if (nc > 1) {  // the tiles of the cluster's other CTAs: their maps, in order
       if (warp == 0) {
-        float4 m;
-        rec_compose(sm.maps[par], cuts, false, m);
-        for (int q = 0; q < nc; ++q) {
-          cluster.map_shared_rank(&sm.cta[par][rank][0], q)[lane] = m;
-          if (lane == 0) *cluster.map_shared_rank(&sm.cta_cut[par][rank], q) = cuts;
-        }
+        if (lane == 0) rec_bar_expect(&sm.peers[par], nc * 32 * (uint32_t)sizeof(float4));
+        const float4 m = rec_compose([&](int w) { return sm.maps[par][w][lane]; }, cuts, false);
+        for (int q = 0; q < nc; ++q) rec_send(&sm.cta[par][rank][lane], &sm.peers[par], q, m);
       }
-      cluster.sync();
-    }
-    u64 h = carry;
-    if (nc > 1) {
-      u64 next = carry;
+      if (alive) alive = rec_bar_wait(&sm.peers[par], (it >> 1) & 1);
+      h = carry;
       for (int q = 0; q < nc; ++q) {
-        if (q == rank) h = next;
-        next = rec_step_map(sm.cta[par][q][lane], packed && sm.cta_cut[par][q] != 0, next);
+        if (q == rank) h = carry;
+        carry = rec_step_map(sm.cta[par][q][lane], sm.cta[par][q][lane].x < 0.f, carry);
       }
-      carry = next;
+    } else {
+      h = it > 0 ? sm.carry[par][lane] : carry;
     }
     if (P.ckpt && warp == 0 && tile < P.tiles)
       rec_put_vec(P.ckpt + ((long long)b * P.tiles + tile) * P.E + ch0, h, VEC, nch);
-    {
-      u64 v = h;
-#pragma unroll
-      for (int w = 0; w < REC_WARPS; ++w) {
-        if (w == warp) h = v;
-        v = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, v);
-      }
-      if (nc == 1) carry = v;
-    }
+    for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
 
     // the states, and what leaves
+    T* out = py + (long long)t0 * P.E;
+    auto states = [&](auto all) {
 #pragma unroll
-    for (int j = 0; j < S; ++j)
-      if (j < n) {
-        if (marks.starts >> j & 1) {
-          const int q = __shfl_sync(0xffffffffu, marks.mine, j);
-          h = rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
-        }
+      for (int j = 0; j < S; ++j) {
+        if (!all.value && j >= n) break;
+        if (!all.value && (marks.starts >> j & 1)) h = h0_of(marks, j);
         h = fma2(a[j], h, bb[j]);
-        rec_put<T, VEC>(py + (long long)(t0 + j) * P.E, has_z ? mul2(h, sz[j]) : h, nch);
-        if (P.ht && (marks.ends >> j & 1)) {
+        rec_put<T, VEC>(out + (long long)j * P.E, Z ? mul2(h, sz[j]) : h, nch);
+        if (!all.value && P.ht && (marks.ends >> j & 1)) {
           const int q = __shfl_sync(0xffffffffu, marks.mine, 8 + j);
           rec_put_vec(P.ht + (long long)q * P.E + ch0, h, VEC, nch);
         }
       }
+    };
+    if (whole) states(RecTrue{});
+    else states(RecFalse{});
+    if (warp == REC_WARPS - 1) {  // behind the tile's last token
+      if (nc == 1) carry = h;
+      sm.carry[par ^ 1][lane] = h;
+    }
   }
-  if (!packed && P.ht && rank == 0 && warp == 0) rec_put_vec(P.ht + (long long)b * P.E + ch0, carry, VEC, nch);
-  cp_async_wait<0>();
+  if (!packed && P.ht && rank == 0 && warp == REC_WARPS - 1)
+    rec_put_vec(P.ht + (long long)b * P.E + ch0, carry, VEC, nch);
+  if (!alive) atomicExch(P.err, 12);
+  if (VEC) {
+    if (!alive) {  // a copy or a map did not arrive: let what is in flight land (waiting again, as long)
+      if (threadIdx.x == 0)
+        for (int it = max(0, iters - STAGES); it < iters; ++it) rec_bar_wait(&sm.full[it % STAGES], (it / STAGES) & 1);
+    }
+  } else {
+    cp_async_wait<0>();
+  }
   if (nc > 1) cluster.sync();  // no CTA leaves while another may still write its maps here
 }
 
@@ -405,108 +500,133 @@ struct RecBwdSmem {
   float4 maps[2][REC_WARPS][32];  // states: P, P, c, c
   float2 back[2][REC_WARPS][32];  // gradients: d, d (P as above)
   float4 cta[2][REC_MAX_CLUSTER][32];
+  u64 carry[2][32];
+  uint64_t full[REC_BWD_STAGES], peers[2];
   unsigned cuts[2][REC_WARPS], ends[2][REC_WARPS];
-  unsigned cta_cut[2][REC_MAX_CLUSTER];
 };
 
 // Adds v to a compensated sum (s, c).
 __device__ __forceinline__ void rec_add(u64& s, u64& c, u64 v) {
-  const u64 y = add2(v, neg2(c)), t = add2(s, y);
-  c = add2(add2(t, neg2(s)), neg2(y));
+  const u64 y = sub2(v, c), t = add2(s, y);
+  c = sub2(sub2(t, s), y);
   s = t;
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(RecParams P) {
-  constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>();
-  extern __shared__ __align__(16) char stages[];
+template <typename T, bool VEC, bool Z>
+__global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_constant__ RecParams P) {
+  constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>(), STAGES = REC_BWD_STAGES;
+  constexpr int STAGE_BYTES = (Z ? 5 : 4) * TB;
+  extern __shared__ __align__(128) char stages[];
   __shared__ RecBwdSmem sm;
   cg::cluster_group cluster = cg::this_cluster();
   const int nc = P.cluster, rank = nc > 1 ? (int)blockIdx.x % nc : 0;
   const int b = blockIdx.y, ch0 = (int)blockIdx.x / nc * REC_CH, nch = min(REC_CH, P.E - ch0);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool has_z = P.z.p != nullptr, packed = P.seq.start != nullptr;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const bool packed = P.seq.start != nullptr;
   const T* px = row_ptr<T>(P.x, b, 0) + ch0;
   const T* pd = row_ptr<T>(P.decay, b, 0) + ch0;
   const T* pg = row_ptr<T>(P.gate, b, 0) + ch0;
-  const T* pz = has_z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
+  const T* pz = Z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
   const T* pdy = row_ptr<T>(P.dy, b, 0) + ch0;
   const long long out0 = (long long)b * P.T * P.E + ch0;
-  const int stage_bytes = (has_z ? 5 : 4) * TB;
   const int iters = (P.tiles + nc - 1) / nc;
 
+  bool alive = true;
+
   auto fetch = [&](int k) {  // the k-th tile from the end
-    if (k < iters) {
-      const int t0 = ((iters - 1 - k) * nc + rank) * TILE;
-      char* s = stages + (k % REC_BWD_STAGES) * stage_bytes;
-      rec_copy<T, VEC>(s, pd, P.decay.st, t0, P.T, nch);
-      rec_copy<T, VEC>(s + TB, px, P.x.st, t0, P.T, nch);
-      rec_copy<T, VEC>(s + 2 * TB, pg, P.gate.st, t0, P.T, nch);
-      rec_copy<T, VEC>(s + 3 * TB, pdy, P.dy.st, t0, P.T, nch);
-      if (has_z) rec_copy<T, VEC>(s + 4 * TB, pz, P.z.st, t0, P.T, nch);
-    }
-    cp_async_commit();
-  };
+    char* s = stages + (k % STAGES) * STAGE_BYTES;
+    const int t0 = ((iters - 1 - k) * nc + rank) * TILE;
+    if (VEC) {
+      if (threadIdx.x == 0 && k < iters && alive) {
+        uint64_t* bar = &sm.full[k % STAGES];
+        rec_bar_expect(bar, STAGE_BYTES);
 #pragma unroll
-  for (int k = 0; k < REC_BWD_STAGES - 1; ++k) fetch(k);
+        for (int q = 0; q < (Z ? 5 : 4); ++q) rec_tma(s + q * TB, &P.map[q], ch0, t0, b, bar);
+      }
+    } else {
+      if (k < iters) {
+        rec_copy<T>(s, pd, P.decay.st, t0, P.T, nch);
+        rec_copy<T>(s + TB, px, P.x.st, t0, P.T, nch);
+        rec_copy<T>(s + 2 * TB, pg, P.gate.st, t0, P.T, nch);
+        rec_copy<T>(s + 3 * TB, pdy, P.dy.st, t0, P.T, nch);
+        if (Z) rec_copy<T>(s + 4 * TB, pz, P.z.st, t0, P.T, nch);
+      }
+      cp_async_commit();
+    }
+  };
+  if (threadIdx.x == 0) {
+    for (int q = 0; q < STAGES; ++q) rec_bar_init(&sm.full[q]);
+    rec_bar_init(&sm.peers[0]);
+    rec_bar_init(&sm.peers[1]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (nc > 1) cluster.sync();  // before any other CTA sends here
+  else __syncthreads();
+#pragma unroll
+  for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
   const u64 A1 = rec_vec(P.A + ch0, VEC, nch, 0.f), A2 = mul2(A1, all2(LOG2E));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   u64 carry = packed ? 0ull : rec_vec(P.dht ? P.dht + (long long)b * P.E + ch0 : nullptr, VEC, nch, 0.f);
+  auto h0_of = [&](const RecMarks& m, int j) {
+    const int q = __shfl_sync(0xffffffffu, m.mine, j);
+    return rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+  };
+  auto dht_of = [&](const RecMarks& m, int j) {
+    const int q = __shfl_sync(0xffffffffu, m.mine, 8 + j);
+    return rec_vec(P.dht ? P.dht + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
+  };
   u64 sumA = 0ull, lowA = 0ull, sumD = 0ull, lowD = 0ull, sumG = 0ull, lowG = 0ull;
 
   for (int k = 0; k < iters; ++k) {
     const int tile = (iters - 1 - k) * nc + rank, t0 = tile * TILE + warp * S, par = k & 1;
-    const char* s = stages + (k % REC_BWD_STAGES) * stage_bytes;
+    const char* s = stages + (k % STAGES) * STAGE_BYTES;
     u64 h = tile < P.tiles ? rec_vec(P.ckpt + ((long long)b * P.tiles + tile) * P.E + ch0, VEC, nch, 0.f) : 0ull;
-    cp_async_wait<REC_BWD_STAGES - 2>();
-    __syncthreads();
-    fetch(k + REC_BWD_STAGES - 1);
+    if (!VEC) cp_async_wait<STAGES - 2>();
+    __syncthreads();  // nobody reads the tile before this one any more
+    fetch(k + STAGES - 1);
+    if (VEC && alive) alive = rec_bar_wait(&sm.full[k % STAGES], (k / STAGES) & 1);
     const int n = min(S, P.T - t0);
     const RecMarks marks = rec_marks<S>(P.seq, t0);
 
     auto get = [&](int which, const T* base, long long st, int j) {
       return rec_get<T, VEC>(s + which * TB, warp * S + j, rec_odd<T, VEC>(base, st, t0 + j));
     };
-    auto h0_of = [&](int j) {
-      const int q = __shfl_sync(0xffffffffu, marks.mine, j);
-      return rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
-    };
-    auto dht_of = [&](int j) {
-      const int q = __shfl_sync(0xffffffffu, marks.mine, 8 + j);
-      return rec_vec(P.dht ? P.dht + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
-    };
-
+    const bool whole = n == S && !(marks.starts | marks.ends);
     u64 a[S], hs[S], rr[S], ii[S], zz[S];  // decay; b, then the state; the sigmoids
     {
       u64 p = all2(1.f), c = 0ull, d = 0ull;
-      bool open = true;  // no end among the tokens so far
+      auto gates = [&](auto all) {
+        bool open = true;  // no end among the tokens so far
 #pragma unroll
-      for (int j = 0; j < S; ++j)
-        if (j < n) {
-          rr[j] = rec_sig(rec_expneg(get(0, pd, P.decay.st, j), nd));
+        for (int j = 0; j < S; ++j) {
+          if (!all.value && j >= n) break;
+          rr[j] = rec_sig(P.k, rec_expneg(P.k, get(0, pd, P.decay.st, j), nd));
           u64 w;
-          rec_decay(mul2(A2, rr[j]), a[j], w);
-          ii[j] = rec_sig(rec_expneg(get(2, pg, P.gate.st, j), ng));
-          hs[j] = mul2(mul2(mul2(w, rec_rsqrt(w)), ii[j]), get(1, px, P.x.st, j));
+          rec_decay(P.k, mul2(A2, rr[j]), a[j], w);
+          ii[j] = rec_sig(P.k, rec_expneg(P.k, get(2, pg, P.gate.st, j), ng));
+          hs[j] = mul2(mul2(rec_root(w), ii[j]), get(1, px, P.x.st, j));
           u64 g = get(3, pdy, P.dy.st, j);
-          if (has_z) {
+          if (Z) {
             const u64 z = get(4, pz, P.z.st, j);
-            zz[j] = rec_sig(rec_expneg(z, 0ull));
+            zz[j] = rec_sig(P.k, ex2_2(mul2(z, P.k.log2e)));
             g = mul2(g, mul2(z, zz[j]));
           }
-          if (marks.starts >> j & 1) c = h0_of(j);
+          if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
           c = fma2(a[j], c, hs[j]);
           p = mul2(p, a[j]);
-          if (open) {
-            if (marks.ends >> j & 1) {
-              g = add2(g, dht_of(j));
+          if (all.value || open) {
+            if (!all.value && (marks.ends >> j & 1)) {
+              g = add2(g, dht_of(marks, j));
               open = false;
             }
             d = fma2(p, g, d);
           }
         }
+      };
+      if (whole) gates(RecTrue{});
+      else gates(RecFalse{});
       const float2 pf = upk2(p), cf = upk2(c);
       sm.maps[par][warp][lane] = make_float4(pf.x, pf.y, cf.x, cf.y);
       sm.back[par][warp][lane] = upk2(d);
@@ -522,103 +642,100 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(RecParams P) {
       const float2 d = sm.back[par][w][lane];
       return make_float4(m.x, m.y, d.x, d.y);
     };
+    u64 U;
     if (nc > 1) {
       if (warp == 0) {
-        u64 p = all2(1.f), d = 0ull;
-#pragma unroll
-        for (int w = REC_WARPS - 1; w >= 0; --w) {
-          const float4 m = back(w);
-          d = rec_step_map(m, ends >> w & 1, d);
-          p = mul2(p, pk2(m.x, m.y));
-        }
-        const float2 pf = upk2(p), df = upk2(d);
-        for (int q = 0; q < nc; ++q) {
-          cluster.map_shared_rank(&sm.cta[par][rank][0], q)[lane] = make_float4(pf.x, pf.y, df.x, df.y);
-          if (lane == 0) *cluster.map_shared_rank(&sm.cta_cut[par][rank], q) = ends;
-        }
+        if (lane == 0) rec_bar_expect(&sm.peers[par], nc * 32 * (uint32_t)sizeof(float4));
+        const float4 m = rec_compose(back, ends, true);
+        for (int q = 0; q < nc; ++q) rec_send(&sm.cta[par][rank][lane], &sm.peers[par], q, m);
       }
-      cluster.sync();
-    }
-    u64 U = carry;
-    if (nc > 1) {
-      u64 next = carry;
+      if (alive) alive = rec_bar_wait(&sm.peers[par], (k >> 1) & 1);
+      U = carry;
       for (int q = nc - 1; q >= 0; --q) {
-        if (q == rank) U = next;
-        next = rec_step_map(sm.cta[par][q][lane], packed && sm.cta_cut[par][q] != 0, next);
+        if (q == rank) U = carry;
+        carry = rec_step_map(sm.cta[par][q][lane], sm.cta[par][q][lane].x < 0.f, carry);
       }
-      carry = next;
+    } else {
+      U = k > 0 ? sm.carry[par][lane] : carry;
     }
-    {
-      u64 v = U;
-#pragma unroll
-      for (int w = REC_WARPS - 1; w >= 0; --w) {
-        if (w == warp) U = v;
-        v = rec_step_map(back(w), ends >> w & 1, v);
-      }
-      if (nc == 1) carry = v;
-      for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
-    }
+    for (int w = REC_WARPS - 1; w > warp; --w) U = rec_step_map(back(w), ends >> w & 1, U);
+    for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
 
-    const u64 h_in = h;
+    u64 tA = 0ull, tD = 0ull, tG = 0ull;
+    const long long out = out0 + (long long)t0 * P.E;
+    auto grads = [&](auto all) {
+      const u64 h_in = h;
 #pragma unroll
-    for (int j = 0; j < S; ++j)
-      if (j < n) {
-        if (marks.starts >> j & 1) h = h0_of(j);
+      for (int j = 0; j < S; ++j) {
+        if (!all.value && j >= n) break;
+        if (!all.value && (marks.starts >> j & 1)) h = h0_of(marks, j);
         h = fma2(a[j], h, hs[j]);
         hs[j] = h;
       }
-
-    u64 tA = 0ull, tD = 0ull, tG = 0ull;
 #pragma unroll
-    for (int j = S - 1; j >= 0; --j)
-      if (j < n) {
-        const long long at = out0 + (long long)(t0 + j) * P.E;
+      for (int j = S - 1; j >= 0; --j) {
+        if (!all.value && j >= n) continue;
+        const long long at = out + (long long)j * P.E;
         u64 prev = j > 0 ? hs[j > 0 ? j - 1 : 0] : h_in;
-        if (marks.starts >> j & 1) prev = h0_of(j);
+        if (!all.value && (marks.starts >> j & 1)) prev = h0_of(marks, j);
         u64 G = get(3, pdy, P.dy.st, j);
-        if (has_z) {
+        if (Z) {
           const u64 z = get(4, pz, P.z.st, j), dyh = mul2(G, hs[j]);
           G = mul2(G, mul2(z, zz[j]));
           // silu' = s (1 + z (1 - s))
-          const u64 one = fma2(zz[j], all2(-1.f), all2(1.f));
-          rec_put<T, VEC>(static_cast<T*>(P.dz) + at, mul2(dyh, mul2(zz[j], fma2(z, one, all2(1.f)))), nch);
+          rec_put<T, VEC>(static_cast<T*>(P.dz) + at,
+                          mul2(dyh, mul2(zz[j], fma2(z, sub2(P.k.one, zz[j]), P.k.one))), nch);
         }
-        if (marks.ends >> j & 1) U = dht_of(j);
+        if (!all.value && (marks.ends >> j & 1)) U = dht_of(marks, j);
         G = add2(G, U);
         U = mul2(a[j], G);
-        if ((marks.starts >> j & 1) && P.dh0) {
+        if (!all.value && (marks.starts >> j & 1) && P.dh0) {
           const int q = __shfl_sync(0xffffffffu, marks.mine, j);
           rec_put_vec(P.dh0 + (long long)q * P.E + ch0, U, VEC, nch);
         }
         const u64 x = get(1, px, P.x.st, j);
-        const u64 er = rec_expneg(get(0, pd, P.decay.st, j), nd), ei = rec_expneg(get(2, pg, P.gate.st, j), ng);
+        const u64 er = rec_expneg(P.k, get(0, pd, P.decay.st, j), nd), ei = rec_expneg(P.k, get(2, pg, P.gate.st, j), ng);
         u64 aa, w;
-        rec_decay(mul2(A2, rr[j]), aa, w);
+        rec_decay(P.k, mul2(A2, rr[j]), aa, w);
         const u64 rs = rec_rsqrt(w), norm = mul2(w, rs);
         const u64 Gn = mul2(G, norm), ix = mul2(ii[j], x);
         rec_put<T, VEC>(static_cast<T*>(P.dx) + at, mul2(Gn, ii[j]), nch);
-        const u64 dg = mul2(mul2(Gn, ix), rec_one_minus(ii[j], ei));
+        const u64 dg = mul2(mul2(Gn, ix), rec_one_minus(P.k, ii[j], ei));
         rec_put<T, VEC>(static_cast<T*>(P.dgate) + at, dg, nch);
         tG = add2(tG, dg);
         // d(A r) r = G (a h' r - a^2 i x r / n): the small factors first, so that nothing overflows
         const u64 ar = mul2(a[j], rr[j]);
-        const u64 q = mul2(mul2(ar, rs), mul2(a[j], ix));
-        const u64 dAr = mul2(G, fma2(ar, prev, neg2(q)));
+        const u64 dAr = mul2(G, sub2(mul2(ar, prev), mul2(mul2(ar, rs), mul2(a[j], ix))));
         tA = add2(tA, dAr);
-        const u64 dd = mul2(mul2(dAr, A1), rec_one_minus(rr[j], er));
+        const u64 dd = mul2(mul2(dAr, A1), rec_one_minus(P.k, rr[j], er));
         rec_put<T, VEC>(static_cast<T*>(P.ddecay) + at, dd, nch);
         tD = add2(tD, dd);
       }
+    };
+    if (whole) grads(RecTrue{});
+    else grads(RecFalse{});
+    if (warp == 0) {  // in front of the tile's first token
+      if (nc == 1) carry = U;
+      sm.carry[par ^ 1][lane] = U;
+    }
     rec_add(sumA, lowA, tA);
     rec_add(sumD, lowD, tD);
     rec_add(sumG, lowG, tG);
   }
   if (!packed && P.dh0 && rank == 0 && warp == 0) rec_put_vec(P.dh0 + (long long)b * P.E + ch0, carry, VEC, nch);
-  cp_async_wait<0>();
+  if (!alive) atomicExch(P.err, 12);
+  if (VEC) {
+    if (!alive) {
+      if (threadIdx.x == 0)
+        for (int k = max(0, iters - STAGES); k < iters; ++k) rec_bar_wait(&sm.full[k % STAGES], (k / STAGES) & 1);
+    }
+  } else {
+    cp_async_wait<0>();
+  }
   __syncthreads();
   // the CTA's sums: the warps in order
   float* red = reinterpret_cast<float*>(stages);  // [warps][3][64]
-  const u64 sums[3] = {add2(sumA, neg2(lowA)), add2(sumD, neg2(lowD)), add2(sumG, neg2(lowG))};
+  const u64 sums[3] = {sub2(sumA, lowA), sub2(sumD, lowD), sub2(sumG, lowG)};
 #pragma unroll
   for (int q = 0; q < 3; ++q) rec_put_vec(red + (warp * 3 + q) * REC_CH, sums[q], VEC, REC_CH);
   __syncthreads();
@@ -635,6 +752,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(RecParams P) {
 // ---------------------------------------------------------------- single tokens
 
 struct RecStepParams {
+  RecConst k;
   const void *x, *decay, *gate, *z;
   long long sx, sd, sg, sz;
   const float *A, *decay_bias, *gate_bias;
@@ -650,7 +768,7 @@ constexpr int REC_STEP_THREADS = 128;
 // A thread has two neighbouring channels (VEC) or one, and strides over the rows: latency, not
 // bandwidth, bounds every size that a decoding batch has.  The arithmetic is the prompt's, operation by operation.
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(RecStepParams P) {
+__global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(const __grid_constant__ RecStepParams P) {
   constexpr int V = VEC ? 2 : 1;
   const int c = (blockIdx.x * REC_STEP_THREADS + threadIdx.x) * V;
   if (c >= P.E) return;
@@ -673,15 +791,15 @@ __global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(RecStepParam
     float* sp = P.state + (long long)slot * P.E + c;
     float hf[V];
     io_load<float, V>(sp, hf);
-    const u64 rd = rec_sig(rec_expneg(in(P.decay, P.sd), nd)), gi = rec_sig(rec_expneg(in(P.gate, P.sg), ng));
+    const u64 rd = rec_sig(P.k, rec_expneg(P.k, in(P.decay, P.sd), nd)), gi = rec_sig(P.k, rec_expneg(P.k, in(P.gate, P.sg), ng));
     u64 a, w;
-    rec_decay(mul2(A2, rd), a, w);
-    const u64 b = mul2(mul2(mul2(w, rec_rsqrt(w)), gi), in(P.x, P.sx));
+    rec_decay(P.k, mul2(A2, rd), a, w);
+    const u64 b = mul2(mul2(rec_root(w), gi), in(P.x, P.sx));
     const u64 h = fma2(a, pk2(hf[0], hf[V - 1]), b);
     u64 o = h;
     if (P.z) {
       const u64 z = in(P.z, P.sz);
-      o = mul2(h, mul2(z, rec_sig(rec_expneg(z, 0ull))));
+      o = mul2(h, mul2(z, rec_sig(P.k, ex2_2(mul2(z, P.k.log2e)))));
     }
     const float2 hn = upk2(h), on = upk2(o);
     const float h2[2] = {hn.x, hn.y}, o2[2] = {on.x, on.y};

@@ -352,6 +352,21 @@ int* kda::device_error_flag() {
   return static_cast<int*>(p);
 }
 
+bool kda::encode_tiled_map(void* map, const void* base, int dtype, int rank, const unsigned long long* dims,
+                           const unsigned long long* strides, const unsigned* box) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  const cuuint32_t elem[5] = {1u, 1u, 1u, 1u, 1u};
+  const CUtensorMapDataType type = dtype == KDA_IO_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == KDA_IO_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                          : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  static_assert(sizeof(cuuint64_t) == sizeof(unsigned long long) && sizeof(cuuint32_t) == sizeof(unsigned), "types");
+  return enc && enc(static_cast<CUtensorMap*>(map), type, (cuuint32_t)rank, const_cast<void*>(base),
+                    reinterpret_cast<const cuuint64_t*>(dims), reinterpret_cast<const cuuint64_t*>(strides),
+                    reinterpret_cast<const cuuint32_t*>(box), elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 extern "C" {
 
 const char* kda_b200_version(void) { return "kda_b200 0.1.0 (sm_100a)"; }

@@ -108,4 +108,10 @@ inline int sm_count() {
 // failure.  Defined in kda_api.cu.
 int* device_error_flag();
 
+// Tensor map of an activation of type KDA_IO_* (no swizzle; a box reads zeros outside the tensor): `rank` dims and box
+// sides, innermost first, and the byte strides of all but the innermost.  False where the driver takes no such map.
+// Defined in kda_api.cu.
+bool encode_tiled_map(void* map, const void* base, int dtype, int rank, const unsigned long long* dims,
+                     const unsigned long long* strides, const unsigned* box);
+
 }  // namespace kda

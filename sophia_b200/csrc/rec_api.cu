@@ -46,6 +46,7 @@ int check_rec(const kda_b200_recurrence_args* a, bool step) {
 
 RecParams rec_params(const kda_b200_recurrence_args* a) {
   RecParams p{};
+  p.k = rec_const();
   p.x = {a->x, a->x_sb, a->x_st};
   p.decay = {a->decay, a->decay_sb, a->decay_st};
   p.gate = {a->gate, a->gate_sb, a->gate_st};
@@ -65,6 +66,24 @@ bool rec_vec_ok(const RecParams& p, int dtype) {
   auto ok = [&](const RowView& r) { return !r.p || vec_rows(r.p, r.sb, r.st, p.B, p.T, V, esz); };
   return p.E % V == 0 && ok(p.x) && ok(p.decay) && ok(p.gate) && ok(p.z) && ok(p.dy) && aligned(p.y, 16) &&
          aligned(p.dx, 16) && aligned(p.ddecay, 16) && aligned(p.dgate, 16) && aligned(p.dz, 16);
+}
+
+// The tensor maps of a call's activations: boxes of a tile's tokens x 64 channels of a row.  False where a layout has
+// none (a row or token that is expanded has the stride 0): the kernels then copy by words.
+bool rec_maps(RecParams& p, int dtype, bool backward) {
+  const RowView fwd[4] = {p.decay, p.x, p.gate, p.z}, bwd[5] = {p.decay, p.x, p.gate, p.dy, p.z};
+  const RowView* r = backward ? bwd : fwd;
+  const int n = (backward ? 5 : 4) - (p.z.p ? 0 : 1);
+  const size_t esz = io_size(dtype);
+  for (int i = 0; i < n; ++i) {
+    // (a stride that is never taken, of a single row or token, may be anything: give the encoder a legal one)
+    const unsigned long long st = (p.T > 1 ? r[i].st : p.E) * esz, sb = (p.B > 1 ? r[i].sb : p.E) * esz;
+    const unsigned long long dims[3] = {(unsigned long long)p.E, (unsigned long long)p.T, (unsigned long long)p.B};
+    const unsigned long long strides[2] = {st, sb};
+    const unsigned box[3] = {REC_CH, (unsigned)rec_tokens(dtype), 1u};
+    if (!st || !sb || !encode_tiled_map(&p.map[i], r[i].p, dtype, 3, dims, strides, box)) return false;
+  }
+  return true;
 }
 
 int launch_rec(void (*kernel)(RecParams), const RecParams& p, int smem, int id, const char* what, cudaStream_t st) {
@@ -89,22 +108,26 @@ int launch_rec(void (*kernel)(RecParams), const RecParams& p, int smem, int id, 
   return launch_check(what);
 }
 
+template <typename T, bool VEC>
+int rec_fwd_z(const RecParams& p, cudaStream_t st) {
+  const int smem = rec_fwd_stages<VEC>() * (p.z.p ? 4 : 3) * rec_tensor_bytes<T, VEC>();
+  return launch_rec(p.z.p ? rec_fwd_kernel<T, VEC, true> : rec_fwd_kernel<T, VEC, false>, p, smem, K_REC_FWD,
+                    "recurrence forward", st);
+}
 template <typename T>
 int rec_fwd(const RecParams& p, bool vec, cudaStream_t st) {
-  const int n = p.z.p ? 4 : 3;
-  return vec ? launch_rec(rec_fwd_kernel<T, true>, p, rec_fwd_stages<true>() * n * rec_tensor_bytes<T, true>(), K_REC_FWD,
-                          "recurrence forward", st)
-             : launch_rec(rec_fwd_kernel<T, false>, p, rec_fwd_stages<false>() * n * rec_tensor_bytes<T, false>(),
-                          K_REC_FWD, "recurrence forward", st);
+  return vec ? rec_fwd_z<T, true>(p, st) : rec_fwd_z<T, false>(p, st);
 }
 
+template <typename T, bool VEC>
+int rec_bwd_z(const RecParams& p, cudaStream_t st) {
+  const int smem = REC_BWD_STAGES * (p.z.p ? 5 : 4) * rec_tensor_bytes<T, VEC>();
+  return launch_rec(p.z.p ? rec_bwd_kernel<T, VEC, true> : rec_bwd_kernel<T, VEC, false>, p, smem, K_REC_BWD,
+                    "recurrence backward", st);
+}
 template <typename T>
 int rec_bwd(const RecParams& p, bool vec, cudaStream_t st) {
-  const int n = p.z.p ? 5 : 4;
-  return vec ? launch_rec(rec_bwd_kernel<T, true>, p, REC_BWD_STAGES * n * rec_tensor_bytes<T, true>(), K_REC_BWD,
-                          "recurrence backward", st)
-             : launch_rec(rec_bwd_kernel<T, false>, p, REC_BWD_STAGES * n * rec_tensor_bytes<T, false>(), K_REC_BWD,
-                          "recurrence backward", st);
+  return vec ? rec_bwd_z<T, true>(p, st) : rec_bwd_z<T, false>(p, st);
 }
 
 template <typename T>
@@ -151,11 +174,13 @@ int kda_b200_recurrence_fwd(const kda_b200_recurrence_args* a, void* workspace, 
                    a->saved_bytes < kda_b200_recurrence_saved_bytes(a->B, a->T, a->E, a->dtype)))
     return fail(KDA_ERR_INVALID, "saved buffer too small: kda_b200_recurrence_saved_bytes() bytes are needed");
   RecParams p = rec_params(a);
+  if (!(p.err = device_error_flag())) return fail(KDA_ERR_CUDA, "the device error flag has no address");
   p.y = a->y;
   p.ht = a->ht;
   Carver cv(workspace);
   if ((rc = build_map(p.seq, cv, a->cu_seqlens, p.T, a->nseq, a->h0, a->ht, a->E, st))) return rc;
-  return SSM_DISPATCH(a->dtype, rec_fwd, p, rec_vec_ok(p, a->dtype), st);
+  const bool vec = rec_vec_ok(p, a->dtype) && rec_maps(p, a->dtype, false);
+  return SSM_DISPATCH(a->dtype, rec_fwd, p, vec, st);
 }
 
 int kda_b200_recurrence_bwd(const kda_b200_recurrence_args* a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -177,13 +202,15 @@ int kda_b200_recurrence_bwd(const kda_b200_recurrence_args* a, void* workspace, 
       workspace_bytes < kda_b200_recurrence_workspace_bytes(a->B, a->T, a->E, a->dtype, a->cu_seqlens != nullptr, 1))
     return fail(KDA_ERR_INVALID, "workspace too small: kda_b200_recurrence_workspace_bytes() bytes are needed");
   RecParams p = rec_params(a);
+  if (!(p.err = device_error_flag())) return fail(KDA_ERR_CUDA, "the device error flag has no address");
   p.dy = {a->dy, a->dy_sb, a->dy_st};
   p.dht = a->dht; p.dh0 = a->dh0;
   p.dx = a->dx; p.ddecay = a->ddecay; p.dgate = a->dgate; p.dz = a->z ? a->dz : nullptr;
   Carver cv(workspace);
   if ((rc = build_map(p.seq, cv, a->cu_seqlens, p.T, a->nseq, a->dht, a->dh0, a->E, st))) return rc;
   p.partial = cv.take<float>((size_t)p.B * p.cluster * p.E * 3 * 4);
-  if ((rc = SSM_DISPATCH(a->dtype, rec_bwd, p, rec_vec_ok(p, a->dtype), st))) return rc;
+  const bool vec = rec_vec_ok(p, a->dtype) && rec_maps(p, a->dtype, true);
+  if ((rc = SSM_DISPATCH(a->dtype, rec_bwd, p, vec, st))) return rc;
   const long long cols = 3LL * p.E;
   {
     TimedLaunch tl(K_REC_BWD, st);
@@ -199,7 +226,7 @@ int kda_b200_recurrence_step(const kda_b200_recurrence_args* a, void* stream) {
   if (a->rows == 0) return KDA_OK;
   int* err = device_error_flag();
   if (!err) return fail(KDA_ERR_CUDA, "the device error flag has no address");
-  RecStepParams p{a->x, a->decay, a->gate, a->z, a->x_sb, a->decay_sb, a->gate_sb, a->z_sb, a->A, a->decay_bias,
+  RecStepParams p{rec_const(), a->x, a->decay, a->gate, a->z, a->x_sb, a->decay_sb, a->gate_sb, a->z_sb, a->A, a->decay_bias,
                   a->gate_bias, a->state, a->slots, a->rows, a->E, a->pool, a->y, err};
   return SSM_DISPATCH(a->dtype, rec_step, p, static_cast<cudaStream_t>(stream));
 }
