@@ -102,29 +102,20 @@ __device__ __forceinline__ u64 rec_expneg(const RecConst& k, u64 v, u64 nb) { re
 __device__ __forceinline__ u64 rec_sig(const RecConst& k, u64 e) { return rcp_2(add2(e, k.one)); }
 // v sigmoid(v)
 __device__ __forceinline__ u64 rec_silu(const RecConst& k, u64 v) { return mul2(v, rec_sig(k, ex2_2(mul2(v, k.log2e)))); }
-// 1 - sigmoid without cancellation: 1 - r below one half, e r above (e is finite there)
-__device__ __forceinline__ u64 rec_one_minus(const RecConst& k, u64 r, u64 e) {
-  const float2 p = upk2(sub2(k.one, r)), q = upk2(mul2(e, r)), f = upk2(r);
-  return pk2(f.x < 0.5f ? p.x : q.x, f.y < 0.5f ? p.y : q.y);
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ float rsq(float v) {
-  float r;
-  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
 // a = 2^l and w = 1 - a^2 for l <= 0, both with fp32 relative accuracy.  l = n + f, n the nearest whole
 // number; q = 1 - 2^f is a polynomial times f, which keeps q accurate in relative terms next to 0;
-// a = 2^n (1 - q), m = 1 - a = 2^n q + (1 - 2^n) cancels nowhere, w = m (2 - m).
+// a = 2^n (1 - q), m = 1 - a = 2^n q + (1 - 2^n) cancels nowhere, w = m (2 - m).  CLAMP: l may be below -126.
+template <bool CLAMP>
 __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64& w) {
-  float2 lf = upk2(l);
-  lf.x = max_nan(lf.x, -126.f);
-  lf.y = max_nan(lf.y, -126.f);
-  l = pk2(lf.x, lf.y);
+  if (CLAMP) {
+    const float2 lf = upk2(l);
+    l = pk2(max_nan(lf.x, -126.f), max_nan(lf.y, -126.f));
+  }
   const u64 t = add2(l, k.round);  // the sum's low bits are n
   const u64 f = sub2(l, sub2(t, k.round));
   u64 p = fma2(k.poly[0], f, k.poly[1]);
@@ -138,15 +129,16 @@ __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64&
   const u64 m = fma2(s, q, sub2(k.one, s));
   w = mul2(m, sub2(k.two, m));
 }
-// sqrt(w) as w / sqrt(w): 0 for w = 0, NaN for NaN (a denormal w counts as 0).
-__device__ __forceinline__ u64 rec_root(u64 w) {
-  const float2 f = upk2(w);
-  return mul2(w, pk2(rsq(fmaxf(f.x, 1.17549435e-38f)), rsq(fmaxf(f.y, 1.17549435e-38f))));
+__device__ __forceinline__ u64 rec_sqrt(u64 w) {
+  float2 f = upk2(w);
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(f.x));
+  asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(f.y));
+  return pk2(f.x, f.y);
 }
-// 1 / sqrt(w), but 0 for w = 0: nothing decays, so nothing enters.
-__device__ __forceinline__ u64 rec_rsqrt(u64 w) {
-  const float2 f = upk2(w);
-  return pk2(f.x < 1.17549435e-38f ? 0.f : rsq(f.x), f.y < 1.17549435e-38f ? 0.f : rsq(f.y));
+// 1 / v, but 0 for v = 0: where nothing decays, nothing enters
+__device__ __forceinline__ u64 rec_inverse(u64 v) {
+  const float2 f = upk2(v);
+  return pk2(f.x == 0.f ? 0.f : rcp(f.x), f.y == 0.f ? 0.f : rcp(f.y));
 }
 
 // ---------------------------------------------------------------- staged tiles
@@ -292,6 +284,19 @@ __device__ __forceinline__ u64 rec_step_map(const float4& m, bool cut, u64 h) {
   return cut ? c : n;
 }
 
+// h through the maps from..to - 1 (REV: last first), one per 32 lanes; `marked`: P < 0 stands for a cut.
+template <bool REV>
+__device__ __forceinline__ void rec_fold(u64& h, const float4* maps, int from, int to, bool marked) {
+  if (!marked) {
+    for (int i = from; i < to; ++i) h = rec_step_map(maps[32 * (REV ? to - 1 - (i - from) : i)], false, h);
+  } else {
+    for (int i = from; i < to; ++i) {
+      const float4 m = maps[32 * (REV ? to - 1 - (i - from) : i)];
+      h = rec_step_map(m, m.x < 0.f, h);
+    }
+  }
+}
+
 // The whole CTA's map: the warps' maps m[0..7] in order (reverse: last first; `mask`: their cuts).  P < 0 stands for a
 // cut inside (a product of decays is not negative).
 template <typename Get>
@@ -381,6 +386,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
   const u64 A2 = mul2(rec_vec(P.A + ch0, VEC, nch, 0.f), all2(LOG2E));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  const bool steep = __any_sync(0xffffffffu, upk2(A2).x < -126.f || upk2(A2).y < -126.f);
   // the state in front of the cluster's first tile; then (one CTA) in shared memory, (several) composed by everyone
   u64 carry = packed ? 0ull : rec_vec(P.h0 ? P.h0 + (long long)b * P.E + ch0 : nullptr, VEC, nch, 0.f);
   auto h0_of = [&](const RecMarks& m, int j) {  // the state that the sequence starting at a warp's token j starts from
@@ -388,20 +394,21 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
     return rec_vec(P.h0 ? P.h0 + (long long)q * P.E + ch0 : nullptr, VEC, nch, 0.f);
   };
 
-  for (int it = 0; it < iters; ++it) {
+  int slot = 0, turn = 0;  // the tile's place among the stages, and the parity of its arrival
+  for (int it = 0; it < iters; ++it, turn ^= slot == STAGES - 1, slot = slot == STAGES - 1 ? 0 : slot + 1) {
     const int tile = it * nc + rank, t0 = tile * TILE + warp * S, par = it & 1;
-    const char* s = stages + (it % STAGES) * STAGE_BYTES;
+    const char* s = stages + slot * STAGE_BYTES;
     const int n = min(S, P.T - t0);  // tokens of this warp (may be <= 0)
     const RecMarks marks = rec_marks<S>(P.seq, t0);
     if (VEC) {
-      if (alive) alive = rec_bar_wait(&sm.full[it % STAGES], (it / STAGES) & 1);
+      if (alive) alive = rec_bar_wait(&sm.full[slot], turn);
     } else {
       cp_async_wait<STAGES - 2>();
       __syncthreads();
     }
 
     // gates, and the map of this warp's tokens
-    const bool whole = n == S && !(marks.starts | marks.ends);  // all there, no sequence starts or ends among them
+    const bool whole = n == S && !(marks.starts | marks.ends) && !steep;  // nothing special about them
     u64 a[S], bb[S], sz[S];
     u64 p = all2(1.f), c = 0ull;
     auto gates = [&](auto all) {
@@ -411,10 +418,10 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
         const int row = warp * S + j, t = t0 + j;
         const u64 r = rec_sig(P.k, rec_expneg(P.k, rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
         u64 w;
-        rec_decay(P.k, mul2(A2, r), a[j], w);
+        rec_decay<!all.value>(P.k, mul2(A2, r), a[j], w);
         const u64 g = rec_sig(P.k, rec_expneg(P.k, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng));
         const u64 x = rec_get<T, VEC>(s + TB, row, rec_odd<T, VEC>(px, P.x.st, t));
-        bb[j] = mul2(mul2(rec_root(w), g), x);
+        bb[j] = mul2(mul2(rec_sqrt(w), g), x);
         if (Z) sz[j] = rec_silu(P.k, rec_get<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t)));
         if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
         c = fma2(a[j], c, bb[j]);
@@ -440,17 +447,17 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
         for (int q = 0; q < nc; ++q) rec_send(&sm.cta[par][rank][lane], &sm.peers[par], q, m);
       }
       if (alive) alive = rec_bar_wait(&sm.peers[par], (it >> 1) & 1);
+      rec_fold<false>(carry, &sm.cta[par][0][lane], 0, rank, packed);
       h = carry;
-      for (int q = 0; q < nc; ++q) {
-        if (q == rank) h = carry;
-        carry = rec_step_map(sm.cta[par][q][lane], sm.cta[par][q][lane].x < 0.f, carry);
-      }
+      rec_fold<false>(carry, &sm.cta[par][0][lane], rank, nc, packed);
     } else {
       h = it > 0 ? sm.carry[par][lane] : carry;
     }
     if (P.ckpt && warp == 0 && tile < P.tiles)
       rec_put_vec(P.ckpt + ((long long)b * P.tiles + tile) * P.E + ch0, h, VEC, nch);
-    for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
+    if (!cuts) rec_fold<false>(h, &sm.maps[par][0][lane], 0, warp, false);
+    else
+      for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
 
     // the states, and what leaves
     T* out = py + (long long)t0 * P.E;
@@ -568,6 +575,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
   const u64 A1 = rec_vec(P.A + ch0, VEC, nch, 0.f), A2 = mul2(A1, all2(LOG2E));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
+  const bool steep = __any_sync(0xffffffffu, upk2(A2).x < -126.f || upk2(A2).y < -126.f);
   u64 carry = packed ? 0ull : rec_vec(P.dht ? P.dht + (long long)b * P.E + ch0 : nullptr, VEC, nch, 0.f);
   auto h0_of = [&](const RecMarks& m, int j) {
     const int q = __shfl_sync(0xffffffffu, m.mine, j);
@@ -593,8 +601,8 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
     auto get = [&](int which, const T* base, long long st, int j) {
       return rec_get<T, VEC>(s + which * TB, warp * S + j, rec_odd<T, VEC>(base, st, t0 + j));
     };
-    const bool whole = n == S && !(marks.starts | marks.ends);
-    u64 a[S], hs[S], rr[S], ii[S], zz[S];  // decay; b, then the state; the sigmoids
+    const bool whole = n == S && !(marks.starts | marks.ends) && !steep;
+    u64 a[S], hs[S], rr[S], ii[S], be[S];  // decay; b, then the state; the sigmoids; the normaliser
     {
       u64 p = all2(1.f), c = 0ull, d = 0ull;
       auto gates = [&](auto all) {
@@ -604,15 +612,12 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
           if (!all.value && j >= n) break;
           rr[j] = rec_sig(P.k, rec_expneg(P.k, get(0, pd, P.decay.st, j), nd));
           u64 w;
-          rec_decay(P.k, mul2(A2, rr[j]), a[j], w);
+          rec_decay<!all.value>(P.k, mul2(A2, rr[j]), a[j], w);
+          be[j] = rec_sqrt(w);
           ii[j] = rec_sig(P.k, rec_expneg(P.k, get(2, pg, P.gate.st, j), ng));
-          hs[j] = mul2(mul2(rec_root(w), ii[j]), get(1, px, P.x.st, j));
+          hs[j] = mul2(mul2(be[j], ii[j]), get(1, px, P.x.st, j));
           u64 g = get(3, pdy, P.dy.st, j);
-          if (Z) {
-            const u64 z = get(4, pz, P.z.st, j);
-            zz[j] = rec_sig(P.k, ex2_2(mul2(z, P.k.log2e)));
-            g = mul2(g, mul2(z, zz[j]));
-          }
+          if (Z) g = mul2(g, rec_silu(P.k, get(4, pz, P.z.st, j)));
           if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
           c = fma2(a[j], c, hs[j]);
           p = mul2(p, a[j]);
@@ -650,16 +655,19 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
         for (int q = 0; q < nc; ++q) rec_send(&sm.cta[par][rank][lane], &sm.peers[par], q, m);
       }
       if (alive) alive = rec_bar_wait(&sm.peers[par], (k >> 1) & 1);
+      rec_fold<true>(carry, &sm.cta[par][0][lane], rank + 1, nc, packed);
       U = carry;
-      for (int q = nc - 1; q >= 0; --q) {
-        if (q == rank) U = carry;
-        carry = rec_step_map(sm.cta[par][q][lane], sm.cta[par][q][lane].x < 0.f, carry);
-      }
+      rec_fold<true>(carry, &sm.cta[par][0][lane], 0, rank + 1, packed);
     } else {
       U = k > 0 ? sm.carry[par][lane] : carry;
     }
-    for (int w = REC_WARPS - 1; w > warp; --w) U = rec_step_map(back(w), ends >> w & 1, U);
-    for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
+    if (!(cuts | ends)) {
+      for (int w = REC_WARPS - 1; w > warp; --w) U = rec_step_map(back(w), false, U);
+      rec_fold<false>(h, &sm.maps[par][0][lane], 0, warp, false);
+    } else {
+      for (int w = REC_WARPS - 1; w > warp; --w) U = rec_step_map(back(w), ends >> w & 1, U);
+      for (int w = 0; w < warp; ++w) h = rec_step_map(sm.maps[par][w][lane], cuts >> w & 1, h);
+    }
 
     u64 tA = 0ull, tD = 0ull, tG = 0ull;
     const long long out = out0 + (long long)t0 * P.E;
@@ -679,12 +687,11 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
         u64 prev = j > 0 ? hs[j > 0 ? j - 1 : 0] : h_in;
         if (!all.value && (marks.starts >> j & 1)) prev = h0_of(marks, j);
         u64 G = get(3, pdy, P.dy.st, j);
-        if (Z) {
+        if (Z) {  // silu' = s (1 + z (1 - s)) = s + z s (1 - s)
           const u64 z = get(4, pz, P.z.st, j), dyh = mul2(G, hs[j]);
-          G = mul2(G, mul2(z, zz[j]));
-          // silu' = s (1 + z (1 - s))
-          rec_put<T, VEC>(static_cast<T*>(P.dz) + at,
-                          mul2(dyh, mul2(zz[j], fma2(z, sub2(P.k.one, zz[j]), P.k.one))), nch);
+          const u64 sg = rec_sig(P.k, ex2_2(mul2(z, P.k.log2e))), zs = mul2(z, sg);
+          G = mul2(G, zs);
+          rec_put<T, VEC>(static_cast<T*>(P.dz) + at, mul2(dyh, fma2(zs, sub2(P.k.one, sg), sg)), nch);
         }
         if (!all.value && (marks.ends >> j & 1)) U = dht_of(marks, j);
         G = add2(G, U);
@@ -693,21 +700,16 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
           const int q = __shfl_sync(0xffffffffu, marks.mine, j);
           rec_put_vec(P.dh0 + (long long)q * P.E + ch0, U, VEC, nch);
         }
-        const u64 x = get(1, px, P.x.st, j);
-        const u64 er = rec_expneg(P.k, get(0, pd, P.decay.st, j), nd), ei = rec_expneg(P.k, get(2, pg, P.gate.st, j), ng);
-        u64 aa, w;
-        rec_decay(P.k, mul2(A2, rr[j]), aa, w);
-        const u64 rs = rec_rsqrt(w), norm = mul2(w, rs);
-        const u64 Gn = mul2(G, norm), ix = mul2(ii[j], x);
+        const u64 ix = mul2(ii[j], get(1, px, P.x.st, j)), Gn = mul2(G, be[j]);
         rec_put<T, VEC>(static_cast<T*>(P.dx) + at, mul2(Gn, ii[j]), nch);
-        const u64 dg = mul2(mul2(Gn, ix), rec_one_minus(P.k, ii[j], ei));
+        const u64 dg = mul2(mul2(Gn, ix), sub2(P.k.one, ii[j]));
         rec_put<T, VEC>(static_cast<T*>(P.dgate) + at, dg, nch);
         tG = add2(tG, dg);
         // d(A r) r = G (a h' r - a^2 i x r / n): the small factors first, so that nothing overflows
         const u64 ar = mul2(a[j], rr[j]);
-        const u64 dAr = mul2(G, sub2(mul2(ar, prev), mul2(mul2(ar, rs), mul2(a[j], ix))));
+        const u64 dAr = mul2(G, sub2(mul2(ar, prev), mul2(mul2(ar, rec_inverse(be[j])), mul2(a[j], ix))));
         tA = add2(tA, dAr);
-        const u64 dd = mul2(mul2(dAr, A1), rec_one_minus(P.k, rr[j], er));
+        const u64 dd = mul2(mul2(dAr, A1), sub2(P.k.one, rr[j]));
         rec_put<T, VEC>(static_cast<T*>(P.ddecay) + at, dd, nch);
         tD = add2(tD, dd);
       }
@@ -793,8 +795,8 @@ __global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(const __grid
     io_load<float, V>(sp, hf);
     const u64 rd = rec_sig(P.k, rec_expneg(P.k, in(P.decay, P.sd), nd)), gi = rec_sig(P.k, rec_expneg(P.k, in(P.gate, P.sg), ng));
     u64 a, w;
-    rec_decay(P.k, mul2(A2, rd), a, w);
-    const u64 b = mul2(mul2(rec_root(w), gi), in(P.x, P.sx));
+    rec_decay<true>(P.k, mul2(A2, rd), a, w);
+    const u64 b = mul2(mul2(rec_sqrt(w), gi), in(P.x, P.sx));
     const u64 h = fma2(a, pk2(hf[0], hf[V - 1]), b);
     u64 o = h;
     if (P.z) {
