@@ -32,6 +32,7 @@ namespace cg = cooperative_groups;
 
 constexpr int REC_THREADS = 256;
 constexpr int REC_WARPS = REC_THREADS / 32;
+constexpr int REC_CTAS = 2;          // per SM: 128 registers a thread
 constexpr int REC_CH = 64;           // channels of a CTA, two a lane
 constexpr int REC_MAX_CLUSTER = 8;   // the portable limit
 // Tokens of a thread: a tile of 8 S tokens of one tensor is 8 KB in every type.
@@ -50,6 +51,22 @@ template <bool VEC>
 __host__ __device__ constexpr int rec_fwd_stages() { return VEC ? 3 : 2; }
 constexpr int REC_BWD_STAGES = 2;
 
+// ---------------------------------------------------------------- arithmetic on two channels
+
+__device__ __forceinline__ u64 ex2_2(u64 v) {
+  const float2 f = upk2(v);
+  return pk2(ex2(f.x), ex2(f.y));
+}
+__device__ __forceinline__ u64 rcp_2(u64 v) {
+  const float2 f = upk2(v);
+  return pk2(rcp(f.x), rcp(f.y));
+}
+__device__ __forceinline__ u64 all2(float v) { return pk2(v, v); }
+__device__ __forceinline__ u64 sub2(u64 a, u64 b) {
+  u64 r;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // The packed arithmetic's constants, as kernel parameters: operands from the constant bank or uniform registers
 // where literals would be moved into a pair of registers at every use (28 of 141 instructions a pair of elements).
 struct RecConst {
@@ -67,36 +84,6 @@ inline RecConst rec_const() {
            two(-0.693147182f)}};
 }
 
-struct RecParams {
-  RecConst k;
-  CUtensorMap map[5];  // decay, x, gate, then forward z, backward dy and z: [B][T][E], boxes of a tile (16-byte pieces only)
-  int* err;
-  RowView x, decay, gate, z, dy;  // z.p null = no output gate
-  const float *A, *decay_bias, *gate_bias, *h0, *dht;
-  void *y, *dx, *ddecay, *dgate, *dz;
-  float *ht, *dh0;
-  float* ckpt;     // [B][tiles][E] states in front of every tile
-  float* partial;  // [B * cluster][E][3]: dA, ddecay_bias, dgate_bias
-  int B, T, E, tiles, cluster;
-  SeqMap seq;
-};
-
-// ---------------------------------------------------------------- arithmetic on two channels
-
-__device__ __forceinline__ u64 ex2_2(u64 v) {
-  const float2 f = upk2(v);
-  return pk2(ex2(f.x), ex2(f.y));
-}
-__device__ __forceinline__ u64 rcp_2(u64 v) {
-  const float2 f = upk2(v);
-  return pk2(rcp(f.x), rcp(f.y));
-}
-__device__ __forceinline__ u64 all2(float v) { return pk2(v, v); }
-__device__ __forceinline__ u64 sub2(u64 a, u64 b) {
-  u64 r;
-  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // e = exp(-(v + bias)) from v and nb = -bias log2 e
 __device__ __forceinline__ u64 rec_expneg(const RecConst& k, u64 v, u64 nb) { return ex2_2(fma2(v, k.log2e, nb)); }
 __device__ __forceinline__ u64 rec_sig(const RecConst& k, u64 e) { return rcp_2(add2(e, k.one)); }
@@ -129,6 +116,14 @@ __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64&
   const u64 m = fma2(s, q, sub2(k.one, s));
   w = mul2(m, sub2(k.two, m));
 }
+// sqrt(w) / d: one special function in the place of a root and a reciprocal
+__device__ __forceinline__ u64 rec_sqrt_over(u64 w, u64 d) {
+  const float2 f = upk2(mul2(mul2(d, d), w));  // (an infinite d^2 gives 0, its limit)
+  float x = max_nan(f.x, 1.17549435e-38f), y = max_nan(f.y, 1.17549435e-38f);
+  asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(x));
+  asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(y));
+  return mul2(w, pk2(x, y));
+}
 __device__ __forceinline__ u64 rec_sqrt(u64 w) {
   float2 f = upk2(w);
   asm("sqrt.approx.ftz.f32 %0, %0;" : "+f"(f.x));
@@ -140,6 +135,20 @@ __device__ __forceinline__ u64 rec_inverse(u64 v) {
   const float2 f = upk2(v);
   return pk2(f.x == 0.f ? 0.f : rcp(f.x), f.y == 0.f ? 0.f : rcp(f.y));
 }
+
+struct RecParams {
+  RecConst k;
+  CUtensorMap map[5];  // decay, x, gate, then forward z, backward dy and z: [B][T][E], boxes of a tile (16-byte pieces only)
+  int* err;
+  RowView x, decay, gate, z, dy;  // z.p null = no output gate
+  const float *A, *decay_bias, *gate_bias, *h0, *dht;
+  void *y, *dx, *ddecay, *dgate, *dz;
+  float *ht, *dh0;
+  float* ckpt;     // [B][tiles][E] states in front of every tile
+  float* partial;  // [B * cluster][E][3]: dA, ddecay_bias, dgate_bias
+  int B, T, E, tiles, cluster;
+  SeqMap seq;
+};
 
 // ---------------------------------------------------------------- staged tiles
 
@@ -213,6 +222,18 @@ __device__ __forceinline__ u64 rec_get(const char* tile, int row, int odd) {
   }
   const T* e = reinterpret_cast<const T*>(p) + odd + lane;
   return pk2(io_to_f(e[0]), io_to_f(e[32]));
+}
+// The same as it is stored, to be converted later.
+template <typename T, bool VEC>
+__device__ __forceinline__ IoVec<T, 2> rec_raw(const char* tile, int row, int odd) {
+  const int lane = threadIdx.x & 31;
+  const char* p = tile + row * rec_pitch<T, VEC>();
+  if (VEC) return *reinterpret_cast<const IoVec<T, 2>*>(p + lane * 2 * sizeof(T));
+  const T* e = reinterpret_cast<const T*>(p) + odd + lane;
+  IoVec<T, 2> v;
+  v.v[0] = e[0];
+  v.v[1] = e[32];
+  return v;
 }
 __device__ __forceinline__ int rec_lane_ch(bool vec, int k) {
   const int lane = threadIdx.x & 31;
@@ -297,7 +318,7 @@ __device__ __forceinline__ void rec_fold(u64& h, const float4* maps, int from, i
   }
 }
 
-// The whole CTA's map: the warps' maps m[0..7] in order (reverse: last first; `mask`: their cuts).  P < 0 stands for a
+// The whole CTA's map: the warps' maps in order (reverse: last first; `mask`: their cuts).  P < 0 stands for a
 // cut inside (a product of decays is not negative).
 template <typename Get>
 __device__ __forceinline__ float4 rec_compose(Get get, unsigned mask, bool reverse) {
@@ -320,7 +341,6 @@ struct RecFalse { static constexpr bool value = false; };
 
 struct RecFwdSmem {
   float4 maps[2][REC_WARPS][32];
-  float4 cta[2][REC_MAX_CLUSTER][32];
   u64 carry[2][32];
   uint64_t full[3], peers[2];
   unsigned cuts[2][REC_WARPS];
@@ -334,7 +354,7 @@ __device__ __forceinline__ unsigned rec_cuts(const unsigned (&c)[REC_WARPS]) {
 }
 
 template <typename T, bool VEC, bool Z>
-__global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_constant__ RecParams P) {
+__global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_fwd_kernel(const __grid_constant__ RecParams P) {
   constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>(), STAGES = rec_fwd_stages<VEC>();
   constexpr int STAGE_BYTES = (Z ? 4 : 3) * TB;
   extern __shared__ __align__(128) char stages[];
@@ -350,6 +370,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
   const T* pz = Z ? row_ptr<T>(P.z, b, 0) + ch0 : nullptr;
   T* py = static_cast<T*>(P.y) + (long long)b * P.T * P.E + ch0;
   const int iters = (P.tiles + nc - 1) / nc;
+  float4* peer_maps = reinterpret_cast<float4*>(stages + STAGES * STAGE_BYTES);  // [2][nc][32]: the cluster's
   bool alive = true;
 
   auto fetch = [&](int it) {
@@ -383,6 +404,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
+  const RecConst& K = P.k;
   const u64 A2 = mul2(rec_vec(P.A + ch0, VEC, nch, 0.f), all2(LOG2E));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
@@ -409,20 +431,21 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
 
     // gates, and the map of this warp's tokens
     const bool whole = n == S && !(marks.starts | marks.ends) && !steep;  // nothing special about them
-    u64 a[S], bb[S], sz[S];
+    u64 a[S], bb[S];
+    IoVec<T, 2> zr[S];
     u64 p = all2(1.f), c = 0ull;
     auto gates = [&](auto all) {
 #pragma unroll
       for (int j = 0; j < S; ++j) {
         if (!all.value && j >= n) break;
         const int row = warp * S + j, t = t0 + j;
-        const u64 r = rec_sig(P.k, rec_expneg(P.k, rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
+        const u64 r = rec_sig(K, rec_expneg(K, rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
         u64 w;
-        rec_decay<!all.value>(P.k, mul2(A2, r), a[j], w);
-        const u64 g = rec_sig(P.k, rec_expneg(P.k, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng));
+        rec_decay<!all.value>(K, mul2(A2, r), a[j], w);
+        const u64 g = add2(rec_expneg(K, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng), K.one);
         const u64 x = rec_get<T, VEC>(s + TB, row, rec_odd<T, VEC>(px, P.x.st, t));
-        bb[j] = mul2(mul2(rec_sqrt(w), g), x);
-        if (Z) sz[j] = rec_silu(P.k, rec_get<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t)));
+        bb[j] = mul2(rec_sqrt_over(w, g), x);
+        if (Z) zr[j] = rec_raw<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t));
         if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
         c = fma2(a[j], c, bb[j]);
         p = mul2(p, a[j]);
@@ -444,12 +467,12 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
       if (warp == 0) {
         if (lane == 0) rec_bar_expect(&sm.peers[par], nc * 32 * (uint32_t)sizeof(float4));
         const float4 m = rec_compose([&](int w) { return sm.maps[par][w][lane]; }, cuts, false);
-        for (int q = 0; q < nc; ++q) rec_send(&sm.cta[par][rank][lane], &sm.peers[par], q, m);
+        for (int q = 0; q < nc; ++q) rec_send(&peer_maps[(par * nc + rank) * 32 + lane], &sm.peers[par], q, m);
       }
       if (alive) alive = rec_bar_wait(&sm.peers[par], (it >> 1) & 1);
-      rec_fold<false>(carry, &sm.cta[par][0][lane], 0, rank, packed);
+      rec_fold<false>(carry, &peer_maps[par * nc * 32 + lane], 0, rank, packed);
       h = carry;
-      rec_fold<false>(carry, &sm.cta[par][0][lane], rank, nc, packed);
+      rec_fold<false>(carry, &peer_maps[par * nc * 32 + lane], rank, nc, packed);
     } else {
       h = it > 0 ? sm.carry[par][lane] : carry;
     }
@@ -467,7 +490,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
         if (!all.value && j >= n) break;
         if (!all.value && (marks.starts >> j & 1)) h = h0_of(marks, j);
         h = fma2(a[j], h, bb[j]);
-        rec_put<T, VEC>(out + (long long)j * P.E, Z ? mul2(h, sz[j]) : h, nch);
+        rec_put<T, VEC>(out + (long long)j * P.E, Z ? mul2(h, rec_silu(K, pk2(io_to_f(zr[j].v[0]), io_to_f(zr[j].v[1])))) : h, nch);
         if (!all.value && P.ht && (marks.ends >> j & 1)) {
           const int q = __shfl_sync(0xffffffffu, marks.mine, 8 + j);
           rec_put_vec(P.ht + (long long)q * P.E + ch0, h, VEC, nch);
@@ -506,7 +529,6 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_fwd_kernel(const __grid_co
 struct RecBwdSmem {
   float4 maps[2][REC_WARPS][32];  // states: P, P, c, c
   float2 back[2][REC_WARPS][32];  // gradients: d, d (P as above)
-  float4 cta[2][REC_MAX_CLUSTER][32];
   u64 carry[2][32];
   uint64_t full[REC_BWD_STAGES], peers[2];
   unsigned cuts[2][REC_WARPS], ends[2][REC_WARPS];
@@ -520,7 +542,7 @@ __device__ __forceinline__ void rec_add(u64& s, u64& c, u64 v) {
 }
 
 template <typename T, bool VEC, bool Z>
-__global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_constant__ RecParams P) {
+__global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_bwd_kernel(const __grid_constant__ RecParams P) {
   constexpr int S = rec_s<T>(), TILE = rec_tile<T>(), TB = rec_tensor_bytes<T, VEC>(), STAGES = REC_BWD_STAGES;
   constexpr int STAGE_BYTES = (Z ? 5 : 4) * TB;
   extern __shared__ __align__(128) char stages[];
@@ -537,6 +559,7 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
   const T* pdy = row_ptr<T>(P.dy, b, 0) + ch0;
   const long long out0 = (long long)b * P.T * P.E + ch0;
   const int iters = (P.tiles + nc - 1) / nc;
+  float4* peer_maps = reinterpret_cast<float4*>(stages + STAGES * STAGE_BYTES);  // [2][nc][32]: the cluster's
 
   bool alive = true;
 
@@ -652,12 +675,12 @@ __global__ void __launch_bounds__(REC_THREADS, 2) rec_bwd_kernel(const __grid_co
       if (warp == 0) {
         if (lane == 0) rec_bar_expect(&sm.peers[par], nc * 32 * (uint32_t)sizeof(float4));
         const float4 m = rec_compose(back, ends, true);
-        for (int q = 0; q < nc; ++q) rec_send(&sm.cta[par][rank][lane], &sm.peers[par], q, m);
+        for (int q = 0; q < nc; ++q) rec_send(&peer_maps[(par * nc + rank) * 32 + lane], &sm.peers[par], q, m);
       }
       if (alive) alive = rec_bar_wait(&sm.peers[par], (k >> 1) & 1);
-      rec_fold<true>(carry, &sm.cta[par][0][lane], rank + 1, nc, packed);
+      rec_fold<true>(carry, &peer_maps[par * nc * 32 + lane], rank + 1, nc, packed);
       U = carry;
-      rec_fold<true>(carry, &sm.cta[par][0][lane], 0, rank + 1, packed);
+      rec_fold<true>(carry, &peer_maps[par * nc * 32 + lane], 0, rank + 1, packed);
     } else {
       U = k > 0 ? sm.carry[par][lane] : carry;
     }
@@ -793,10 +816,10 @@ __global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(const __grid
     float* sp = P.state + (long long)slot * P.E + c;
     float hf[V];
     io_load<float, V>(sp, hf);
-    const u64 rd = rec_sig(P.k, rec_expneg(P.k, in(P.decay, P.sd), nd)), gi = rec_sig(P.k, rec_expneg(P.k, in(P.gate, P.sg), ng));
+    const u64 rd = rec_sig(P.k, rec_expneg(P.k, in(P.decay, P.sd), nd)), gi = add2(rec_expneg(P.k, in(P.gate, P.sg), ng), P.k.one);
     u64 a, w;
     rec_decay<true>(P.k, mul2(A2, rd), a, w);
-    const u64 b = mul2(mul2(rec_sqrt(w), gi), in(P.x, P.sx));
+    const u64 b = mul2(rec_sqrt_over(w, gi), in(P.x, P.sx));
     const u64 h = fma2(a, pk2(hf[0], hf[V - 1]), b);
     u64 o = h;
     if (P.z) {

@@ -20,7 +20,7 @@ long long rec_tiles(long long T, int dtype) { return (T + rec_tokens(dtype) - 1)
 
 // CTAs that share a row's tiles: as many as two CTAs per SM allow, never more than there are tiles.
 int rec_cluster(long long B, long long T, int E, int dtype) {
-  const long long lanes = B * ((E + REC_CH - 1) / REC_CH), tiles = rec_tiles(T, dtype), slots = 2LL * sm_count();
+  const long long lanes = B * ((E + REC_CH - 1) / REC_CH), tiles = rec_tiles(T, dtype), slots = (long long)REC_CTAS * sm_count();
   int c = 1;
   while (2 * c <= REC_MAX_CLUSTER && 2 * c * lanes <= slots && 2 * c <= tiles) c *= 2;
   return c;
@@ -87,6 +87,7 @@ bool rec_maps(RecParams& p, int dtype, bool backward) {
 }
 
 int launch_rec(void (*kernel)(RecParams), const RecParams& p, int smem, int id, const char* what, cudaStream_t st) {
+  if (p.cluster > 1) smem += 2 * p.cluster * 32 * (int)sizeof(float4);  // the maps of the cluster's CTAs
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string(what) + " smem: " + cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
