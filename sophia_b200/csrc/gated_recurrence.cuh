@@ -118,8 +118,9 @@ __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64&
 }
 // sqrt(w) / d: one special function in the place of a root and a reciprocal
 __device__ __forceinline__ u64 rec_sqrt_over(u64 w, u64 d) {
-  const float2 f = upk2(mul2(mul2(d, d), w));  // (an infinite d^2 gives 0, its limit)
-  float x = max_nan(f.x, 1.17549435e-38f), y = max_nan(f.y, 1.17549435e-38f);
+  const float2 f = upk2(w);  // w = 0 and an infinite d both give 0, their limits
+  const float2 g = upk2(mul2(mul2(pk2(max_nan(f.x, 1.17549435e-38f), max_nan(f.y, 1.17549435e-38f)), d), d));
+  float x = g.x, y = g.y;
   asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(x));
   asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(y));
   return mul2(w, pk2(x, y));
