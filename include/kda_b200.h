@@ -208,7 +208,9 @@ int kda_b200_device_error(int reset);
  *         swizzled tensor-core tiles need it): the kernel did nothing;
  *   10    a tensor-core completion wait of the forward chunk kernel ran out;
  *   11    a single-token call named a state slot past its pool (that row was
- *         treated as padding).
+ *         treated as padding);
+ *   12    a wait of the gated recurrence for a tile, or for the states of the
+ *         cluster's other CTAs, ran out: the call's outputs are not valid.
  * A kernel that records a timeout lets its copies in flight land (a second
  * bounded wait), frees what it holds and returns; later calls are unaffected.
  */
@@ -437,6 +439,44 @@ size_t kda_b200_recurrence_workspace_bytes(int64_t B, int64_t T, int E, int dtyp
 int kda_b200_recurrence_fwd(const kda_b200_recurrence_args* args, void* workspace, size_t workspace_bytes, void* stream);
 int kda_b200_recurrence_bwd(const kda_b200_recurrence_args* args, void* workspace, size_t workspace_bytes, void* stream);
 int kda_b200_recurrence_step(const kda_b200_recurrence_args* args, void* stream);
+
+/*
+ * What stands between two blocks of a stack, per row of D <= 8192 channels:
+ *     u = o, or rms_norm(o) wb;   u = u sigmoid(gate);   u = dropout(u)
+ *     v = x + scale u,   n = rms_norm(v) w        rms_norm(a) = a / sqrt(mean(a^2) + eps)
+ * o, gate, n and their gradients are of one type (dtype), the residual stream x, v, dv, dx of that type or fp32
+ * (stream_dtype); rows [B, T, D] with strides as above.  w, wb, scale [D] fp32; w NULL: no n; wb, gate, scale NULL: that
+ * part is left out.  v is rounded when it is stored; n comes from the value before that.
+ * Dropout (dropout_p > 0) draws 32 bits per element from Philox4x32-10: the key is *seed_ptr (device int64) or
+ * seed, the counter (channel / 4, row, row >> 32, offset) with row = b T + t, and the four words are those of four
+ * neighbouring channels.  An element whose word is below round(dropout_p 2^32) is dropped, the others are divided by
+ * 1 - dropout_p.  No mask is stored; the backward needs the same seed and offset.
+ * rstd: [B T][2] fp32, written by the forward (NULL for inference) and read by the backward.
+ * kda_b200_norm_bwd takes the same inputs, dv and dn (either may be NULL = zero) and writes dx, d_o, dgate and, where
+ * not NULL, the sums over rows dw, dwb, dscale [D] fp32, in a fixed order.
+ */
+typedef struct kda_b200_norm_args {
+  int64_t B, T;
+  int32_t D, dtype, stream_dtype;
+  uint32_t offset;
+  const void *x, *o, *gate;
+  int64_t x_sb, x_st, o_sb, o_st, gate_sb, gate_st;
+  const float *w, *wb, *scale;
+  const int64_t* seed_ptr;
+  uint64_t seed;
+  double dropout_p;
+  float eps;
+  void *v, *n;
+  float* rstd;
+  /* backward */
+  const void *dv, *dn;
+  int64_t dv_sb, dv_st, dn_sb, dn_st;
+  void *dx, *d_o, *dgate;
+  float *dw, *dwb, *dscale;
+} kda_b200_norm_args;
+size_t kda_b200_norm_workspace_bytes(int64_t B, int64_t T, int D, int dtype);
+int kda_b200_norm_fwd(const kda_b200_norm_args* args, void* stream);
+int kda_b200_norm_bwd(const kda_b200_norm_args* args, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Global gradient norm over `count` tensors, and clipping:

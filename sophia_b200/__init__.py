@@ -12,6 +12,7 @@ from .integration import install  # noqa: F401
 from .packing import document_cu_seqlens  # noqa: F401
 from .ssm import selective_scan, selective_scan_step, short_conv, short_conv_step  # noqa: F401
 from .recurrence import gated_recurrence, gated_recurrence_step  # noqa: F401
+from .residual import residual_norm  # noqa: F401
 from .clip import clip_grad_norm_, grad_norm  # noqa: F401
 
 __version__ = "0.1.0"

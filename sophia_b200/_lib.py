@@ -48,6 +48,20 @@ class RecArgs(ctypes.Structure):
                 + [("pool", ctypes.c_int32)])
 
 
+class NormArgs(ctypes.Structure):
+    """``kda_b200_norm_args``."""
+
+    _fields_ = ([(n, c_int64) for n in ("B", "T")]
+                + [(n, ctypes.c_int32) for n in ("D", "dtype", "stream_dtype")] + [("offset", ctypes.c_uint32)]
+                + [(n, c_void_p) for n in ("x", "o", "gate")]
+                + [(n, c_int64) for n in ("x_sb", "x_st", "o_sb", "o_st", "gate_sb", "gate_st")]
+                + [(n, c_void_p) for n in ("w", "wb", "scale", "seed_ptr")]
+                + [("seed", ctypes.c_uint64), ("dropout_p", ctypes.c_double), ("eps", c_float)]
+                + [(n, c_void_p) for n in ("v", "n", "rstd", "dv", "dn")]
+                + [(n, c_int64) for n in ("dv_sb", "dv_st", "dn_sb", "dn_st")]
+                + [(n, c_void_p) for n in ("dx", "d_o", "dgate", "dw", "dwb", "dscale")])
+
+
 class GradArgs(ctypes.Structure):
     """``kda_b200_grad_args`` (host arrays; the types as bytes objects)."""
 
@@ -107,6 +121,9 @@ SIGNATURES = {
     "kda_b200_recurrence_fwd": ([ctypes.POINTER(RecArgs), c_void_p, c_size_t, c_void_p], c_int),
     "kda_b200_recurrence_bwd": ([ctypes.POINTER(RecArgs), c_void_p, c_size_t, c_void_p], c_int),
     "kda_b200_recurrence_step": ([ctypes.POINTER(RecArgs), c_void_p], c_int),
+    "kda_b200_norm_workspace_bytes": ([c_int64, c_int64] + [c_int] * 2, c_size_t),
+    "kda_b200_norm_fwd": ([ctypes.POINTER(NormArgs), c_void_p], c_int),
+    "kda_b200_norm_bwd": ([ctypes.POINTER(NormArgs), c_void_p, c_size_t, c_void_p], c_int),
     "kda_b200_grad_workspace_bytes": ([c_int64], c_size_t),
     "kda_b200_grad_clip": ([ctypes.POINTER(GradArgs), c_void_p, c_size_t, c_void_p], c_int),
 }

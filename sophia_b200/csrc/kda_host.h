@@ -42,7 +42,7 @@ enum KernelId {
   K_TABLE = 0, K_FWD_INTRA, K_FWD_STATE, K_BWD_STATE, K_BWD_INTRA, K_BWD_POST, K_REDUCE, K_RECURRENT,
   K_GNORM_FWD, K_GNORM_BWD, K_F32_PREP, K_F32_FWD, K_F32_BWD, K_F32_DC, K_F32_CONV, K_DOC_BOUNDS,
   K_CONV_FWD, K_CONV_BWD, K_CONV_STEP, K_SCAN_FWD, K_SCAN_BWD, K_SCAN_STEP, K_GRAD_NORM, K_GRAD_SCALE,
-  K_REC_FWD, K_REC_BWD, K_REC_STEP, K_COUNT
+  K_REC_FWD, K_REC_BWD, K_REC_STEP, K_NORM_FWD, K_NORM_BWD, K_COUNT
 };
 inline const char* const kKernelNames[K_COUNT] = {"chunk_table", "fwd_intra", "fwd_state",       "bwd_state",
                                            "bwd_intra",   "bwd_post",  "reduce",          "recurrent",
@@ -50,7 +50,8 @@ inline const char* const kKernelNames[K_COUNT] = {"chunk_table", "fwd_intra", "f
                                            "f32_bwd",     "f32_dc",    "f32_conv_bwd",    "doc_bounds",
                                            "conv_fwd",    "conv_bwd",  "conv_step",       "scan_fwd",
                                            "scan_bwd",    "scan_step", "grad_norm",       "grad_scale",
-                                           "rec_fwd",     "rec_bwd",   "rec_step"};
+                                           "rec_fwd",     "rec_bwd",   "rec_step",        "norm_fwd",
+                                           "norm_bwd"};
 
 struct Timing {
   std::mutex mu;
