@@ -22,6 +22,7 @@ int check_norm(const kda_b200_norm_args* a) {
   if (a->B < 0 || a->T < 0 || a->D < 1) return fail(KDA_ERR_INVALID, "B >= 0, T >= 0 and D >= 1 are required");
   if (a->D > RN_MAX_WIDTH) return fail(KDA_ERR_UNSUPPORTED, "more than 8192 channels");
   if (a->T > INT32_MAX) return fail(KDA_ERR_UNSUPPORTED, "too many tokens");
+  if (!aligned(a->rstd, 8)) return fail(KDA_ERR_INVALID, "rstd must be 8-byte aligned");
   if (!(a->dropout_p >= 0.0 && a->dropout_p <= 1.0)) return fail(KDA_ERR_INVALID, "dropout_p must be in [0, 1]");
   if (a->B * a->T > 0 && (!a->x || !a->o)) return fail(KDA_ERR_INVALID, "null input pointer");
   return KDA_OK;
@@ -61,9 +62,12 @@ bool norm_vec(const RnParams& p, long long B, int dtype, int stream_dtype) {
          aligned(p.dg, 16) && aligned(p.w, 16) && aligned(p.wb, 16) && aligned(p.scale, 16);
 }
 
-// One stride over all rows?
+// One stride over all rows?  And which tensors' rows lie end to end.
 void norm_flatten(RnParams& p, long long B) {
   auto flat = [&](const RowView& r) { return !r.p || B <= 1 || r.sb == (long long)p.T * r.st; };
+  const RowView* all[5] = {&p.x, &p.o, &p.g, &p.dv, &p.dn};
+  for (int i = 0; i < 5; ++i)
+    if (all[i]->st == p.D && flat(*all[i])) p.dense |= 1u << i;
   if (flat(p.x) && flat(p.o) && flat(p.g) && flat(p.dv) && flat(p.dn)) p.T = 0;
 }
 
@@ -83,9 +87,15 @@ struct Bwd {
   static int run(RnParams& p, bool vec, cudaStream_t st) { return rn_bwd<TX, TO>(p, vec, st); }
 };
 
-// CTAs of a backward call, whichever way its rows are read.
-long long norm_parts(long long rows, int D, int dtype, bool vec) {
-  return rn_bwd_grid(rows, rn_shape(D, io_size(dtype), vec, true));
+// The most CTAs that a backward call may have, whichever way its rows are read and whatever parts it has.
+long long norm_parts(long long rows, int D, int dtype) {
+  const size_t o = io_size(dtype);
+  long long most = rn_plain_ctas(rows, rn_plain_shape(D));
+  const RnShape s = rn_ring_shape(D, o);
+  for (size_t x : {o, (size_t)4})
+    for (int parts = 0; parts < 8; ++parts)
+      most = std::max(most, rn_fit(s, rows, rn_bwd_row(D, x, o, parts & 1, parts & 2, parts & 4), (size_t)3 * D * 4).ctas);
+  return most;
 }
 
 }  // namespace
@@ -95,7 +105,7 @@ extern "C" {
 size_t kda_b200_norm_workspace_bytes(int64_t B, int64_t T, int D, int dtype) {
   if (B < 0 || T < 0 || D < 1 || D > RN_MAX_WIDTH || dtype < KDA_IO_F32 || dtype > KDA_IO_F16) return 0;
   const long long rows = B * T;
-  return std::max<size_t>(16, (size_t)std::max(norm_parts(rows, D, dtype, true), norm_parts(rows, D, dtype, false)) * 3 * D * 4);
+  return std::max<size_t>(16, (size_t)norm_parts(rows, D, dtype) * 3 * D * 4);
 }
 
 int kda_b200_norm_fwd(const kda_b200_norm_args* a, void* stream) {
@@ -103,6 +113,7 @@ int kda_b200_norm_fwd(const kda_b200_norm_args* a, void* stream) {
   if (rc) return rc;
   RnParams p = norm_params(a);
   if (p.rows == 0) return KDA_OK;
+  if (!(p.err = device_error_flag())) return fail(KDA_ERR_CUDA, "the device error flag has no address");
   if (!a->v || (a->w && !a->n)) return fail(KDA_ERR_INVALID, "null output pointer");
   p.v = a->v;
   p.n = a->n;
@@ -121,6 +132,7 @@ int kda_b200_norm_bwd(const kda_b200_norm_args* a, void* workspace, size_t works
       if ((rc = zero_floats(q, a->D, st))) return rc;
     return KDA_OK;
   }
+  if (!(p.err = device_error_flag())) return fail(KDA_ERR_CUDA, "the device error flag has no address");
   p.dv = {a->dv, a->dv_sb, a->dv_st};
   if (a->w) p.dn = {a->dn, a->dn_sb, a->dn_st};
   p.dx = a->dx; p.d_o = a->d_o; p.dg = a->dgate;
@@ -136,7 +148,7 @@ int kda_b200_norm_bwd(const kda_b200_norm_args* a, void* workspace, size_t works
   {
     TimedLaunch tl(K_NORM_BWD, st);
     rn_reduce_kernel<<<dim3((a->D + RN_REDUCE_COLS - 1) / RN_REDUCE_COLS, 3), RN_REDUCE_COLS * RN_REDUCE_SLICES, 0, st>>>(
-        p.partial, (int)norm_parts(p.rows, a->D, a->dtype, vec), a->D, a->dw, a->dwb, a->dscale);
+        p.partial, p.parts, a->D, a->dw, a->dwb, a->dscale);
   }
   return launch_check("residual norm sums");
 }

@@ -9,30 +9,70 @@
 
 namespace kda {
 
-// How a row is laid over threads: `warps` of a group, k pieces of v channels a thread, groups of a CTA.
+// How a row is laid over threads: `warps` of a group (or, of one, `lanes` lanes a row), k pieces of v channels a thread,
+// `groups` of a CTA.
 struct RnShape {
-  int v, k, warps, groups;
+  int v, k, warps, groups, lanes;
 };
-// Whole pieces (16 bytes of the branch's type) wherever rows are aligned to them, else single channels.  Backward as few
-// pieces a thread as 16 warps allow: its registers hold five tensors.
-inline RnShape rn_shape(int D, size_t branch_size, bool vec, bool backward) {
-  RnShape s;
-  s.v = vec ? (int)(16 / branch_size) : 1;
-  const int pieces = (D + s.v - 1) / s.v;
-  if (vec) {
-    s.k = 1;
-    while (pieces > 32 * s.k * (backward ? RN_MAX_WARPS : 8)) s.k *= 2;
-    if (s.k > 4) s.k = 4;
-  } else {
-    s.k = pieces <= 64 * 8 ? 2 : (pieces <= 32 * 4 * RN_MAX_WARPS ? 4 : 16);
-  }
-  s.warps = (pieces + 32 * s.k - 1) / (32 * s.k);
+// Rows that are read as they lie, channel by channel.
+inline RnShape rn_plain_shape(int D) {
+  RnShape s{1, D <= 64 * 8 ? 2 : (D <= 128 * RN_MAX_WARPS ? 4 : 16), 0, 0, 32};
+  s.warps = (D + 32 * s.k - 1) / (32 * s.k);
   s.groups = std::max(1, 8 / s.warps);
   return s;
 }
-inline int rn_bwd_ctas(const RnShape& s) { return std::max(1, 24 / (s.warps * s.groups)); }  // per SM
-inline long long rn_bwd_grid(long long rows, const RnShape& s) {
-  return std::max(1LL, std::min((rows + s.groups - 1) / s.groups, (long long)rn_bwd_ctas(s) * sm_count()));
+// Rows in pieces of 16 bytes of the branch's type: 16 channels a thread, or 8 where a row has no more than 256.  Fewer
+// channels a thread mean more warps a row and more waiting for their sums: 16384 x 1536, forward, 91 us with 16 and 124
+// with 8.
+inline RnShape rn_ring_shape(int D, size_t branch_size) {
+  RnShape s;
+  s.v = (int)(16 / branch_size);
+  s.k = (D <= 256 ? 8 : 16) / s.v;
+  const int threads = (D + s.v * s.k - 1) / (s.v * s.k);
+  s.warps = (threads + 31) / 32;
+  s.groups = std::max(1, 8 / s.warps);
+  s.lanes = 1;
+  while (s.lanes < threads && s.lanes < 32) s.lanes *= 2;
+  return s;
+}
+inline long long rn_units(long long rows, int rows_a_cta) { return std::max(1LL, (rows + rows_a_cta - 1) / rows_a_cta); }
+
+// The ring: rows of a stage, stages, and the CTAs of an SM.  A stage has 4 KB at least, unless that left groups
+// without rows; two stages at least where the SM's shared memory has room for them, up to four.  No stage: the rows are
+// too wide.
+struct RnFit {
+  int batch, stages;
+  long long ctas;
+  size_t smem;
+};
+inline RnFit rn_fit(const RnShape& s, long long rows, size_t row_bytes, size_t fixed) {
+  const size_t room = 227 * 1024, own = 2048;  // own: static and reserved
+  const int per = s.warps > 1 ? 1 : 32 / s.lanes, threads = s.warps * s.groups * 32;
+  RnFit f;
+  long long sm_ctas = std::max(1, 512 / threads);  // 128 registers a thread
+  f.batch = 1;
+  while (f.batch * per * row_bytes < 4096 && rows >= 4LL * f.batch * per * s.groups * sm_ctas * sm_count()) f.batch *= 2;
+  const size_t stage = (size_t)s.groups * f.batch * per * row_bytes;
+  while (sm_ctas > 1 && sm_ctas * (2 * stage + fixed + own) > room) --sm_ctas;
+  const size_t share = room / sm_ctas;
+  f.stages = (int)std::min<size_t>(RN_MAX_STAGES, (share - std::min(share, fixed + own)) / stage);
+  f.smem = f.stages * stage + fixed;
+  f.ctas = std::min(rn_units(rows, s.groups * per * f.batch), sm_ctas * sm_count());
+  return f;
+}
+template <typename TX, typename TO>
+RnFit rn_fwd_fit(const RnParams& p, const RnShape& s) {
+  return rn_fit(s, p.rows, (size_t)p.D * (sizeof(TX) + (p.g.p ? 2 : 1) * sizeof(TO)), 0);
+}
+inline size_t rn_bwd_row(int D, size_t x, size_t o, bool g, bool dv, bool dn) {
+  return (size_t)D * (x + o + (g ? o : 0) + (dv ? x : 0) + (dn ? o : 0));
+}
+template <typename TX, typename TO>
+RnFit rn_bwd_fit(const RnParams& p, const RnShape& s) {
+  return rn_fit(s, p.rows, rn_bwd_row(p.D, sizeof(TX), sizeof(TO), p.g.p, p.dv.p, p.dn.p), (size_t)3 * p.D * 4);
+}
+inline long long rn_plain_ctas(long long rows, const RnShape& s) {
+  return std::min(rn_units(rows, s.groups), (long long)std::max(1, 24 / (s.warps * s.groups)) * sm_count());
 }
 
 template <typename TX, typename TO>
@@ -40,28 +80,59 @@ int rn_fwd(RnParams& p, bool vec, cudaStream_t st);
 template <typename TX, typename TO>
 int rn_bwd(RnParams& p, bool vec, cudaStream_t st);
 
-template <typename TX, typename TO, int V, int K>
+template <typename TX, typename TO, int K>
 int launch_rn_fwd(const RnParams& p, const RnShape& s, cudaStream_t st) {
-  const long long ctas = (p.rows + s.groups - 1) / s.groups;
   {
     TimedLaunch tl(K_NORM_FWD, st);
-    rn_fwd_kernel<TX, TO, V, K>
-        <<<(unsigned)std::min(ctas, 1LL << 20), s.warps * s.groups * 32, 0, st>>>(p);
+    rn_fwd_kernel<TX, TO, 1, K>
+        <<<(unsigned)std::min(rn_units(p.rows, s.groups), 1LL << 20), s.warps * s.groups * 32, 0, st>>>(p);
   }
   return launch_check("residual norm forward");
 }
 
-template <typename TX, typename TO, int V, int K>
-int launch_rn_bwd(const RnParams& p, const RnShape& s, cudaStream_t st) {
-  const size_t smem = (size_t)s.groups * 3 * p.D * 4;
-  auto kernel = rn_bwd_kernel<TX, TO, V, K>;
-  if (smem > 40 * 1024) {  // (48 KB go without asking, the static ones included)
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("residual norm smem: ") + cudaGetErrorString(e));
+template <typename K>
+int rn_smem(K kernel, size_t smem) {
+  if (smem <= 40 * 1024) return KDA_OK;  // (48 KB go without asking, the static ones included)
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  return e == cudaSuccess ? KDA_OK : fail(KDA_ERR_CUDA, std::string("residual norm smem: ") + cudaGetErrorString(e));
+}
+
+template <typename TX, typename TO, int K>
+int launch_rn_fwd_ring(RnParams& p, const RnShape& s, const RnFit& fit, cudaStream_t st) {
+  p.stages = fit.stages;
+  p.batch = fit.batch;
+  auto kernel = rn_fwd_ring_kernel<TX, TO, K>;
+  if (int rc = rn_smem(kernel, fit.smem)) return rc;
+  {
+    TimedLaunch tl(K_NORM_FWD, st);
+    kernel<<<(unsigned)fit.ctas, s.warps * s.groups * 32, fit.smem, st>>>(p);
   }
+  return launch_check("residual norm forward");
+}
+
+template <typename TX, typename TO, int K>
+int launch_rn_bwd_ring(RnParams& p, const RnShape& s, const RnFit& fit, cudaStream_t st) {
+  p.stages = fit.stages;
+  p.batch = fit.batch;
+  p.parts = (int)fit.ctas;
+  auto kernel = rn_bwd_ring_kernel<TX, TO, K>;
+  if (int rc = rn_smem(kernel, fit.smem)) return rc;
   {
     TimedLaunch tl(K_NORM_BWD, st);
-    kernel<<<(unsigned)rn_bwd_grid(p.rows, s), s.warps * s.groups * 32, smem, st>>>(p);
+    kernel<<<(unsigned)fit.ctas, s.warps * s.groups * 32, fit.smem, st>>>(p);
+  }
+  return launch_check("residual norm backward");
+}
+
+template <typename TX, typename TO, int K>
+int launch_rn_bwd(RnParams& p, const RnShape& s, cudaStream_t st) {
+  const size_t smem = (size_t)s.groups * 3 * p.D * 4;
+  auto kernel = rn_bwd_kernel<TX, TO, 1, K>;
+  if (int rc = rn_smem(kernel, smem)) return rc;
+  p.parts = (int)rn_plain_ctas(p.rows, s);
+  {
+    TimedLaunch tl(K_NORM_BWD, st);
+    kernel<<<(unsigned)p.parts, s.warps * s.groups * 32, smem, st>>>(p);
   }
   return launch_check("residual norm backward");
 }
