@@ -1,0 +1,3 @@
+#include "norm_fwd.cuh"
+
+template int kda::rn_fwd<float, kda::bf16>(kda::RnParams&, bool, cudaStream_t);

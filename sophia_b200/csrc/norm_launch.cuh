@@ -2,6 +2,7 @@
 #pragma once
 
 #include <algorithm>
+#include <climits>
 #include <string>
 
 #include "kda_host.h"
@@ -30,7 +31,7 @@ inline RnShape rn_ring_shape(int D, size_t branch_size) {
   s.k = (D <= 256 ? 8 : 16) / s.v;
   const int threads = (D + s.v * s.k - 1) / (s.v * s.k);
   s.warps = (threads + 31) / 32;
-  s.groups = std::max(1, 8 / s.warps);
+  s.groups = std::max(1, RN_MAX_WARPS / s.warps);
   s.lanes = 1;
   while (s.lanes < threads && s.lanes < 32) s.lanes *= 2;
   return s;
@@ -41,31 +42,33 @@ inline long long rn_units(long long rows, int rows_a_cta) { return std::max(1LL,
 // without rows; two stages at least where the SM's shared memory has room for them, up to four.  No stage: the rows are
 // too wide.
 struct RnFit {
-  int batch, stages;
+  int batch, stages, groups;
   long long ctas;
   size_t smem;
 };
 inline RnFit rn_fit(const RnShape& s, long long rows, size_t row_bytes, size_t fixed) {
-  const size_t room = 227 * 1024, own = 2048;  // own: static and reserved
-  const int per = s.warps > 1 ? 1 : 32 / s.lanes, threads = s.warps * s.groups * 32;
+  // of an SM, whose registers hold one CTA; 8 KB are static
+  const size_t room = 227 * 1024 - 8 * 1024 - fixed;
+  const int per = s.warps > 1 ? 1 : 32 / s.lanes;
   RnFit f;
-  long long sm_ctas = std::max(1, 512 / threads);  // 128 registers a thread
+  // few rows: a group to an SM before the second
+  f.groups = (int)std::max<long long>(1, std::min<long long>(s.groups, rows / ((long long)per * sm_count())));
+  while (f.groups > 1 && 2 * f.groups * per * row_bytes > room) --f.groups;
   f.batch = 1;
-  while (f.batch * per * row_bytes < 4096 && rows >= 4LL * f.batch * per * s.groups * sm_ctas * sm_count()) f.batch *= 2;
-  const size_t stage = (size_t)s.groups * f.batch * per * row_bytes;
-  while (sm_ctas > 1 && sm_ctas * (2 * stage + fixed + own) > room) --sm_ctas;
-  const size_t share = room / sm_ctas;
-  f.stages = (int)std::min<size_t>(RN_MAX_STAGES, (share - std::min(share, fixed + own)) / stage);
+  while (f.batch * per * row_bytes < 4096 && 4 * f.groups * f.batch * per * row_bytes <= room &&
+         rows >= 4LL * f.batch * per * f.groups * sm_count()) f.batch *= 2;
+  const size_t stage = (size_t)f.groups * f.batch * per * row_bytes;
+  f.stages = (int)std::min<size_t>(RN_MAX_STAGES, room / stage);
   f.smem = f.stages * stage + fixed;
-  f.ctas = std::min(rn_units(rows, s.groups * per * f.batch), sm_ctas * sm_count());
+  f.ctas = std::min<long long>(rn_units(rows, f.groups * per * f.batch), sm_count());
   return f;
+}
+inline size_t rn_bwd_row(int D, size_t x, size_t o, bool g, bool dv, bool dn) {
+  return (size_t)D * (x + o + (g ? o : 0) + (dv ? x : 0) + (dn ? o : 0));
 }
 template <typename TX, typename TO>
 RnFit rn_fwd_fit(const RnParams& p, const RnShape& s) {
   return rn_fit(s, p.rows, (size_t)p.D * (sizeof(TX) + (p.g.p ? 2 : 1) * sizeof(TO)), 0);
-}
-inline size_t rn_bwd_row(int D, size_t x, size_t o, bool g, bool dv, bool dn) {
-  return (size_t)D * (x + o + (g ? o : 0) + (dv ? x : 0) + (dn ? o : 0));
 }
 template <typename TX, typename TO>
 RnFit rn_bwd_fit(const RnParams& p, const RnShape& s) {
@@ -97,31 +100,28 @@ int rn_smem(K kernel, size_t smem) {
   return e == cudaSuccess ? KDA_OK : fail(KDA_ERR_CUDA, std::string("residual norm smem: ") + cudaGetErrorString(e));
 }
 
-template <typename TX, typename TO, int K>
-int launch_rn_fwd_ring(RnParams& p, const RnShape& s, const RnFit& fit, cudaStream_t st) {
-  p.stages = fit.stages;
-  p.batch = fit.batch;
-  auto kernel = rn_fwd_ring_kernel<TX, TO, K>;
-  if (int rc = rn_smem(kernel, fit.smem)) return rc;
-  {
-    TimedLaunch tl(K_NORM_FWD, st);
-    kernel<<<(unsigned)fit.ctas, s.warps * s.groups * 32, fit.smem, st>>>(p);
-  }
-  return launch_check("residual norm forward");
+// The ring kernel for a call's parts.
+template <template <typename, typename, bool, bool, bool, bool> class Kernel, typename TX, typename TO, bool NARROW, bool FULL>
+auto rn_pick(bool gate, bool drop) {
+  return gate ? (drop ? Kernel<TX, TO, NARROW, FULL, true, true>::get() : Kernel<TX, TO, NARROW, FULL, true, false>::get())
+              : (drop ? Kernel<TX, TO, NARROW, FULL, false, true>::get() : Kernel<TX, TO, NARROW, FULL, false, false>::get());
 }
-
-template <typename TX, typename TO, int K>
-int launch_rn_bwd_ring(RnParams& p, const RnShape& s, const RnFit& fit, cudaStream_t st) {
+template <template <typename, typename, bool, bool, bool, bool> class Kernel, typename TX, typename TO>
+int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, const char* what, cudaStream_t st) {
   p.stages = fit.stages;
   p.batch = fit.batch;
   p.parts = (int)fit.ctas;
-  auto kernel = rn_bwd_ring_kernel<TX, TO, K>;
+  p.params = (long long)(fit.smem / 4) - 3LL * p.D;
+  const bool gate = p.g.p != nullptr, full = p.D == s.warps * 32 * s.v * s.k;
+  auto kernel = p.D <= 256 ? rn_pick<Kernel, TX, TO, true, false>(gate, p.dropout)
+                : full     ? rn_pick<Kernel, TX, TO, false, true>(gate, p.dropout)
+                           : rn_pick<Kernel, TX, TO, false, false>(gate, p.dropout);
   if (int rc = rn_smem(kernel, fit.smem)) return rc;
   {
-    TimedLaunch tl(K_NORM_BWD, st);
-    kernel<<<(unsigned)fit.ctas, s.warps * s.groups * 32, fit.smem, st>>>(p);
+    TimedLaunch tl(id, st);
+    kernel<<<(unsigned)fit.ctas, s.warps * fit.groups * 32, fit.smem, st>>>(p);
   }
-  return launch_check("residual norm backward");
+  return launch_check(what);
 }
 
 template <typename TX, typename TO, int K>

@@ -43,6 +43,7 @@ struct RnParams {
   long long rows;
   int T;  // rows per batch entry, or 0 where all rows of every tensor have one stride (no division)
   int stages, batch;  // of the ring: stages, and how many times a group's rows a stage holds
+  long long params;   // floats from the ring's start to the backward's parameters
   unsigned dense;     // bit per tensor (x, o, g, dv, dn): rows lie end to end
   int D, warps, lanes;  // a row's threads: warps of a group, or (one warp) that many lanes
   int parts;  // CTAs of the backward, set by its launch
@@ -249,12 +250,15 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
 // ---------------------------------------------------------------- rows by bulk copies
 
 // Aligned rows come into a ring of stages in shared memory by bulk copies, so that the next rows are on their way
-// while one is worked on.  A group of W warps owns a row at a time (of narrow rows `lanes` lanes of a single warp, which
-// has 32 / lanes rows at once), and a stage holds enough consecutive rows for copies of a few KB: rows that lie end to
-// end are one copy (small copies cost the copy engine as much as large ones).  A thread has at most 16 channels, the same
-// in every row, in packed fp32 arithmetic; parameters (forward) and sums over rows (backward) stay in its registers.
+// while one is worked on.  A group of W warps owns a row at a time (NARROW rows, up to 256 channels: `lanes` lanes of a
+// single warp, which has 32 / lanes rows at once); rows that lie end to end are one copy (small copies cost the copy
+// engine as much as large ones), so a stage of short rows holds several.  A thread has 16 channels (NARROW 8), the same in
+// every row, in packed fp32 arithmetic; the forward's parameters and the backward's sums over rows stay in its registers.
+// What a row costs beside its arithmetic -- waiting, barriers, sums over warps, addresses -- is what bounds these
+// kernels, so the parts that a call has are known to the compiler as far as they change the loops (FULL: a row fills its
+// threads; GATE; DROP).
 constexpr int RN_MAX_STAGES = 4;
-constexpr int RN_MAX_GROUPS = 8;
+constexpr int RN_MAX_GROUPS = 16;
 
 __device__ __forceinline__ void rn_bar_init(uint64_t* bar) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(bar)) : "memory");
@@ -262,8 +266,8 @@ __device__ __forceinline__ void rn_bar_init(uint64_t* bar) {
 __device__ __forceinline__ void rn_expect(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void rn_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+__device__ __forceinline__ void rn_bulk(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
@@ -279,66 +283,223 @@ __device__ __forceinline__ bool rn_wait(uint64_t* bar, uint32_t parity) {
   return false;
 }
 
-// Where a thread stands.
-struct RnPlace {
-  int group, mine;   // its group of the CTA, its number in it
-  int per, sub, me;  // rows that a group works on at once, which of them, and its number in that row
-  int stride;        // channels between a thread's pieces
-  long long step, first;  // rows between a group's stages, and its first
+// A tensor of the ring, held by one lane of a group's first warp: the lanes issue a stage's copies side by side (one after
+// the other, with the addresses of five tensors, they held the group up for 1100 to 1800 cycles a row).
+struct RnSource {
+  const char* p;
+  long long sb, st;    // bytes
+  uint32_t row, off;   // bytes of a row, of the tensors in front of it in a stage (per row)
+  bool dense, any;     // rows lie end to end; there is such a tensor for this lane
 };
-template <int V>
-__device__ __forceinline__ RnPlace rn_place(const RnParams& P) {
-  RnPlace a;
-  const int groups = (int)(blockDim.x >> 5) / P.warps;
-  a.group = (int)(threadIdx.x >> 5) / P.warps;
-  a.mine = threadIdx.x - a.group * P.warps * 32;
-  a.per = P.warps > 1 ? 1 : 32 / P.lanes;
-  a.sub = P.warps > 1 ? 0 : a.mine / P.lanes;
-  a.me = P.warps > 1 ? a.mine : a.mine % P.lanes;
-  a.stride = (P.warps > 1 ? P.warps * 32 : P.lanes) * V;
-  const long long rows = (long long)a.per * P.batch;
-  a.step = (long long)gridDim.x * groups * rows;
-  a.first = ((long long)blockIdx.x * groups + a.group) * rows;
-  return a;
+__device__ __forceinline__ RnSource rn_source(const RowView& r, uint32_t esz, uint32_t off, bool dense, int D) {
+  return {static_cast<const char*>(r.p), r.sb * (long long)esz, r.st * (long long)esz, D * esz, off, dense, r.p != nullptr};
 }
-
-// n rows of a tensor from row0 on to `dst`; `dense`: they lie end to end.  (Called by the first warp of a group.)
-template <typename T>
-__device__ __forceinline__ void rn_fetch(char* dst, const RowView& r, bool dense, long long row0, int n, const RnParams& P,
-                                         uint64_t* bar) {
-  const int lane = threadIdx.x & 31;
-  const uint32_t bytes = P.D * (uint32_t)sizeof(T);
-  if (dense) {
-    if (lane == 0) rn_bulk(dst, rn_row<T>(r, row0, P.T), n * bytes, bar);
+// n rows from row0 on to the stage at `at`, which has room for `rows`.
+__device__ __forceinline__ void rn_copy(const RnSource& t, uint32_t at, int rows, long long row0, int n, int T, uint64_t* bar) {
+  const uint32_t dst = at + rows * t.off;
+  auto src = [&](long long row) {
+    if (T == 0) return t.p + row * t.st;
+    const long long b = row / T;
+    return t.p + b * t.sb + (row - b * T) * t.st;
+  };
+  if (!t.any) return;
+  if (t.dense) {
+    rn_bulk(dst, src(row0), n * t.row, bar);
   } else {
-    for (int i = lane; i < n; i += 32) rn_bulk(dst + (size_t)i * bytes, rn_row<T>(r, row0 + i, P.T), bytes, bar);
+    for (int i = 0; i < n; ++i) rn_bulk(dst + i * t.row, src(row0 + i), t.row, bar);
   }
 }
-// The sum over a row's threads: `lanes` of a warp, or `warps` warps.
-__device__ __forceinline__ float rn_total(float a, float (*part)[RN_MAX_WARPS], int slot, int group, const RnParams& P) {
-  if (P.warps > 1) return rn_sum(a, part, slot, group, P.warps);
-  for (int m = P.lanes >> 1; m >= 1; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
-  return a;
-}
+// What a CTA shares: the sums' places (two for each group: a sum's may be written while the last one is read) and the
+// stages' arrivals.
+template <int N>
+struct RnShared {
+  float part[2][RN_MAX_GROUPS][N][RN_MAX_WARPS];
+  uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES];
+};
 
-// V channels as pairs.
+// A group's walk through its rows: where it and its thread stand, and its stages.
+template <typename T, bool NARROW, int N>
+struct RnGroup {
+  int group, warps, lanes;
+  int per, sub, me;   // rows that it works on at once, which of them, and the thread's number in that row
+  int stride;         // channels between a thread's pieces
+  int rows, batch;    // of a stage: rows, and how often `per`
+  int first, step;    // its first row, and the rows between its stages
+  int total;          // rows of the call
+  bool leads, alive;  // the first warp; no wait has run out
+  uint32_t base, stage_bytes, row_bytes;
+  uint64_t* full;
+  float (*part)[RN_MAX_GROUPS][N][RN_MAX_WARPS];
+  int slot, turn, stages, flip;
+  int refill, spare;  // the first row of the stage to be filled again once everyone has read it (or total), and that stage
+  int T_;
+  RnSource mine;
+
+  __device__ __forceinline__ RnGroup(const RnParams& P, RnShared<N>& sh, uint32_t ring, uint32_t bytes_a_row) {
+    constexpr int V = 16 / sizeof(T);
+    warps = NARROW ? 1 : P.warps;
+    lanes = P.lanes;
+    const int groups = (int)(blockDim.x >> 5) / warps;
+    group = (int)(threadIdx.x >> 5) / warps;
+    const int in = threadIdx.x - group * warps * 32;
+    per = NARROW ? 32 / lanes : 1;
+    sub = NARROW ? in / lanes : 0;
+    me = NARROW ? in % lanes : in;
+    stride = (NARROW ? lanes : warps * 32) * V;
+    batch = P.batch;
+    rows = per * batch;
+    total = (int)P.rows;
+    first = ((int)blockIdx.x * groups + group) * rows;
+    step = (int)gridDim.x * groups * rows;
+    leads = in < 32;
+    alive = true;
+    row_bytes = bytes_a_row;
+    stage_bytes = rows * row_bytes;
+    stages = P.stages;
+    base = ring + group * stages * stage_bytes;
+    full = sh.full[group];
+    part = sh.part;
+    slot = turn = flip = spare = 0;
+    refill = total;
+    T_ = P.T;
+    mine = RnSource{};
+    if (in == 0)
+      for (int q = 0; q < stages; ++q) rn_bar_init(&full[q]);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int i = threadIdx.x; i < 2 * RN_MAX_GROUPS * N * RN_MAX_WARPS; i += blockDim.x) (&sh.part[0][0][0][0])[i] = 0.f;
+  }
+  __device__ __forceinline__ void sync() const {
+    if (warps == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
+  }
+  __device__ __forceinline__ void fetch(int row0, int s) {  // (the first warp)
+    if (row0 >= total || !alive) return;
+    const int n = min(rows, total - row0);
+    if ((threadIdx.x & 31) == 0) rn_expect(&full[s], n * row_bytes);
+    rn_copy(mine, base + s * stage_bytes, rows, row0, n, T_, &full[s]);
+  }
+  __device__ __forceinline__ void start() {
+    if (leads)
+      for (int q = 0; q < stages; ++q)
+        if (first + (long long)q * step < total) fetch(first + q * step, q);
+  }
+  // Behind a barrier of the group in a row, everyone has read the stage before the row's own.
+  __device__ __forceinline__ void again() {
+    if (leads && refill < total) fetch(refill, spare);
+    refill = total;
+  }
+  __device__ __forceinline__ void wait() {
+    if (alive) alive = rn_wait(&full[slot], turn);
+  }
+  __device__ __forceinline__ void next(int row0) {
+    spare = slot;
+    refill = (long long)row0 + (long long)stages * step < total ? row0 + stages * step : total;
+    if (stages == 1) {  // nothing on its way meanwhile
+      sync();
+      again();
+    }
+    if (++slot == stages) slot = 0, turn ^= 1;
+  }
+  __device__ __forceinline__ void finish(int* err) {
+    if (alive) return;  // a copy did not arrive: report it, and let what is in flight land (waiting again, as long)
+    atomicExch(err, 12);
+    if (leads)
+      for (int q = 0; q < stages; ++q) rn_wait(&full[q], q < slot ? turn ^ 1 : turn);
+  }
+  // The sums over a row's threads, the same in all of them.
+  __device__ __forceinline__ void sum(float (&a)[N]) {
+    if (NARROW) {
+      for (int m = lanes >> 1; m >= 1; m >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], m);
+      __syncwarp();
+    } else {
+#pragma unroll
+      for (int m = 16; m >= 1; m >>= 1)
+#pragma unroll
+        for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], m);
+      if (warps > 1) {
+        float (*p)[RN_MAX_WARPS] = part[flip][group];
+        flip ^= 1;
+        if ((threadIdx.x & 31) == 0)
+#pragma unroll
+          for (int i = 0; i < N; ++i) p[i][(threadIdx.x >> 5) - group * warps] = a[i];
+        sync();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float4* q = reinterpret_cast<const float4*>(p[i]);
+          float4 f = q[0];
+          float t = (f.x + f.y) + (f.z + f.w);
+          for (int w = 4; w < warps; w += 4) {
+            f = q[w / 4];
+            t += (f.x + f.y) + (f.z + f.w);
+          }
+          a[i] = t;
+        }
+      } else {
+        __syncwarp();
+      }
+    }
+    again();
+  }
+};
+
+// V channels as pairs, from and to pieces of 16 bytes.
+__device__ __forceinline__ u64 rn_pair(bf16, uint32_t u) { return pk2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)); }
+__device__ __forceinline__ u64 rn_pair(f16, uint32_t u) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u));
+  return pk2(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t rn_word(bf16, u64 v) {
+  const float2 f = upk2(v);
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t rn_word(f16, u64 v) {
+  const float2 f = upk2(v);
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
 template <typename T, int V>
 __device__ __forceinline__ void rn_get(const T* q, u64 (&f)[V / 2]) {
-  RnVec<T, V> v;
-  v.load(q);
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) f[i] = pk2(v.get(2 * i), v.get(2 * i + 1));
+    for (int i = 0; i < V / 4; ++i) {
+      const ulonglong2 r = reinterpret_cast<const ulonglong2*>(q)[i];
+      f[2 * i] = r.x;
+      f[2 * i + 1] = r.y;
+    }
+  } else {
+    static_assert(V == 8, "16-bit rows go in pieces of eight channels");
+    const uint4 r = *reinterpret_cast<const uint4*>(q);
+    f[0] = rn_pair(T(), r.x);
+    f[1] = rn_pair(T(), r.y);
+    f[2] = rn_pair(T(), r.z);
+    f[3] = rn_pair(T(), r.w);
+  }
+}
+// The same from shared memory.
+template <typename T, int V>
+__device__ __forceinline__ void rn_take(uint32_t at, u64 (&f)[V / 2]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(f[2 * i]), "=l"(f[2 * i + 1]) : "r"(at + 16 * i));
+  } else {
+    uint32_t r[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = rn_pair(T(), r[i]);
+  }
 }
 template <typename T, int V>
 __device__ __forceinline__ void rn_put(T* q, const u64 (&f)[V / 2]) {
-  float o[V];
+  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-  for (int i = 0; i < V / 2; ++i) {
-    const float2 t = upk2(f[i]);
-    o[2 * i] = t.x;
-    o[2 * i + 1] = t.y;
+    for (int i = 0; i < V / 4; ++i) reinterpret_cast<ulonglong2*>(q)[i] = make_ulonglong2(f[2 * i], f[2 * i + 1]);
+  } else {
+    *reinterpret_cast<uint4*>(q) = make_uint4(rn_word(T(), f[0]), rn_word(T(), f[1]), rn_word(T(), f[2]), rn_word(T(), f[3]));
   }
-  rn_store<T, V>(q, o);
 }
 __device__ __forceinline__ u64 rn_all(float v) { return pk2(v, v); }
 __device__ __forceinline__ u64 rn_neg1_plus(u64 v) { return fma2(v, rn_all(-1.f), rn_all(1.f)); }  // 1 - v
@@ -368,360 +529,320 @@ __device__ __forceinline__ u64 rn_mask(u64 v, unsigned bits, int pair) {
   return pk2(bits >> (2 * pair) & 1 ? t.x : 0.f, bits >> (2 * pair + 1) & 1 ? t.y : 0.f);
 }
 
-template <typename TX, typename TO, int K>
-__global__ void __launch_bounds__(512, 1) rn_fwd_ring_kernel(const __grid_constant__ RnParams P) {
-  constexpr int V = 16 / sizeof(TO), H = V / 2;
+
+template <typename TX, typename TO, bool NARROW, bool FULL, bool GATE, bool DROP>
+__global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const __grid_constant__ RnParams P) {
+  constexpr int V = 16 / sizeof(TO), H = V / 2, K = (NARROW ? 8 : 16) / V;
   extern __shared__ __align__(128) char ring[];
-  __shared__ float part[2][RN_MAX_WARPS];
-  __shared__ uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES];
-  const RnPlace a = rn_place<V>(P);
-  const int rows = a.per * P.batch;
-  const uint32_t xb = P.D * sizeof(TX), ob = P.D * sizeof(TO), row_bytes = xb + (P.g.p ? 2 : 1) * ob;
-  char* stages = ring + (size_t)a.group * P.stages * rows * row_bytes;
-  const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
-  const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
-  const float inv = 1.f / P.D;
-  if (a.mine == 0) {
-    for (int q = 0; q < P.stages; ++q) rn_bar_init(&full[a.group][q]);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  __shared__ __align__(16) RnShared<1> sh;
+  const int D = P.D;
+  const uint32_t xb = D * sizeof(TX), ob = D * sizeof(TO);
+  RnGroup<TO, NARROW, 1> a(P, sh, smem_u32(ring), xb + (GATE ? 2 : 1) * ob);
+  {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) a.mine = rn_source(P.x, sizeof(TX), 0, P.dense & 1, D);
+    if (lane == 1) a.mine = rn_source(P.o, sizeof(TO), xb, P.dense >> 1 & 1, D);
+    if (GATE && lane == 2) a.mine = rn_source(P.g, sizeof(TO), xb + ob, P.dense >> 2 & 1, D);
   }
   __syncthreads();
-
-  bool alive = true;
-  auto fetch = [&](long long row0, int s) {
-    if (row0 >= P.rows || a.mine >= 32 || !alive) return;
-    const int n = (int)min((long long)rows, P.rows - row0);
-    uint64_t* bar = &full[a.group][s];
-    char* d = stages + (size_t)s * rows * row_bytes;
-    if (a.mine == 0) rn_expect(bar, n * row_bytes);
-    rn_fetch<TX>(d, P.x, P.dense & 1, row0, n, P, bar);
-    rn_fetch<TO>(d + (size_t)rows * xb, P.o, P.dense >> 1 & 1, row0, n, P, bar);
-    if (P.g.p) rn_fetch<TO>(d + (size_t)rows * (xb + ob), P.g, P.dense >> 2 & 1, row0, n, P, bar);
-  };
-  for (int q = 0; q < P.stages; ++q) fetch(a.first + q * a.step, q);
-
+  a.start();
+  const bool has_w = P.w != nullptr, has_wb = P.wb != nullptr, scaled = P.scale || DROP, keeps = P.rstd && a.me == 0;
+  unsigned long long seed = 0;
+  if (DROP) seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
+  const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+  const float inv = 1.f / D, eps = P.eps;
+  bool mine[K];  // the thread's pieces that there are
   u64 w[K][H], wb[K][H], sc[K][H];  // the scale with 1 / (1 - p) in it
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = a.me * V + k * a.stride;
-    const u64 keep = rn_all(P.dropout ? P.keep_scale : 1.f);
+    mine[k] = FULL || c < D;
+    const u64 keep = rn_all(DROP ? P.keep_scale : 1.f);
 #pragma unroll
     for (int i = 0; i < H; ++i) w[k][i] = wb[k][i] = sc[k][i] = 0ull;
-    if (c < P.D) {
-      if (P.w) rn_get<float, V>(P.w + c, w[k]);
-      if (P.wb) rn_get<float, V>(P.wb + c, wb[k]);
+    if (mine[k]) {
+      if (has_w) rn_get<float, V>(P.w + c, w[k]);
+      if (has_wb) rn_get<float, V>(P.wb + c, wb[k]);
       if (P.scale) rn_get<float, V>(P.scale + c, sc[k]);
     }
 #pragma unroll
     for (int i = 0; i < H; ++i) sc[k][i] = P.scale ? mul2(sc[k][i], keep) : keep;
   }
-  const bool scaled = P.scale || P.dropout;
-  int s = 0, turn = 0;
-  for (long long row0 = a.first; row0 < P.rows; row0 += a.step) {
-    if (alive) alive = rn_wait(&full[a.group][s], turn);
-    const char* d = stages + (size_t)s * rows * row_bytes;
-    for (int j = 0; j < P.batch; ++j) {
-      const int at = j * a.per + a.sub;
-      const long long row = row0 + at;
-      if (row0 + j * a.per >= P.rows) break;  // (the whole group at once)
-      const bool here = row < P.rows;
-      const TX* px = reinterpret_cast<const TX*>(d) + (size_t)at * P.D;
-      const TO* po = reinterpret_cast<const TO*>(d + (size_t)rows * xb) + (size_t)at * P.D;
-      const TO* pg = reinterpret_cast<const TO*>(d + (size_t)rows * (xb + ob)) + (size_t)at * P.D;
+  const uint32_t at_x = a.sub * xb + a.me * (V * (uint32_t)sizeof(TX)), at_o = a.rows * xb + a.sub * ob + a.me * 16;
+  const uint32_t kx = a.stride * (uint32_t)sizeof(TX), ko = a.stride * (uint32_t)sizeof(TO), at_g = a.rows * ob;
+  for (int row0 = a.first; row0 < a.total; row0 += a.step) {
+    a.wait();
+    uint32_t px = a.base + a.slot * a.stage_bytes + at_x, po = a.base + a.slot * a.stage_bytes + at_o;
+    int row = row0 + a.sub;
+    for (int j = 0; j < a.batch && row - a.sub < a.total; ++j, row += a.per, px += a.per * xb, po += a.per * ob) {
+      const bool here = !NARROW || row < a.total;
+      const long long out = (long long)row * D + a.me * V;
       u64 v[K][H], ss = 0ull;
-      float rb = 1.f;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = a.me * V + k * a.stride;
+        if (mine[k] && here) rn_take<TO, V>(po + k * ko, v[k]);
+        else
 #pragma unroll
-        for (int i = 0; i < H; ++i) v[k][i] = 0ull;
-        if (c < P.D && here) {
-          rn_get<TO, V>(po + c, v[k]);
+          for (int i = 0; i < H; ++i) v[k][i] = 0ull;
+      }
+      float rb = 1.f, t[1];
+      if (has_wb) {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < H; ++i) ss = fma2(v[k][i], v[k][i], ss);
-        }
-      }
-      if (P.wb) {
-        rb = rsqrtf(fmaf(rn_total(rn_hsum(ss), part, 0, a.group, P), inv, P.eps));
+        t[0] = rn_hsum(ss);
+        a.sum(t);
+        rb = rsqrtf(fmaf(t[0], inv, eps));
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
           for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(wb[k][i], rn_all(rb)));
+        ss = 0ull;
       }
-      ss = 0ull;
-      TX* pv = static_cast<TX*>(P.v) + row * P.D;
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = a.me * V + k * a.stride;
-        if (c < P.D && here) {
+      for (int k = 0; k < K; ++k)
+        if (mine[k] && here) {
           u64 f[H];
-          if (P.g.p) {
-            rn_get<TO, V>(pg + c, f);
+          if (GATE) {
+            rn_take<TO, V>(po + at_g + k * ko, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], rn_sigmoid(f[i]));
           }
           if (scaled)
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], sc[k][i]);
-          if (P.dropout) {
-            const unsigned bits = rn_bits<V>(P, k0, k1, row, c);
+          if (DROP) {
+            const unsigned bits = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = rn_mask(v[k][i], bits, i);
           }
-          rn_get<TX, V>(px + c, f);
+          rn_take<TX, V>(px + k * kx, f);
 #pragma unroll
           for (int i = 0; i < H; ++i) {
             v[k][i] = add2(v[k][i], f[i]);
             ss = fma2(v[k][i], v[k][i], ss);
           }
-          rn_put<TX, V>(pv + c, v[k]);
+          rn_put<TX, V>(static_cast<TX*>(P.v) + out + k * a.stride, v[k]);
         }
-      }
       float r = 0.f;
-      if (P.w) {
-        r = rsqrtf(fmaf(rn_total(rn_hsum(ss), part, 1, a.group, P), inv, P.eps));
-        TO* pn = static_cast<TO*>(P.n) + row * P.D;
+      if (has_w) {
+        t[0] = rn_hsum(ss);
+        a.sum(t);
+        r = rsqrtf(fmaf(t[0], inv, eps));
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int c = a.me * V + k * a.stride;
-          if (c < P.D && here) {
+        for (int k = 0; k < K; ++k)
+          if (mine[k] && here) {
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(w[k][i], rn_all(r)));
-            rn_put<TO, V>(pn + c, v[k]);
+            rn_put<TO, V>(static_cast<TO*>(P.n) + out + k * a.stride, v[k]);
           }
-        }
       }
-      if (P.rstd && a.me == 0 && here) *reinterpret_cast<float2*>(P.rstd + 2 * row) = make_float2(rb, r);
-      // everyone has read the row (two sums: the second one's barrier says so, and keeps their slots apart)
-      if (P.warps == 1) __syncwarp();
-      else if (!P.w || !P.wb) asm volatile("bar.sync %0, %1;" ::"r"(a.group + 1), "r"(P.warps * 32) : "memory");
+      if (keeps && here) *reinterpret_cast<float2*>(P.rstd + 2LL * row) = make_float2(rb, r);
+      if (!has_w && !has_wb) {
+        a.sync();
+        a.again();
+      }
     }
-    fetch(row0 + P.stages * a.step, s);
-    if (++s == P.stages) s = 0, turn ^= 1;
+    a.next(row0);
   }
-  if (!alive) {  // a copy did not arrive: report it, and let what is in flight land (waiting again, as long)
-    atomicExch(P.err, 12);
-    if (a.mine == 0)
-      for (int q = 0; q < P.stages; ++q) rn_wait(&full[a.group][q], q < s ? turn ^ 1 : turn);
-  }
+  a.finish(P.err);
 }
 
-template <typename TX, typename TO, int K>
-__global__ void __launch_bounds__(512, 1) rn_bwd_ring_kernel(const __grid_constant__ RnParams P) {
-  constexpr int V = 16 / sizeof(TO), H = V / 2;
-  extern __shared__ __align__(128) char ring[];  // the parameters [3][D], then the groups' stages
-  __shared__ float part[2][RN_MAX_WARPS];
-  __shared__ uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES];
-  const RnPlace a = rn_place<V>(P);
-  const int rows = a.per * P.batch;
-  const bool has_g = P.g.p != nullptr, has_dv = P.dv.p != nullptr, has_dn = P.dn.p != nullptr;
-  const uint32_t xb = P.D * sizeof(TX), ob = P.D * sizeof(TO);
-  const uint32_t off_o = xb, off_g = off_o + ob, off_dv = off_g + (has_g ? ob : 0), off_dn = off_dv + (has_dv ? xb : 0);
-  const uint32_t row_bytes = off_dn + (has_dn ? ob : 0);
-  float* params = reinterpret_cast<float*>(ring);
-  char* stages = ring + (size_t)3 * P.D * 4 + (size_t)a.group * P.stages * rows * row_bytes;
-  const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
-  const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
-  const float inv = 1.f / P.D;
-  if (a.mine == 0) {
-    for (int q = 0; q < P.stages; ++q) rn_bar_init(&full[a.group][q]);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+// One round of sums a row: with t = scale m s u (what the stream got from the branch), the sum that the branch's norm
+// needs is that of t dv', and dv' = dv + r (tw - v r^2 S1 / D) with tw = dn w, S1 = sum tw v: sum t dv' =
+// sum t (dv + r tw) - r^3 S1 / D sum t v, and do = r_b (du w_b - o r_b / D sum t dv').
+template <typename TX, typename TO, bool NARROW, bool FULL, bool GATE, bool DROP>
+__global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const __grid_constant__ RnParams P) {
+  constexpr int V = 16 / sizeof(TO), H = V / 2, K = (NARROW ? 8 : 16) / V;
+  extern __shared__ __align__(128) char ring[];  // the groups' stages, then the parameters [3][D], at the end the sums
+  __shared__ __align__(16) RnShared<3> sh;
+  const int D = P.D;
+  const bool has_dv = P.dv.p != nullptr, has_dn = P.dn.p != nullptr, has_wb = P.wb != nullptr, has_scale = P.scale != nullptr;
+  const uint32_t xb = D * sizeof(TX), ob = D * sizeof(TO);
+  const uint32_t off_g = xb + ob, off_dv = off_g + (GATE ? ob : 0), off_dn = off_dv + (has_dv ? xb : 0);
+  RnGroup<TO, NARROW, 3> a(P, sh, smem_u32(ring), off_dn + (has_dn ? ob : 0));
+  {
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) a.mine = rn_source(P.x, sizeof(TX), 0, P.dense & 1, D);
+    if (lane == 1) a.mine = rn_source(P.o, sizeof(TO), xb, P.dense >> 1 & 1, D);
+    if (GATE && lane == 2) a.mine = rn_source(P.g, sizeof(TO), off_g, P.dense >> 2 & 1, D);
+    if (lane == 3) a.mine = rn_source(P.dv, sizeof(TX), off_dv, P.dense >> 3 & 1, D);
+    if (lane == 4) a.mine = rn_source(P.dn, sizeof(TO), off_dn, P.dense >> 4 & 1, D);
   }
-  for (int i = threadIdx.x; i < P.D; i += blockDim.x) {
+  float* params = reinterpret_cast<float*>(ring) + P.params;
+  for (int i = threadIdx.x; i < D; i += blockDim.x) {  // what a part that is left out multiplies with: 1
     params[i] = P.w ? P.w[i] : 0.f;
-    params[P.D + i] = P.wb ? P.wb[i] : 1.f;
-    params[2 * P.D + i] = (P.scale ? P.scale[i] : 1.f) * (P.dropout ? P.keep_scale : 1.f);
+    params[D + i] = has_wb ? P.wb[i] : 1.f;
+    params[2 * D + i] = (has_scale ? P.scale[i] : 1.f) * (DROP ? P.keep_scale : 1.f);
   }
   __syncthreads();
-
-  bool alive = true;
-  auto fetch = [&](long long row0, int s) {
-    if (row0 >= P.rows || a.mine >= 32 || !alive) return;
-    const int n = (int)min((long long)rows, P.rows - row0);
-    uint64_t* bar = &full[a.group][s];
-    char* d = stages + (size_t)s * rows * row_bytes;
-    if (a.mine == 0) rn_expect(bar, n * row_bytes);
-    rn_fetch<TX>(d, P.x, P.dense & 1, row0, n, P, bar);
-    rn_fetch<TO>(d + (size_t)rows * off_o, P.o, P.dense >> 1 & 1, row0, n, P, bar);
-    if (has_g) rn_fetch<TO>(d + (size_t)rows * off_g, P.g, P.dense >> 2 & 1, row0, n, P, bar);
-    if (has_dv) rn_fetch<TX>(d + (size_t)rows * off_dv, P.dv, P.dense >> 3 & 1, row0, n, P, bar);
-    if (has_dn) rn_fetch<TO>(d + (size_t)rows * off_dn, P.dn, P.dense >> 4 & 1, row0, n, P, bar);
-  };
-  for (int q = 0; q < P.stages; ++q) fetch(a.first + q * a.step, q);
-
+  a.start();
+  unsigned long long seed = 0;
+  if (DROP) seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
+  const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
+  const float inv = 1.f / D, keep = DROP ? P.keep_scale : 1.f;
+  bool mine[K];
   u64 sw[K][H], sb[K][H], ssc[K][H];  // sums over this thread's rows
 #pragma unroll
-  for (int k = 0; k < K; ++k)
+  for (int k = 0; k < K; ++k) {
+    mine[k] = FULL || a.me * V + k * a.stride < D;
 #pragma unroll
     for (int i = 0; i < H; ++i) sw[k][i] = sb[k][i] = ssc[k][i] = 0ull;
-  const float keep = P.dropout ? P.keep_scale : 1.f;
-  int s = 0, turn = 0;
-  for (long long row0 = a.first; row0 < P.rows; row0 += a.step) {
-    if (alive) alive = rn_wait(&full[a.group][s], turn);
-    const char* d = stages + (size_t)s * rows * row_bytes;
-    for (int j = 0; j < P.batch; ++j) {
-      const int at = j * a.per + a.sub;
-      const long long row = row0 + at;
-      if (row0 + j * a.per >= P.rows) break;
-      const bool here = row < P.rows;
-      const TX* px = reinterpret_cast<const TX*>(d) + (size_t)at * P.D;
-      const TO* po = reinterpret_cast<const TO*>(d + (size_t)rows * off_o) + (size_t)at * P.D;
-      const TO* pg = reinterpret_cast<const TO*>(d + (size_t)rows * off_g) + (size_t)at * P.D;
-      const TX* pdv = reinterpret_cast<const TX*>(d + (size_t)rows * off_dv) + (size_t)at * P.D;
-      const TO* pdn = reinterpret_cast<const TO*>(d + (size_t)rows * off_dn) + (size_t)at * P.D;
-      const float2 roots = here ? *reinterpret_cast<const float2*>(P.rstd + 2 * row) : make_float2(0.f, 0.f);
-      const float rb = roots.x, r = roots.y;
-      // the stream again, and the next norm's sum of t v
-      u64 v[K][H], dot = 0ull;
+  }
+  const uint32_t at_x = a.sub * xb + a.me * (V * (uint32_t)sizeof(TX)), at_o = a.rows * xb + a.sub * ob + a.me * 16;
+  const uint32_t to_dv = a.rows * off_dv, to_g = a.rows * (off_g - xb), to_dn = a.rows * (off_dn - xb);
+  const uint32_t kx = a.stride * (uint32_t)sizeof(TX), ko = a.stride * (uint32_t)sizeof(TO), kp = a.stride * 4;
+  const uint32_t pw = smem_u32(params) + a.me * V * 4, pwb = pw + 4 * D, psc = pwb + 4 * D;
+  auto roots_of = [&](int row) {
+    return row < a.total ? __ldg(reinterpret_cast<const float2*>(P.rstd + 2LL * row)) : make_float2(0.f, 0.f);
+  };
+  float2 ahead = roots_of(min(a.first, a.total) + a.sub);  // of the row to come
+  for (int row0 = a.first; row0 < a.total; row0 += a.step) {
+    a.wait();
+    uint32_t px = a.base + a.slot * a.stage_bytes + at_x, po = a.base + a.slot * a.stage_bytes + at_o;
+    int row = row0 + a.sub;
+    for (int j = 0; j < a.batch && row - a.sub < a.total; ++j, row += a.per, px += a.per * xb, po += a.per * ob) {
+      const bool here = !NARROW || row < a.total;
+      const long long out = (long long)row * D + a.me * V;
+      const float rb = ahead.x, r = ahead.y;
+      ahead = roots_of(j + 1 < a.batch ? row + a.per : (int)min((long long)row0 + a.step, (long long)a.total) + a.sub);
+      u64 v[K][H], s1 = 0ull, s2 = 0ull, s3 = 0ull;
       unsigned bits[K];
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = a.me * V + k * a.stride;
         bits[k] = 0xffffffffu;
 #pragma unroll
         for (int i = 0; i < H; ++i) v[k][i] = 0ull;
-        if (c < P.D && here) {
-          u64 f[H];
-          if (P.dropout) bits[k] = rn_bits<V>(P, k0, k1, row, c);
+        if (mine[k] && here) {
+          u64 f[H], t[H];
+          rn_take<TO, V>(po + k * ko, t);
+          rn_take<float, V>(pwb + k * kp, f);
+#pragma unroll
+          for (int i = 0; i < H; ++i) t[i] = mul2(t[i], mul2(f[i], rn_all(rb)));
+          if (GATE) {
+            rn_take<TO, V>(po + to_g + k * ko, f);
+#pragma unroll
+            for (int i = 0; i < H; ++i) t[i] = mul2(t[i], rn_sigmoid(f[i]));
+          }
+          rn_take<float, V>(psc + k * kp, f);
+#pragma unroll
+          for (int i = 0; i < H; ++i) t[i] = mul2(t[i], f[i]);
+          if (DROP) {
+            bits[k] = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
+#pragma unroll
+            for (int i = 0; i < H; ++i) t[i] = rn_mask(t[i], bits[k], i);
+          }
+          rn_take<TX, V>(px + k * kx, f);
+#pragma unroll
+          for (int i = 0; i < H; ++i) v[k][i] = add2(f[i], t[i]);
           if (has_dn) {
-            rn_get<TO, V>(po + c, v[k]);
-            rn_get<float, V>(params + P.D + c, f);
+            u64 q[H];
+            rn_take<TO, V>(po + to_dn + k * ko, q);
+            rn_take<float, V>(pw + k * kp, f);
 #pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(f[i], rn_all(rb)));
-            if (has_g) {
-              rn_get<TO, V>(pg + c, f);
-#pragma unroll
-              for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], rn_sigmoid(f[i]));
+            for (int i = 0; i < H; ++i) {
+              q[i] = mul2(q[i], f[i]);
+              s1 = fma2(q[i], v[k][i], s1);
+              s2 = fma2(t[i], mul2(q[i], rn_all(r)), s2);
+              s3 = fma2(t[i], v[k][i], s3);
             }
-            rn_get<float, V>(params + 2 * P.D + c, f);
+          }
+          if (has_dv) {
+            rn_take<TX, V>(px + to_dv + k * kx, f);
 #pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], f[i]);
-            if (P.dropout)
-#pragma unroll
-              for (int i = 0; i < H; ++i) v[k][i] = rn_mask(v[k][i], bits[k], i);
-            rn_get<TX, V>(px + c, f);
-#pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = add2(v[k][i], f[i]);
-            u64 t[H];
-            rn_get<TO, V>(pdn + c, t);
-            rn_get<float, V>(params + c, f);
-#pragma unroll
-            for (int i = 0; i < H; ++i) dot = fma2(mul2(t[i], f[i]), v[k][i], dot);
+            for (int i = 0; i < H; ++i) s2 = fma2(t[i], f[i], s2);
           }
         }
       }
-      float mean = 0.f;
-      if (has_dn) mean = rn_total(rn_hsum(dot), part, 0, a.group, P) * inv * r * r;
-      dot = 0ull;
-      TX* pdx = static_cast<TX*>(P.dx) + row * P.D;
-      TO* pdg = static_cast<TO*>(P.dg) + row * P.D;
-      TO* pdo = static_cast<TO*>(P.d_o) + row * P.D;
+      float t[3] = {rn_hsum(s1), rn_hsum(s2), rn_hsum(s3)};
+      a.sum(t);
+      const float mean = t[0] * inv * r * r;                                 // of tw v, times r^2
+      const float back = has_wb ? (t[1] - r * mean * t[2]) * inv * rb : 0.f;  // of t dv', times r_b
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = a.me * V + k * a.stride;
-        if (c < P.D && here) {
-          u64 g[H], f[H], t[H];  // g: gradient of the stream
+      for (int k = 0; k < K; ++k)
+        if (mine[k] && here) {
+          u64 g[H], f[H], q[H], u[H], sg[H];  // g: gradient of the stream, then of less and less of the branch
+#pragma unroll
+          for (int i = 0; i < H; ++i) g[i] = 0ull;
           if (has_dn) {
-            rn_get<TO, V>(pdn + c, t);
-            rn_get<float, V>(params + c, f);
+            rn_take<TO, V>(po + to_dn + k * ko, q);
+            rn_take<float, V>(pw + k * kp, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) {
-              g[i] = mul2(rn_all(r), fma2(v[k][i], rn_all(-mean), mul2(f[i], t[i])));
-              sw[k][i] = fma2(mul2(t[i], v[k][i]), rn_all(r), sw[k][i]);
+              g[i] = mul2(rn_all(r), fma2(v[k][i], rn_all(-mean), mul2(f[i], q[i])));
+              sw[k][i] = fma2(mul2(q[i], v[k][i]), rn_all(r), sw[k][i]);
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < H; ++i) g[i] = 0ull;
           }
           if (has_dv) {
-            rn_get<TX, V>(pdv + c, f);
+            rn_take<TX, V>(px + to_dv + k * kx, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) g[i] = add2(g[i], f[i]);
           }
-          rn_put<TX, V>(pdx + c, g);
-          if (P.dropout)
+          rn_put<TX, V>(static_cast<TX*>(P.dx) + out + k * a.stride, g);
+          if (DROP)
 #pragma unroll
             for (int i = 0; i < H; ++i) g[i] = rn_mask(g[i], bits[k], i);
-          u64 u[H], sg[H];
-          rn_get<TO, V>(po + c, u);
-          rn_get<float, V>(params + P.D + c, f);
-          if (has_g) rn_get<TO, V>(pg + c, sg);
-          rn_get<float, V>(params + 2 * P.D + c, t);
+          rn_take<TO, V>(po + k * ko, u);
+          rn_take<float, V>(pwb + k * kp, f);
+          if (GATE) rn_take<TO, V>(po + to_g + k * ko, sg);
+          rn_take<float, V>(psc + k * kp, q);
 #pragma unroll
           for (int i = 0; i < H; ++i) {
-            const u64 n = mul2(u[i], rn_all(rb));        // the branch, normed
-            const u64 ui = mul2(n, f[i]);
-            const u64 si = has_g ? rn_sigmoid(sg[i]) : rn_all(1.f);
-            u64 us = mul2(ui, si);
-            if (P.dropout) us = rn_mask(us, bits[k], i);  // a dropped element may hold anything
-            if (P.scale) ssc[k][i] = fma2(mul2(g[i], us), rn_all(keep), ssc[k][i]);
-            const u64 ds = mul2(g[i], t[i]);              // of u s
-            if (has_g) sg[i] = mul2(mul2(ds, us), rn_neg1_plus(si));
-            u64 du = mul2(ds, si);
-            if (P.dropout) {
-              du = rn_mask(du, bits[k], i);
-              if (has_g) sg[i] = rn_mask(sg[i], bits[k], i);
+            const u64 n = mul2(u[i], rn_all(rb));
+            u64 us = mul2(n, f[i]), s = 0ull;
+            if (GATE) {
+              s = rn_sigmoid(sg[i]);
+              us = mul2(us, s);
             }
-            if (P.wb) {
-              sb[k][i] = fma2(du, n, sb[k][i]);
-              du = mul2(du, f[i]);
-              dot = fma2(du, u[i], dot);
+            if (DROP) us = rn_mask(us, bits[k], i);  // (a dropped element may hold anything)
+            ssc[k][i] = fma2(g[i], us, ssc[k][i]);
+            u64 e = mul2(g[i], q[i]);
+            if (GATE) {
+              sg[i] = mul2(mul2(e, us), rn_neg1_plus(s));
+              e = mul2(e, s);
+              if (DROP) {
+                sg[i] = rn_mask(sg[i], bits[k], i);
+                e = rn_mask(e, bits[k], i);
+              }
             }
-            v[k][i] = du;
+            if (has_wb) {
+              sb[k][i] = fma2(e, n, sb[k][i]);
+              e = mul2(rn_all(rb), fma2(u[i], rn_all(-back), mul2(e, f[i])));
+            }
+            g[i] = e;
           }
-          if (has_g) rn_put<TO, V>(pdg + c, sg);
-          if (!P.wb) rn_put<TO, V>(pdo + c, v[k]);
+          if (GATE) rn_put<TO, V>(static_cast<TO*>(P.dg) + out + k * a.stride, sg);
+          rn_put<TO, V>(static_cast<TO*>(P.d_o) + out + k * a.stride, g);
         }
-      }
-      if (P.wb) {
-        mean = rn_total(rn_hsum(dot), part, 1, a.group, P) * inv * rb * rb;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-          const int c = a.me * V + k * a.stride;
-          if (c < P.D && here) {
-            u64 u[H];
-            rn_get<TO, V>(po + c, u);
-#pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = mul2(rn_all(rb), fma2(u[i], rn_all(-mean), v[k][i]));
-            rn_put<TO, V>(pdo + c, v[k]);
-          }
-        }
-      }
-      // everyone has read the row, and the sums' slots may be written again
-      if (P.warps == 1) __syncwarp();
-      else asm volatile("bar.sync %0, %1;" ::"r"(a.group + 1), "r"(P.warps * 32) : "memory");
     }
-    fetch(row0 + P.stages * a.step, s);
-    if (++s == P.stages) s = 0, turn ^= 1;
+    a.next(row0);
   }
-  if (!alive) {
-    atomicExch(P.err, 12);
-    if (a.mine == 0)
-      for (int q = 0; q < P.stages; ++q) rn_wait(&full[a.group][q], q < s ? turn ^ 1 : turn);
-  }
-  // the CTA's sums: its threads of a channel in order (groups, then rows at once), through the parameters' place
+  a.finish(P.err);
+  // the CTA's sums: its threads of a channel in order (groups, then rows at once)
   __syncthreads();
-  float* out = P.partial + (long long)blockIdx.x * 3 * P.D;
-  const int groups = (int)(blockDim.x >> 5) / P.warps;
+  float* out = P.partial + (long long)blockIdx.x * 3 * D;
+  const int groups = (int)(blockDim.x >> 5) / a.warps;
   for (int q = 0; q < groups * a.per; ++q) {
     if (a.group == q / a.per && a.sub == q % a.per)
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const int c = a.me * V + k * a.stride;
-        if (c < P.D)
+        if (mine[k])
 #pragma unroll
           for (int i = 0; i < H; ++i) {
             u64* f0 = reinterpret_cast<u64*>(params + c) + i;
-            u64* f1 = reinterpret_cast<u64*>(params + P.D + c) + i;
-            u64* f2 = reinterpret_cast<u64*>(params + 2 * P.D + c) + i;
+            u64* f1 = reinterpret_cast<u64*>(params + D + c) + i;
+            u64* f2 = reinterpret_cast<u64*>(params + 2 * D + c) + i;
+            const u64 scale = mul2(ssc[k][i], rn_all(keep));
             *f0 = q ? add2(*f0, sw[k][i]) : sw[k][i];
             *f1 = q ? add2(*f1, sb[k][i]) : sb[k][i];
-            *f2 = q ? add2(*f2, ssc[k][i]) : ssc[k][i];
+            *f2 = q ? add2(*f2, scale) : scale;
           }
       }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < 3 * P.D; i += blockDim.x) out[i] = params[i];
+  for (int i = threadIdx.x; i < 3 * D; i += blockDim.x) out[i] = params[i];
 }
 
 // ---------------------------------------------------------------- backward

@@ -124,6 +124,11 @@ CASES = [  # shape, stream, branch, next norm, branch norm, gate, scale, p, elem
     ((2, 3, 4, 100), f32, f32, True, True, True, True, 0.1, 4),
     ((40,), f32, f32, True, True, True, True, 0.1, 0),
     ((2000, 40), bf16, bf16, True, True, True, True, 0.1, 3),
+    ((330, 7008), bf16, bf16, True, True, True, True, 0.1, 0),
+    ((700, 4096), f32, bf16, True, True, True, True, 0.1, 0),
+    ((5, 200, 520), f32, f32, True, True, True, True, 0.0, 4),
+    ((40000, 64), bf16, bf16, True, True, True, True, 0.1, 0),
+    ((9, 1000, 24), f32, f16, True, True, True, True, 0.1, 8),
 ]
 
 
