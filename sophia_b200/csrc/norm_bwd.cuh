@@ -5,19 +5,24 @@
 
 namespace kda {
 
-template <typename TX, typename TO, bool NARROW, bool FULL, bool GATE, bool DROP>
+template <typename TX, typename TO, bool NARROW>
 struct RnBackward {
-  static auto get() { return rn_bwd_ring_kernel<TX, TO, NARROW, FULL, GATE, DROP>; }
+  template <bool FULL, bool GATE, bool DROP>
+  static auto get() { return rn_bwd_ring_kernel<TX, TO, NARROW, FULL && !NARROW, GATE, DROP>; }
 };
 
 template <typename TX, typename TO>
 int rn_bwd(RnParams& p, bool vec, cudaStream_t st) {
   if (vec && p.rows <= INT32_MAX / 2) {
-    const RnShape s = rn_ring_shape(p.D, sizeof(TO));
+    const RnShape s = rn_bwd_shape(p.D, sizeof(TO));
     const RnFit fit = rn_bwd_fit<TX, TO>(p, s);
     p.warps = s.warps;
     p.lanes = s.lanes;
-    if (fit.stages > 0) return launch_rn_ring<RnBackward, TX, TO>(p, s, fit, K_NORM_BWD, "residual norm backward", st);
+    if (fit.stages > 0) {
+      const char* what = "residual norm backward";
+      if (p.D <= 256) return launch_rn_ring<RnBackward<TX, TO, true>>(p, s, fit, K_NORM_BWD, what, st);
+      return launch_rn_ring<RnBackward<TX, TO, false>>(p, s, fit, K_NORM_BWD, what, st);
+    }
   }
   const RnShape s = rn_plain_shape(p.D);
   p.warps = s.warps;

@@ -22,13 +22,11 @@ inline RnShape rn_plain_shape(int D) {
   s.groups = std::max(1, 8 / s.warps);
   return s;
 }
-// Rows in pieces of 16 bytes of the branch's type: 16 channels a thread, or 8 where a row has no more than 256.  Fewer
-// channels a thread mean more warps a row and more waiting for their sums: 16384 x 1536, forward, 91 us with 16 and 124
-// with 8.
-inline RnShape rn_ring_shape(int D, size_t branch_size) {
+// Rows in pieces of 16 bytes of the branch's type, `channels` of them a thread (8 where a row has no more than 256).
+inline RnShape rn_ring_shape(int D, size_t branch_size, int channels) {
   RnShape s;
   s.v = (int)(16 / branch_size);
-  s.k = (D <= 256 ? 8 : 16) / s.v;
+  s.k = (D <= 256 ? 8 : channels) / s.v;
   const int threads = (D + s.v * s.k - 1) / (s.v * s.k);
   s.warps = (threads + 31) / 32;
   s.groups = std::max(1, RN_MAX_WARPS / s.warps);
@@ -36,6 +34,17 @@ inline RnShape rn_ring_shape(int D, size_t branch_size) {
   while (s.lanes < threads && s.lanes < 32) s.lanes *= 2;
   return s;
 }
+// The forward's channels a thread: 32, 24 or 16, whichever leaves the fewest threads idle, the most of them at a tie.  More
+// channels a thread mean fewer warps a row that wait for one another.
+inline RnShape rn_fwd_shape(int D, size_t branch_size) {
+  RnShape best = rn_ring_shape(D, branch_size, 32);
+  for (int channels : {24, 16}) {
+    const RnShape s = rn_ring_shape(D, branch_size, channels);
+    if (s.warps * s.k < best.warps * best.k) best = s;
+  }
+  return best;
+}
+inline RnShape rn_bwd_shape(int D, size_t branch_size) { return rn_ring_shape(D, branch_size, 16); }
 inline long long rn_units(long long rows, int rows_a_cta) { return std::max(1LL, (rows + rows_a_cta - 1) / rows_a_cta); }
 
 // The ring: rows of a stage, stages, and the CTAs of an SM.  A stage has 4 KB at least, unless that left groups
@@ -68,7 +77,7 @@ inline size_t rn_bwd_row(int D, size_t x, size_t o, bool g, bool dv, bool dn) {
 }
 template <typename TX, typename TO>
 RnFit rn_fwd_fit(const RnParams& p, const RnShape& s) {
-  return rn_fit(s, p.rows, (size_t)p.D * (sizeof(TX) + (p.g.p ? 2 : 1) * sizeof(TO)), 0);
+  return rn_fit(s, p.rows, (size_t)p.D * (sizeof(TX) + (p.g.p ? 2 : 1) * sizeof(TO)), (size_t)3 * p.D * 4);
 }
 template <typename TX, typename TO>
 RnFit rn_bwd_fit(const RnParams& p, const RnShape& s) {
@@ -100,22 +109,22 @@ int rn_smem(K kernel, size_t smem) {
   return e == cudaSuccess ? KDA_OK : fail(KDA_ERR_CUDA, std::string("residual norm smem: ") + cudaGetErrorString(e));
 }
 
-// The ring kernel for a call's parts.
-template <template <typename, typename, bool, bool, bool, bool> class Kernel, typename TX, typename TO, bool NARROW, bool FULL>
-auto rn_pick(bool gate, bool drop) {
-  return gate ? (drop ? Kernel<TX, TO, NARROW, FULL, true, true>::get() : Kernel<TX, TO, NARROW, FULL, true, false>::get())
-              : (drop ? Kernel<TX, TO, NARROW, FULL, false, true>::get() : Kernel<TX, TO, NARROW, FULL, false, false>::get());
+// The ring kernel for a call's parts: Kernel::get<FULL, GATE, DROP>().
+template <typename Kernel>
+auto rn_pick(bool full, bool gate, bool drop) {
+  if (full)
+    return gate ? (drop ? Kernel::template get<true, true, true>() : Kernel::template get<true, true, false>())
+                : (drop ? Kernel::template get<true, false, true>() : Kernel::template get<true, false, false>());
+  return gate ? (drop ? Kernel::template get<false, true, true>() : Kernel::template get<false, true, false>())
+              : (drop ? Kernel::template get<false, false, true>() : Kernel::template get<false, false, false>());
 }
-template <template <typename, typename, bool, bool, bool, bool> class Kernel, typename TX, typename TO>
+template <typename Kernel>
 int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, const char* what, cudaStream_t st) {
   p.stages = fit.stages;
   p.batch = fit.batch;
   p.parts = (int)fit.ctas;
   p.params = (long long)(fit.smem / 4) - 3LL * p.D;
-  const bool gate = p.g.p != nullptr, full = p.D == s.warps * 32 * s.v * s.k;
-  auto kernel = p.D <= 256 ? rn_pick<Kernel, TX, TO, true, false>(gate, p.dropout)
-                : full     ? rn_pick<Kernel, TX, TO, false, true>(gate, p.dropout)
-                           : rn_pick<Kernel, TX, TO, false, false>(gate, p.dropout);
+  auto kernel = rn_pick<Kernel>(p.D == s.warps * 32 * s.v * s.k, p.g.p != nullptr, p.dropout);
   if (int rc = rn_smem(kernel, fit.smem)) return rc;
   {
     TimedLaunch tl(id, st);

@@ -116,8 +116,10 @@ __device__ __forceinline__ float rn_sum(float a, float (*part)[RN_MAX_WARPS], in
 __device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
-    const u64 p0 = (u64)0xD2511F53u * c.x, p1 = (u64)0xCD9E8D57u * c.z;
-    c = make_uint4((unsigned)(p1 >> 32) ^ c.y ^ k0, (unsigned)p1, (unsigned)(p0 >> 32) ^ c.w ^ k1, (unsigned)p0);
+    // (halves apart: as 64-bit products, 154 us against 90 of the forward of 16384 x 1536)
+    const unsigned l0 = 0xD2511F53u * c.x, h0 = __umulhi(0xD2511F53u, c.x);
+    const unsigned l1 = 0xCD9E8D57u * c.z, h1 = __umulhi(0xCD9E8D57u, c.z);
+    c = make_uint4(h1 ^ c.y ^ k0, l1, h0 ^ c.w ^ k1, l0);
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
@@ -252,8 +254,9 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
 // Aligned rows come into a ring of stages in shared memory by bulk copies, so that the next rows are on their way
 // while one is worked on.  A group of W warps owns a row at a time (NARROW rows, up to 256 channels: `lanes` lanes of a
 // single warp, which has 32 / lanes rows at once); rows that lie end to end are one copy (small copies cost the copy
-// engine as much as large ones), so a stage of short rows holds several.  A thread has 16 channels (NARROW 8), the same in
-// every row, in packed fp32 arithmetic; the forward's parameters and the backward's sums over rows stay in its registers.
+// engine as much as large ones), so a stage of short rows holds several.  A thread has the same channels in every
+// row -- 16 to 32 forward, 16 backward, whose sums over rows stay in its registers, 8 of NARROW rows -- and computes in
+// packed fp32 arithmetic; the parameters lie in shared memory.
 // What a row costs beside its arithmetic -- waiting, barriers, sums over warps, addresses -- is what bounds these
 // kernels, so the parts that a call has are known to the compiler as far as they change the loops (FULL: a row fills its
 // threads; GATE; DROP).
@@ -530,10 +533,10 @@ __device__ __forceinline__ u64 rn_mask(u64 v, unsigned bits, int pair) {
 }
 
 
-template <typename TX, typename TO, bool NARROW, bool FULL, bool GATE, bool DROP>
+template <typename TX, typename TO, int K, bool NARROW, bool FULL, bool GATE, bool DROP>
 __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const __grid_constant__ RnParams P) {
-  constexpr int V = 16 / sizeof(TO), H = V / 2, K = (NARROW ? 8 : 16) / V;
-  extern __shared__ __align__(128) char ring[];
+  constexpr int V = 16 / sizeof(TO), H = V / 2;
+  extern __shared__ __align__(128) char ring[];  // the groups' stages, then the parameters [3][D]
   __shared__ __align__(16) RnShared<1> sh;
   const int D = P.D;
   const uint32_t xb = D * sizeof(TX), ob = D * sizeof(TO);
@@ -544,6 +547,12 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
     if (lane == 1) a.mine = rn_source(P.o, sizeof(TO), xb, P.dense >> 1 & 1, D);
     if (GATE && lane == 2) a.mine = rn_source(P.g, sizeof(TO), xb + ob, P.dense >> 2 & 1, D);
   }
+  float* params = reinterpret_cast<float*>(ring) + P.params;
+  for (int i = threadIdx.x; i < D; i += blockDim.x) {  // (the scale with 1 / (1 - p) in it)
+    params[i] = P.w ? P.w[i] : 0.f;
+    params[D + i] = P.wb ? P.wb[i] : 0.f;
+    params[2 * D + i] = (P.scale ? P.scale[i] : 1.f) * (DROP ? P.keep_scale : 1.f);
+  }
   __syncthreads();
   a.start();
   const bool has_w = P.w != nullptr, has_wb = P.wb != nullptr, scaled = P.scale || DROP, keeps = P.rstd && a.me == 0;
@@ -552,22 +561,9 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / D, eps = P.eps;
   bool mine[K];  // the thread's pieces that there are
-  u64 w[K][H], wb[K][H], sc[K][H];  // the scale with 1 / (1 - p) in it
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = a.me * V + k * a.stride;
-    mine[k] = FULL || c < D;
-    const u64 keep = rn_all(DROP ? P.keep_scale : 1.f);
-#pragma unroll
-    for (int i = 0; i < H; ++i) w[k][i] = wb[k][i] = sc[k][i] = 0ull;
-    if (mine[k]) {
-      if (has_w) rn_get<float, V>(P.w + c, w[k]);
-      if (has_wb) rn_get<float, V>(P.wb + c, wb[k]);
-      if (P.scale) rn_get<float, V>(P.scale + c, sc[k]);
-    }
-#pragma unroll
-    for (int i = 0; i < H; ++i) sc[k][i] = P.scale ? mul2(sc[k][i], keep) : keep;
-  }
+  for (int k = 0; k < K; ++k) mine[k] = FULL || a.me * V + k * a.stride < D;
+  const uint32_t pw = smem_u32(params) + a.me * V * 4, pwb = pw + 4 * D, psc = pwb + 4 * D, kp = a.stride * 4;
   const uint32_t at_x = a.sub * xb + a.me * (V * (uint32_t)sizeof(TX)), at_o = a.rows * xb + a.sub * ob + a.me * 16;
   const uint32_t kx = a.stride * (uint32_t)sizeof(TX), ko = a.stride * (uint32_t)sizeof(TO), at_g = a.rows * ob;
   for (int row0 = a.first; row0 < a.total; row0 += a.step) {
@@ -594,24 +590,27 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
         t[0] = rn_hsum(ss);
         a.sum(t);
         rb = rsqrtf(fmaf(t[0], inv, eps));
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-          for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(wb[k][i], rn_all(rb)));
         ss = 0ull;
       }
 #pragma unroll
       for (int k = 0; k < K; ++k)
         if (mine[k] && here) {
           u64 f[H];
+          if (has_wb) {
+            rn_take<float, V>(pwb + k * kp, f);
+#pragma unroll
+            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(f[i], rn_all(rb)));
+          }
           if (GATE) {
             rn_take<TO, V>(po + at_g + k * ko, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], rn_sigmoid(f[i]));
           }
-          if (scaled)
+          if (scaled) {
+            rn_take<float, V>(psc + k * kp, f);
 #pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], sc[k][i]);
+            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], f[i]);
+          }
           if (DROP) {
             const unsigned bits = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
 #pragma unroll
@@ -633,8 +632,10 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
 #pragma unroll
         for (int k = 0; k < K; ++k)
           if (mine[k] && here) {
+            u64 f[H];
+            rn_take<float, V>(pw + k * kp, f);
 #pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(w[k][i], rn_all(r)));
+            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(f[i], rn_all(r)));
             rn_put<TO, V>(static_cast<TO*>(P.n) + out + k * a.stride, v[k]);
           }
       }
