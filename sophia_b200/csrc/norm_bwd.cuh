@@ -27,8 +27,7 @@ int rn_bwd(RnParams& p, bool vec, cudaStream_t st) {
   const RnShape s = rn_plain_shape(p.D);
   p.warps = s.warps;
   if (s.k == 2) return launch_rn_bwd<TX, TO, 2>(p, s, st);
-  if (s.k == 4) return launch_rn_bwd<TX, TO, 4>(p, s, st);
-  return launch_rn_bwd<TX, TO, 16>(p, s, st);
+  return launch_rn_bwd<TX, TO, 4>(p, s, st);
 }
 
 }  // namespace kda

@@ -15,10 +15,10 @@ namespace kda {
 struct RnShape {
   int v, k, warps, groups, lanes;
 };
-// Rows that are read as they lie, channel by channel.
+// Rows that are read as they lie, element by element: four neighbours a piece, 8 or 16 channels a thread.
 inline RnShape rn_plain_shape(int D) {
-  RnShape s{1, D <= 64 * 8 ? 2 : (D <= 128 * RN_MAX_WARPS ? 4 : 16), 0, 0, 32};
-  s.warps = (D + 32 * s.k - 1) / (32 * s.k);
+  RnShape s{4, D <= 512 ? 2 : 4, 0, 0, 32};
+  s.warps = (D + 128 * s.k - 1) / (128 * s.k);
   s.groups = std::max(1, 8 / s.warps);
   return s;
 }
@@ -96,7 +96,7 @@ template <typename TX, typename TO, int K>
 int launch_rn_fwd(const RnParams& p, const RnShape& s, cudaStream_t st) {
   {
     TimedLaunch tl(K_NORM_FWD, st);
-    rn_fwd_kernel<TX, TO, 1, K>
+    rn_fwd_kernel<TX, TO, K>
         <<<(unsigned)std::min(rn_units(p.rows, s.groups), 1LL << 20), s.warps * s.groups * 32, 0, st>>>(p);
   }
   return launch_check("residual norm forward");
@@ -135,8 +135,8 @@ int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, cons
 
 template <typename TX, typename TO, int K>
 int launch_rn_bwd(RnParams& p, const RnShape& s, cudaStream_t st) {
-  const size_t smem = (size_t)s.groups * 3 * p.D * 4;
-  auto kernel = rn_bwd_kernel<TX, TO, 1, K>;
+  const size_t smem = (size_t)s.groups * 3 * ((p.D + 3) / 4) * 16;
+  auto kernel = rn_bwd_kernel<TX, TO, K>;
   if (int rc = rn_smem(kernel, smem)) return rc;
   p.parts = (int)rn_plain_ctas(p.rows, s);
   {

@@ -53,43 +53,29 @@ struct RnParams {
 
 // ---------------------------------------------------------------- rows
 
-// V channels in pieces of up to 16 bytes.
-template <typename T, int V>
-struct RnVec {
-  static constexpr int PER = V * sizeof(T) > 16 ? 16 / (int)sizeof(T) : V;
-  IoVec<T, PER> p[V / PER];
-  __device__ __forceinline__ void load(const T* q) {
-#pragma unroll
-    for (int i = 0; i < V / PER; ++i) p[i] = reinterpret_cast<const IoVec<T, PER>*>(q)[i];
-  }
+// Four neighbouring channels, of which the first n are there, wherever they lie: element by element.
+template <typename T>
+struct RnFour {
+  T v[4];
   __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < V / PER; ++i)
-#pragma unroll
-      for (int j = 0; j < PER; ++j) p[i].v[j] = io_from_f<T>(0.f);
+    for (int i = 0; i < 4; ++i) v[i] = io_from_f<T>(0.f);
   }
-  __device__ __forceinline__ float get(int i) const { return io_to_f(p[i / PER].v[i % PER]); }
+  __device__ __forceinline__ void load(const T* q, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? q[i] : io_from_f<T>(0.f);
+  }
+  __device__ __forceinline__ float get(int i) const { return io_to_f(v[i]); }
 };
-template <typename T, int V>
-__device__ __forceinline__ void rn_store(T* q, const float (&f)[V]) {
-  constexpr int PER = RnVec<T, V>::PER;
+template <typename T>
+__device__ __forceinline__ void rn_store(T* q, const float (&f)[4], int n) {
 #pragma unroll
-  for (int i = 0; i < V / PER; ++i) {
-    IoVec<T, PER> r;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) r.v[j] = io_from_f<T>(f[i * PER + j]);
-    reinterpret_cast<IoVec<T, PER>*>(q)[i] = r;
-  }
+  for (int i = 0; i < 4; ++i)
+    if (i < n) q[i] = io_from_f<T>(f[i]);
 }
-template <int V>
-__device__ __forceinline__ void rn_param(const float* p, int c, float (&f)[V]) {
-  constexpr int PER = V > 4 ? 4 : V;
+__device__ __forceinline__ void rn_param(const float* p, int c, int n, float (&f)[4]) {
 #pragma unroll
-  for (int i = 0; i < V / PER; ++i) {
-    const IoVec<float, PER> r = reinterpret_cast<const IoVec<float, PER>*>(p + c)[i];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) f[i * PER + j] = r.v[j];
-  }
+  for (int i = 0; i < 4; ++i) f[i] = i < n ? __ldg(p + c + i) : 0.f;
 }
 template <typename T>
 __device__ __forceinline__ const T* rn_row(const RowView& r, long long row, int T_) {
@@ -125,38 +111,28 @@ __device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
   }
   return c;
 }
-// keep / (1 - p) of the V channels from c on (V = 1, or a multiple of 4 with c a multiple of 4)
-template <int V>
-__device__ __forceinline__ void rn_keep(const RnParams& P, unsigned k0, unsigned k1, long long row, int c, float (&m)[V]) {
+// keep / (1 - p) of the four channels from c on, c a multiple of 4
+__device__ __forceinline__ void rn_keep(const RnParams& P, unsigned k0, unsigned k1, long long row, int c, float (&m)[4]) {
   if (!P.dropout) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) m[i] = 1.f;
+    for (int i = 0; i < 4; ++i) m[i] = 1.f;
     return;
   }
+  const uint4 r = philox(make_uint4((unsigned)c / 4, (unsigned)row, (unsigned)(row >> 32), P.offset), k0, k1);
+  const unsigned word[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-  for (int q = 0; q < (V + 3) / 4; ++q) {
-    const uint4 r = philox(make_uint4((unsigned)c / 4 + q, (unsigned)row, (unsigned)(row >> 32), P.offset), k0, k1);
-    const unsigned word[4] = {r.x, r.y, r.z, r.w};
-    if (V == 1) {
-      const unsigned w = (c & 2) ? ((c & 1) ? r.w : r.z) : ((c & 1) ? r.y : r.x);
-      m[0] = w < P.drop || P.drop_all ? 0.f : P.keep_scale;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (q * 4 + i < V) m[q * 4 + i] = word[i] < P.drop || P.drop_all ? 0.f : P.keep_scale;
-    }
-  }
+  for (int i = 0; i < 4; ++i) m[i] = word[i] < P.drop || P.drop_all ? 0.f : P.keep_scale;
 }
 // a product with keep / (1 - p) that is 0 where the element is dropped, whatever it holds
 __device__ __forceinline__ float rn_drop(float m, float a) { return m == 0.f ? 0.f : m * a; }
 
 // ---------------------------------------------------------------- forward
 
-template <typename TX, typename TO, int V, int K>
+template <typename TX, typename TO, int K>
 __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnParams P) {
   __shared__ float part[2][RN_MAX_WARPS];
   const int warps = P.warps, group = (threadIdx.x >> 5) / warps, groups = (blockDim.x >> 5) / warps;
-  const int me = threadIdx.x - group * warps * 32, stride = warps * 32 * V;
+  const int me = threadIdx.x - group * warps * 32, stride = warps * 32 * 4;
   const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / P.D;
@@ -164,15 +140,15 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
     const TX* px = rn_row<TX>(P.x, row, P.T);
     const TO* po = rn_row<TO>(P.o, row, P.T);
     const TO* pg = P.g.p ? rn_row<TO>(P.g, row, P.T) : nullptr;
-    RnVec<TO, V> o[K], g[K];
-    RnVec<TX, V> x[K];
+    RnFour<TO> o[K], g[K];
+    RnFour<TX> x[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * V + k * stride;
+      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
       if (c < P.D) {
-        o[k].load(po + c);
-        x[k].load(px + c);
-        if (pg) g[k].load(pg + c);
+        o[k].load(po + c, n4);
+        x[k].load(px + c, n4);
+        if (pg) g[k].load(pg + c, n4);
       } else {
         o[k].zero();
         x[k].zero();
@@ -184,44 +160,44 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) ss = fmaf(o[k].get(i), o[k].get(i), ss);
+        for (int i = 0; i < 4; ++i) ss = fmaf(o[k].get(i), o[k].get(i), ss);
       rb = rsqrtf(fmaf(rn_sum(ss, part, 0, group, warps), inv, P.eps));
     }
-    float v[K][V], ss = 0.f;
+    float v[K][4], ss = 0.f;
     TX* pv = static_cast<TX*>(P.v) + row * P.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * V + k * stride;
+      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[k][i] = 0.f;
+      for (int i = 0; i < 4; ++i) v[k][i] = 0.f;
       if (c < P.D) {
-        float f[V], m[V], u[V];
+        float f[4], m[4], u[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) u[i] = o[k].get(i);
+        for (int i = 0; i < 4; ++i) u[i] = o[k].get(i);
         if (P.wb) {
-          rn_param<V>(P.wb, c, f);
+          rn_param(P.wb, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[i] *= rb * f[i];
+          for (int i = 0; i < 4; ++i) u[i] *= rb * f[i];
         }
         if (pg)
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[i] *= sigmoidf_(g[k].get(i));
+          for (int i = 0; i < 4; ++i) u[i] *= sigmoidf_(g[k].get(i));
         if (P.dropout) {
-          rn_keep<V>(P, k0, k1, row, c, m);
+          rn_keep(P, k0, k1, row, c, m);
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[i] = rn_drop(m[i], u[i]);
+          for (int i = 0; i < 4; ++i) u[i] = rn_drop(m[i], u[i]);
         }
         if (P.scale) {
-          rn_param<V>(P.scale, c, f);
+          rn_param(P.scale, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[i] *= f[i];
+          for (int i = 0; i < 4; ++i) u[i] *= f[i];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+        for (int i = 0; i < 4; ++i) {
           v[k][i] = x[k].get(i) + u[i];
           ss = fmaf(v[k][i], v[k][i], ss);
         }
-        rn_store<TX, V>(pv + c, v[k]);
+        rn_store(pv + c, v[k], n4);
       }
     }
     float r = 0.f;
@@ -230,13 +206,13 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
       TO* pn = static_cast<TO*>(P.n) + row * P.D;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = me * V + k * stride;
+        const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
         if (c < P.D) {
-          float f[V];
-          rn_param<V>(P.w, c, f);
+          float f[4];
+          rn_param(P.w, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) f[i] *= v[k][i] * r;
-          rn_store<TO, V>(pn + c, f);
+          for (int i = 0; i < 4; ++i) f[i] *= v[k][i] * r;
+          rn_store(pn + c, f, n4);
         }
       }
     }
@@ -317,8 +293,18 @@ __device__ __forceinline__ void rn_copy(const RnSource& t, uint32_t at, int rows
 template <int N>
 struct RnShared {
   float part[2][RN_MAX_GROUPS][N][RN_MAX_WARPS];
-  uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES];
+  uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES], params;
 };
+// The parameters w, w_b and scale into shared memory [3][D]; one that is left out counts as 1.  The first thread, behind
+// the barriers' initialisation.
+__device__ __forceinline__ void rn_params(const RnParams& P, float* dst, uint64_t* bar) {
+  const float* src[3] = {P.w, P.wb, P.scale};
+  const uint32_t bytes = P.D * 4;
+  rn_expect(bar, ((P.w ? 1 : 0) + (P.wb ? 1 : 0) + (P.scale ? 1 : 0)) * bytes);
+#pragma unroll
+  for (int q = 0; q < 3; ++q)
+    if (src[q]) rn_bulk(smem_u32(dst + q * P.D), src[q], bytes, bar);
+}
 
 // A group's walk through its rows: where it and its thread stand, and its stages.
 template <typename T, bool NARROW, int N>
@@ -368,6 +354,7 @@ struct RnGroup {
     mine = RnSource{};
     if (in == 0)
       for (int q = 0; q < stages; ++q) rn_bar_init(&full[q]);
+    if (threadIdx.x == 0) rn_bar_init(&sh.params);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     for (int i = threadIdx.x; i < 2 * RN_MAX_GROUPS * N * RN_MAX_WARPS; i += blockDim.x) (&sh.part[0][0][0][0])[i] = 0.f;
   }
@@ -548,24 +535,21 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
     if (GATE && lane == 2) a.mine = rn_source(P.g, sizeof(TO), xb + ob, P.dense >> 2 & 1, D);
   }
   float* params = reinterpret_cast<float*>(ring) + P.params;
-  for (int i = threadIdx.x; i < D; i += blockDim.x) {  // (the scale with 1 / (1 - p) in it)
-    params[i] = P.w ? P.w[i] : 0.f;
-    params[D + i] = P.wb ? P.wb[i] : 0.f;
-    params[2 * D + i] = (P.scale ? P.scale[i] : 1.f) * (DROP ? P.keep_scale : 1.f);
-  }
   __syncthreads();
   a.start();
-  const bool has_w = P.w != nullptr, has_wb = P.wb != nullptr, scaled = P.scale || DROP, keeps = P.rstd && a.me == 0;
+  if (threadIdx.x == 0) rn_params(P, params, &sh.params);
+  const bool has_w = P.w != nullptr, has_wb = P.wb != nullptr, has_scale = P.scale != nullptr, keeps = P.rstd && a.me == 0;
   unsigned long long seed = 0;
   if (DROP) seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
-  const float inv = 1.f / D, eps = P.eps;
+  const float inv = 1.f / D, eps = P.eps, keep = DROP ? P.keep_scale : 1.f;
   bool mine[K];  // the thread's pieces that there are
 #pragma unroll
   for (int k = 0; k < K; ++k) mine[k] = FULL || a.me * V + k * a.stride < D;
   const uint32_t pw = smem_u32(params) + a.me * V * 4, pwb = pw + 4 * D, psc = pwb + 4 * D, kp = a.stride * 4;
   const uint32_t at_x = a.sub * xb + a.me * (V * (uint32_t)sizeof(TX)), at_o = a.rows * xb + a.sub * ob + a.me * 16;
   const uint32_t kx = a.stride * (uint32_t)sizeof(TX), ko = a.stride * (uint32_t)sizeof(TO), at_g = a.rows * ob;
+  a.alive = rn_wait(&sh.params, 0);
   for (int row0 = a.first; row0 < a.total; row0 += a.step) {
     a.wait();
     uint32_t px = a.base + a.slot * a.stage_bytes + at_x, po = a.base + a.slot * a.stage_bytes + at_o;
@@ -606,7 +590,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], rn_sigmoid(f[i]));
           }
-          if (scaled) {
+          if (has_scale) {
             rn_take<float, V>(psc + k * kp, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], f[i]);
@@ -614,7 +598,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
           if (DROP) {
             const unsigned bits = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
 #pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = rn_mask(v[k][i], bits, i);
+            for (int i = 0; i < H; ++i) v[k][i] = rn_mask(mul2(v[k][i], rn_all(keep)), bits, i);
           }
           rn_take<TX, V>(px + k * kx, f);
 #pragma unroll
@@ -672,13 +656,13 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
     if (lane == 4) a.mine = rn_source(P.dn, sizeof(TO), off_dn, P.dense >> 4 & 1, D);
   }
   float* params = reinterpret_cast<float*>(ring) + P.params;
-  for (int i = threadIdx.x; i < D; i += blockDim.x) {  // what a part that is left out multiplies with: 1
-    params[i] = P.w ? P.w[i] : 0.f;
-    params[D + i] = has_wb ? P.wb[i] : 1.f;
-    params[2 * D + i] = (has_scale ? P.scale[i] : 1.f) * (DROP ? P.keep_scale : 1.f);
+  for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    if (!has_wb) params[D + i] = 1.f;
+    if (!has_scale) params[2 * D + i] = 1.f;
   }
   __syncthreads();
   a.start();
+  if (threadIdx.x == 0) rn_params(P, params, &sh.params);
   unsigned long long seed = 0;
   if (DROP) seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
@@ -699,6 +683,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
     return row < a.total ? __ldg(reinterpret_cast<const float2*>(P.rstd + 2LL * row)) : make_float2(0.f, 0.f);
   };
   float2 ahead = roots_of(min(a.first, a.total) + a.sub);  // of the row to come
+  a.alive = rn_wait(&sh.params, 0);
   for (int row0 = a.first; row0 < a.total; row0 += a.step) {
     a.wait();
     uint32_t px = a.base + a.slot * a.stage_bytes + at_x, po = a.base + a.slot * a.stage_bytes + at_o;
@@ -732,7 +717,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
           if (DROP) {
             bits[k] = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
 #pragma unroll
-            for (int i = 0; i < H; ++i) t[i] = rn_mask(t[i], bits[k], i);
+            for (int i = 0; i < H; ++i) t[i] = rn_mask(mul2(t[i], rn_all(keep)), bits[k], i);
           }
           rn_take<TX, V>(px + k * kx, f);
 #pragma unroll
@@ -783,7 +768,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
           rn_put<TX, V>(static_cast<TX*>(P.dx) + out + k * a.stride, g);
           if (DROP)
 #pragma unroll
-            for (int i = 0; i < H; ++i) g[i] = rn_mask(g[i], bits[k], i);
+            for (int i = 0; i < H; ++i) g[i] = rn_mask(mul2(g[i], rn_all(keep)), bits[k], i);
           rn_take<TO, V>(po + k * ko, u);
           rn_take<float, V>(pwb + k * kp, f);
           if (GATE) rn_take<TO, V>(po + to_g + k * ko, sg);
@@ -835,10 +820,9 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
             u64* f0 = reinterpret_cast<u64*>(params + c) + i;
             u64* f1 = reinterpret_cast<u64*>(params + D + c) + i;
             u64* f2 = reinterpret_cast<u64*>(params + 2 * D + c) + i;
-            const u64 scale = mul2(ssc[k][i], rn_all(keep));
             *f0 = q ? add2(*f0, sw[k][i]) : sw[k][i];
             *f1 = q ? add2(*f1, sb[k][i]) : sb[k][i];
-            *f2 = q ? add2(*f2, scale) : scale;
+            *f2 = q ? add2(*f2, ssc[k][i]) : ssc[k][i];
           }
       }
     __syncthreads();
@@ -848,34 +832,26 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
 
 // ---------------------------------------------------------------- backward
 
-template <typename TX, typename TO, int V, int K>
+template <typename TX, typename TO, int K>
 __global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnParams P) {
-  extern __shared__ __align__(16) float acc[];  // [groups][3][D]: every thread adds to its own channels
+  extern __shared__ __align__(16) float acc[];  // [groups][3][D, in whole fours]: every thread adds to its own channels
   __shared__ float part[2][RN_MAX_WARPS];
   const int warps = P.warps, group = (threadIdx.x >> 5) / warps, groups = (blockDim.x >> 5) / warps;
-  const int me = threadIdx.x - group * warps * 32, stride = warps * 32 * V;
+  const int me = threadIdx.x - group * warps * 32, stride = warps * 32 * 4;
   const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / P.D;
-  float* sums = acc + (long long)group * 3 * P.D;
+  const int D4 = (P.D + 3) & ~3;
+  float* sums = acc + (long long)group * 3 * D4;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int c = me * V + k * stride;
+    const int c = me * 4 + k * stride;
     if (c < P.D)
-      for (int q = 0; q < 3; ++q)
-#pragma unroll
-        for (int i = 0; i < V; ++i) sums[q * P.D + c + i] = 0.f;
+      for (int q = 0; q < 3; ++q) *reinterpret_cast<float4*>(sums + q * D4 + c) = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  auto add = [&](int q, int c, const float (&f)[V]) {
-    constexpr int PER = V > 4 ? 4 : V;
-    IoVec<float, PER>* s = reinterpret_cast<IoVec<float, PER>*>(sums + q * P.D + c);
-#pragma unroll
-    for (int i = 0; i < V / PER; ++i) {
-      IoVec<float, PER> t = s[i];
-#pragma unroll
-      for (int j = 0; j < PER; ++j) t.v[j] += f[i * PER + j];
-      s[i] = t;
-    }
+  auto add = [&](int q, int c, const float (&f)[4]) {
+    float4& t = *reinterpret_cast<float4*>(sums + q * D4 + c);
+    t = make_float4(t.x + f[0], t.y + f[1], t.z + f[2], t.w + f[3]);
   };
   for (long long row = (long long)blockIdx.x * groups + group; row < P.rows; row += (long long)gridDim.x * groups) {
     const TX* px = rn_row<TX>(P.x, row, P.T);
@@ -883,82 +859,82 @@ __global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnP
     const TO* pg = P.g.p ? rn_row<TO>(P.g, row, P.T) : nullptr;
     const TX* pdv = P.dv.p ? rn_row<TX>(P.dv, row, P.T) : nullptr;
     const TO* pdn = P.dn.p ? rn_row<TO>(P.dn, row, P.T) : nullptr;
-    RnVec<TO, V> o[K], g[K], dn[K];
-    RnVec<TX, V> x[K], dv[K];
+    RnFour<TO> o[K], g[K], dn[K];
+    RnFour<TX> x[K], dv[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * V + k * stride;
+      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
       o[k].zero(), g[k].zero(), dn[k].zero(), x[k].zero(), dv[k].zero();
       if (c < P.D) {
-        o[k].load(po + c);
-        x[k].load(px + c);
-        if (pg) g[k].load(pg + c);
-        if (pdv) dv[k].load(pdv + c);
-        if (pdn) dn[k].load(pdn + c);
+        o[k].load(po + c, n4);
+        x[k].load(px + c, n4);
+        if (pg) g[k].load(pg + c, n4);
+        if (pdv) dv[k].load(pdv + c, n4);
+        if (pdn) dn[k].load(pdn + c, n4);
       }
     }
     const float rb = P.rstd[2 * row], r = P.rstd[2 * row + 1];
     // the stream again, and the next norm's mean(t v)
-    float v[K][V], m[K][V], dot = 0.f;
+    float v[K][4], m[K][4], dot = 0.f;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * V + k * stride;
+      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[k][i] = 0.f, m[k][i] = 0.f;
+      for (int i = 0; i < 4; ++i) v[k][i] = 0.f, m[k][i] = 0.f;
       if (c < P.D) {
-        float f[V], u[V];
+        float f[4], u[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) u[i] = o[k].get(i);
+        for (int i = 0; i < 4; ++i) u[i] = o[k].get(i);
         if (P.wb) {
-          rn_param<V>(P.wb, c, f);
+          rn_param(P.wb, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[i] *= rb * f[i];
+          for (int i = 0; i < 4; ++i) u[i] *= rb * f[i];
         }
         if (pg)
 #pragma unroll
-          for (int i = 0; i < V; ++i) u[i] *= sigmoidf_(g[k].get(i));
-        rn_keep<V>(P, k0, k1, row, c, m[k]);
-        if (P.scale) rn_param<V>(P.scale, c, f);
+          for (int i = 0; i < 4; ++i) u[i] *= sigmoidf_(g[k].get(i));
+        rn_keep(P, k0, k1, row, c, m[k]);
+        if (P.scale) rn_param(P.scale, c, n4, f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[k][i] = x[k].get(i) + rn_drop(m[k][i], u[i]) * (P.scale ? f[i] : 1.f);
+        for (int i = 0; i < 4; ++i) v[k][i] = x[k].get(i) + rn_drop(m[k][i], u[i]) * (P.scale ? f[i] : 1.f);
         if (pdn) {
-          rn_param<V>(P.w, c, f);
+          rn_param(P.w, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) dot = fmaf(f[i] * dn[k].get(i), v[k][i], dot);
+          for (int i = 0; i < 4; ++i) dot = fmaf(f[i] * dn[k].get(i), v[k][i], dot);
         }
       }
     }
     float mean = 0.f;
     if (pdn) mean = rn_sum(dot, part, 0, group, warps) * inv * r * r;
     dot = 0.f;
-    float du[K][V];
+    float du[K][4];
     TX* pdx = static_cast<TX*>(P.dx) + row * P.D;
     TO* pdg = static_cast<TO*>(P.dg) + row * P.D;
     TO* pdo = static_cast<TO*>(P.d_o) + row * P.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * V + k * stride;
+      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
 #pragma unroll
-      for (int i = 0; i < V; ++i) du[k][i] = 0.f;
+      for (int i = 0; i < 4; ++i) du[k][i] = 0.f;
       if (c < P.D) {
-        float d[V], f[V], t[V], wb[V];
+        float d[4], f[4], t[4], wb[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) d[i] = dv[k].get(i);
+        for (int i = 0; i < 4; ++i) d[i] = dv[k].get(i);
         if (pdn) {
-          rn_param<V>(P.w, c, f);
+          rn_param(P.w, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
+          for (int i = 0; i < 4; ++i) {
             d[i] = fmaf(r, fmaf(-v[k][i], mean, f[i] * dn[k].get(i)), d[i]);
             t[i] = dn[k].get(i) * v[k][i] * r;
           }
           add(0, c, t);
         }
-        rn_store<TX, V>(pdx + c, d);
-        if (P.wb) rn_param<V>(P.wb, c, wb);
-        if (P.scale) rn_param<V>(P.scale, c, f);
-        float u[V], s[V];
+        rn_store(pdx + c, d, n4);
+        if (P.wb) rn_param(P.wb, c, n4, wb);
+        if (P.scale) rn_param(P.scale, c, n4, f);
+        float u[4], s[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
+        for (int i = 0; i < 4; ++i) {
           u[i] = P.wb ? o[k].get(i) * rb * wb[i] : o[k].get(i);
           s[i] = pg ? sigmoidf_(g[k].get(i)) : 1.f;
           const float dm = rn_drop(m[k][i], d[i]);           // gradient of scale u s
@@ -968,17 +944,17 @@ __global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnP
           s[i] = m[k][i] == 0.f ? 0.f : ds * u[i] * (s[i] * (1.f - s[i]));
         }
         if (P.scale) add(2, c, t);
-        if (pg) rn_store<TO, V>(pdg + c, s);
+        if (pg) rn_store(pdg + c, s, n4);
         if (P.wb) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
+          for (int i = 0; i < 4; ++i) {
             t[i] = du[k][i] * o[k].get(i) * rb;
             du[k][i] *= wb[i];
             dot = fmaf(du[k][i], o[k].get(i), dot);
           }
           add(1, c, t);
         } else {
-          rn_store<TO, V>(pdo + c, du[k]);
+          rn_store(pdo + c, du[k], n4);
         }
       }
     }
@@ -986,11 +962,11 @@ __global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnP
       mean = rn_sum(dot, part, 1, group, warps) * inv * rb * rb;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = me * V + k * stride;
+        const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
         if (c < P.D) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) du[k][i] = rb * fmaf(-o[k].get(i), mean, du[k][i]);
-          rn_store<TO, V>(pdo + c, du[k]);
+          for (int i = 0; i < 4; ++i) du[k][i] = rb * fmaf(-o[k].get(i), mean, du[k][i]);
+          rn_store(pdo + c, du[k], n4);
         }
       }
     }
@@ -998,8 +974,9 @@ __global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnP
   }
   __syncthreads();
   for (int i = threadIdx.x; i < 3 * P.D; i += blockDim.x) {  // the CTA's sums, its groups in order
+    const int at = i / P.D * D4 + i % P.D;
     float t = 0.f;
-    for (int q = 0; q < groups; ++q) t += acc[(long long)q * 3 * P.D + i];
+    for (int q = 0; q < groups; ++q) t += acc[(long long)q * 3 * D4 + at];
     P.partial[(long long)blockIdx.x * 3 * P.D + i] = t;
   }
 }
