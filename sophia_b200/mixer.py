@@ -63,9 +63,12 @@ class KDAMixerBlock(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         """x [B, T, dim] -> [B, T, dim]."""
-        B, T, _ = x.shape
+        return self.mix(F.rms_norm(x, (self.dim,), self.in_norm.to(x.dtype), self.eps))
+
+    def mix(self, h: torch.Tensor) -> torch.Tensor:
+        """The block behind its input norm: h [B, T, dim] -> [B, T, dim]."""
+        B, T, _ = h.shape
         H, D = self.heads, HEAD_DIM
-        h = F.rms_norm(x, (self.dim,), self.in_norm.to(x.dtype), self.eps)
         # four GEMMs from row blocks of the one weight: each output is a
         # contiguous [B, T, H*D] tensor, so the kernels read it without a copy
         q, k, v, gate = (F.linear(h, w) for w in self.w_qkvg.split(H * D, dim=0))

@@ -58,16 +58,18 @@ class SSMMixerBlock(nn.Module):
         self.D = nn.Parameter(torch.ones(inner, **kw))
         self.o_proj = normal(dim, inner)
 
-    def _in(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-        h = F.rms_norm(x, (self.dim,), self.in_norm.to(x.dtype), self.eps)
+    def _norm(self, x: torch.Tensor) -> torch.Tensor:
+        return F.rms_norm(x, (self.dim,), self.in_norm.to(x.dtype), self.eps)
+
+    def _in(self, h: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         return F.linear(h, self.w_xz).split(self.inner, dim=-1)  # x and z, read in place
 
     def _dbc(self, x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         low, B, C = F.linear(x, self.w_dbc).split([self.dt_rank, self.state, self.state], dim=-1)
         return F.linear(low, self.dt_up), B, C
 
-    def _mix(self, x, cu_seqlens=None, want_state=False):
-        x, z = self._in(x)
+    def _mix(self, h, cu_seqlens=None, want_state=False):
+        x, z = self._in(h)
         x, conv = short_conv(x, self.conv_weight, self.conv_bias, output_final_state=want_state, cu_seqlens=cu_seqlens)
         dt, B, C = self._dbc(x)
         y, scan = selective_scan(x, dt, -self.A_log.exp(), B, C, self.D, z, self.dt_bias,
@@ -76,7 +78,11 @@ class SSMMixerBlock(nn.Module):
 
     def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
         """x [B, T, dim] -> [B, T, dim]; documents may be packed along T (B = 1, ``cu_seqlens``)."""
-        return self._mix(x, cu_seqlens)[0]
+        return self.mix(self._norm(x), cu_seqlens)
+
+    def mix(self, h: torch.Tensor, cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+        """The block behind its input norm: h [B, T, dim] -> [B, T, dim]."""
+        return self._mix(h, cu_seqlens)[0]
 
     def make_pool(self, slots: int) -> SSMPool:
         """Zero states for `slots` requests."""
@@ -87,7 +93,12 @@ class SSMMixerBlock(nn.Module):
     def prefill(self, x: torch.Tensor, cu_seqlens: torch.Tensor, pool: SSMPool, slots: torch.Tensor) -> torch.Tensor:
         """Prompts packed along T: x [1, T, dim], cu_seqlens [R + 1], slots [R]; the requests' states go
         to their slots of the pool.  A negative slot marks a padding request, as in ``step``.  Returns [1, T, dim]."""
-        y, conv, scan = self._mix(x, cu_seqlens, want_state=True)
+        return self.mix_prefill(self._norm(x), cu_seqlens, pool, slots)
+
+    @torch.no_grad()
+    def mix_prefill(self, h: torch.Tensor, cu_seqlens: torch.Tensor, pool: SSMPool, slots: torch.Tensor) -> torch.Tensor:
+        """``prefill`` behind the input norm."""
+        y, conv, scan = self._mix(h, cu_seqlens, want_state=True)
         if slots.dtype != torch.int32:
             slots = slots.clamp(-1, 2 ** 31 - 1).to(torch.int32)
         slots = slots.contiguous()
@@ -98,7 +109,12 @@ class SSMMixerBlock(nn.Module):
     @torch.no_grad()
     def step(self, x: torch.Tensor, pool: SSMPool, slots: torch.Tensor) -> torch.Tensor:
         """One token of each request: x [R, dim], slots int32 [R] (negative: a padding row) -> [R, dim]."""
-        x, z = self._in(x)
+        return self.mix_step(self._norm(x), pool, slots)
+
+    @torch.no_grad()
+    def mix_step(self, h: torch.Tensor, pool: SSMPool, slots: torch.Tensor) -> torch.Tensor:
+        """``step`` behind the input norm."""
+        x, z = self._in(h)
         x = short_conv_step(x, pool.conv, self.conv_weight, self.conv_bias, slots=slots)
         dt, B, C = self._dbc(x)
         y = selective_scan_step(x, dt, -self.A_log.exp(), B, C, pool.scan, self.D, z, self.dt_bias, slots=slots)
