@@ -17,6 +17,9 @@
 // of three sigmoids, rsqrt), which the SM makes at 16 a clock: both take about as long
 // (50 us per 4 x 4096 x 2048 elements), so the decay's exponential is a polynomial on
 // packed fp32 arithmetic, which also gives 1 - a^2 without cancellation.
+//
+// A run's decay P is the exponential of its tokens' summed logarithms: one rounding of 2^-24 where their product has one a
+// token, which is what a state that remembers thousands of tokens would feel.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -434,7 +437,7 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_fwd_kernel(const __
     const bool whole = n == S && !(marks.starts | marks.ends) && !steep;  // nothing special about them
     u64 a[S], bb[S];
     IoVec<T, 2> zr[S];
-    u64 p = all2(1.f), c = 0ull;
+    u64 logs = 0ull, c = 0ull;
     auto gates = [&](auto all) {
 #pragma unroll
       for (int j = 0; j < S; ++j) {
@@ -442,19 +445,22 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_fwd_kernel(const __
         const int row = warp * S + j, t = t0 + j;
         const u64 r = rec_sig(K, rec_expneg(K, rec_get<T, VEC>(s, row, rec_odd<T, VEC>(pd, P.decay.st, t)), nd));
         u64 w;
-        rec_decay<!all.value>(K, mul2(A2, r), a[j], w);
+        const u64 l = mul2(A2, r);
+        rec_decay<!all.value>(K, l, a[j], w);
+        logs = add2(logs, l);
         const u64 g = add2(rec_expneg(K, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng), K.one);
         const u64 x = rec_get<T, VEC>(s + TB, row, rec_odd<T, VEC>(px, P.x.st, t));
         bb[j] = mul2(rec_sqrt_over(w, g), x);
         if (Z) zr[j] = rec_raw<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t));
         if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
         c = fma2(a[j], c, bb[j]);
-        p = mul2(p, a[j]);
       }
     };
     if (whole) gates(RecTrue{});
     else gates(RecFalse{});
     {
+      u64 p, w;
+      rec_decay<true>(K, logs, p, w);
       const float2 pf = upk2(p), cf = upk2(c);
       sm.maps[par][warp][lane] = make_float4(pf.x, pf.y, cf.x, cf.y);
       if (lane == 0) sm.cuts[par][warp] = marks.starts;
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_bwd_kernel(const __
     const bool whole = n == S && !(marks.starts | marks.ends) && !steep;
     u64 a[S], hs[S], rr[S], ii[S], be[S];  // decay; b, then the state; the sigmoids; the normaliser
     {
-      u64 p = all2(1.f), c = 0ull, d = 0ull;
+      u64 p = all2(1.f), logs = 0ull, c = 0ull, d = 0ull;
       auto gates = [&](auto all) {
         bool open = true;  // no end among the tokens so far
 #pragma unroll
@@ -636,7 +642,9 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_bwd_kernel(const __
           if (!all.value && j >= n) break;
           rr[j] = rec_sig(P.k, rec_expneg(P.k, get(0, pd, P.decay.st, j), nd));
           u64 w;
-          rec_decay<!all.value>(P.k, mul2(A2, rr[j]), a[j], w);
+          const u64 l = mul2(A2, rr[j]);
+          rec_decay<!all.value>(P.k, l, a[j], w);
+          logs = add2(logs, l);
           be[j] = rec_sqrt(w);
           ii[j] = rec_sig(P.k, rec_expneg(P.k, get(2, pg, P.gate.st, j), ng));
           hs[j] = mul2(mul2(be[j], ii[j]), get(1, px, P.x.st, j));
@@ -656,6 +664,8 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_bwd_kernel(const __
       };
       if (whole) gates(RecTrue{});
       else gates(RecFalse{});
+      u64 w;
+      rec_decay<true>(P.k, logs, p, w);
       const float2 pf = upk2(p), cf = upk2(c);
       sm.maps[par][warp][lane] = make_float4(pf.x, pf.y, cf.x, cf.y);
       sm.back[par][warp][lane] = upk2(d);
