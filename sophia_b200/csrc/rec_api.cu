@@ -168,8 +168,9 @@ int kda_b200_recurrence_fwd(const kda_b200_recurrence_args* a, void* workspace, 
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->T == 0) return pass_state(a->h0, a->ht, (long long)a->nseq * a->E, st);
   if (!a->y) return fail(KDA_ERR_INVALID, "null output pointer");
-  if (!workspace || !aligned(workspace, 16) ||
-      workspace_bytes < kda_b200_recurrence_workspace_bytes(a->B, a->T, a->E, a->dtype, a->cu_seqlens != nullptr, 0))
+  if (a->cu_seqlens &&  // (plain rows need none)
+      (!workspace || !aligned(workspace, 16) ||
+       workspace_bytes < kda_b200_recurrence_workspace_bytes(a->B, a->T, a->E, a->dtype, 1, 0)))
     return fail(KDA_ERR_INVALID, "workspace too small: kda_b200_recurrence_workspace_bytes() bytes are needed");
   if (a->saved && (!aligned(a->saved, 16) ||
                    a->saved_bytes < kda_b200_recurrence_saved_bytes(a->B, a->T, a->E, a->dtype)))

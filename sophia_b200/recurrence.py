@@ -25,8 +25,18 @@ __all__ = ["gated_recurrence", "gated_recurrence_step"]
 TILE = {torch.float32: 32, torch.bfloat16: 64, torch.float16: 64}  # tokens between the states kept for a backward
 
 
-def _strides(t: Tensor | None) -> tuple[int, int]:
-    return (0, 0) if t is None else (t.stride(0), t.stride(1))
+def _new(t: Tensor) -> Tensor:
+    """A contiguous tensor of t's shape and type."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _workspace(lib, x: Tensor, cu: Tensor | None, backward: bool) -> Tensor | None:
+    """A prompt of plain rows needs none."""
+    if cu is None and not backward:
+        return None
+    b, T, E = x.shape
+    return x.new_empty(lib.kda_b200_recurrence_workspace_bytes(b, T, E, _IO[x.dtype], int(cu is not None), int(backward)),
+                       dtype=torch.uint8)
 
 
 def _inputs(x, decay, gate, z):
@@ -37,9 +47,12 @@ def _args(rows, nseq, A, decay_bias, gate_bias, h0, cu):
     """The fields that both directions share."""
     x, decay, gate, z = rows
     b, T, E = x.shape
-    return RecArgs(b, T, E, nseq, _IO[x.dtype], 0, _ptr(x), _ptr(decay), _ptr(gate), _ptr(z), *_strides(x),
-                   *_strides(decay), *_strides(gate), *_strides(z), _ptr(A), _ptr(decay_bias), _ptr(gate_bias), _ptr(h0),
-                   _ptr(cu))
+    xb, xt, _ = x.stride()
+    db, dt, _ = decay.stride()
+    gb, gt, _ = gate.stride()
+    zb, zt, _ = (0, 0, 0) if z is None else z.stride()
+    return RecArgs(b, T, E, nseq, _IO[x.dtype], 0, x.data_ptr(), decay.data_ptr(), gate.data_ptr(), _ptr(z), xb, xt, db, dt,
+                   gb, gt, zb, zt, A.data_ptr(), _ptr(decay_bias), _ptr(gate_bias), _ptr(h0), _ptr(cu))
 
 
 def _fwd_impl(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, want_final, training):
@@ -49,14 +62,14 @@ def _fwd_impl(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, want_
     lib, io = _lib.load(), _IO[x.dtype]
     rows = _inputs(x, decay, gate, z)
     A, decay_bias, gate_bias, h0, cu = _param(A), _param(decay_bias), _param(gate_bias), _param(h0), _cu(cu_seqlens)
-    y = x.new_empty((b, T, E))
+    y = _new(x)
     ht = x.new_empty((nseq, E) if want_final else 0, dtype=torch.float32)
     saved = x.new_empty(lib.kda_b200_recurrence_saved_bytes(b, T, E, io) if training else 0, dtype=torch.uint8)
     if b:
-        ws = x.new_empty(lib.kda_b200_recurrence_workspace_bytes(b, T, E, io, int(cu is not None), 0), dtype=torch.uint8)
+        ws = _workspace(lib, x, cu, False)
         a = _args(rows, nseq, A, decay_bias, gate_bias, h0, cu)
-        a.y, a.ht, a.saved, a.saved_bytes = _ptr(y), _ptr(ht), _ptr(saved), saved.numel()
-        _call(lib.kda_b200_recurrence_fwd, x.device, a, _ptr(ws), ws.numel())
+        a.y, a.ht, a.saved, a.saved_bytes = y.data_ptr(), ht.data_ptr(), saved.data_ptr(), saved.numel()
+        _call(lib.kda_b200_recurrence_fwd, x.device, a, _ptr(ws), 0 if ws is None else ws.numel())
     return y, ht, saved
 
 
@@ -64,22 +77,22 @@ def _bwd_impl(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, saved
     """Returns (dx, ddecay, dgate, dA, dz, ddecay_bias, dgate_bias, dh0); absent ones empty."""
     b, T, E = x.shape
     nseq = b if cu_seqlens is None else cu_seqlens.shape[0] - 1
-    lib, io = _lib.load(), _IO[x.dtype]
+    lib = _lib.load()
     rows, dyr = _inputs(x, decay, gate, z), _rows(dy, x.dtype)
     Af, dbias, gbias, h, cu, dh = (_param(A), _param(decay_bias), _param(gate_bias), _param(h0), _cu(cu_seqlens),
                                    _param(dht))
-    dx, ddecay, dgate = (x.new_empty((b, T, E)) for _ in range(3))
-    dz = x.new_empty((b, T, E) if z is not None else 0)
+    dx, ddecay, dgate = _new(x), _new(x), _new(x)
+    dz = _new(x) if z is not None else x.new_empty(0)
     dA, ddb, dgb = (x.new_empty(E, dtype=torch.float32) for _ in range(3))
     dh0 = x.new_empty((nseq, E) if want_dh0 else 0, dtype=torch.float32)
     if b:
-        ws = x.new_empty(lib.kda_b200_recurrence_workspace_bytes(b, T, E, io, int(cu is not None), 1), dtype=torch.uint8)
+        ws = _workspace(lib, x, cu, True)
         a = _args(rows, nseq, Af, dbias, gbias, h, cu)
-        a.saved, a.saved_bytes = _ptr(saved), saved.numel()
-        a.dy, a.dy_sb, a.dy_st = _ptr(dyr), dyr.stride(0), dyr.stride(1)
+        a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
+        a.dy, (a.dy_sb, a.dy_st, _) = dyr.data_ptr(), dyr.stride()
         a.dht, a.dx, a.ddecay, a.dgate, a.dz, a.dh0 = _ptr(dh), _ptr(dx), _ptr(ddecay), _ptr(dgate), _ptr(dz), _ptr(dh0)
         a.dA, a.ddecay_bias, a.dgate_bias = _ptr(dA), _ptr(ddb), _ptr(dgb)
-        _call(lib.kda_b200_recurrence_bwd, x.device, a, _ptr(ws), ws.numel())
+        _call(lib.kda_b200_recurrence_bwd, x.device, a, ws.data_ptr(), ws.numel())
     else:
         dA.zero_(), ddb.zero_(), dgb.zero_()
     return dx, ddecay, dgate, dA, dz, ddb, dgb, dh0
@@ -145,19 +158,16 @@ class _RecEager(torch.autograd.Function):
     """The eager path: the custom ops' implementation without their dispatch."""
 
     @staticmethod
-    def forward(ctx, x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, want_final, grad_mode):
-        # (the caller's grad mode: it is off in here, and ctx.needs_input_grad follows requires_grad alone)
-        training = grad_mode and any(ctx.needs_input_grad)
-        y, ht, saved = _fwd_impl(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, want_final, training)
-        if training:
-            ctx.save_for_backward(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, saved)
+    def forward(ctx, x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, want_final):
+        y, ht, saved = _fwd_impl(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, want_final, True)
+        ctx.save_for_backward(x, decay, gate, A, z, decay_bias, gate_bias, h0, cu_seqlens, saved)
         ctx.set_materialize_grads(False)
         return y, ht
 
     @staticmethod
     def backward(ctx, dy, dht):
         grads = _first_order("gated_recurrence", ctx, _grads(ctx, dy, dht, _bwd_impl), dy, dht)
-        return (*grads, None, None, None)
+        return (*grads, None, None)
 
 
 def _check(what, x, dims, decay, gate, A, z, decay_bias, gate_bias) -> torch.dtype:
@@ -204,10 +214,14 @@ def gated_recurrence(x: Tensor, decay: Tensor, gate: Tensor, A: Tensor, z: Tenso
     like = x.dtype
     x, decay, gate, z = _promoted(io, x, decay, gate, z)
     args = (x, decay, gate, A, z, decay_bias, gate_bias, initial_state, cu_seqlens, bool(output_final_state))
+    training = _needs_grad(x, decay, gate, A, z, decay_bias, gate_bias, initial_state)
     if torch.compiler.is_compiling():
-        y, ht, _ = _rec_fwd(*args, _needs_grad(x, decay, gate, A, z, decay_bias, gate_bias, initial_state))
+        y, ht, _ = _rec_fwd(*args, training)
+    elif training:
+        y, ht = _RecEager.apply(*args)
     else:
-        y, ht = _RecEager.apply(*args, torch.is_grad_enabled())
+        _check_no_tangents(what, x, decay, gate, A, z, decay_bias, gate_bias, initial_state)
+        y, ht, _ = _fwd_impl(*args, False)
     return (y if y.dtype == like else y.to(like)), (ht if output_final_state else None)
 
 

@@ -17,7 +17,8 @@ from torch import Tensor
 
 from . import _lib
 from ._lib import NormArgs
-from .ssm import _IO, _call, _check_activations, _check_params, _first_order, _needs_grad, _param, _ptr, _rows
+from .ssm import (_IO, _call, _check_activations, _check_no_tangents, _check_params, _first_order, _needs_grad, _param, _ptr,
+                  _rows)
 
 __all__ = ["residual_norm"]
 
@@ -26,45 +27,55 @@ MAX_WIDTH = 8192
 
 def _args(x, o, gate, w, wb, scale, seed, seed_value, offset, p, eps):
     b, t, D = x.shape
-    gs = (0, 0) if gate is None else (gate.stride(0), gate.stride(1))
-    return NormArgs(b, t, D, _IO[o.dtype], _IO[x.dtype], offset, _ptr(x), _ptr(o), _ptr(gate), x.stride(0), x.stride(1),
-                    o.stride(0), o.stride(1), *gs, _ptr(w), _ptr(wb), _ptr(scale), _ptr(seed), seed_value & (2 ** 64 - 1), p,
-                    eps)
+    xb, xt, _ = x.stride()
+    ob, ot, _ = o.stride()
+    gb, gt, _ = (0, 0, 0) if gate is None else gate.stride()
+    return NormArgs(b, t, D, _IO[o.dtype], _IO[x.dtype], offset, x.data_ptr(), o.data_ptr(), _ptr(gate), xb, xt, ob, ot, gb,
+                    gt, _ptr(w), _ptr(wb), _ptr(scale), _ptr(seed), seed_value & (2 ** 64 - 1), p, eps)
+
+
+def _new(t: Tensor) -> Tensor:
+    """A contiguous tensor of t's shape and type."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _fwd_impl(x, o, gate, weight, branch_weight, scale, seed, seed_value, offset, p, eps, training):
     """x, o, gate [B, T, D].  Returns (stream, next block's input or empty, reciprocal roots or empty)."""
     xr, orr, gr = _rows(x, x.dtype), _rows(o, o.dtype), None if gate is None else _rows(gate, o.dtype)
-    w, wb, sc = _param(weight), _param(branch_weight), _param(scale)
-    v = x.new_empty(x.shape)
-    n = o.new_empty(o.shape if weight is not None else 0)
+    a = _args(xr, orr, gr, _param(weight), _param(branch_weight), _param(scale), seed, seed_value, offset, p, eps)
+    v = _new(x)
+    n = _new(o) if weight is not None else o.new_empty(0)
     rstd = x.new_empty((x.shape[0] * x.shape[1], 2) if training else 0, dtype=torch.float32)
-    a = _args(xr, orr, gr, w, wb, sc, seed, seed_value, offset, p, eps)
-    a.v, a.n, a.rstd = _ptr(v), _ptr(n), _ptr(rstd)
+    a.v, a.n, a.rstd = v.data_ptr(), n.data_ptr(), rstd.data_ptr()
     _call(_lib.load().kda_b200_norm_fwd, x.device, a)
     return v, n, rstd
+
+
+def _sum_of(t: Tensor | None, x: Tensor) -> Tensor:
+    """Where the gradient of a parameter goes: float32, empty where there is no parameter."""
+    if t is not None and t.dtype == torch.float32:
+        return _new(t)
+    return x.new_empty(0 if t is None else t.shape, dtype=torch.float32)
 
 
 def _bwd_impl(x, o, gate, weight, branch_weight, scale, seed, rstd, dv, dn, seed_value, offset, p, eps):
     """Returns (dx, do, dgate, dweight, dbranch_weight, dscale); absent ones empty."""
     lib = _lib.load()
     xr, orr, gr = _rows(x, x.dtype), _rows(o, o.dtype), None if gate is None else _rows(gate, o.dtype)
-    w, wb, sc = _param(weight), _param(branch_weight), _param(scale)
+    a = _args(xr, orr, gr, _param(weight), _param(branch_weight), _param(scale), seed, seed_value, offset, p, eps)
     dvr = None if dv is None else _rows(dv, x.dtype)
     dnr = None if dn is None else _rows(dn, o.dtype)
-    D = x.shape[2]
-    dx, do = x.new_empty(x.shape), o.new_empty(o.shape)
-    dgate = o.new_empty(o.shape if gate is not None else 0)
-    dw, dwb, dscale = (x.new_empty(0 if t is None else D, dtype=torch.float32) for t in (weight, branch_weight, scale))
-    ws = x.new_empty(lib.kda_b200_norm_workspace_bytes(x.shape[0], x.shape[1], D, _IO[o.dtype]), dtype=torch.uint8)
-    a = _args(xr, orr, gr, w, wb, sc, seed, seed_value, offset, p, eps)
-    a.rstd = _ptr(rstd)
+    dx, do = _new(x), _new(o)
+    dgate = _new(o) if gate is not None else o.new_empty(0)
+    dw, dwb, dscale = _sum_of(weight, x), _sum_of(branch_weight, x), _sum_of(scale, x)
+    ws = x.new_empty(lib.kda_b200_norm_workspace_bytes(a.B, a.T, a.D, a.dtype), dtype=torch.uint8)
+    a.rstd = rstd.data_ptr()
     if dvr is not None:
-        a.dv, a.dv_sb, a.dv_st = _ptr(dvr), dvr.stride(0), dvr.stride(1)
+        a.dv, (a.dv_sb, a.dv_st, _) = dvr.data_ptr(), dvr.stride()
     if dnr is not None:
-        a.dn, a.dn_sb, a.dn_st = _ptr(dnr), dnr.stride(0), dnr.stride(1)
-    a.dx, a.d_o, a.dgate, a.dw, a.dwb, a.dscale = (_ptr(t) for t in (dx, do, dgate, dw, dwb, dscale))
-    _call(lib.kda_b200_norm_bwd, x.device, a, _ptr(ws), ws.numel())
+        a.dn, (a.dn_sb, a.dn_st, _) = dnr.data_ptr(), dnr.stride()
+    a.dx, a.d_o, a.dgate, a.dw, a.dwb, a.dscale = (t.data_ptr() for t in (dx, do, dgate, dw, dwb, dscale))
+    _call(lib.kda_b200_norm_bwd, x.device, a, ws.data_ptr(), ws.numel())
     return dx, do, dgate, dw, dwb, dscale
 
 
@@ -119,20 +130,17 @@ class _NormEager(torch.autograd.Function):
     """The eager path: the custom ops' implementation without their dispatch."""
 
     @staticmethod
-    def forward(ctx, x, o, gate, weight, branch_weight, scale, seed, seed_value, offset, p, eps, grad_mode):
-        # (the caller's grad mode: it is off in here, and ctx.needs_input_grad follows requires_grad alone)
-        training = grad_mode and any(ctx.needs_input_grad)
-        v, n, rstd = _fwd_impl(x, o, gate, weight, branch_weight, scale, seed, seed_value, offset, p, eps, training)
-        if training:
-            ctx.save_for_backward(x, o, gate, weight, branch_weight, scale, seed, rstd)
-            ctx.numbers = (seed_value, offset, p, eps)
+    def forward(ctx, x, o, gate, weight, branch_weight, scale, seed, seed_value, offset, p, eps):
+        v, n, rstd = _fwd_impl(x, o, gate, weight, branch_weight, scale, seed, seed_value, offset, p, eps, True)
+        ctx.save_for_backward(x, o, gate, weight, branch_weight, scale, seed, rstd)
+        ctx.numbers = (seed_value, offset, p, eps)
         ctx.set_materialize_grads(False)
         return v, n
 
     @staticmethod
     def backward(ctx, dv, dn):
         grads = _first_order("residual_norm", ctx, _grads(ctx, dv, dn, _bwd_impl), dv, dn)
-        return (*grads, *[None] * 6)
+        return (*grads, *[None] * 5)
 
 
 def _seed_of(seed, device):
@@ -211,12 +219,20 @@ def residual_norm(residual: Tensor, branch: Tensor, weight: Tensor | None = None
     if io != torch.float32 and residual.dtype not in (io, torch.float32):  # bf16 beside fp16
         io = torch.float32
     shape = branch.shape
-    x, o, g = (_three(t if t is None or t.dtype == d else t.to(d)) for t, d in ((residual, wide), (branch, io), (gate, io)))
+    x = residual if residual.dtype == wide else residual.to(wide)
+    o = branch if branch.dtype == io else branch.to(io)
+    g = gate if gate is None or gate.dtype == io else gate.to(io)
+    if branch.dim() != 3:
+        x, o, g = _three(x), _three(o), _three(g)
     args = (x, o, g, weight, branch_weight, scale, seed, value, offset, float(dropout_p), float(eps))
+    training = _needs_grad(residual, branch, weight, branch_weight, gate, scale)
     if torch.compiler.is_compiling():
-        v, n, _ = _norm_fwd(*args, _needs_grad(residual, branch, weight, branch_weight, gate, scale))
+        v, n, _ = _norm_fwd(*args, training)
+    elif training:
+        v, n = _NormEager.apply(*args)
     else:
-        v, n = _NormEager.apply(*args, torch.is_grad_enabled())
+        _check_no_tangents(what, residual, branch, weight, branch_weight, gate, scale)
+        v, n, _ = _fwd_impl(*args, False)
     if v.shape != shape:
         v = v.reshape(shape)
     if v.dtype != residual.dtype:
