@@ -209,8 +209,9 @@ int kda_b200_device_error(int reset);
  *   10    a tensor-core completion wait of the forward chunk kernel ran out;
  *   11    a single-token call named a state slot past its pool (that row was
  *         treated as padding);
- *   12    a wait of the gated recurrence for a tile, or for the states of the
- *         cluster's other CTAs, ran out: the call's outputs are not valid.
+ *   12    a wait of the gated recurrence for a tile or for the states of the
+ *         cluster's other CTAs, or of the residual norm for its rows, ran out: the
+ *         call's outputs are not valid.
  * A kernel that records a timeout lets its copies in flight land (a second
  * bounded wait), frees what it holds and returns; later calls are unaffected.
  */

@@ -265,6 +265,11 @@ __device__ __forceinline__ void rec_put(T* row, u64 v, int nch) {
     if (c1 < nch) row[c1] = io_from_f<T>(f.y);
   }
 }
+// The rates in log2 units: NaN for a positive one, whose normaliser is not real.
+__device__ __forceinline__ u64 rec_rates(u64 a) {
+  const float2 f = upk2(a);
+  return pk2(f.x > 0.f ? __int_as_float(0x7fffffff) : f.x * LOG2E, f.y > 0.f ? __int_as_float(0x7fffffff) : f.y * LOG2E);
+}
 // fp32 vectors over the channels
 __device__ __forceinline__ u64 rec_vec(const float* p, bool vec, int nch, float none) {
   const int c0 = rec_lane_ch(vec, 0), c1 = rec_lane_ch(vec, 1);
@@ -409,7 +414,7 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_fwd_kernel(const __
   for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
   const RecConst& K = P.k;
-  const u64 A2 = mul2(rec_vec(P.A + ch0, VEC, nch, 0.f), all2(LOG2E));
+  const u64 A2 = rec_rates(rec_vec(P.A + ch0, VEC, nch, 0.f));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const bool steep = __any_sync(0xffffffffu, upk2(A2).x < -126.f || upk2(A2).y < -126.f);
@@ -602,7 +607,7 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_bwd_kernel(const __
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
-  const u64 A1 = rec_vec(P.A + ch0, VEC, nch, 0.f), A2 = mul2(A1, all2(LOG2E));
+  const u64 A1 = rec_vec(P.A + ch0, VEC, nch, 0.f), A2 = rec_rates(A1);
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const bool steep = __any_sync(0xffffffffu, upk2(A2).x < -126.f || upk2(A2).y < -126.f);
@@ -809,7 +814,7 @@ __global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(const __grid
   const int c = (blockIdx.x * REC_STEP_THREADS + threadIdx.x) * V;
   if (c >= P.E) return;
   auto vec = [&](const float* p) { return p ? pk2(__ldg(p + c), VEC ? __ldg(p + c + 1) : 0.f) : 0ull; };
-  const u64 A2 = mul2(vec(P.A), all2(LOG2E));
+  const u64 A2 = rec_rates(vec(P.A));
   const u64 nd = mul2(vec(P.decay_bias), all2(-LOG2E)), ng = mul2(vec(P.gate_bias), all2(-LOG2E));
   for (int r = blockIdx.y; r < P.rows; r += gridDim.y) {
     const int slot = step_slot(P.slots, r, P.pool, P.err);

@@ -235,6 +235,40 @@ def test_gates_at_their_ends():
 
 
 @gpu
+def test_positive_rate_is_not_a_number_in_its_channel():
+    rn = gen(14)
+    ts = inputs(rn, torch.float32, 2, 40, 70, 2, grad=False)
+    y, ht = call(ts, None)
+    bad = dict(ts, A=ts["A"].clone())
+    bad["A"][[3, 68]] = torch.tensor([0.5, float("nan")], device="cuda")
+    by, bht = call(bad, None)
+    hit = torch.zeros(70, dtype=torch.bool, device="cuda")
+    hit[[3, 68]] = True
+    assert by[..., hit].isnan().all() and torch.equal(by[..., ~hit], y[..., ~hit]) and torch.equal(bht[:, ~hit], ht[:, ~hit])
+    pool = ts["h0"].clone()
+    step = sophia_b200.gated_recurrence_step(*(bad[k][:, 0] for k in ("x", "decay", "gate")), bad["A"], pool)
+    assert step[:, hit].isnan().all() and torch.isfinite(step[:, ~hit]).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_expanded_transposed_and_far_rows(dtype):
+    """Strides that the tile copies have no map for, and rows more than 2^31 elements apart: the same bits."""
+    rn = gen(15)
+    A = -torch.ones(64, device="cuda")
+    run = lambda t: sophia_b200.gated_recurrence(t, t, t, A, t)[0]  # noqa: E731
+    wide = torch.empty(2 ** 31 + 2 ** 20, device="cuda", dtype=dtype)
+    far = torch.as_strided(wide, (2, 40, 64), (2 ** 31, 64, 1))
+    far.copy_(rn(2, 40, 64))
+    apart = torch.as_strided(wide, (1, 33, 64), (0, 2 ** 26, 1))
+    for t in (rn(1, 40, 64, dtype=dtype).expand(3, 40, 64), rn(3, 1, 64, dtype=dtype).expand(3, 40, 64),
+              rn(40, 3, 64, dtype=dtype).transpose(0, 1), rn(3, 64, 40, dtype=dtype).transpose(1, 2), far):
+        close("y", run(t), run(t.contiguous()).double(), dtype)
+    apart.copy_(rn(1, 33, 64))
+    close("y", run(apart), run(apart.contiguous()).double(), dtype)
+
+
+@gpu
 def test_not_a_number_stays_in_its_document_and_channel():
     rn = gen(4)
     cu = cu_of((70, 3, 127))
