@@ -15,9 +15,9 @@ namespace kda {
 struct RnShape {
   int v, k, warps, groups, lanes;
 };
-// Rows that are read as they lie, element by element: four neighbours a piece, 8 or 16 channels a thread.
+// Rows that are read as they lie, element by element: 8 or 16 channels a thread.
 inline RnShape rn_plain_shape(int D) {
-  RnShape s{4, D <= 512 ? 2 : 4, 0, 0, 32};
+  RnShape s{4, D <= 2048 ? 2 : 4, 0, 0, 32};
   s.warps = (D + 128 * s.k - 1) / (128 * s.k);
   s.groups = std::max(1, 8 / s.warps);
   return s;
@@ -83,8 +83,9 @@ template <typename TX, typename TO>
 RnFit rn_bwd_fit(const RnParams& p, const RnShape& s) {
   return rn_fit(s, p.rows, rn_bwd_row(p.D, sizeof(TX), sizeof(TO), p.g.p, p.dv.p, p.dn.p), (size_t)3 * p.D * 4);
 }
+// (the backward: as many as the SMs hold at once, which is one of more than eight warps)
 inline long long rn_plain_ctas(long long rows, const RnShape& s) {
-  return std::min(rn_units(rows, s.groups), (long long)std::max(1, 24 / (s.warps * s.groups)) * sm_count());
+  return std::min(rn_units(rows, s.groups), (long long)(s.warps <= 8 ? 2 : 1) * sm_count());
 }
 
 template <typename TX, typename TO>
@@ -135,7 +136,7 @@ int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, cons
 
 template <typename TX, typename TO, int K>
 int launch_rn_bwd(RnParams& p, const RnShape& s, cudaStream_t st) {
-  const size_t smem = (size_t)s.groups * 3 * ((p.D + 3) / 4) * 16;
+  const size_t smem = (size_t)s.groups * 3 * p.D * 4;
   auto kernel = rn_bwd_kernel<TX, TO, K>;
   if (int rc = rn_smem(kernel, smem)) return rc;
   p.parts = (int)rn_plain_ctas(p.rows, s);

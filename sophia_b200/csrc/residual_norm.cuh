@@ -12,9 +12,9 @@
 // (s the gate's sigmoid, u the branch behind its norm).  The sums over rows go by
 // CTA into partial rows, summed in order by one more kernel.
 //
-// HBM-bound: 10 bytes an element forward and 16 backward when all is 16-bit.  W
-// warps own a row, K pieces of V channels a thread; the row stays in registers
-// between its two reductions.
+// 10 bytes an element forward and 16 backward when all is 16-bit; how rows are laid over
+// threads, and what bounds that, stands at the two sorts of kernels: rows by bulk
+// copies, and rows wherever they lie.
 //
 // Dropout draws 32 bits per element from Philox4x32-10 (Salmon, Moraes, Dror and Shaw,
 // 2011): key = the seed, counter = (channel / 4, row, row >> 32, offset), the four words
@@ -53,17 +53,15 @@ struct RnParams {
 
 // ---------------------------------------------------------------- rows
 
-// Four neighbouring channels, of which the first n are there, wherever they lie: element by element.
+// Rows wherever they lie go element by element: four channels 32 apart, of which the first n are there, so that a warp's
+// lanes have neighbours (with neighbours in a thread, a store touched four times the sectors: 98 and 320 us against 95 and
+// 295, the two directions at 8192 x 2043).
 template <typename T>
 struct RnFour {
   T v[4];
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = io_from_f<T>(0.f);
-  }
   __device__ __forceinline__ void load(const T* q, int n) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = i < n ? q[i] : io_from_f<T>(0.f);
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? q[32 * i] : io_from_f<T>(0.f);
   }
   __device__ __forceinline__ float get(int i) const { return io_to_f(v[i]); }
 };
@@ -71,12 +69,17 @@ template <typename T>
 __device__ __forceinline__ void rn_store(T* q, const float (&f)[4], int n) {
 #pragma unroll
   for (int i = 0; i < 4; ++i)
-    if (i < n) q[i] = io_from_f<T>(f[i]);
+    if (i < n) q[32 * i] = io_from_f<T>(f[i]);
 }
 __device__ __forceinline__ void rn_param(const float* p, int c, int n, float (&f)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = i < n ? __ldg(p + c + i) : 0.f;
+  for (int i = 0; i < 4; ++i) f[i] = i < n ? __ldg(p + c + 32 * i) : 0.f;
 }
+__device__ __forceinline__ int rn_there(int c, int D) { return min(4, max(0, (D - c + 31) >> 5)); }
+// K = 2, eight channels a thread: four CTAs an SM forward and two backward, whose column sums then stay in registers;
+// K = 4, rows above 2048 channels.  (8192 x 2043: 77 and 162 us, floors 36 and 56; with K = 4, its column sums in shared
+// memory and three CTAs an SM launched where two fitted, 95 and 295.)
+__host__ __device__ constexpr int rn_plain_threads(int k) { return k == 2 ? 256 : 512; }
 template <typename T>
 __device__ __forceinline__ const T* rn_row(const RowView& r, long long row, int T_) {
   if (T_ == 0) return static_cast<const T*>(r.p) + row * r.st;
@@ -84,17 +87,24 @@ __device__ __forceinline__ const T* rn_row(const RowView& r, long long row, int 
   return static_cast<const T*>(r.p) + b * r.sb + (row - b * T_) * r.st;
 }
 
-// Sum over the `warps` warps of a row's group, the same in every thread.  `slot` alternates, so that one barrier is enough.
-__device__ __forceinline__ float rn_sum(float a, float (*part)[RN_MAX_WARPS], int slot, int group, int warps) {
+// Sums over the `warps` warps of a row's group, the same in every thread.  `part` is another one than at the sum before, so
+// that one barrier is enough.
+template <int N>
+__device__ __forceinline__ void rn_sum(float (&a)[N], float (*part)[RN_MAX_WARPS], int group, int warps) {
 #pragma unroll
-  for (int m = 16; m >= 1; m >>= 1) a += __shfl_xor_sync(0xffffffffu, a, m);
-  if (warps == 1) return a;
-  const int warp = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) part[slot][warp] = a;
+  for (int m = 16; m >= 1; m >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], m);
+  if (warps == 1) return;
+  if ((threadIdx.x & 31) == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) part[i][threadIdx.x >> 5] = a[i];
   asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
-  float t = 0.f;
-  for (int w = 0; w < warps; ++w) t += part[slot][group * warps + w];
-  return t;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    a[i] = 0.f;
+    for (int w = 0; w < warps; ++w) a[i] += part[i][group * warps + w];
+  }
 }
 
 // ---------------------------------------------------------------- dropout
@@ -111,28 +121,28 @@ __device__ __forceinline__ uint4 philox(uint4 c, unsigned k0, unsigned k1) {
   }
   return c;
 }
-// keep / (1 - p) of the four channels from c on, c a multiple of 4
-__device__ __forceinline__ void rn_keep(const RnParams& P, unsigned k0, unsigned k1, long long row, int c, float (&m)[4]) {
-  if (!P.dropout) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) m[i] = 1.f;
-    return;
-  }
-  const uint4 r = philox(make_uint4((unsigned)c / 4, (unsigned)row, (unsigned)(row >> 32), P.offset), k0, k1);
-  const unsigned word[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = word[i] < P.drop || P.drop_all ? 0.f : P.keep_scale;
+// Bit i: channel c + 32 i is kept.  c - lane is a multiple of 128; the whole warp calls.  A lane draws the four words of
+// the lane % 4-th 32 channels' group lane / 4, and the warp's votes on them give every lane its own.
+__device__ __forceinline__ unsigned rn_kept(const RnParams& P, unsigned k0, unsigned k1, long long row, int c) {
+  const int lane = threadIdx.x & 31, first = c - lane;
+  const uint4 r = philox(make_uint4((unsigned)first / 4 + 8 * (lane & 3) + lane / 4, (unsigned)row, (unsigned)(row >> 32), P.offset),
+                         k0, k1);
+  const unsigned b0 = __ballot_sync(0xffffffffu, r.x >= P.drop), b1 = __ballot_sync(0xffffffffu, r.y >= P.drop);
+  const unsigned b2 = __ballot_sync(0xffffffffu, r.z >= P.drop), b3 = __ballot_sync(0xffffffffu, r.w >= P.drop);
+  const unsigned b = lane & 2 ? (lane & 1 ? b3 : b2) : (lane & 1 ? b1 : b0);
+  return P.drop_all ? 0u : b >> (lane & ~3) & 15u;
 }
-// a product with keep / (1 - p) that is 0 where the element is dropped, whatever it holds
-__device__ __forceinline__ float rn_drop(float m, float a) { return m == 0.f ? 0.f : m * a; }
 
-// ---------------------------------------------------------------- forward
+// ---------------------------------------------------------------- forward, rows wherever they lie
 
+// A group of warps has a row, in registers between its two reductions.  Instructions bound it: 80 an element at 50 % of
+// the issue slots (predicates and addresses of single elements), DRAM at 26 %.
 template <typename TX, typename TO, int K>
-__global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnParams P) {
-  __shared__ float part[2][RN_MAX_WARPS];
+__global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 4 : 1) rn_fwd_kernel(const __grid_constant__ RnParams P) {
+  __shared__ float part[2][1][RN_MAX_WARPS];
+  int flip = 0;
   const int warps = P.warps, group = (threadIdx.x >> 5) / warps, groups = (blockDim.x >> 5) / warps;
-  const int me = threadIdx.x - group * warps * 32, stride = warps * 32 * 4;
+  const int me = threadIdx.x - group * warps * 32, stride = warps * 128, c0 = me / 32 * 128 + me % 32;
   const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / P.D;
@@ -144,34 +154,31 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
     RnFour<TX> x[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
-      if (c < P.D) {
-        o[k].load(po + c, n4);
-        x[k].load(px + c, n4);
-        if (pg) g[k].load(pg + c, n4);
-      } else {
-        o[k].zero();
-        x[k].zero();
-      }
+      const int c = c0 + k * stride, n4 = rn_there(c, P.D);
+      o[k].load(po + c, n4);
+      x[k].load(px + c, n4);
+      if (pg) g[k].load(pg + c, n4);
     }
     float rb = 1.f;
     if (P.wb) {
-      float ss = 0.f;
+      float ss[1] = {0.f};
 #pragma unroll
       for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ss = fmaf(o[k].get(i), o[k].get(i), ss);
-      rb = rsqrtf(fmaf(rn_sum(ss, part, 0, group, warps), inv, P.eps));
+        for (int i = 0; i < 4; ++i) ss[0] = fmaf(o[k].get(i), o[k].get(i), ss[0]);
+      rn_sum(ss, part[flip ^= 1], group, warps);
+      rb = rsqrtf(fmaf(ss[0], inv, P.eps));
     }
-    float v[K][4], ss = 0.f;
+    float v[K][4], ss[1] = {0.f};
     TX* pv = static_cast<TX*>(P.v) + row * P.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
+      const int c = c0 + k * stride, n4 = rn_there(c, P.D);
+      const unsigned kept = P.dropout ? rn_kept(P, k0, k1, row, c) : 15u;
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[k][i] = 0.f;
-      if (c < P.D) {
-        float f[4], m[4], u[4];
+      if (n4 > 0) {
+        float f[4], u[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = o[k].get(i);
         if (P.wb) {
@@ -182,11 +189,9 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
         if (pg)
 #pragma unroll
           for (int i = 0; i < 4; ++i) u[i] *= sigmoidf_(g[k].get(i));
-        if (P.dropout) {
-          rn_keep(P, k0, k1, row, c, m);
+        if (P.dropout)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[i] = rn_drop(m[i], u[i]);
-        }
+          for (int i = 0; i < 4; ++i) u[i] = kept >> i & 1 ? P.keep_scale * u[i] : 0.f;
         if (P.scale) {
           rn_param(P.scale, c, n4, f);
 #pragma unroll
@@ -195,19 +200,20 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           v[k][i] = x[k].get(i) + u[i];
-          ss = fmaf(v[k][i], v[k][i], ss);
+          ss[0] = fmaf(v[k][i], v[k][i], ss[0]);
         }
         rn_store(pv + c, v[k], n4);
       }
     }
     float r = 0.f;
     if (P.w) {
-      r = rsqrtf(fmaf(rn_sum(ss, part, 1, group, warps), inv, P.eps));
+      rn_sum(ss, part[flip ^= 1], group, warps);
+      r = rsqrtf(fmaf(ss[0], inv, P.eps));
       TO* pn = static_cast<TO*>(P.n) + row * P.D;
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
-        if (c < P.D) {
+        const int c = c0 + k * stride, n4 = rn_there(c, P.D);
+        if (n4 > 0) {
           float f[4];
           rn_param(P.w, c, n4, f);
 #pragma unroll
@@ -220,8 +226,6 @@ __global__ void __launch_bounds__(512) rn_fwd_kernel(const __grid_constant__ RnP
       P.rstd[2 * row] = rb;
       P.rstd[2 * row + 1] = r;
     }
-    if (warps > 1 && !(P.wb && P.w))  // one reduction a row: its slot is written again for the next row
-      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
   }
 }
 
@@ -450,25 +454,6 @@ __device__ __forceinline__ uint32_t rn_word(f16, u64 v) {
   const __half2 h = __floats2half2_rn(f.x, f.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-template <typename T, int V>
-__device__ __forceinline__ void rn_get(const T* q, u64 (&f)[V / 2]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-      const ulonglong2 r = reinterpret_cast<const ulonglong2*>(q)[i];
-      f[2 * i] = r.x;
-      f[2 * i + 1] = r.y;
-    }
-  } else {
-    static_assert(V == 8, "16-bit rows go in pieces of eight channels");
-    const uint4 r = *reinterpret_cast<const uint4*>(q);
-    f[0] = rn_pair(T(), r.x);
-    f[1] = rn_pair(T(), r.y);
-    f[2] = rn_pair(T(), r.z);
-    f[3] = rn_pair(T(), r.w);
-  }
-}
-// The same from shared memory.
 template <typename T, int V>
 __device__ __forceinline__ void rn_take(uint32_t at, u64 (&f)[V / 2]) {
   if constexpr (sizeof(T) == 4) {
@@ -830,28 +815,32 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
   for (int i = threadIdx.x; i < 3 * D; i += blockDim.x) out[i] = params[i];
 }
 
-// ---------------------------------------------------------------- backward
+// ---------------------------------------------------------------- backward, rows wherever they lie
 
+// (The row's three sums, and what they are for, as in the kernel above.)
 template <typename TX, typename TO, int K>
-__global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnParams P) {
-  extern __shared__ __align__(16) float acc[];  // [groups][3][D, in whole fours]: every thread adds to its own channels
-  __shared__ float part[2][RN_MAX_WARPS];
+__global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 2 : 1) rn_bwd_kernel(const __grid_constant__ RnParams P) {
+  extern __shared__ __align__(16) float acc[];  // [groups][3][D] column sums: a thread's own channels (K = 2: at the end)
+  __shared__ float part[2][3][RN_MAX_WARPS];
+  int flip = 0;
   const int warps = P.warps, group = (threadIdx.x >> 5) / warps, groups = (blockDim.x >> 5) / warps;
-  const int me = threadIdx.x - group * warps * 32, stride = warps * 32 * 4;
+  const int me = threadIdx.x - group * warps * 32, stride = warps * 128, c0 = me / 32 * 128 + me % 32;
   const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / P.D;
-  const int D4 = (P.D + 3) & ~3;
-  float* sums = acc + (long long)group * 3 * D4;
+  float* sums = acc + group * 3 * P.D;
+  float mine[3][K][4] = {};  // (K = 2)
+  if (K > 2)
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int c = me * 4 + k * stride;
-    if (c < P.D)
-      for (int q = 0; q < 3; ++q) *reinterpret_cast<float4*>(sums + q * D4 + c) = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  auto add = [&](int q, int c, const float (&f)[4]) {
-    float4& t = *reinterpret_cast<float4*>(sums + q * D4 + c);
-    t = make_float4(t.x + f[0], t.y + f[1], t.z + f[2], t.w + f[3]);
+    for (int k = 0; k < K; ++k)
+      for (int i = 0; i < rn_there(c0 + k * stride, P.D); ++i)
+        for (int q = 0; q < 3; ++q) sums[q * P.D + c0 + k * stride + 32 * i] = 0.f;
+  auto add = [&](int q, int k, int c, int n, const float (&f)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (K == 2) mine[q][k][i] += f[i];
+      else if (i < n) sums[q * P.D + c + 32 * i] += f[i];
+    }
   };
   for (long long row = (long long)blockIdx.x * groups + group; row < P.rows; row += (long long)gridDim.x * groups) {
     const TX* px = rn_row<TX>(P.x, row, P.T);
@@ -863,120 +852,112 @@ __global__ void __launch_bounds__(512) rn_bwd_kernel(const __grid_constant__ RnP
     RnFour<TX> x[K], dv[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
-      o[k].zero(), g[k].zero(), dn[k].zero(), x[k].zero(), dv[k].zero();
-      if (c < P.D) {
-        o[k].load(po + c, n4);
-        x[k].load(px + c, n4);
-        if (pg) g[k].load(pg + c, n4);
-        if (pdv) dv[k].load(pdv + c, n4);
-        if (pdn) dn[k].load(pdn + c, n4);
-      }
+      const int c = c0 + k * stride, n4 = rn_there(c, P.D);
+      o[k].load(po + c, n4);
+      x[k].load(px + c, n4);
+      if (pg) g[k].load(pg + c, n4);
+      dv[k].load(pdv + c, pdv ? n4 : 0);
+      dn[k].load(pdn + c, pdn ? n4 : 0);
     }
     const float rb = P.rstd[2 * row], r = P.rstd[2 * row + 1];
-    // the stream again, and the next norm's mean(t v)
-    float v[K][4], m[K][4], dot = 0.f;
+    // the stream again, and the row's sums (as above)
+    float v[K][4], sum[3] = {0.f, 0.f, 0.f};
+    unsigned kept[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
+      const int c = c0 + k * stride, n4 = rn_there(c, P.D);
+      kept[k] = P.dropout ? rn_kept(P, k0, k1, row, c) : 15u;
+      float f[4], t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[k][i] = 0.f, m[k][i] = 0.f;
-      if (c < P.D) {
-        float f[4], u[4];
+      for (int i = 0; i < 4; ++i) t[i] = o[k].get(i);
+      if (P.wb) {
+        rn_param(P.wb, c, n4, f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = o[k].get(i);
-        if (P.wb) {
-          rn_param(P.wb, c, n4, f);
+        for (int i = 0; i < 4; ++i) t[i] *= rb * f[i];
+      }
+      if (pg)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[i] *= rb * f[i];
-        }
-        if (pg)
+        for (int i = 0; i < 4; ++i) t[i] *= sigmoidf_(g[k].get(i));
+      if (P.scale) {
+        rn_param(P.scale, c, n4, f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[i] *= sigmoidf_(g[k].get(i));
-        rn_keep(P, k0, k1, row, c, m[k]);
-        if (P.scale) rn_param(P.scale, c, n4, f);
+        for (int i = 0; i < 4; ++i) t[i] *= f[i];
+      }
+      if (P.dropout)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[k][i] = x[k].get(i) + rn_drop(m[k][i], u[i]) * (P.scale ? f[i] : 1.f);
-        if (pdn) {
-          rn_param(P.w, c, n4, f);
+        for (int i = 0; i < 4; ++i) t[i] = kept[k] >> i & 1 ? P.keep_scale * t[i] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dot = fmaf(f[i] * dn[k].get(i), v[k][i], dot);
-        }
+      for (int i = 0; i < 4; ++i) f[i] = 0.f;
+      if (pdn) rn_param(P.w, c, n4, f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[k][i] = x[k].get(i) + t[i];
+        const float q = f[i] * dn[k].get(i);
+        sum[0] = fmaf(q, v[k][i], sum[0]);
+        sum[1] = fmaf(t[i], fmaf(r, q, dv[k].get(i)), sum[1]);
+        sum[2] = fmaf(t[i], v[k][i], sum[2]);
       }
     }
-    float mean = 0.f;
-    if (pdn) mean = rn_sum(dot, part, 0, group, warps) * inv * r * r;
-    dot = 0.f;
-    float du[K][4];
+    if (pdn || P.wb) rn_sum(sum, part[flip ^= 1], group, warps);
+    const float mean = sum[0] * inv * r * r, back = P.wb ? (sum[1] - r * mean * sum[2]) * inv * rb : 0.f;
     TX* pdx = static_cast<TX*>(P.dx) + row * P.D;
     TO* pdg = static_cast<TO*>(P.dg) + row * P.D;
     TO* pdo = static_cast<TO*>(P.d_o) + row * P.D;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
+      const int c = c0 + k * stride, n4 = rn_there(c, P.D);
+      float d[4], f[4], t[4], wb[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) du[k][i] = 0.f;
-      if (c < P.D) {
-        float d[4], f[4], t[4], wb[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = dv[k].get(i);
-        if (pdn) {
-          rn_param(P.w, c, n4, f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            d[i] = fmaf(r, fmaf(-v[k][i], mean, f[i] * dn[k].get(i)), d[i]);
-            t[i] = dn[k].get(i) * v[k][i] * r;
-          }
-          add(0, c, t);
-        }
-        rn_store(pdx + c, d, n4);
-        if (P.wb) rn_param(P.wb, c, n4, wb);
-        if (P.scale) rn_param(P.scale, c, n4, f);
-        float u[4], s[4];
+      for (int i = 0; i < 4; ++i) d[i] = dv[k].get(i);
+      if (pdn) {
+        rn_param(P.w, c, n4, f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          u[i] = P.wb ? o[k].get(i) * rb * wb[i] : o[k].get(i);
-          s[i] = pg ? sigmoidf_(g[k].get(i)) : 1.f;
-          const float dm = rn_drop(m[k][i], d[i]);           // gradient of scale u s
-          t[i] = m[k][i] == 0.f ? 0.f : dm * (u[i] * s[i]);  // of scale
-          const float ds = P.scale ? dm * f[i] : dm;         // of u s
-          du[k][i] = m[k][i] == 0.f ? 0.f : ds * s[i];
-          s[i] = m[k][i] == 0.f ? 0.f : ds * u[i] * (s[i] * (1.f - s[i]));
+          d[i] = fmaf(r, fmaf(-v[k][i], mean, f[i] * dn[k].get(i)), d[i]);
+          t[i] = dn[k].get(i) * v[k][i] * r;
         }
-        if (P.scale) add(2, c, t);
-        if (pg) rn_store(pdg + c, s, n4);
-        if (P.wb) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            t[i] = du[k][i] * o[k].get(i) * rb;
-            du[k][i] *= wb[i];
-            dot = fmaf(du[k][i], o[k].get(i), dot);
-          }
-          add(1, c, t);
-        } else {
-          rn_store(pdo + c, du[k], n4);
-        }
+        add(0, k, c, n4, t);
       }
-    }
-    if (P.wb) {
-      mean = rn_sum(dot, part, 1, group, warps) * inv * rb * rb;
+      rn_store(pdx + c, d, n4);
+      if (P.wb) rn_param(P.wb, c, n4, wb);
+      if (P.scale) rn_param(P.scale, c, n4, f);
+      float s[4];
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        const int c = me * 4 + k * stride, n4 = min(4, P.D - c);
-        if (c < P.D) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) du[k][i] = rb * fmaf(-o[k].get(i), mean, du[k][i]);
-          rn_store(pdo + c, du[k], n4);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const bool on = kept[k] >> i & 1;
+        const float u = P.wb ? o[k].get(i) * rb * wb[i] : o[k].get(i);
+        s[i] = pg ? sigmoidf_(g[k].get(i)) : 1.f;
+        const float dm = on ? (P.dropout ? P.keep_scale * d[i] : d[i]) : 0.f;  // gradient of scale u s
+        t[i] = on ? dm * (u * s[i]) : 0.f;                                      // of scale
+        const float ds = P.scale ? dm * f[i] : dm;                              // of u s
+        d[i] = on ? ds * s[i] : 0.f;                                            // of u
+        s[i] = on ? ds * u * (s[i] * (1.f - s[i])) : 0.f;
       }
+      if (P.scale) add(2, k, c, n4, t);
+      if (pg) rn_store(pdg + c, s, n4);
+      if (P.wb) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          t[i] = d[i] * o[k].get(i) * rb;
+          d[i] = rb * fmaf(-o[k].get(i), back, d[i] * wb[i]);
+        }
+        add(1, k, c, n4, t);
+      }
+      rn_store(pdo + c, d, n4);
     }
-    if (warps > 1 && !(P.wb && pdn)) asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(warps * 32) : "memory");
   }
+  if (K == 2)
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < rn_there(c0 + k * stride, P.D))
+#pragma unroll
+          for (int q = 0; q < 3; ++q) sums[q * P.D + c0 + k * stride + 32 * i] = mine[q][k][i];
   __syncthreads();
   for (int i = threadIdx.x; i < 3 * P.D; i += blockDim.x) {  // the CTA's sums, its groups in order
-    const int at = i / P.D * D4 + i % P.D;
     float t = 0.f;
-    for (int q = 0; q < groups; ++q) t += acc[(long long)q * 3 * D4 + at];
+    for (int q = 0; q < groups; ++q) t += acc[q * 3 * P.D + i];
     P.partial[(long long)blockIdx.x * 3 * P.D + i] = t;
   }
 }

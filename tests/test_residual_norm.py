@@ -140,6 +140,15 @@ def test_forward_and_gradients(case):
     check(inputs(rn, shape, wide, dtype, norm, post, gate, scale, pad), rn, p, 0x123456789ABCDEF if p else None, 41)
 
 
+@gpu
+@pytest.mark.parametrize("shape,dtype", [((900, 2043), bf16), ((650, 2501), bf16), ((1200, 131), f16), ((3, 211, 2047), f32)],
+                         ids=str)
+def test_odd_rows_many(shape, dtype):
+    """More odd rows than run at once, at both widths of a thread: the column sums go over several rows of a group."""
+    rn = gen(23)
+    check(inputs(rn, shape, f32, dtype, True, True, True, True, 0), rn, 0.1, 77, 3)
+
+
 def test_generator_known_answers():
     """The published vectors of Philox4x32-10, and the tensor form against the integers."""
     assert ref.philox([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
