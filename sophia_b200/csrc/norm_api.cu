@@ -94,7 +94,7 @@ long long norm_parts(long long rows, int D, int dtype) {
   const RnShape s = rn_bwd_shape(D, o);
   for (size_t x : {o, (size_t)4})
     for (int parts = 0; parts < 8; ++parts)
-      most = std::max(most, rn_fit(s, rows, rn_bwd_row(D, x, o, parts & 1, parts & 2, parts & 4), (size_t)3 * D * 4).ctas);
+      most = std::max(most, rn_fit(s, rows, rn_bwd_row(D, x, o, parts & 1, parts & 2, parts & 4), rn_fixed(D)).ctas);
   return most;
 }
 

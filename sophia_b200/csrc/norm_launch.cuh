@@ -56,8 +56,9 @@ struct RnFit {
   size_t smem;
 };
 inline RnFit rn_fit(const RnShape& s, long long rows, size_t row_bytes, size_t fixed) {
-  // of an SM, whose registers hold one CTA; 8 KB are static
-  const size_t room = 227 * 1024 - 8 * 1024 - fixed;
+  // of an SM, whose registers hold one CTA; up to 2 KB are static
+  static_assert(sizeof(RnShared<3>) <= 2048, "what the kernels share beside the ring");
+  const size_t room = 227 * 1024 - 2 * 1024 - fixed;
   const int per = s.warps > 1 ? 1 : 32 / s.lanes;
   RnFit f;
   // few rows: a group to an SM before the second
@@ -72,16 +73,17 @@ inline RnFit rn_fit(const RnShape& s, long long rows, size_t row_bytes, size_t f
   f.ctas = std::min<long long>(rn_units(rows, f.groups * per * f.batch), sm_count());
   return f;
 }
+inline size_t rn_fixed(int D) { return (size_t)2 * D * 4; }  // the parameters
 inline size_t rn_bwd_row(int D, size_t x, size_t o, bool g, bool dv, bool dn) {
   return (size_t)D * (x + o + (g ? o : 0) + (dv ? x : 0) + (dn ? o : 0));
 }
 template <typename TX, typename TO>
 RnFit rn_fwd_fit(const RnParams& p, const RnShape& s) {
-  return rn_fit(s, p.rows, (size_t)p.D * (sizeof(TX) + (p.g.p ? 2 : 1) * sizeof(TO)), (size_t)3 * p.D * 4);
+  return rn_fit(s, p.rows, (size_t)p.D * (sizeof(TX) + (p.g.p ? 2 : 1) * sizeof(TO)), rn_fixed(p.D));
 }
 template <typename TX, typename TO>
 RnFit rn_bwd_fit(const RnParams& p, const RnShape& s) {
-  return rn_fit(s, p.rows, rn_bwd_row(p.D, sizeof(TX), sizeof(TO), p.g.p, p.dv.p, p.dn.p), (size_t)3 * p.D * 4);
+  return rn_fit(s, p.rows, rn_bwd_row(p.D, sizeof(TX), sizeof(TO), p.g.p, p.dv.p, p.dn.p), rn_fixed(p.D));
 }
 // (the backward: as many as the SMs hold at once, which is one of more than eight warps)
 inline long long rn_plain_ctas(long long rows, const RnShape& s) {
@@ -124,7 +126,7 @@ int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, cons
   p.stages = fit.stages;
   p.batch = fit.batch;
   p.parts = (int)fit.ctas;
-  p.params = (long long)(fit.smem / 4) - 3LL * p.D;
+  p.params = (long long)(fit.smem / 4) - 2LL * p.D;
   auto kernel = rn_pick<Kernel>(p.D == s.warps * 32 * s.v * s.k, p.g.p != nullptr, p.dropout);
   if (int rc = rn_smem(kernel, fit.smem)) return rc;
   {

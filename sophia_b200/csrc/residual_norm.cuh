@@ -292,22 +292,23 @@ __device__ __forceinline__ void rn_copy(const RnSource& t, uint32_t at, int rows
     for (int i = 0; i < n; ++i) rn_bulk(dst + i * t.row, src(row0 + i), t.row, bar);
   }
 }
-// What a CTA shares: the sums' places (two for each group: a sum's may be written while the last one is read) and the
-// stages' arrivals.
+// What a CTA shares: the sums' places (two for each group: a sum's may be written while the last one is read; a group's
+// warps take whole fours of them) and the stages' arrivals.
+constexpr int RN_PARTS = 32;
 template <int N>
 struct RnShared {
-  float part[2][RN_MAX_GROUPS][N][RN_MAX_WARPS];
-  uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES], params;
+  float part[2][N][RN_PARTS];
+  uint64_t full[RN_MAX_GROUPS][RN_MAX_STAGES];
 };
-// The parameters w, w_b and scale into shared memory [3][D]; one that is left out counts as 1.  The first thread, behind
-// the barriers' initialisation.
-__device__ __forceinline__ void rn_params(const RnParams& P, float* dst, uint64_t* bar) {
-  const float* src[3] = {P.w, P.wb, P.scale};
-  const uint32_t bytes = P.D * 4;
-  rn_expect(bar, ((P.w ? 1 : 0) + (P.wb ? 1 : 0) + (P.scale ? 1 : 0)) * bytes);
-#pragma unroll
-  for (int q = 0; q < 3; ++q)
-    if (src[q]) rn_bulk(smem_u32(dst + q * P.D), src[q], bytes, bar);
+// The parameters in shared memory [2][D]: w, and w_b scale, the only form in which a row needs those two.
+__device__ __forceinline__ void rn_params(const RnParams& P, float* dst) {
+  const float4 one = make_float4(1.f, 1.f, 1.f, 1.f);
+  for (int c = threadIdx.x * 4; c < P.D; c += blockDim.x * 4) {
+    const float4 b = P.wb ? __ldg(reinterpret_cast<const float4*>(P.wb + c)) : one;
+    const float4 s = P.scale ? __ldg(reinterpret_cast<const float4*>(P.scale + c)) : one;
+    if (P.w) *reinterpret_cast<float4*>(dst + c) = __ldg(reinterpret_cast<const float4*>(P.w + c));
+    *reinterpret_cast<float4*>(dst + P.D + c) = make_float4(b.x * s.x, b.y * s.y, b.z * s.z, b.w * s.w);
+  }
 }
 
 // A group's walk through its rows: where it and its thread stand, and its stages.
@@ -322,7 +323,8 @@ struct RnGroup {
   bool leads, alive;  // the first warp; no wait has run out
   uint32_t base, stage_bytes, row_bytes;
   uint64_t* full;
-  float (*part)[RN_MAX_GROUPS][N][RN_MAX_WARPS];
+  float (*part)[N][RN_PARTS];
+  int place;  // its first of the sums' places
   int slot, turn, stages, flip;
   int refill, spare;  // the first row of the stage to be filled again once everyone has read it (or total), and that stage
   int T_;
@@ -352,15 +354,15 @@ struct RnGroup {
     base = ring + group * stages * stage_bytes;
     full = sh.full[group];
     part = sh.part;
+    place = group * ((warps + 3) & ~3);
     slot = turn = flip = spare = 0;
     refill = total;
     T_ = P.T;
     mine = RnSource{};
     if (in == 0)
       for (int q = 0; q < stages; ++q) rn_bar_init(&full[q]);
-    if (threadIdx.x == 0) rn_bar_init(&sh.params);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    for (int i = threadIdx.x; i < 2 * RN_MAX_GROUPS * N * RN_MAX_WARPS; i += blockDim.x) (&sh.part[0][0][0][0])[i] = 0.f;
+    for (int i = threadIdx.x; i < 2 * N * RN_PARTS; i += blockDim.x) (&sh.part[0][0][0])[i] = 0.f;
   }
   __device__ __forceinline__ void sync() const {
     if (warps == 1) __syncwarp();
@@ -413,15 +415,15 @@ struct RnGroup {
 #pragma unroll
         for (int i = 0; i < N; ++i) a[i] += __shfl_xor_sync(0xffffffffu, a[i], m);
       if (warps > 1) {
-        float (*p)[RN_MAX_WARPS] = part[flip][group];
+        float (*p)[RN_PARTS] = part[flip];
         flip ^= 1;
         if ((threadIdx.x & 31) == 0)
 #pragma unroll
-          for (int i = 0; i < N; ++i) p[i][(threadIdx.x >> 5) - group * warps] = a[i];
+          for (int i = 0; i < N; ++i) p[i][place + (threadIdx.x >> 5) - group * warps] = a[i];
         sync();
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float4* q = reinterpret_cast<const float4*>(p[i]);
+          const float4* q = reinterpret_cast<const float4*>(p[i] + place);
           float4 f = q[0];
           float t = (f.x + f.y) + (f.z + f.w);
           for (int w = 4; w < warps; w += 4) {
@@ -508,7 +510,7 @@ __device__ __forceinline__ u64 rn_mask(u64 v, unsigned bits, int pair) {
 template <typename TX, typename TO, int K, bool NARROW, bool FULL, bool GATE, bool DROP>
 __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const __grid_constant__ RnParams P) {
   constexpr int V = 16 / sizeof(TO), H = V / 2;
-  extern __shared__ __align__(128) char ring[];  // the groups' stages, then the parameters [3][D]
+  extern __shared__ __align__(128) char ring[];  // the groups' stages, then the parameters [2][D]
   __shared__ __align__(16) RnShared<1> sh;
   const int D = P.D;
   const uint32_t xb = D * sizeof(TX), ob = D * sizeof(TO);
@@ -522,8 +524,9 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
   float* params = reinterpret_cast<float*>(ring) + P.params;
   __syncthreads();
   a.start();
-  if (threadIdx.x == 0) rn_params(P, params, &sh.params);
-  const bool has_w = P.w != nullptr, has_wb = P.wb != nullptr, has_scale = P.scale != nullptr, keeps = P.rstd && a.me == 0;
+  rn_params(P, params);
+  __syncthreads();
+  const bool has_w = P.w != nullptr, has_wb = P.wb != nullptr, has_ws = P.wb || P.scale, keeps = P.rstd && a.me == 0;
   unsigned long long seed = 0;
   if (DROP) seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
@@ -531,10 +534,9 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
   bool mine[K];  // the thread's pieces that there are
 #pragma unroll
   for (int k = 0; k < K; ++k) mine[k] = FULL || a.me * V + k * a.stride < D;
-  const uint32_t pw = smem_u32(params) + a.me * V * 4, pwb = pw + 4 * D, psc = pwb + 4 * D, kp = a.stride * 4;
+  const uint32_t pw = smem_u32(params) + a.me * V * 4, pws = pw + 4 * D, kp = a.stride * 4;
   const uint32_t at_x = a.sub * xb + a.me * (V * (uint32_t)sizeof(TX)), at_o = a.rows * xb + a.sub * ob + a.me * 16;
   const uint32_t kx = a.stride * (uint32_t)sizeof(TX), ko = a.stride * (uint32_t)sizeof(TO), at_g = a.rows * ob;
-  a.alive = rn_wait(&sh.params, 0);
   for (int row0 = a.first; row0 < a.total; row0 += a.step) {
     a.wait();
     uint32_t px = a.base + a.slot * a.stage_bytes + at_x, po = a.base + a.slot * a.stage_bytes + at_o;
@@ -565,8 +567,8 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
       for (int k = 0; k < K; ++k)
         if (mine[k] && here) {
           u64 f[H];
-          if (has_wb) {
-            rn_take<float, V>(pwb + k * kp, f);
+          if (has_ws) {
+            rn_take<float, V>(pws + k * kp, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], mul2(f[i], rn_all(rb)));
           }
@@ -574,11 +576,6 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
             rn_take<TO, V>(po + at_g + k * ko, f);
 #pragma unroll
             for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], rn_sigmoid(f[i]));
-          }
-          if (has_scale) {
-            rn_take<float, V>(psc + k * kp, f);
-#pragma unroll
-            for (int i = 0; i < H; ++i) v[k][i] = mul2(v[k][i], f[i]);
           }
           if (DROP) {
             const unsigned bits = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
@@ -621,14 +618,15 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_fwd_ring_kernel(const
 
 // One round of sums a row: with t = scale m s u (what the stream got from the branch), the sum that the branch's norm
 // needs is that of t dv', and dv' = dv + r (tw - v r^2 S1 / D) with tw = dn w, S1 = sum tw v: sum t dv' =
-// sum t (dv + r tw) - r^3 S1 / D sum t v, and do = r_b (du w_b - o r_b / D sum t dv').
+// sum t (dv + r tw) - r^3 S1 / D sum t v, and do = r_b (du w_b - o r_b / D sum t dv').  And one column sum serves two
+// parameters: with Q = sum over the rows of m dv' s o r_b, dw_b = scale Q and dscale = w_b Q.
 template <typename TX, typename TO, bool NARROW, bool FULL, bool GATE, bool DROP>
 __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const __grid_constant__ RnParams P) {
   constexpr int V = 16 / sizeof(TO), H = V / 2, K = (NARROW ? 8 : 16) / V;
-  extern __shared__ __align__(128) char ring[];  // the groups' stages, then the parameters [3][D], at the end the sums
+  extern __shared__ __align__(128) char ring[];  // the groups' stages, then the parameters [2][D], at the end the column sums
   __shared__ __align__(16) RnShared<3> sh;
   const int D = P.D;
-  const bool has_dv = P.dv.p != nullptr, has_dn = P.dn.p != nullptr, has_wb = P.wb != nullptr, has_scale = P.scale != nullptr;
+  const bool has_dv = P.dv.p != nullptr, has_dn = P.dn.p != nullptr, has_wb = P.wb != nullptr;
   const uint32_t xb = D * sizeof(TX), ob = D * sizeof(TO);
   const uint32_t off_g = xb + ob, off_dv = off_g + (GATE ? ob : 0), off_dn = off_dv + (has_dv ? xb : 0);
   RnGroup<TO, NARROW, 3> a(P, sh, smem_u32(ring), off_dn + (has_dn ? ob : 0));
@@ -641,34 +639,30 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
     if (lane == 4) a.mine = rn_source(P.dn, sizeof(TO), off_dn, P.dense >> 4 & 1, D);
   }
   float* params = reinterpret_cast<float*>(ring) + P.params;
-  for (int i = threadIdx.x; i < D; i += blockDim.x) {
-    if (!has_wb) params[D + i] = 1.f;
-    if (!has_scale) params[2 * D + i] = 1.f;
-  }
   __syncthreads();
   a.start();
-  if (threadIdx.x == 0) rn_params(P, params, &sh.params);
+  rn_params(P, params);
+  __syncthreads();
   unsigned long long seed = 0;
   if (DROP) seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / D, keep = DROP ? P.keep_scale : 1.f;
   bool mine[K];
-  u64 sw[K][H], sb[K][H], ssc[K][H];  // sums over this thread's rows
+  u64 sw[K][H], sq[K][H];  // sums over this thread's rows: dw, Q
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     mine[k] = FULL || a.me * V + k * a.stride < D;
 #pragma unroll
-    for (int i = 0; i < H; ++i) sw[k][i] = sb[k][i] = ssc[k][i] = 0ull;
+    for (int i = 0; i < H; ++i) sw[k][i] = sq[k][i] = 0ull;
   }
   const uint32_t at_x = a.sub * xb + a.me * (V * (uint32_t)sizeof(TX)), at_o = a.rows * xb + a.sub * ob + a.me * 16;
   const uint32_t to_dv = a.rows * off_dv, to_g = a.rows * (off_g - xb), to_dn = a.rows * (off_dn - xb);
   const uint32_t kx = a.stride * (uint32_t)sizeof(TX), ko = a.stride * (uint32_t)sizeof(TO), kp = a.stride * 4;
-  const uint32_t pw = smem_u32(params) + a.me * V * 4, pwb = pw + 4 * D, psc = pwb + 4 * D;
+  const uint32_t pw = smem_u32(params) + a.me * V * 4, pws = pw + 4 * D;
   auto roots_of = [&](int row) {
     return row < a.total ? __ldg(reinterpret_cast<const float2*>(P.rstd + 2LL * row)) : make_float2(0.f, 0.f);
   };
   float2 ahead = roots_of(min(a.first, a.total) + a.sub);  // of the row to come
-  a.alive = rn_wait(&sh.params, 0);
   for (int row0 = a.first; row0 < a.total; row0 += a.step) {
     a.wait();
     uint32_t px = a.base + a.slot * a.stage_bytes + at_x, po = a.base + a.slot * a.stage_bytes + at_o;
@@ -688,7 +682,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
         if (mine[k] && here) {
           u64 f[H], t[H];
           rn_take<TO, V>(po + k * ko, t);
-          rn_take<float, V>(pwb + k * kp, f);
+          rn_take<float, V>(pws + k * kp, f);
 #pragma unroll
           for (int i = 0; i < H; ++i) t[i] = mul2(t[i], mul2(f[i], rn_all(rb)));
           if (GATE) {
@@ -696,9 +690,6 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
 #pragma unroll
             for (int i = 0; i < H; ++i) t[i] = mul2(t[i], rn_sigmoid(f[i]));
           }
-          rn_take<float, V>(psc + k * kp, f);
-#pragma unroll
-          for (int i = 0; i < H; ++i) t[i] = mul2(t[i], f[i]);
           if (DROP) {
             bits[k] = rn_bits<V>(P, k0, k1, row, a.me * V + k * a.stride);
 #pragma unroll
@@ -755,32 +746,23 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
 #pragma unroll
             for (int i = 0; i < H; ++i) g[i] = rn_mask(mul2(g[i], rn_all(keep)), bits[k], i);
           rn_take<TO, V>(po + k * ko, u);
-          rn_take<float, V>(pwb + k * kp, f);
+          rn_take<float, V>(pws + k * kp, f);
           if (GATE) rn_take<TO, V>(po + to_g + k * ko, sg);
-          rn_take<float, V>(psc + k * kp, q);
 #pragma unroll
           for (int i = 0; i < H; ++i) {
-            const u64 n = mul2(u[i], rn_all(rb));
-            u64 us = mul2(n, f[i]), s = 0ull;
+            u64 n = mul2(u[i], rn_all(rb)), e = mul2(g[i], f[i]);
+            if (DROP) n = rn_mask(n, bits[k], i);  // (a dropped element may hold anything)
             if (GATE) {
-              s = rn_sigmoid(sg[i]);
-              us = mul2(us, s);
+              const u64 s = rn_sigmoid(sg[i]), gs = DROP ? rn_mask(mul2(g[i], s), bits[k], i) : mul2(g[i], s);
+              sq[k][i] = fma2(gs, n, sq[k][i]);
+              const u64 es = mul2(gs, f[i]);
+              sg[i] = mul2(mul2(es, n), rn_neg1_plus(s));
+              if (DROP) sg[i] = rn_mask(sg[i], bits[k], i);
+              e = es;
+            } else {
+              sq[k][i] = fma2(g[i], n, sq[k][i]);
             }
-            if (DROP) us = rn_mask(us, bits[k], i);  // (a dropped element may hold anything)
-            ssc[k][i] = fma2(g[i], us, ssc[k][i]);
-            u64 e = mul2(g[i], q[i]);
-            if (GATE) {
-              sg[i] = mul2(mul2(e, us), rn_neg1_plus(s));
-              e = mul2(e, s);
-              if (DROP) {
-                sg[i] = rn_mask(sg[i], bits[k], i);
-                e = rn_mask(e, bits[k], i);
-              }
-            }
-            if (has_wb) {
-              sb[k][i] = fma2(e, n, sb[k][i]);
-              e = mul2(rn_all(rb), fma2(u[i], rn_all(-back), mul2(e, f[i])));
-            }
+            if (has_wb) e = mul2(rn_all(rb), fma2(u[i], rn_all(-back), e));
             g[i] = e;
           }
           if (GATE) rn_put<TO, V>(static_cast<TO*>(P.dg) + out + k * a.stride, sg);
@@ -804,15 +786,17 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
           for (int i = 0; i < H; ++i) {
             u64* f0 = reinterpret_cast<u64*>(params + c) + i;
             u64* f1 = reinterpret_cast<u64*>(params + D + c) + i;
-            u64* f2 = reinterpret_cast<u64*>(params + 2 * D + c) + i;
             *f0 = q ? add2(*f0, sw[k][i]) : sw[k][i];
-            *f1 = q ? add2(*f1, sb[k][i]) : sb[k][i];
-            *f2 = q ? add2(*f2, ssc[k][i]) : ssc[k][i];
+            *f1 = q ? add2(*f1, sq[k][i]) : sq[k][i];
           }
       }
     __syncthreads();
   }
-  for (int i = threadIdx.x; i < 3 * D; i += blockDim.x) out[i] = params[i];
+  for (int i = threadIdx.x; i < D; i += blockDim.x) {
+    out[i] = params[i];
+    out[D + i] = params[D + i] * (P.scale ? P.scale[i] : 1.f);
+    out[2 * D + i] = params[D + i] * (P.wb ? P.wb[i] : 1.f);
+  }
 }
 
 // ---------------------------------------------------------------- backward, rows wherever they lie
