@@ -13,10 +13,19 @@
 // exchanges their maps through distributed shared memory, in the order of the
 // tiles -- one pass over the data at any number of rows.
 //
-// 10 bytes an element (bf16, with z) against seven special functions (ex2 and rcp
-// of three sigmoids, rsqrt), which the SM makes at 16 a clock: both take about as long
-// (50 us per 4 x 4096 x 2048 elements), so the decay's exponential is a polynomial on
-// packed fp32 arithmetic, which also gives 1 - a^2 without cancellation.
+// 10 bytes an element (bf16, with z) against six special functions (ex2 of three
+// sigmoids, rcp of two, rsqrt), which the SM makes at 16 a clock: 51 and 45 us per
+// 4 x 4096 x 2048 elements, so the decay's exponential is a polynomial on packed fp32
+// arithmetic, which also gives 1 - a^2 without cancellation.
+//
+// Measured at 4 x 4096 x 2048 bf16 with z: forward 108 us, backward 195 us (floors 51 and
+// 92 us of bytes), 128 channel groups on 148 SMs in clusters of two; 32 x 512 x 2048, no
+// cluster: 79 and 164 us.  What bounds them: latency at 128 registers and 3.3 warps a
+// scheduler (48 % of the issue slots, 44 and 40 % of the special functions, 32 % of DRAM)
+// and SMs left over.  Tried: CTAs of 512 threads, one an SM, without a cluster (111 and
+// 195 us, but 268 against 230 for the forward of one row of 16384 tokens); 4 tokens a
+// thread and three CTAs an SM (142 and 289 us); CTAs of 128 threads; a tile's gates ahead
+// of the states of the one before (5 % slower).
 //
 // A run's decay P is the exponential of its tokens' summed logarithms: one rounding of 2^-24 where their product has one a
 // token, which is what a state that remembers thousands of tokens would feel.
@@ -70,8 +79,8 @@ __device__ __forceinline__ u64 sub2(u64 a, u64 b) {
   asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// The packed arithmetic's constants, as kernel parameters: operands from the constant bank or uniform registers
-// where literals would be moved into a pair of registers at every use (28 of 141 instructions a pair of elements).
+// The packed arithmetic's constants, as kernel parameters: operands from the constant bank or uniform registers;
+// literals were moved into a pair of registers at every use (28 of then 141 instructions a pair of elements).
 struct RecConst {
   u64 one, two, log2e, round, poly[6];
 };

@@ -138,7 +138,7 @@ int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, cons
 
 template <typename TX, typename TO, int K>
 int launch_rn_bwd(RnParams& p, const RnShape& s, cudaStream_t st) {
-  const size_t smem = (size_t)s.groups * 3 * p.D * 4;
+  const size_t smem = (size_t)s.groups * 2 * p.D * 4;
   auto kernel = rn_bwd_kernel<TX, TO, K>;
   if (int rc = rn_smem(kernel, smem)) return rc;
   p.parts = (int)rn_plain_ctas(p.rows, s);

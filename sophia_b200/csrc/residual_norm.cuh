@@ -43,7 +43,7 @@ struct RnParams {
   long long rows;
   int T;  // rows per batch entry, or 0 where all rows of every tensor have one stride (no division)
   int stages, batch;  // of the ring: stages, and how many times a group's rows a stage holds
-  long long params;   // floats from the ring's start to the backward's parameters
+  long long params;   // floats from the ring's start to the parameters
   unsigned dense;     // bit per tensor (x, o, g, dv, dn): rows lie end to end
   int D, warps, lanes;  // a row's threads: warps of a group, or (one warp) that many lanes
   int parts;  // CTAs of the backward, set by its launch
@@ -77,7 +77,7 @@ __device__ __forceinline__ void rn_param(const float* p, int c, int n, float (&f
 }
 __device__ __forceinline__ int rn_there(int c, int D) { return min(4, max(0, (D - c + 31) >> 5)); }
 // K = 2, eight channels a thread: four CTAs an SM forward and two backward, whose column sums then stay in registers;
-// K = 4, rows above 2048 channels.  (8192 x 2043: 77 and 162 us, floors 36 and 56; with K = 4, its column sums in shared
+// K = 4, rows above 2048 channels.  (8192 x 2043: 77 and 158 us, floors 36 and 56; with K = 4, its column sums in shared
 // memory and three CTAs an SM launched where two fitted, 95 and 295.)
 __host__ __device__ constexpr int rn_plain_threads(int k) { return k == 2 ? 256 : 512; }
 template <typename T>
@@ -135,8 +135,8 @@ __device__ __forceinline__ unsigned rn_kept(const RnParams& P, unsigned k0, unsi
 
 // ---------------------------------------------------------------- forward, rows wherever they lie
 
-// A group of warps has a row, in registers between its two reductions.  Instructions bound it: 80 an element at 50 % of
-// the issue slots (predicates and addresses of single elements), DRAM at 26 %.
+// A group of warps has a row, in registers between its two reductions.  Instructions bound it: 116 an element at 75 % of
+// the issue slots (predicates and addresses of single elements), DRAM at 33 %; the backward 169 at 55 %.
 template <typename TX, typename TO, int K>
 __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 4 : 1) rn_fwd_kernel(const __grid_constant__ RnParams P) {
   __shared__ float part[2][1][RN_MAX_WARPS];
@@ -239,7 +239,11 @@ __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 4 : 1) rn_fwd_ke
 // packed fp32 arithmetic; the parameters lie in shared memory.
 // What a row costs beside its arithmetic -- waiting, barriers, sums over warps, addresses -- is what bounds these
 // kernels, so the parts that a call has are known to the compiler as far as they change the loops (FULL: a row fills its
-// threads; GATE; DROP).
+// threads; GATE; DROP).  Measured at 4 x 4096 x 1536, bf16 with an fp32 stream, norms on both sides, gate and dropout:
+// forward 71 us and backward 128 us (floors 46 and 61 us of bytes, 65 and 48 % of the copy bandwidth); 2 x 4096 x 4096 bf16
+// without gate and dropout: 51 and 106 us (30 and 52).
+// Tried: a warp of its own for the copies (17 warps: 96 registers, spills); parameters from global memory; 8 channels a
+// thread (forward 124 us); 16 channels of narrow rows (backward of 32768 x 256 88 us against 69).
 constexpr int RN_MAX_STAGES = 4;
 constexpr int RN_MAX_GROUPS = 16;
 
@@ -804,7 +808,7 @@ __global__ void __launch_bounds__(RN_MAX_WARPS * 32, 1) rn_bwd_ring_kernel(const
 // (The row's three sums, and what they are for, as in the kernel above.)
 template <typename TX, typename TO, int K>
 __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 2 : 1) rn_bwd_kernel(const __grid_constant__ RnParams P) {
-  extern __shared__ __align__(16) float acc[];  // [groups][3][D] column sums: a thread's own channels (K = 2: at the end)
+  extern __shared__ __align__(16) float acc[];  // [groups][2][D] column sums of dw and Q (K = 2: at the end)
   __shared__ float part[2][3][RN_MAX_WARPS];
   int flip = 0;
   const int warps = P.warps, group = (threadIdx.x >> 5) / warps, groups = (blockDim.x >> 5) / warps;
@@ -812,13 +816,13 @@ __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 2 : 1) rn_bwd_ke
   const unsigned long long seed = P.seed_ptr ? (unsigned long long)*P.seed_ptr : P.seed;
   const unsigned k0 = (unsigned)seed, k1 = (unsigned)(seed >> 32);
   const float inv = 1.f / P.D;
-  float* sums = acc + group * 3 * P.D;
-  float mine[3][K][4] = {};  // (K = 2)
+  float* sums = acc + group * 2 * P.D;
+  float mine[2][K][4] = {};  // (K = 2)
   if (K > 2)
 #pragma unroll
     for (int k = 0; k < K; ++k)
       for (int i = 0; i < rn_there(c0 + k * stride, P.D); ++i)
-        for (int q = 0; q < 3; ++q) sums[q * P.D + c0 + k * stride + 32 * i] = 0.f;
+        for (int q = 0; q < 2; ++q) sums[q * P.D + c0 + k * stride + 32 * i] = 0.f;
   auto add = [&](int q, int k, int c, int n, const float (&f)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -909,24 +913,16 @@ __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 2 : 1) rn_bwd_ke
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const bool on = kept[k] >> i & 1;
-        const float u = P.wb ? o[k].get(i) * rb * wb[i] : o[k].get(i);
+        const float n = o[k].get(i) * rb;
         s[i] = pg ? sigmoidf_(g[k].get(i)) : 1.f;
-        const float dm = on ? (P.dropout ? P.keep_scale * d[i] : d[i]) : 0.f;  // gradient of scale u s
-        t[i] = on ? dm * (u * s[i]) : 0.f;                                      // of scale
-        const float ds = P.scale ? dm * f[i] : dm;                              // of u s
-        d[i] = on ? ds * s[i] : 0.f;                                            // of u
-        s[i] = on ? ds * u * (s[i] * (1.f - s[i])) : 0.f;
+        const float gs = on ? (P.dropout ? P.keep_scale * d[i] : d[i]) * s[i] : 0.f;
+        t[i] = on ? gs * n : 0.f;
+        d[i] = on ? gs * ((P.scale ? f[i] : 1.f) * (P.wb ? wb[i] : 1.f)) : 0.f;
+        s[i] = on ? d[i] * n * (1.f - s[i]) : 0.f;
+        if (P.wb) d[i] = rb * fmaf(-o[k].get(i), back, d[i]);
       }
-      if (P.scale) add(2, k, c, n4, t);
+      add(1, k, c, n4, t);
       if (pg) rn_store(pdg + c, s, n4);
-      if (P.wb) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          t[i] = d[i] * o[k].get(i) * rb;
-          d[i] = rb * fmaf(-o[k].get(i), back, d[i] * wb[i]);
-        }
-        add(1, k, c, n4, t);
-      }
       rn_store(pdo + c, d, n4);
     }
   }
@@ -937,12 +933,15 @@ __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 2 : 1) rn_bwd_ke
       for (int i = 0; i < 4; ++i)
         if (i < rn_there(c0 + k * stride, P.D))
 #pragma unroll
-          for (int q = 0; q < 3; ++q) sums[q * P.D + c0 + k * stride + 32 * i] = mine[q][k][i];
+          for (int q = 0; q < 2; ++q) sums[q * P.D + c0 + k * stride + 32 * i] = mine[q][k][i];
   __syncthreads();
-  for (int i = threadIdx.x; i < 3 * P.D; i += blockDim.x) {  // the CTA's sums, its groups in order
-    float t = 0.f;
-    for (int q = 0; q < groups; ++q) t += acc[q * 3 * P.D + i];
-    P.partial[(long long)blockIdx.x * 3 * P.D + i] = t;
+  float* out = P.partial + (long long)blockIdx.x * 3 * P.D;
+  for (int i = threadIdx.x; i < P.D; i += blockDim.x) {  // the CTA's sums, its groups in order
+    float t = 0.f, q = 0.f;
+    for (int w = 0; w < groups; ++w) t += acc[w * 2 * P.D + i], q += acc[(w * 2 + 1) * P.D + i];
+    out[i] = t;
+    out[P.D + i] = q * (P.scale ? P.scale[i] : 1.f);
+    out[2 * P.D + i] = q * (P.wb ? P.wb[i] : 1.f);
   }
 }
 
