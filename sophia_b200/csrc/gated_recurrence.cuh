@@ -23,7 +23,7 @@
 // cluster: 79 and 164 us.  What bounds them: latency at 128 registers and 3.3 warps a
 // scheduler (48 % of the issue slots, 44 and 40 % of the special functions, 32 % of DRAM)
 // and SMs left over.  Tried: CTAs of 512 threads, one an SM, without a cluster (111 and
-// 195 us, but 268 against 230 for the forward of one row of 16384 tokens); 4 tokens a
+// 195 us, but 273 against 233 for the forward of one row of 32768 tokens); 4 tokens a
 // thread and three CTAs an SM (142 and 289 us); CTAs of 128 threads; a tile's gates ahead
 // of the states of the one before (5 % slower).
 //

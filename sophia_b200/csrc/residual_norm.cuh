@@ -240,8 +240,8 @@ __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 4 : 1) rn_fwd_ke
 // What a row costs beside its arithmetic -- waiting, barriers, sums over warps, addresses -- is what bounds these
 // kernels, so the parts that a call has are known to the compiler as far as they change the loops (FULL: a row fills its
 // threads; GATE; DROP).  Measured at 4 x 4096 x 1536, bf16 with an fp32 stream, norms on both sides, gate and dropout:
-// forward 71 us and backward 128 us (floors 46 and 61 us of bytes, 65 and 48 % of the copy bandwidth); 2 x 4096 x 4096 bf16
-// without gate and dropout: 51 and 106 us (30 and 52).
+// forward 72 us and backward 128 us (75 and 66 % of the copy bandwidth); 2 x 4096 x 4096 bf16 without gate and dropout:
+// 51 and 104 us (80 and 59 %).
 // Tried: a warp of its own for the copies (17 warps: 96 registers, spills); parameters from global memory; 8 channels a
 // thread (forward 124 us); 16 channels of narrow rows (backward of 32768 x 256 88 us against 69).
 constexpr int RN_MAX_STAGES = 4;
