@@ -149,6 +149,15 @@ def test_odd_rows_many(shape, dtype):
     check(inputs(rn, shape, f32, dtype, True, True, True, True, 0), rn, 0.1, 77, 3)
 
 
+@gpu
+@pytest.mark.parametrize("shape,wide,dtype", [((400, 8192), f32, f32), ((310, 8192), f32, f16), ((1000, 4096), f32, f32)],
+                         ids=str)
+def test_widest_rows_many(shape, wide, dtype):
+    """Rows of which shared memory holds one or two beside the parameters, more of them than there are SMs."""
+    rn = gen(29)
+    check(inputs(rn, shape, wide, dtype, True, True, True, True, 0), rn, 0.1, 78, 4)
+
+
 def test_generator_known_answers():
     """The published vectors of Philox4x32-10, and the tensor form against the integers."""
     assert ref.philox([0] * 4, [0] * 2) == [0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
