@@ -42,7 +42,8 @@ def _new(t: Tensor) -> Tensor:
 def _fwd_impl(x, o, gate, weight, branch_weight, scale, seed, seed_value, offset, p, eps, training):
     """x, o, gate [B, T, D].  Returns (stream, next block's input or empty, reciprocal roots or empty)."""
     xr, orr, gr = _rows(x, x.dtype), _rows(o, o.dtype), None if gate is None else _rows(gate, o.dtype)
-    a = _args(xr, orr, gr, _param(weight), _param(branch_weight), _param(scale), seed, seed_value, offset, p, eps)
+    w, wb, sc = _param(weight), _param(branch_weight), _param(scale)  # (held: the arguments are addresses)
+    a = _args(xr, orr, gr, w, wb, sc, seed, seed_value, offset, p, eps)
     v = _new(x)
     n = _new(o) if weight is not None else o.new_empty(0)
     rstd = x.new_empty((x.shape[0] * x.shape[1], 2) if training else 0, dtype=torch.float32)
@@ -62,7 +63,8 @@ def _bwd_impl(x, o, gate, weight, branch_weight, scale, seed, rstd, dv, dn, seed
     """Returns (dx, do, dgate, dweight, dbranch_weight, dscale); absent ones empty."""
     lib = _lib.load()
     xr, orr, gr = _rows(x, x.dtype), _rows(o, o.dtype), None if gate is None else _rows(gate, o.dtype)
-    a = _args(xr, orr, gr, _param(weight), _param(branch_weight), _param(scale), seed, seed_value, offset, p, eps)
+    w, wb, sc = _param(weight), _param(branch_weight), _param(scale)
+    a = _args(xr, orr, gr, w, wb, sc, seed, seed_value, offset, p, eps)
     dvr = None if dv is None else _rows(dv, x.dtype)
     dnr = None if dn is None else _rows(dn, o.dtype)
     dx, do = _new(x), _new(o)

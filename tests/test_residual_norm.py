@@ -405,3 +405,42 @@ def test_refusals():
     (g,) = torch.autograd.grad(f(x, x, w)[0].sum(), x, create_graph=True)
     with pytest.raises(NotImplementedError):
         g.sum().backward()
+
+
+def converted(ts, kind):
+    """The parameters as the kernels have to convert them: in bf16, or with a stride."""
+    def one(t):
+        t = t.detach()
+        return (t.to(bf16) if kind == "bf16" else torch.stack([t, t + 1], -1)[:, 0]).requires_grad_()
+    return {k: one(t) if k in ("weight", "branch_weight", "scale") else t for k, t in ts.items()}
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "strided"])
+@pytest.mark.parametrize("shape,wide,dtype", [((1, 64), f32, bf16), ((2, 1536), bf16, bf16), ((8, 1003), f32, f32),
+                                              ((700, 1536), f32, bf16), ((300, 2043), f32, f16)], ids=str)
+def test_parameters_that_have_to_be_converted(kind, shape, wide, dtype):
+    """Eager against the formulas, with allocations of the parameters' size before and after; captured with the same bits."""
+    rn = gen(31)
+    ts = converted(inputs(rn, shape, wide, dtype), kind)
+    for _ in range(3):
+        check(ts, rn, 0.1, 79, 5)
+    leaves = [ts[k] for k in NAMES]
+    up = rn(*shape, dtype=wide), rn(*shape, dtype=dtype)
+
+    def step():
+        out = call(ts, dropout_p=0.1, seed=79, offset=5)
+        return (*out, *torch.autograd.grad(out, leaves, up))
+
+    want = [t.detach() for t in step()]  # (no eager graph of the leaves lives while one is captured)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(), step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
