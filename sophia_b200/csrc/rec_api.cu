@@ -86,14 +86,16 @@ bool rec_maps(RecParams& p, int dtype, bool backward) {
   return true;
 }
 
+// `smem`: the kernel's stages.
 int launch_rec(void (*kernel)(RecParams), const RecParams& p, int smem, int id, const char* what, cudaStream_t st) {
-  if (p.cluster > 1) smem += 2 * p.cluster * 32 * (int)sizeof(float4);  // the maps of the cluster's CTAs
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  auto maps = [](int cluster) { return cluster > 1 ? 2 * cluster * 32 * (int)sizeof(float4) : 0; };  // of the cluster's CTAs
+  // The kernel's limit is the same for every call: host threads with clusters of other sizes may be here too.
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem + maps(REC_MAX_CLUSTER));
   if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string(what) + " smem: " + cudaGetErrorString(e));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)((p.E + REC_CH - 1) / REC_CH * p.cluster), (unsigned)p.B);
   cfg.blockDim = dim3(REC_THREADS);
-  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.dynamicSmemBytes = (size_t)(smem + maps(p.cluster));
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
