@@ -47,6 +47,9 @@ inline RnShape rn_fwd_shape(int D, size_t branch_size) {
 inline RnShape rn_bwd_shape(int D, size_t branch_size) { return rn_ring_shape(D, branch_size, 16); }
 inline long long rn_units(long long rows, int rows_a_cta) { return std::max(1LL, (rows + rows_a_cta - 1) / rows_a_cta); }
 
+// An SM's shared memory, whose registers hold one CTA; up to 2 KB are static.
+constexpr size_t RN_RING_SMEM = 227 * 1024 - 2 * 1024;
+static_assert(sizeof(RnShared<3>) <= 2048, "what the kernels share beside the ring");
 // The ring: rows of a stage, stages, and the CTAs of an SM.  A stage has 4 KB at least, unless that left groups
 // without rows; two stages at least where the SM's shared memory has room for them, up to four.  No stage: the rows are
 // too wide.
@@ -56,9 +59,7 @@ struct RnFit {
   size_t smem;
 };
 inline RnFit rn_fit(const RnShape& s, long long rows, size_t row_bytes, size_t fixed) {
-  // of an SM, whose registers hold one CTA; up to 2 KB are static
-  static_assert(sizeof(RnShared<3>) <= 2048, "what the kernels share beside the ring");
-  const size_t room = 227 * 1024 - 2 * 1024 - fixed;
+  const size_t room = RN_RING_SMEM - fixed;
   const int per = s.warps > 1 ? 1 : 32 / s.lanes;
   RnFit f;
   // few rows: a group to an SM before the second
@@ -105,10 +106,11 @@ int launch_rn_fwd(const RnParams& p, const RnShape& s, cudaStream_t st) {
   return launch_check("residual norm forward");
 }
 
+// `most`: the kernel's limit, the same for every call, because host threads with other sizes may be here too.
 template <typename K>
-int rn_smem(K kernel, size_t smem) {
+int rn_smem(K kernel, size_t smem, size_t most) {
   if (smem <= 40 * 1024) return KDA_OK;  // (48 KB go without asking, the static ones included)
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
   return e == cudaSuccess ? KDA_OK : fail(KDA_ERR_CUDA, std::string("residual norm smem: ") + cudaGetErrorString(e));
 }
 
@@ -128,7 +130,7 @@ int launch_rn_ring(RnParams& p, const RnShape& s, const RnFit& fit, int id, cons
   p.parts = (int)fit.ctas;
   p.params = (long long)(fit.smem / 4) - 2LL * p.D;
   auto kernel = rn_pick<Kernel>(p.D == s.warps * 32 * s.v * s.k, p.g.p != nullptr, p.dropout);
-  if (int rc = rn_smem(kernel, fit.smem)) return rc;
+  if (int rc = rn_smem(kernel, fit.smem, RN_RING_SMEM)) return rc;
   {
     TimedLaunch tl(id, st);
     kernel<<<(unsigned)fit.ctas, s.warps * fit.groups * 32, fit.smem, st>>>(p);
@@ -140,7 +142,7 @@ template <typename TX, typename TO, int K>
 int launch_rn_bwd(RnParams& p, const RnShape& s, cudaStream_t st) {
   const size_t smem = (size_t)s.groups * 2 * p.D * 4;
   auto kernel = rn_bwd_kernel<TX, TO, K>;
-  if (int rc = rn_smem(kernel, smem)) return rc;
+  if (int rc = rn_smem(kernel, smem, (size_t)2 * RN_MAX_WIDTH * 4)) return rc;  // (above 2048 channels one group)
   p.parts = (int)rn_plain_ctas(p.rows, s);
   {
     TimedLaunch tl(K_NORM_BWD, st);

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import sophia_b200
-from sophia_b200 import _lib, recurrence
+from sophia_b200 import _lib, recurrence, residual
 
 gpu = pytest.mark.gpu
 bf16 = torch.bfloat16
@@ -70,3 +70,20 @@ def rec(tokens, backward):
 @pytest.mark.parametrize("backward", [False, True])
 def test_recurrence(monkeypatch, backward):
     in_threads(monkeypatch, recurrence, [rec(t, backward) for t in (60, 120, 250, 500)])
+
+
+def norm(rows, backward):
+    rn = gen(rows)
+    x, o, gate, w = rn(rows, 1536).to(bf16), rn(rows, 1536).to(bf16), rn(rows, 1536).to(bf16), rn(1536)
+
+    def run():
+        leaf = o.detach().requires_grad_(backward)
+        n = sophia_b200.residual_norm(x, leaf, w, gate=gate)[1]
+        return torch.autograd.grad(n, leaf, x)[0] if backward else n
+    return run
+
+
+@gpu
+@pytest.mark.parametrize("backward", [False, True])
+def test_residual_norm(monkeypatch, backward):
+    in_threads(monkeypatch, residual, [norm(r, backward) for r in (2, 500, 900, 1400)])
