@@ -103,14 +103,21 @@ inline long long scan_part_floats(long long B, long long T, int E, int N, int G)
 }
 
 #ifdef SSM_SCAN_INSTANTIATE
+// Sets a kernel's shared-memory limit to what its most states need: the same for every call, because host threads with
+// fewer states may be here too.
+template <typename K>
+int scan_limit(K kernel, int most, const char* what) {
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  return e == cudaSuccess ? KDA_OK : fail(KDA_ERR_CUDA, std::string(what) + " smem: " + cudaGetErrorString(e));
+}
 // P and c of the spans, if there are several.
 template <typename T, int L, bool PAD, bool REV>
 int launch_scan_carry(const ScanParams& p, cudaStream_t st) {
   if (p.spans == 1) return KDA_OK;
-  const int smem = scan_carry_smem<T, ScanCarryGeo<T, L, SCAN_S>>(p.N, REV ? 3 : 2);
+  auto bytes = [](int N) { return scan_carry_smem<T, ScanCarryGeo<T, L, SCAN_S>>(N, REV ? 3 : 2); };
+  const int smem = bytes(p.N);
   auto kernel = ssm_scan_carry_kernel<T, L, SCAN_S, PAD, REV>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan carry smem: ") + cudaGetErrorString(e));
+  if (int rc = scan_limit(kernel, bytes(L * SCAN_S), "scan carry")) return rc;
   {
     TimedLaunch tl(REV ? K_SCAN_BWD : K_SCAN_FWD, st);
     kernel<<<dim3(p.G * p.blocks, p.B, p.spans - 1), SCAN_THREADS, smem, st>>>(p);
@@ -124,8 +131,7 @@ int launch_scan_fwd_tile(const ScanParams& p, cudaStream_t st) {
   using G = ScanGeo<T, L, S, TT>;
   const int smem = scan_fwd_smem<T, G>(p.N);
   auto kernel = ssm_scan_fwd_kernel<T, L, S, TT, PAD>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan forward smem: ") + cudaGetErrorString(e));
+  if (int rc = scan_limit(kernel, scan_fwd_smem<T, G>(L * S), "scan forward")) return rc;
   {
     TimedLaunch tl(K_SCAN_FWD, st);
     kernel<<<dim3(p.G * p.blocks, p.B, p.spans), SCAN_THREADS, smem, st>>>(p);
@@ -149,12 +155,10 @@ int launch_scan_bwd(ScanParams p, const ScanGrads& g, cudaStream_t st) {
   constexpr int S = SCAN_S;
   using G = ScanBwdGeo<T, L, S>;
   p.blocks = scan_blocks(p.E, p.G, L);
-  const int rc = launch_scan_carry<T, L, PAD, true>(p, st);
-  if (rc) return rc;
+  if (int rc = launch_scan_carry<T, L, PAD, true>(p, st)) return rc;
   const int smem = scan_bwd_smem<T, G>(p.N);
   auto kernel = ssm_scan_bwd_kernel<T, L, S, PAD>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(KDA_ERR_CUDA, std::string("scan backward smem: ") + cudaGetErrorString(e));
+  if (int rc = scan_limit(kernel, scan_bwd_smem<T, G>(L * S), "scan backward")) return rc;
   const int tiles = (p.T + G::TT - 1) / G::TT, per = G::TT * 2 * p.N;
   const long long cols = (long long)p.E * (p.N + 2);
   {

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import sophia_b200
-from sophia_b200 import _lib, recurrence, residual
+from sophia_b200 import _lib, recurrence, residual, ssm
 
 gpu = pytest.mark.gpu
 bf16 = torch.bfloat16
@@ -87,3 +87,21 @@ def norm(rows, backward):
 @pytest.mark.parametrize("backward", [False, True])
 def test_residual_norm(monkeypatch, backward):
     in_threads(monkeypatch, residual, [norm(r, backward) for r in (2, 500, 900, 1400)])
+
+
+def scan(states, backward):
+    rn = gen(states)
+    ts = [rn(1, 40, 64).to(bf16) for _ in range(2)]
+    B, C, A = rn(1, 40, 1, states).to(bf16), rn(1, 40, 1, states).to(bf16), -torch.ones(64, states, device="cuda")
+
+    def run():
+        x = ts[0].detach().requires_grad_(backward)
+        y = sophia_b200.selective_scan(x, ts[1], A, B, C)[0]
+        return torch.autograd.grad(y, x, ts[0])[0] if backward else y
+    return run
+
+
+@gpu
+@pytest.mark.parametrize("backward", [False, True])
+def test_selective_scan(monkeypatch, backward):
+    in_threads(monkeypatch, ssm, [scan(n, backward) for n in (33, 40, 50, 63)])
