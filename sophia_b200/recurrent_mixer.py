@@ -130,9 +130,10 @@ class ResidualStack(nn.Module):
         for every block i:
             x, h = residual_norm(x, block.mix(h), next norm's weight, branch norm, gate, scale, dropout)
 
-    The norm in front of a block is the block's own ``in_norm``, the one behind the last is ``out_norm``.  ``post_norm``
-    norms every block's output, ``gate`` multiplies it with a sigmoid of a projection of the block's input, ``scale_init``
-    gives each block a scale per channel that starts there.  ``forward`` returns (stream, normed stream)."""
+    The norm in front of a block is the block's own ``in_norm``, the one behind the last is ``out_norm``; all norms have
+    the eps that the blocks share (blocks that differ in it are refused).  ``post_norm`` norms every block's output,
+    ``gate`` multiplies it with a sigmoid of a projection of the block's input, ``scale_init`` gives each block a scale
+    per channel that starts there.  ``forward`` returns (stream, normed stream)."""
 
     def __init__(self, blocks: Sequence[nn.Module], post_norm: bool = True, gate: bool = False,
                  scale_init: float | None = None, dropout_p: float = 0.0, std: float = 0.02,
@@ -143,6 +144,9 @@ class ResidualStack(nn.Module):
         dims = {b.dim for b in blocks}
         if len(dims) != 1:
             raise ValueError(f"ResidualStack: the blocks' widths differ: {sorted(dims)}")
+        epss = {b.eps for b in blocks}
+        if len(epss) != 1:  # one call norms a block's output and the next block's input
+            raise ValueError(f"ResidualStack: the blocks' eps differ: {sorted(epss)}")
         self.dim, self.eps, self.dropout_p = blocks[0].dim, blocks[0].eps, dropout_p
         self.blocks = nn.ModuleList(blocks)
         like = blocks[0].in_norm

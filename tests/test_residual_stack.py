@@ -177,3 +177,10 @@ def test_stack_refusals():
         ResidualStack([RecurrentMixerBlock(8, 8, 2), RecurrentMixerBlock(16, 8, 2)])
     with pytest.raises(NotImplementedError):
         ResidualStack([KDAMixerBlock(dim=8, heads=1, decay_rank=2)]).make_pools(2)
+
+
+def test_stack_refuses_blocks_of_another_eps():
+    """Each block's own forward norms its input with the block's eps; a stack has one for all of its norms."""
+    with pytest.raises(ValueError, match="eps"):
+        ResidualStack([RecurrentMixerBlock(8, 8, 2), RecurrentMixerBlock(8, 8, 2, eps=1e-6)])
+    assert ResidualStack([RecurrentMixerBlock(8, 8, 2, eps=1e-6), SSMMixerBlock(8, 8, eps=1e-6)]).eps == 1e-6
