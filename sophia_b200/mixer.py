@@ -61,11 +61,11 @@ class KDAMixerBlock(nn.Module):
         self.out_norm = nn.Parameter(torch.ones(HEAD_DIM, **kw))
         self.o_proj = normal(dim, inner)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
-        """x [B, T, dim] -> [B, T, dim]."""
-        return self.mix(F.rms_norm(x, (self.dim,), self.in_norm.to(x.dtype), self.eps))
+    def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
+        """x [B, T, dim] -> [B, T, dim]; documents may be packed along T (B = 1, ``cu_seqlens``)."""
+        return self.mix(F.rms_norm(x, (self.dim,), self.in_norm.to(x.dtype), self.eps), cu_seqlens)
 
-    def mix(self, h: torch.Tensor) -> torch.Tensor:
+    def mix(self, h: torch.Tensor, cu_seqlens: torch.Tensor | None = None) -> torch.Tensor:
         """The block behind its input norm: h [B, T, dim] -> [B, T, dim]."""
         B, T, _ = h.shape
         H, D = self.heads, HEAD_DIM
@@ -76,6 +76,6 @@ class KDAMixerBlock(nn.Module):
         beta = F.linear(h, self.beta_proj)
         o, _ = kda_layer(q.reshape(B, T, H, D), k.reshape(B, T, H, D), v.reshape(B, T, H, D),
                          decay.reshape(B, T, H, D), beta, self.A_log, self.dt_bias,
-                         self.conv_q, self.conv_k, self.conv_v, lower_bound=self.lower_bound)
+                         self.conv_q, self.conv_k, self.conv_v, lower_bound=self.lower_bound, cu_seqlens=cu_seqlens)
         y = gated_rms_norm(o, gate.reshape(B, T, H, D), self.out_norm, self.eps)
         return F.linear(y.reshape(B, T, H * D), self.o_proj)

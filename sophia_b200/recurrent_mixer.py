@@ -173,8 +173,8 @@ class ResidualStack(nn.Module):
 
     def forward(self, x: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
                 seed: torch.Tensor | int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
-        """x [B, T, dim]; documents may be packed along T (blocks that take ``cu_seqlens``).  Dropout needs a ``seed`` of
-        every step's own (an int, or an int64 tensor on the device); without one nothing is dropped."""
+        """x [B, T, dim]; documents may be packed along T (B = 1, ``cu_seqlens``).  Dropout needs a ``seed`` of every step's
+        own (an int, or an int64 tensor on the device); without one nothing is dropped."""
         h = self._first(x)
         for i, block in enumerate(self.blocks):
             branch = block.mix(h) if cu_seqlens is None else block.mix(h, cu_seqlens)

@@ -184,3 +184,47 @@ def test_stack_refuses_blocks_of_another_eps():
     with pytest.raises(ValueError, match="eps"):
         ResidualStack([RecurrentMixerBlock(8, 8, 2), RecurrentMixerBlock(8, 8, 2, eps=1e-6)])
     assert ResidualStack([RecurrentMixerBlock(8, 8, 2, eps=1e-6), SSMMixerBlock(8, 8, eps=1e-6)]).eps == 1e-6
+
+
+@gpu
+def test_packed_stack_against_the_formulas():
+    """Documents packed along T, one of them empty, one of a single token."""
+    s = ResidualStack([recurrent(seed=i) for i in range(3)], scale_init=0.5, gate=True, dropout_p=0.2, generator=gen(9))
+    cu = torch.tensor([0, 1, 20, 20, 37], device="cuda", dtype=torch.int32)
+    x = torch.randn(1, 37, 64, device="cuda", generator=gen(5)).requires_grad_()
+    out = s(x, cu, seed=78)
+    p, xd = doubles(s), x.detach().double().requires_grad_()
+    want = stack_reference(s, p, xd, 78, cu)
+    up = [torch.randn(1, 37, 64, device="cuda", generator=gen(6 + i)) for i in range(2)]
+    for name, a, e in zip(("stream", "normed"), out, want):
+        near(name, a, e)
+    got = torch.autograd.grad(out, [x, *s.parameters()], up)
+    exp = torch.autograd.grad(want, [xd, *p.values()], [u.double() for u in up])
+    for name, a, e in zip(["x", *p], got, exp):
+        near(name, a, e, 1e-3)  # gradients pass every layer twice
+
+
+@gpu
+def test_packed_documents_in_a_stack_of_all_mixers():
+    """Documents packed along T give what each gives alone, outputs and summed gradients, through every mixer of the
+    package in fp32: the same sums, in matrix products of other heights."""
+    blocks = [KDAMixerBlock(dim=128, heads=1, decay_rank=16, std=0.1, generator=gen(0), device="cuda"),
+              SSMMixerBlock(dim=128, inner=128, state=8, dt_rank=16, std=0.1, generator=gen(1), device="cuda"),
+              RecurrentMixerBlock(dim=128, inner=128, rank=16, std=0.1, generator=gen(2), device="cuda")]
+    s = ResidualStack(blocks, scale_init=0.5)
+    x = torch.randn(1, 133, 128, device="cuda", generator=gen(4)).requires_grad_()
+    up = [torch.randn(1, 133, 128, device="cuda", generator=gen(6 + i)) for i in range(2)]
+    bounds = [0, 33, 34, 133]
+    cu = torch.tensor(bounds, device="cuda", dtype=torch.int32)
+    spans = list(zip(bounds[:-1], bounds[1:]))
+    for f in (blocks[0], lambda t, c=None: s(t, c)[0]):
+        near("alone", f(x, cu), torch.cat([f(x[:, a:b].contiguous()) for a, b in spans], 1).double())
+    out = s(x, cu)
+    leaves = [x, *s.parameters()]
+    got = torch.autograd.grad(out, leaves, up)
+    alone = [s(x[:, a:b].contiguous()) for a, b in spans]
+    flat = [t for pair in alone for t in pair]
+    ups = [u[:, a:b].contiguous() for a, b in spans for u in up]
+    want = torch.autograd.grad(flat, leaves, ups)
+    for (name, _), a, e in zip([("x", None), *s.named_parameters()], got, want):
+        near(name, a, e.double(), 1e-3)
