@@ -165,7 +165,7 @@ def _three(t: Tensor | None) -> Tensor | None:
         return t
     if t.dim() < 3:
         return t.reshape(1, -1, t.shape[-1]) if t.dim() == 1 else t.unsqueeze(0)
-    return t.reshape(-1, *t.shape[-2:])
+    return t.flatten(0, -3)  # (reshape(-1, ...) has no answer where a dimension is 0)
 
 
 def residual_norm(residual: Tensor, branch: Tensor, weight: Tensor | None = None, *, branch_weight: Tensor | None = None,

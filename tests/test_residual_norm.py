@@ -444,3 +444,20 @@ def test_parameters_that_have_to_be_converted(kind, shape, wide, dtype):
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("shape", [(2, 3, 0, 8), (0, 3, 2, 8), (2, 0, 1, 4, 8), (0, 8), (2, 0, 8), (8,), (5, 8), (2, 3, 4, 8)], ids=str)
+def test_any_leading_dimensions_as_three(shape):
+    """The kernels' [B, T, D], of the same elements in the same order, also where there are none."""
+    t = sophia_b200.residual._three(torch.arange(torch.Size(shape).numel()).reshape(shape))
+    assert t.dim() == 3 and t.shape[-1] == 8 and torch.equal(t.flatten(), torch.arange(t.numel()))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(2, 3, 0, 8), (0, 3, 2, 8), (2, 0, 1, 4, 8)], ids=str)
+def test_no_rows_of_more_dimensions(shape):
+    ts = inputs(gen(9), shape, f32, bf16)
+    v, n = call(ts, dropout_p=0.1, seed=3)
+    assert v.shape == n.shape == shape
+    grads = torch.autograd.grad((v, n), [ts[k] for k in NAMES], (v.detach(), n.detach()))
+    assert all(g.shape == ts[k].shape and not g.any() for k, g in zip(NAMES, grads))
