@@ -188,12 +188,18 @@ class ResidualStack(nn.Module):
                 raise NotImplementedError(f"{type(b).__name__} keeps no states in a pool")
         return [b.make_pool(slots) for b in self.blocks]
 
+    def _with(self, pools):
+        """The blocks with their pools."""
+        if len(pools) != len(self.blocks):
+            raise ValueError(f"ResidualStack: {len(pools)} pools for {len(self.blocks)} blocks")
+        return enumerate(zip(self.blocks, pools))
+
     @torch.no_grad()
     def prefill(self, x: torch.Tensor, cu_seqlens: torch.Tensor, pools: list,
                 slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """Prompts packed along T (x [1, T, dim]), their states to the requests' slots of every block's pool."""
         h = self._first(x)
-        for i, (block, pool) in enumerate(zip(self.blocks, pools)):
+        for i, (block, pool) in self._with(pools):
             x, h = self._join(i, x, h, block.mix_prefill(h, cu_seqlens, pool, slots), None)
         return x, h
 
@@ -201,6 +207,6 @@ class ResidualStack(nn.Module):
     def step(self, x: torch.Tensor, pools: list, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """One token of each request: x [R, dim]."""
         h = self._first(x)
-        for i, (block, pool) in enumerate(zip(self.blocks, pools)):
+        for i, (block, pool) in self._with(pools):
             x, h = self._join(i, x, h, block.mix_step(h, pool, slots), None)
         return x, h

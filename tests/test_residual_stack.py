@@ -228,3 +228,14 @@ def test_packed_documents_in_a_stack_of_all_mixers():
     want = torch.autograd.grad(flat, leaves, ups)
     for (name, _), a, e in zip([("x", None), *s.named_parameters()], got, want):
         near(name, a, e.double(), 1e-3)
+
+
+def test_stack_refuses_another_number_of_pools():
+    """Blocks without a pool would be left out of the stream silently."""
+    s = ResidualStack([RecurrentMixerBlock(8, 8, 2), RecurrentMixerBlock(8, 8, 2)])
+    pools, slots = s.make_pools(2), torch.zeros(1, dtype=torch.int32)
+    for some in ([], pools[:1], [*pools, pools[0]]):
+        with pytest.raises(ValueError, match="pools"):
+            s.step(torch.zeros(1, 8), some, slots)
+        with pytest.raises(ValueError, match="pools"):
+            s.prefill(torch.zeros(1, 1, 8), torch.tensor([0, 1]), some, slots)
