@@ -34,6 +34,7 @@
 #include <cooperative_groups.h>
 #include <cuda.h>  // CUtensorMap
 
+#include <cfloat>
 #include <cstring>
 
 #include "ssm_common.cuh"
@@ -555,10 +556,11 @@ struct RecBwdSmem {
   unsigned cuts[2][REC_WARPS], ends[2][REC_WARPS];
 };
 
-// Adds v to a compensated sum (s, c).
+// Adds v to a compensated sum (s, c), which an infinity leaves infinite (inf - inf would make NaN of the error).
 __device__ __forceinline__ void rec_add(u64& s, u64& c, u64 v) {
   const u64 y = sub2(v, c), t = add2(s, y);
-  c = sub2(sub2(t, s), y);
+  const float2 e = upk2(sub2(sub2(t, s), y)), f = upk2(t);
+  c = pk2(fabsf(f.x) <= FLT_MAX ? e.x : 0.f, fabsf(f.y) <= FLT_MAX ? e.y : 0.f);
   s = t;
 }
 

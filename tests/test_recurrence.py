@@ -434,3 +434,33 @@ def test_no_grad_keeps_nothing():
     frozen = {k: v.detach() for k, v in ts.items()}
     y2, _ = call(frozen, None)
     assert torch.equal(y, y2) and y2.grad_fn is None
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_infinite_gradient_leaves_infinite_sums(dtype):
+    """dA and the biases' gradients are sums over the tokens: one infinite term makes them infinite, as the plain sum,
+    where it is the only one (a gradient that enters at a sequence's first token reaches no other); other channels
+    keep their bits."""
+    rn = gen(21)
+    E, T = 70, 200
+    ts = inputs(rn, dtype, 2, T, E, 2, z=False)
+    leaves = [ts[k] for k in SUMS]
+    dy = rn(2, T, E, dtype=dtype)
+    base = torch.autograd.grad(call(ts, None, False)[0], leaves, dy)
+    # the token's own factors from the formulas (autograd adds the two parts of d(A r), which may be inf - inf)
+    x, decay, gate, A, db, gb, h0 = (ts[k].detach().double()[i][..., 5] for k, i in (
+        ("x", (1, 0)), ("decay", (1, 0)), ("gate", (1, 0)), ("A", ...), ("decay_bias", ...), ("gate_bias", ...), ("h0", 1)))
+    r, i = torch.sigmoid(decay + db), torch.sigmoid(gate + gb)
+    a = torch.exp(A * r)
+    n = torch.sqrt(1 - a * a)
+    d_rate = a * h0 - a * a / n * i * x
+    want = {"A": d_rate * r, "decay_bias": d_rate * A * r * (1 - r), "gate_bias": n * x * i * (1 - i)}
+    rest = torch.arange(E, device="cuda") != 5
+    for value in (float("inf"), -float("inf")):
+        bad = dy.clone()
+        bad[1, 0, 5] = value
+        got = torch.autograd.grad(call(ts, None, False)[0], leaves, bad)
+        for name, g, b in zip(SUMS, got, base):
+            assert g[5] == value * torch.sign(want[name]), name
+            assert torch.equal(g[rest], b[rest]), name
