@@ -403,10 +403,10 @@ int kda_b200_selective_scan_step(const kda_b200_scan_args* args, void* stream);
  * Gated linear recurrence.  Per sequence and channel e, with r = sigmoid(decay + decay_bias) and
  * i = sigmoid(gate + gate_bias):
  *     a = exp(A[e] r),   h[t] = a h[t-1] + sqrt(1 - a^2) i x[t],   y[t] = h[t] silu(z[t])  (or h[t])
- * A: [E], not positive (a positive rate has no real normaliser: its outputs are NaN).  One state per
- * channel: h0, ht, dht, dh0: [nseq][E].  Unused pointers are NULL: z, decay_bias, gate_bias, h0, ht, dht, dh0,
- * cu_seqlens; saved (kda_b200_recurrence_saved_bytes() bytes) is NULL for inference, and so may the forward's
- * workspace be without cu_seqlens.
+ * A: [E], not positive (a positive rate has no real normaliser: its outputs are NaN; -inf counts as the largest finite
+ * rate, so that a closed gate still keeps the state).  One state per channel: h0, ht, dht, dh0: [nseq][E].  Unused
+ * pointers are NULL: z, decay_bias, gate_bias, h0, ht, dht, dh0, cu_seqlens; saved (kda_b200_recurrence_saved_bytes()
+ * bytes) is NULL for inference, and so may the forward's workspace be without cu_seqlens.
  * kda_b200_recurrence_bwd takes the same inputs, the saved buffer of the forward, dy and dht, and writes dx, ddecay,
  * dgate, dz [B, T, E] in the activations' type and dA, ddecay_bias, dgate_bias [E] (the last two may be
  * NULL) and dh0 in fp32; all sums have a fixed order.  Where nothing decays (a = 1 to the last bit) the input's part of

@@ -109,13 +109,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 // a = 2^l and w = 1 - a^2 for l <= 0, both with fp32 relative accuracy.  l = n + f, n the nearest whole
 // number; q = 1 - 2^f is a polynomial times f, which keeps q accurate in relative terms next to 0;
-// a = 2^n (1 - q), m = 1 - a = 2^n q + (1 - 2^n) cancels nowhere, w = m (2 - m).  CLAMP: l may be below -126.
+// a = 2^n (1 - q), m = 1 - a = 2^n q + (1 - 2^n) cancels nowhere, w = m (2 - m).  CLAMP: l may be below -126; from
+// -150 on, where fp32 has nothing below, a is 0 (2^-126 times a rate of 1e34 would count in the rate's gradient).
 template <bool CLAMP>
 __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64& w) {
-  if (CLAMP) {
-    const float2 lf = upk2(l);
-    l = pk2(max_nan(lf.x, -126.f), max_nan(lf.y, -126.f));
-  }
+  const float2 lf = upk2(l);
+  if (CLAMP) l = pk2(max_nan(lf.x, -126.f), max_nan(lf.y, -126.f));
   const u64 t = add2(l, k.round);  // the sum's low bits are n
   const u64 f = sub2(l, sub2(t, k.round));
   u64 p = fma2(k.poly[0], f, k.poly[1]);
@@ -126,6 +125,10 @@ __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64&
                     __int_as_float((__float_as_int(tf.y) << 23) + 0x3f800000));
   const u64 q = mul2(p, f);
   a = mul2(s, sub2(k.one, q));
+  if (CLAMP) {
+    const float2 af = upk2(a);
+    a = pk2(lf.x < -150.f ? 0.f : af.x, lf.y < -150.f ? 0.f : af.y);
+  }
   const u64 m = fma2(s, q, sub2(k.one, s));
   w = mul2(m, sub2(k.two, m));
 }
@@ -275,10 +278,16 @@ __device__ __forceinline__ void rec_put(T* row, u64 v, int nch) {
     if (c1 < nch) row[c1] = io_from_f<T>(f.y);
   }
 }
-// The rates in log2 units: NaN for a positive one, whose normaliser is not real.
+// The rates: NaN for a positive one, whose normaliser is not real; -inf as the largest finite one (a closed gate times
+// an infinity would be NaN).  And in log2 units.
 __device__ __forceinline__ u64 rec_rates(u64 a) {
+  auto rate = [](float v) { return v > 0.f ? __int_as_float(0x7fffffff) : max_nan(v, -FLT_MAX); };
   const float2 f = upk2(a);
-  return pk2(f.x > 0.f ? __int_as_float(0x7fffffff) : f.x * LOG2E, f.y > 0.f ? __int_as_float(0x7fffffff) : f.y * LOG2E);
+  return pk2(rate(f.x), rate(f.y));
+}
+__device__ __forceinline__ u64 rec_log2_rates(u64 rates) {
+  const float2 f = upk2(rates);
+  return pk2(max_nan(f.x * LOG2E, -FLT_MAX), max_nan(f.y * LOG2E, -FLT_MAX));
 }
 // fp32 vectors over the channels
 __device__ __forceinline__ u64 rec_vec(const float* p, bool vec, int nch, float none) {
@@ -424,7 +433,7 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_fwd_kernel(const __
   for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
   const RecConst& K = P.k;
-  const u64 A2 = rec_rates(rec_vec(P.A + ch0, VEC, nch, 0.f));
+  const u64 A2 = rec_log2_rates(rec_rates(rec_vec(P.A + ch0, VEC, nch, 0.f)));
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const bool steep = __any_sync(0xffffffffu, upk2(A2).x < -126.f || upk2(A2).y < -126.f);
@@ -618,7 +627,7 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_bwd_kernel(const __
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k) fetch(k);
 
-  const u64 A1 = rec_vec(P.A + ch0, VEC, nch, 0.f), A2 = rec_rates(A1);
+  const u64 A1 = rec_rates(rec_vec(P.A + ch0, VEC, nch, 0.f)), A2 = rec_log2_rates(A1);
   const u64 nd = mul2(rec_vec(P.decay_bias ? P.decay_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const u64 ng = mul2(rec_vec(P.gate_bias ? P.gate_bias + ch0 : nullptr, VEC, nch, 0.f), all2(-LOG2E));
   const bool steep = __any_sync(0xffffffffu, upk2(A2).x < -126.f || upk2(A2).y < -126.f);
@@ -825,7 +834,7 @@ __global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(const __grid
   const int c = (blockIdx.x * REC_STEP_THREADS + threadIdx.x) * V;
   if (c >= P.E) return;
   auto vec = [&](const float* p) { return p ? pk2(__ldg(p + c), VEC ? __ldg(p + c + 1) : 0.f) : 0ull; };
-  const u64 A2 = rec_rates(vec(P.A));
+  const u64 A2 = rec_log2_rates(rec_rates(vec(P.A)));
   const u64 nd = mul2(vec(P.decay_bias), all2(-LOG2E)), ng = mul2(vec(P.gate_bias), all2(-LOG2E));
   for (int r = blockIdx.y; r < P.rows; r += gridDim.y) {
     const int slot = step_slot(P.slots, r, P.pool, P.err);

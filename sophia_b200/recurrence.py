@@ -201,8 +201,8 @@ def gated_recurrence(x: Tensor, decay: Tensor, gate: Tensor, A: Tensor, z: Tenso
         y[t] = h[t] * silu(z[t])        (h[t] without z)
 
     x, decay, gate, z: ``[B, T, E]``, the gates as logits; A: ``[E]``, the rates
-    themselves, not positive (a positive one gives NaN); decay_bias, gate_bias:
-    ``[E]``.  ``initial_state`` ``[sequences, E]`` float32; with ``cu_seqlens``
+    themselves, not positive (a positive one gives NaN, -inf is the largest finite one);
+    decay_bias, gate_bias: ``[E]``.  ``initial_state`` ``[sequences, E]`` float32; with ``cu_seqlens``
     (``[sequences + 1]``, B = 1) sequences are packed along T and the state restarts
     at each.  Returns ``(y, final_state | None)``, y in x's type; gradients reach every
     floating-point input.  Where a is 1 to the last bit nothing enters the state, and

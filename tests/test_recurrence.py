@@ -464,3 +464,35 @@ def test_an_infinite_gradient_leaves_infinite_sums(dtype):
         for name, g, b in zip(SUMS, got, base):
             assert g[5] == value * torch.sign(want[name]), name
             assert torch.equal(g[rest], b[rest]), name
+
+
+@gpu
+@pytest.mark.parametrize("dtype,T", [(torch.float32, 75), (torch.bfloat16, 700)])
+def test_states_that_forget_at_once(dtype, T):
+    """Rates so steep that no state outlives a token, -inf the steepest: h = i x, whatever went before, and
+    nothing of the gradients comes through a decay of 0 -- not even times a rate of 1e38.  A closed gate still lets the
+    state through."""
+    rn = gen(22)
+    E = 66
+    ts = inputs(rn, dtype, 2, T, E, 2, z=False, biases=False)
+    leaves = [ts[k] for k in ("x", "decay", "gate", "A", "h0")]
+    dy, dht = rn(2, T, E, dtype=dtype), rn(2, E)
+    runs = []
+    for rate in (-1e30, -1e34, -1e38, -3.4e38, float("-inf")):
+        with torch.no_grad():
+            ts["A"].fill_(rate)
+        y, ht = call(ts, None)
+        runs.append([t.detach() for t in (y, ht, *torch.autograd.grad((y, ht), leaves, (dy, dht)))])
+        close("y", y, torch.sigmoid(ts["gate"].detach().double()) * ts["x"].detach().double(), dtype)
+        pool = ts["h0"].detach().clone()
+        step = sophia_b200.gated_recurrence_step(*(ts[k].detach()[:, 0] for k in ("x", "decay", "gate")), ts["A"].detach(),
+                                                 pool)
+        assert torch.equal(step, y.detach()[:, 0])
+    for run in runs:
+        assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+    d_decay, d_A, d_h0 = runs[0][3], runs[0][5], runs[0][6]
+    assert not d_decay.any() and not d_A.any() and not d_h0.any()
+    with torch.no_grad():
+        ts["decay"].fill_(float("-inf"))
+        y, ht = call(ts, None)
+    assert torch.equal(ht, ts["h0"].detach()) and torch.equal(y[:, 0], ts["h0"].detach().to(dtype))
