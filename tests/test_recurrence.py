@@ -496,3 +496,22 @@ def test_states_that_forget_at_once(dtype, T):
         ts["decay"].fill_(float("-inf"))
         y, ht = call(ts, None)
     assert torch.equal(ht, ts["h0"].detach()) and torch.equal(y[:, 0], ts["h0"].detach().to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_strides_give_the_same_bits(dtype):
+    """Expanded, transposed and odd rows against contiguous ones: the copies differ, a channel's arithmetic and the split
+    over a cluster's CTAs (both by the sizes alone) do not, forward and backward."""
+    rn = gen(16)
+    A = -torch.exp(rn(64))
+
+    def run(t):
+        t = t.detach().requires_grad_()
+        y, ht = sophia_b200.gated_recurrence(t, t, t, A, t, output_final_state=True)
+        return y, ht, torch.autograd.grad((y, ht), t, (torch.ones_like(y), torch.ones_like(ht)))[0]
+
+    for t in (rn(1, 300, 64, dtype=dtype).expand(3, 300, 64), rn(3, 1, 64, dtype=dtype).expand(3, 300, 64),
+              rn(300, 3, 64, dtype=dtype).transpose(0, 1), rn(3, 64, 300, dtype=dtype).transpose(1, 2),
+              rn(3, 300, 67, dtype=dtype)[..., 3:], rn(3, 300, 66, dtype=dtype)[..., 1:65]):
+        assert all(torch.equal(a, b) for a, b in zip(run(t), run(t.contiguous())))

@@ -461,3 +461,24 @@ def test_no_rows_of_more_dimensions(shape):
     assert v.shape == n.shape == shape
     grads = torch.autograd.grad((v, n), [ts[k] for k in NAMES], (v.detach(), n.detach()))
     assert all(g.shape == ts[k].shape and not g.any() for k, g in zip(NAMES, grads))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [bf16, f32])
+def test_gradient_of_a_broadcast_gate_term_by_term(dtype):
+    """Every token's gradient is within the bounds above (2e-5 of its row's ``terms`` and half a step), and so their sum is
+    within the sum of those bounds, for the terms that are summed, and one more rounding: half a step of the result."""
+    rn = gen(33)
+    ts = inputs(rn, (3, 20, 192), f32, dtype)
+    for shape in ((3, 1, 192), (192,), (1, 20, 192)):
+        gate = rn(*shape, dtype=dtype).requires_grad_()
+        out = call(dict(ts, gate=gate))
+        up = [rn(*out[0].shape), rn(*out[1].shape, dtype=dtype)]
+        (got,) = torch.autograd.grad(out, gate, up)
+        r = {k: None if t is None else t.detach().double() for k, t in dict(ts, gate=gate).items()}
+        r["gate"] = r["gate"].expand(3, 20, 192).clone().requires_grad_()
+        want = torch.autograd.grad(ref.residual_norm(*(r[k] for k in NAMES), 0, 0, 0, 1e-5), r["gate"], [u.double() for u in up])[0]
+        each = ROUND[dtype] * want.abs() + 2e-5 * terms(r, up, 0.0, 1e-5)["d_gate"]
+        total, bound = want.sum_to_size(shape), each.sum_to_size(shape)
+        bound = bound + ROUND[dtype] * (total.abs() + bound)
+        assert got.shape == gate.shape and ((got.double() - total).abs() <= bound).all()
