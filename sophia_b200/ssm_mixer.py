@@ -85,8 +85,8 @@ class SSMMixerBlock(nn.Module):
         return self._mix(h, cu_seqlens)[0]
 
     def make_pool(self, slots: int) -> SSMPool:
-        """Zero states for `slots` requests."""
-        new = self.in_norm.new_zeros
+        """Zero states for `slots` requests, in float32 whatever the parameters' type."""
+        new = lambda *s: self.in_norm.new_zeros(s, dtype=torch.float32)  # noqa: E731
         return SSMPool(new(slots, self.inner, self.taps - 1), new(slots, self.inner, self.state))
 
     @torch.no_grad()

@@ -239,3 +239,30 @@ def test_stack_refuses_another_number_of_pools():
             s.step(torch.zeros(1, 8), some, slots)
         with pytest.raises(ValueError, match="pools"):
             s.prefill(torch.zeros(1, 1, 8), torch.tensor([0, 1]), some, slots)
+
+
+@pytest.mark.parametrize("kind", [torch.bfloat16, torch.float16])
+def test_pools_are_float32_for_parameters_in_16_bits(kind):
+    s = ResidualStack([RecurrentMixerBlock(8, 8, 2), SSMMixerBlock(8, 8)]).to(kind)
+    assert all(t.dtype == torch.float32 and not t.any() for pool in s.make_pools(3) for t in pool)
+
+
+@gpu
+def test_stack_in_16_bits_serves():
+    """A model cast to bf16 as a whole: prompts and single tokens run, and continue each other's states.  One layer rounds
+    about ten times (projections, convolution, gates, recurrence, norms), each by 2^-8 of its values, with gains around one,
+    and what is compared went through two layers twice: 40 2^-8 of the largest value."""
+    s = ResidualStack([recurrent(seed=1), recurrent(seed=2)], scale_init=0.5, gate=True, generator=gen(4)).bfloat16()
+    x = torch.randn(2, 20, 64, device="cuda", generator=gen(7)).bfloat16()
+    with torch.no_grad():
+        stream, normed = s(x)
+    pools = s.make_pools(4)
+    slots = torch.tensor([3, 1], device="cuda", dtype=torch.int32)
+    cu = torch.tensor([0, 12, 24], device="cuda", dtype=torch.int32)
+    got = s.prefill(x[:, :12].reshape(1, 24, 64), cu, pools, slots)
+    assert got[0].dtype == got[1].dtype == torch.bfloat16
+    near("prompt", got[1].reshape(2, 12, 64), normed[:, :12].double(), 40 * 2.0 ** -8)
+    for t in range(12, 20):
+        a, b = s.step(x[:, t], pools, slots)
+        near("stream", a, stream[:, t].double(), 40 * 2.0 ** -8)
+        near("normed", b, normed[:, t].double(), 40 * 2.0 ** -8)
