@@ -409,8 +409,8 @@ int kda_b200_selective_scan_step(const kda_b200_scan_args* args, void* stream);
  * bytes) is NULL for inference, and so may the forward's workspace be without cu_seqlens.
  * kda_b200_recurrence_bwd takes the same inputs, the saved buffer of the forward, dy and dht, and writes dx, ddecay,
  * dgate, dz [B, T, E] in the activations' type and dA, ddecay_bias, dgate_bias [E] (the last two may be
- * NULL) and dh0 in fp32; all sums have a fixed order.  Where nothing decays (a = 1 to the last bit) the input's part of
- * ddecay and dA, which has no limit for A = 0, counts as 0.
+ * NULL) and dh0 in fp32; all sums have a fixed order.  Where 1 - a^2 is below fp32's normal range (1.2e-38), it and the
+ * input's part of ddecay and dA, which has no limit for A = 0, count as 0.
  * kda_b200_recurrence_step takes `rows` single tokens: x, decay, gate, z [rows, E] (*_sb: row strides), a pool of
  * states [pool][E] rewritten in place, and slots as kda_b200_short_conv_step; y [rows, E].
  */

@@ -13,10 +13,11 @@
 // exchanges their maps through distributed shared memory, in the order of the
 // tiles -- one pass over the data at any number of rows.
 //
-// 10 bytes an element (bf16, with z) against six special functions (ex2 of three
-// sigmoids, rcp of two, rsqrt), which the SM makes at 16 a clock: 51 and 45 us per
-// 4 x 4096 x 2048 elements, so the decay's exponential is a polynomial on packed fp32
-// arithmetic, which also gives 1 - a^2 without cancellation.
+// 10 bytes an element (bf16, with z) against seven special functions (ex2 and rcp of three
+// sigmoids, sqrt), which the SM makes at 16 a clock: 51 and 52 us per 4 x 4096 x 2048
+// elements, so the decay's exponential is a polynomial on packed fp32 arithmetic, which
+// also gives 1 - a^2 without cancellation.  (One special function less, rsqrt(w d d) w for
+// sqrt(w) / d, took as long, and an input gate's d = 1 + e^44 and above overflowed it.)
 //
 // Measured at 4 x 4096 x 2048 bf16 with z: forward 108 us, backward 195 us (floors 51 and
 // 92 us of bytes), 128 channel groups on 148 SMs in clusters of two; 32 x 512 x 2048, no
@@ -131,15 +132,6 @@ __device__ __forceinline__ void rec_decay(const RecConst& k, u64 l, u64& a, u64&
   }
   const u64 m = fma2(s, q, sub2(k.one, s));
   w = mul2(m, sub2(k.two, m));
-}
-// sqrt(w) / d: one special function in the place of a root and a reciprocal
-__device__ __forceinline__ u64 rec_sqrt_over(u64 w, u64 d) {
-  const float2 f = upk2(w);  // w = 0 and an infinite d both give 0, their limits
-  const float2 g = upk2(mul2(mul2(pk2(max_nan(f.x, 1.17549435e-38f), max_nan(f.y, 1.17549435e-38f)), d), d));
-  float x = g.x, y = g.y;
-  asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(x));
-  asm("rsqrt.approx.ftz.f32 %0, %0;" : "+f"(y));
-  return mul2(w, pk2(x, y));
 }
 __device__ __forceinline__ u64 rec_sqrt(u64 w) {
   float2 f = upk2(w);
@@ -472,9 +464,9 @@ __global__ void __launch_bounds__(REC_THREADS, REC_CTAS) rec_fwd_kernel(const __
         const u64 l = mul2(A2, r);
         rec_decay<!all.value>(K, l, a[j], w);
         logs = add2(logs, l);
-        const u64 g = add2(rec_expneg(K, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng), K.one);
+        const u64 i = rec_sig(K, rec_expneg(K, rec_get<T, VEC>(s + 2 * TB, row, rec_odd<T, VEC>(pg, P.gate.st, t)), ng));
         const u64 x = rec_get<T, VEC>(s + TB, row, rec_odd<T, VEC>(px, P.x.st, t));
-        bb[j] = mul2(rec_sqrt_over(w, g), x);
+        bb[j] = mul2(mul2(rec_sqrt(w), i), x);
         if (Z) zr[j] = rec_raw<T, VEC>(s + 3 * TB, row, rec_odd<T, VEC>(pz, P.z.st, t));
         if (!all.value && (marks.starts >> j & 1)) c = h0_of(marks, j);
         c = fma2(a[j], c, bb[j]);
@@ -852,10 +844,10 @@ __global__ void __launch_bounds__(REC_STEP_THREADS) rec_step_kernel(const __grid
     float* sp = P.state + (long long)slot * P.E + c;
     float hf[V];
     io_load<float, V>(sp, hf);
-    const u64 rd = rec_sig(P.k, rec_expneg(P.k, in(P.decay, P.sd), nd)), gi = add2(rec_expneg(P.k, in(P.gate, P.sg), ng), P.k.one);
+    const u64 rd = rec_sig(P.k, rec_expneg(P.k, in(P.decay, P.sd), nd)), gi = rec_sig(P.k, rec_expneg(P.k, in(P.gate, P.sg), ng));
     u64 a, w;
     rec_decay<true>(P.k, mul2(A2, rd), a, w);
-    const u64 b = mul2(rec_sqrt_over(w, gi), in(P.x, P.sx));
+    const u64 b = mul2(mul2(rec_sqrt(w), gi), in(P.x, P.sx));
     const u64 h = fma2(a, pk2(hf[0], hf[V - 1]), b);
     u64 o = h;
     if (P.z) {

@@ -205,8 +205,8 @@ def gated_recurrence(x: Tensor, decay: Tensor, gate: Tensor, A: Tensor, z: Tenso
     decay_bias, gate_bias: ``[E]``.  ``initial_state`` ``[sequences, E]`` float32; with ``cu_seqlens``
     (``[sequences + 1]``, B = 1) sequences are packed along T and the state restarts
     at each.  Returns ``(y, final_state | None)``, y in x's type; gradients reach every
-    floating-point input.  Where a is 1 to the last bit nothing enters the state, and
-    the gradient that would reach the rate through the input counts as 0."""
+    floating-point input.  Where 1 - a^2 is below fp32's normal range (1.2e-38) it
+    counts as 0: nothing enters the state, and no gradient reaches the rate through the input."""
     what = "gated_recurrence"
     io = _check(what, x, ("B", "T", "E"), decay, gate, A, z, decay_bias, gate_bias)
     nseq = _num_seqs(what, x, cu_seqlens)

@@ -515,3 +515,21 @@ def test_strides_give_the_same_bits(dtype):
               rn(300, 3, 64, dtype=dtype).transpose(0, 1), rn(3, 64, 300, dtype=dtype).transpose(1, 2),
               rn(3, 300, 67, dtype=dtype)[..., 3:], rn(3, 300, 66, dtype=dtype)[..., 1:65]):
         assert all(torch.equal(a, b) for a, b in zip(run(t), run(t.contiguous())))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [-44.0, -60.0, -80.0])
+def test_nearly_closed_input_gates(dtype, shift):
+    """Gates of e^-44 to e^-80 let that share of the inputs in, on a state that starts from nothing: the bounds above,
+    which are relative to the outputs' own size."""
+    rn = gen(24)
+    ts = inputs(rn, dtype, 2, 150, 72, 2, state=False)
+    ts["gate_bias"] = (ts["gate_bias"].detach() + shift).requires_grad_()
+    check(ts, None, rn(2, 150, 72, dtype=dtype), rn(2, 72))
+    d = {k: None if v is None else v.detach() for k, v in ts.items()}
+    pool = torch.zeros(2, 72, device="cuda")
+    y = sophia_b200.gated_recurrence_step(*(d[k][:, 0] for k in ("x", "decay", "gate")), d["A"], pool, d["z"][:, 0],
+                                          d["decay_bias"], d["gate_bias"])
+    r = {k: None if v is None else v.double() for k, v in d.items()}
+    close("step", y, ref.recurrence(*(r[k] for k in NAMES), None)[0][:, 0], dtype)
