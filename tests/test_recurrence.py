@@ -533,3 +533,17 @@ def test_nearly_closed_input_gates(dtype, shift):
                                           d["decay_bias"], d["gate_bias"])
     r = {k: None if v is None else v.double() for k, v in d.items()}
     close("step", y, ref.recurrence(*(r[k] for k in NAMES), None)[0][:, 0], dtype)
+
+
+def test_kept_states_have_the_size_that_the_library_asks_for():
+    """What the traced form allocates is what the library computes, at every size."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    lib, op = sophia_b200._lib.load(), torch.ops.sophia_b200.gated_recurrence_fwd.default
+    with FakeTensorMode():
+        for io, dtype in enumerate((torch.float32, torch.bfloat16, torch.float16)):
+            for B, T, E in ((1, 1, 1), (2, 31, 8), (3, 32, 5), (1, 64, 64), (2, 65, 7), (1, 129, 2048), (2, 0, 3)):
+                x, A = torch.empty(B, T, E, dtype=dtype, device="cuda"), torch.empty(E, device="cuda")
+                y, ht, saved = op(x, x, x, A, None, None, None, None, None, True, True)
+                assert y.shape == x.shape and y.dtype == dtype and ht.shape == (B, E)
+                assert saved.shape == (lib.kda_b200_recurrence_saved_bytes(B, T, E, io),)
