@@ -19,14 +19,15 @@
 // also gives 1 - a^2 without cancellation.  (One special function less, rsqrt(w d d) w for
 // sqrt(w) / d, took as long, and an input gate's d = 1 + e^44 and above overflowed it.)
 //
-// Measured at 4 x 4096 x 2048 bf16 with z: forward 108 us, backward 195 us (floors 51 and
+// Measured at 4 x 4096 x 2048 bf16 with z: forward 108 us, backward 196 us (floors 51 and
 // 92 us of bytes), 128 channel groups on 148 SMs in clusters of two; 32 x 512 x 2048, no
-// cluster: 79 and 164 us.  What bounds them: latency at 128 registers and 3.3 warps a
-// scheduler (48 % of the issue slots, 44 and 40 % of the special functions, 32 % of DRAM)
-// and SMs left over.  Tried: CTAs of 512 threads, one an SM, without a cluster (111 and
-// 195 us, but 273 against 233 for the forward of one row of 32768 tokens); 4 tokens a
-// thread and three CTAs an SM (142 and 289 us); CTAs of 128 threads; a tile's gates ahead
-// of the states of the one before (5 % slower).
+// cluster: 81 and 162 us; fp32, 2 x 4096 x 2048: 78 and 122 us (51 and 92).  What bounds
+// them: latency at 128 registers and 3.3 warps a scheduler (47 and 49 % of the issue slots,
+// 51 and 40 % of the special functions, 31 % of DRAM) and SMs left over; at that number the
+// 16-bit backward spills 72 bytes a thread (48 without z at odd rows).  Tried: CTAs of 512
+// threads, one an SM, without a cluster (111 and 195 us, but 273 against 233 for the forward
+// of one row of 32768 tokens); 4 tokens a thread and three CTAs an SM (142 and 289 us); CTAs
+// of 128 threads; a tile's gates ahead of the states of the one before (5 % slower).
 //
 // A run's decay P is the exponential of its tokens' summed logarithms: one rounding of 2^-24 where their product has one a
 // token, which is what a state that remembers thousands of tokens would feel.
@@ -92,7 +93,7 @@ inline RecConst rec_const() {
     std::memcpy(&u, &v, 4);
     return (u64)u << 32 | u;
   };
-  // a fit of (1 - 2^f) / f on [-1/2, 1/2], relative error 1.1e-8, highest power first; 1.5 2^23
+  // a fit of (1 - 2^f) / f on [-1/2, 1/2], relative error 2.1e-8, highest power first; 1.5 2^23
   return {two(1.f), two(2.f), two(-LOG2E), two(12582912.f),
           {two(-0.000154035122f), two(-0.00133907353f), two(-0.00961823761f), two(-0.0555035733f), two(-0.240226492f),
            two(-0.693147182f)}};

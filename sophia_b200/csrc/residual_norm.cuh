@@ -136,7 +136,7 @@ __device__ __forceinline__ unsigned rn_kept(const RnParams& P, unsigned k0, unsi
 // ---------------------------------------------------------------- forward, rows wherever they lie
 
 // A group of warps has a row, in registers between its two reductions.  Instructions bound it: 116 an element at 75 % of
-// the issue slots (predicates and addresses of single elements), DRAM at 33 %; the backward 169 at 55 %.
+// the issue slots (predicates and addresses of single elements), DRAM at 32 %; the backward 163 at 55 %.
 template <typename TX, typename TO, int K>
 __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 4 : 1) rn_fwd_kernel(const __grid_constant__ RnParams P) {
   __shared__ float part[2][1][RN_MAX_WARPS];
@@ -242,6 +242,11 @@ __global__ void __launch_bounds__(rn_plain_threads(K), K == 2 ? 4 : 1) rn_fwd_ke
 // threads; GATE; DROP).  Measured at 4 x 4096 x 1536, bf16 with an fp32 stream, norms on both sides, gate and dropout:
 // forward 72 us and backward 128 us (75 and 66 % of the copy bandwidth); 2 x 4096 x 4096 bf16 without gate and dropout:
 // 51 and 104 us (80 and 59 %).
+// What each switch brings, known to the compiler and decided in the kernel (between events, forward + backward): GATE at
+// 16384 x 1536 67 + 110 and 66 + 130 us, with dropout 71 + 134 and 71 + 188; DROP there 71 + 134 and 69 + 138, without
+// dropout 67 + 110 and 65 + 122; FULL at 8192 x 4096 55 + 109 and 53 + 114, with gate and dropout 74 + 157 and 79 + 159,
+// at 200 x 1536 13 + 28 and 14 + 30, but at 16384 x 1536 with gate and dropout 71 + 134 and 65 + 126: its rows of 24
+// channels a thread would be better off without.
 // Tried: a warp of its own for the copies (17 warps: 96 registers, spills); parameters from global memory; 8 channels a
 // thread (forward 124 us); 16 channels of narrow rows (backward of 32768 x 256 88 us against 69).
 constexpr int RN_MAX_STAGES = 4;

@@ -181,8 +181,8 @@ def residual_norm(residual: Tensor, branch: Tensor, weight: Tensor | None = None
         normed = rms_norm(stream) * weight
 
     with ``rms_norm(a) = a / sqrt(mean(a^2) + eps)`` over the last dimension, D <= 8192.
-    residual, branch: ``[..., D]``; gate: logits of branch's shape, or of one that
-    broadcasts to it; weight, branch_weight, scale: ``[D]``.  The residual may be
+    residual, branch: ``[..., D]``; gate: logits of branch's shape, or ``[..., D]`` whose
+    leading dimensions broadcast to it; weight, branch_weight, scale: ``[D]``.  The residual may be
     float32 beside a 16-bit branch.  Returns ``(stream, normed)``: the stream in residual's type,
     normed in branch's, or None without weight.
 
